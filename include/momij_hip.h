@@ -188,6 +188,130 @@ mj_status mj_attn_block(mj_ctx* ctx, const mj_attn_config* cfg, const mj_attn_we
                         void* h, void* kcache, void* vcache, int64_t L,
                         const int32_t* parents_host, int M);
 
+/* ------------------------------------------------- a KV cache in 8 bits ------ */
+/* The context of a full-attention layer in two tiers (no counterpart in the reference, whose caches
+ * are fp16): an fp16 ring holds the newest positions, and blocks of MJ_KV8_BLOCK positions are
+ * sealed from it into pages of 8-bit codes.  Attention reads both.  Keys are rotated before they are
+ * cached, so which position a block held does not matter once it is sealed: blocks may be left out
+ * of a call (mj_kv8_select) or for good (mj_kv8_evict).  Heads of 128 only.
+ *
+ * Every call below is asynchronous on the context's stream and takes no host array but
+ * parents_host: with a tree it is refused while the stream is being captured (a replay would run on
+ * the captured call's); with NULL, a chain, it may be captured.  Lengths and positions are
+ * captured as they are.  Calls that need device scratch take it from ws (16-byte aligned,
+ * mj_kv8_workspace bytes), or, ws NULL, from the context's growable scratch, and are then refused
+ * while the stream is being captured (a later call may replace that scratch).  Calls that share a ws
+ * must be ordered by the caller.  Calls that may overlap may share a pool as long as none of them
+ * writes pages, table entries or ring slots that another one touches.  Device pointers must be
+ * 16-byte aligned. */
+#define MJ_KV8_BLOCK 64
+
+/* Pool of pages and the lists of them.  A page holds one block of one KV head: 64 x 128 codes of K
+ * and of V, a scale for each, and the greatest and the least K code of every dim.  A value is
+ * code * scale.  Page bytes are in the order the matrix instructions take them:
+ *   K: byte 2048 (t / 16) + 1024 (d / 64) + 256 (d / 16 % 4) + 16 (t % 16) + d % 16
+ *   V: byte 1024 (d / 16) + 256 (t / 4 % 4) + 16 (d % 16) + 4 (t / 16) + t % 4
+ * of token t, dim d, each byte its code + 128.  table[g * table_stride + i] is the page of the i-th
+ * block of head g: a head's row lists its n_blocks blocks in use, then (after mj_kv8_evict, or as
+ * the caller filled it) its free pages.  An entry outside [0, n_pages) names no block: it is neither
+ * read nor written, and its keys are left out.  Two entries naming one page must not both be
+ * sealed. */
+typedef struct mj_kv8 {
+    int n_kv_heads;
+    int n_pages;           /* pages of the pool, of all heads together */
+    void* k_codes;         /* [n_pages][8192] */
+    void* v_codes;         /* [n_pages][8192] */
+    float* k_scale;        /* [n_pages] */
+    float* v_scale;        /* [n_pages] */
+    int8_t* k_bounds;      /* [n_pages][2][128]: greatest, least code */
+    int32_t* table;        /* [n_kv_heads][table_stride] */
+    int table_stride;      /* blocks a head can list */
+} mj_kv8;
+
+/* fp16 rows [n_kv_heads][capacity][128] of K and V, position p at slot p % capacity (the layout of
+ * mj_attn_block's caches and of mj_model_kv). */
+typedef struct mj_kv_ring {
+    void* k;
+    void* v;
+    int64_t capacity;
+} mj_kv_ring;
+
+/* Queries and keys of a pass finished and appended: per-head RMSNorm(eps) * weight, then RoPE of the
+ * first rope_dim dims (0, 32, 64 or 128; halves (i, i + rope_dim / 2) of a head rotate together) at
+ * the row's position L + depth(r), angles formed in 64 bits; parents_host as in mj_attn_block.  qkv
+ * fp16 [M] rows of ld_qkv halves (0: packed; else a multiple of 8): the q, k and v heads of a raw
+ * projection.  q_out fp16 [M][n_heads * 128]; keys and values of row r go to slot (L + r) %
+ * capacity.  Reads n_heads, n_kv_heads, head_dim, rope_dim, rope_base and eps of cfg. */
+mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv, int64_t ld_qkv,
+                        const void* q_norm_w, const void* k_norm_w, const mj_kv_ring* ring,
+                        int64_t L, const int32_t* parents_host, int M, void* q_out);
+
+/* Positions [pos, pos + 64 count) of the ring sealed into the pages of table entries at .. at +
+ * count - 1 of every head: scale = m / 127 and code = round(x * (127 / m)) to the nearest whole
+ * number, ties to even, each operation in fp32, m the block's greatest finite magnitude (0: all
+ * codes 0).  An infinity takes the code +-127, a NaN 0.  64 count <= capacity. */
+mj_status mj_kv8_seal(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int64_t pos,
+                      int count, int at);
+/* The way back, for a rewind into sealed blocks: entries at .. at + count - 1 to positions
+ * [pos, pos + 64 count) of the ring, half(code * scale). */
+mj_status mj_kv8_unseal(mj_ctx* ctx, const mj_kv8* cache, int at, int count,
+                        const mj_kv_ring* ring, int64_t pos);
+
+/* Blocks for each row to read: sel int32 [M][n_kv_heads][n_sel], indices into the head's list in
+ * increasing order: the first n_first and the last n_last of the n_blocks blocks and, of the others,
+ * those of the greatest score (the lower index on ties); all blocks, then -1, where n_sel >
+ * n_blocks.  n_first + n_last <= n_sel (each is cut to n_blocks).  The score bounds q k over the
+ * block: with c the query's 8-bit codes of scale s_q (formed as sealed ones are),
+ *   max over the group's heads of  (sum_d max(c_d greatest_d, c_d least_d)) * k_scale * s_q,
+ * the sum in whole numbers, the products in fp32 from left to right.  A NaN score counts as the
+ * least.  q fp16 [M] rows of ld_q halves (0: packed; else a multiple of 8). */
+mj_status mj_kv8_select(mj_ctx* ctx, const mj_kv8* cache, int n_heads, const void* q, int64_t ld_q,
+                        int M, int n_blocks, int n_sel, int n_first, int n_last, int32_t* sel,
+                        void* ws, size_t ws_bytes);
+
+/* Attention of M rows: softmax(q k^T / sqrt(128)) v over the sealed blocks [0, n_blocks) of each
+ * head, or (sel, as mj_kv8_select writes it) those listed for the row and head, and over the ring's
+ * positions [start, L) and the row's ancestors and itself among the pass's own rows at L + r
+ * (parents_host as in mj_attn_block).  A listed index outside [0, n_blocks) names no block; one that
+ * is listed twice counts twice.  q as in mj_kv8_select, out fp16 [M] rows of ld_out halves.  0 <=
+ * start <= L, L - start + M <= ring capacity.
+ * mass_out (nullable; not with sel) float [n_kv_heads][table_stride]: for every block its entry of
+ * mass_in (same layout, NULL: zeros; may be mass_out) plus the softmax weight that all rows and the
+ * group's heads gave the block's keys.
+ * Scores, softmax statistics and outputs are summed in fp32; the weights are rounded to fp16 for the
+ * product with V.  A call repeats bit for bit; a row's result in a call of other rows may differ by
+ * rounding (the keys are split differently). */
+mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int n_heads,
+                      const void* q, int64_t ld_q, int M, int n_blocks, const int32_t* sel,
+                      int n_sel, int64_t start, int64_t L, const int32_t* parents_host, void* out,
+                      int64_t ld_out, const float* mass_in, float* mass_out, void* ws,
+                      size_t ws_bytes);
+
+/* Eviction down to `keep` of n_blocks blocks a head: the first n_first, the last n_last and, of the
+ * others, those of the greatest mass stay (the lower index on ties; a NaN counts as the least; each
+ * head by its own masses).  table_out [n_kv_heads][table_stride] lists the kept blocks in their
+ * order, then the evicted ones' pages (free now) in theirs, then the rest of the row unchanged;
+ * mass_out likewise, 0 from `keep` on.  n_first + n_last <= keep <= n_blocks.  table_out must not be
+ * cache->table, nor mass_out be mass_in. */
+mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep, int n_first,
+                       int n_last, const float* mass_in, int32_t* table_out, float* mass_out);
+
+/* Bytes of workspace that mj_kv8_select and mj_kv8_attn with these sizes (ring_rows = L - start + M;
+ * n_sel 0: every block; mass: mass_out given) take at most; 0 where an argument is out of range. */
+size_t mj_kv8_workspace(int n_heads, int n_kv_heads, int M, int n_blocks, int n_sel,
+                        int64_t ring_rows, int mass);
+
+/* mj_attn_block over this cache (full attention: cfg->window must be 0): h += o_proj(attn(rms(h))),
+ * the pass's keys appended to the ring at L + r; start, n_blocks, mass_in and mass_out as in
+ * mj_kv8_attn; n_sel > 0: every row reads the blocks that mj_kv8_select with n_sel, n_first and
+ * n_last chooses (no mass then).  cfg->kv_capacity is not read (the ring's counts).  Scratch is the
+ * context's: refused while the stream is being captured. */
+mj_status mj_attn_block_kv8(mj_ctx* ctx, const mj_attn_config* cfg, const mj_attn_weights* w,
+                            const mj_kv8* cache, const mj_kv_ring* ring, void* h, int n_blocks,
+                            int n_sel, int n_first, int n_last, int64_t start, int64_t L,
+                            const int32_t* parents_host, int M, const float* mass_in,
+                            float* mass_out);
+
 /* lm_head verify -- encodeMetalHead -> maple_lm_head_argmax/reduce
  * (SeedlessDecodeEngine.swift:481-498, SeedlessMetal.swift:3005-3111) for an fp16 head:
  * logits[m][v] = sum_k w[v][k] * x[m][k] (fp32), argmax per row with the lowest id winning

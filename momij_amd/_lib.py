@@ -98,6 +98,19 @@ def sampling(temperature, top_p=1.0, rep=1.0, pres=0.0, freq=0.0, hist=None):
     return sp, (ht, hc)
 
 
+MJ_KV8_BLOCK = 64
+
+
+class Kv8(C.Structure):
+    _fields_ = [("n_kv_heads", i32), ("n_pages", i32), ("k_codes", vp), ("v_codes", vp),
+                ("k_scale", vp), ("v_scale", vp), ("k_bounds", vp), ("table", vp),
+                ("table_stride", i32)]
+
+
+class KvRingStruct(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("capacity", i64)]
+
+
 class Capture(C.Structure):
     _fields_ = [("h", vp), ("inds", vp), ("logits", vp), ("attn_out", vp), ("moe_in", vp),
                 ("router_logits", vp), ("head_in", vp), ("kv_rows", vp)]
@@ -144,6 +157,19 @@ _SIGS = {
     "mj_recycle_index_observe": (i32, [vp, i32, vp, i32]),
     "mj_recycle_index_draft": (i32, [vp, i32, i32, vp, vp]),
     "mj_recycle_index_entries": (i32, [vp]),
+    "mj_qkv_append": (i32, [vp, C.POINTER(AttnConfig), vp, i64, vp, vp, C.POINTER(KvRingStruct), i64,
+                            vp, i32, vp]),
+    "mj_kv8_seal": (i32, [vp, C.POINTER(Kv8), C.POINTER(KvRingStruct), i64, i32, i32]),
+    "mj_kv8_unseal": (i32, [vp, C.POINTER(Kv8), i32, i32, C.POINTER(KvRingStruct), i64]),
+    "mj_kv8_select": (i32, [vp, C.POINTER(Kv8), i32, vp, i64, i32, i32, i32, i32, i32, vp, vp,
+                            C.c_size_t]),
+    "mj_kv8_attn": (i32, [vp, C.POINTER(Kv8), C.POINTER(KvRingStruct), i32, vp, i64, i32, i32, vp,
+                          i32, i64, i64, vp, vp, i64, vp, vp, vp, C.c_size_t]),
+    "mj_kv8_evict": (i32, [vp, C.POINTER(Kv8), i32, i32, i32, i32, vp, vp, vp]),
+    "mj_kv8_workspace": (C.c_size_t, [i32, i32, i32, i32, i32, i64, i32]),
+    "mj_attn_block_kv8": (i32, [vp, C.POINTER(AttnConfig), C.POINTER(AttnWeights), C.POINTER(Kv8),
+                                C.POINTER(KvRingStruct), vp, i32, i32, i32, i32, i64, i64, vp, i32,
+                                vp, vp]),
     "mj_accept_greedy": (i32, [vp, vp, vp, vp, i32, vp]),
     "mj_accept_sampled": (i32, [vp, vp, i32, i32, vp, f32, i32, vp, u64, u64, vp]),
     "mj_accept_sampled_ex": (i32, [vp, vp, i32, i32, vp, C.POINTER(Sampling), i32, vp, u64, u64,

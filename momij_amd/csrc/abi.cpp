@@ -82,6 +82,17 @@ mj_status mj_scratch_reserve(mj_ctx* ctx, size_t bytes) {
     return MJ_OK;
 }
 
+// Calls whose host arrays go with the launch are refused while their stream is captured, as when they
+// were uploaded and waited for: a replay would run on those of the captured call (and an attention
+// block's on scratch that a larger call may have replaced).
+mj_status mj_refuse_capture(mj_ctx* ctx, const char* what) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    mj_status s = mj_hip(ctx, hipStreamIsCapturing(ctx->stream, &cs), what);
+    if (s == MJ_OK && cs != hipStreamCaptureStatusNone)
+        s = mj_fail(ctx, MJ_HIP_ERROR, "%s cannot be captured", what);
+    return s;
+}
+
 void* Arena::take(size_t bytes) {
     off = (off + 255) & ~(size_t)255;
     void* p = base ? (char*)base + off : nullptr;

@@ -97,6 +97,10 @@ struct Prof {
 mj_status mj_fail(mj_ctx* ctx, mj_status st, const char* fmt, ...);
 mj_status mj_hip(mj_ctx* ctx, hipError_t e, const char* what);
 mj_status mj_scratch_reserve(mj_ctx* ctx, size_t bytes);
+// MJ_HIP_ERROR while the context's stream is being captured.
+mj_status mj_refuse_capture(mj_ctx* ctx, const char* what);
+// Parents (NULL: a chain), depths and ancestor masks of a pass's M rows, checked.
+mj_status fill_tree(mj_ctx* ctx, StepDesc* sd, const int32_t* parents, int M);
 // The abort word around one synchronising call: begin at its entry (MJ_ABORTED, and nothing
 // queued, if the word is set; *gen receives the generation), end after its wait.
 mj_status mj_abort_begin(mj_ctx* ctx, unsigned* gen);

@@ -93,7 +93,7 @@ static mj_status model_fail(mj_model* m, mj_status s, const char* what) {
 }
 
 // Depth and ancestor masks of a pass; parents == nullptr means a chain.
-static mj_status fill_tree(mj_ctx* ctx, StepDesc* sd, const int32_t* parents, int M) {
+mj_status fill_tree(mj_ctx* ctx, StepDesc* sd, const int32_t* parents, int M) {
     sd->chain = 1;
     for (int r = 0; r < M; ++r) {
         const int p = parents ? parents[r] : r - 1;
@@ -931,17 +931,6 @@ mj_status mj_verify_sampled(mj_model* m, int32_t y, const int32_t* draft, int n_
 }
 
 // ------------------------------------------------------------------ op-level entries
-// Calls whose host arrays go with the launch are refused while their stream is captured, as when they
-// were uploaded and waited for: a replay would run on those of the captured call (and an attention
-// block's on scratch that a larger call may have replaced).
-static mj_status mj_refuse_capture(mj_ctx* ctx, const char* what) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    mj_status s = mj_hip(ctx, hipStreamIsCapturing(ctx->stream, &cs), what);
-    if (s == MJ_OK && cs != hipStreamCaptureStatusNone)
-        s = mj_fail(ctx, MJ_HIP_ERROR, "%s cannot be captured", what);
-    return s;
-}
-
 mj_status mj_attn_block(mj_ctx* ctx, const mj_attn_config* cfg, const mj_attn_weights* w,
                         void* h, void* kcache, void* vcache, int64_t L,
                         const int32_t* parents_host, int M) {

@@ -1,0 +1,74 @@
+"""The KV cache in 8 bits as its callers hold it: KvRing (fp16 rows, position p at slot p %
+capacity) and Kv8Cache (a pool of pages and each head's list of them), over the mj_kv8_* calls of
+Context.
+
+A layer's context in use:
+
+    cache, ring = Kv8Cache(ctx, n_kv_heads, blocks), KvRing(k, v)
+    ctx.qkv_append(cfg, qkv, q_norm_w, k_norm_w, ring, L, parents, M, q)   # a pass's rows
+    ctx.kv8_attn(cache, ring, q, M, n_heads, n, start, L, parents, out)    # n blocks, then [start, L)
+    # 64 committed positions more than the ring should hold: one more block
+    ctx.kv8_seal(cache, ring, start, 1, n); n, start = n + 1, start + 64
+    # a long context in part: blocks chosen for every row
+    ctx.kv8_select(cache, q, M, n_heads, n, n_sel, 1, 2, sel)
+    ctx.kv8_attn(cache, ring, q, M, n_heads, n, start, L, parents, out, sel=sel)
+    # a bounded cache: the blocks that got the least attention go, their pages are used again
+    ctx.kv8_attn(..., mass_in=cache.mass, mass_out=cache.mass)
+    cache.evict(n, keep, n_first=1, n_last=4); n = keep
+"""
+from __future__ import annotations
+
+from . import _lib
+from .ops import ptr
+
+
+class KvRing:
+    """K and V rows fp16 [n_kv_heads][capacity][128]: torch tensors, or device addresses (those of
+    VerifyEngine.kv) with the capacity given."""
+
+    def __init__(self, k, v, capacity: int | None = None):
+        self.k, self.v = k, v
+        if capacity is None:
+            if k.shape != v.shape or k.dim() != 3 or k.shape[2] != 128 or not (
+                    k.is_contiguous() and v.is_contiguous()):
+                raise ValueError("ring tensors: two contiguous [n_kv_heads][capacity][128]")
+            capacity = k.shape[1]
+        self.capacity = int(capacity)
+        addr = [t if isinstance(t, int) else ptr(t) for t in (k, v)]
+        self.struct = _lib.KvRingStruct(addr[0], addr[1], self.capacity)
+
+
+class Kv8Cache:
+    """A pool for `blocks` blocks of each head, head g's pages g * blocks .. at first; `mass`
+    [n_kv_heads][blocks] holds the blocks' accumulated attention weight."""
+
+    def __init__(self, ctx, n_kv_heads: int, blocks: int, device: str = "cuda"):
+        import torch
+
+        self.ctx, self.n_kv_heads, self.blocks = ctx, n_kv_heads, blocks
+        pages = n_kv_heads * blocks
+
+        def zeros(shape, dtype):
+            return torch.zeros(shape, dtype=dtype, device=device)
+
+        self.k_codes, self.v_codes = (zeros((pages, 8192), torch.uint8) for _ in range(2))
+        self.k_scale, self.v_scale = (zeros(pages, torch.float32) for _ in range(2))
+        self.k_bounds = zeros((pages, 2, 128), torch.int8)
+        self.table = torch.arange(pages, dtype=torch.int32, device=device).reshape(n_kv_heads, blocks)
+        self.mass = zeros((n_kv_heads, blocks), torch.float32)
+        self._spare = torch.empty_like(self.table), torch.empty_like(self.mass)
+        self._bind()
+
+    def _bind(self):
+        self.struct = _lib.Kv8(self.n_kv_heads, self.n_kv_heads * self.blocks, ptr(self.k_codes),
+                               ptr(self.v_codes), ptr(self.k_scale), ptr(self.v_scale),
+                               ptr(self.k_bounds), ptr(self.table), self.blocks)
+
+    def evict(self, n_blocks: int, keep: int, n_first: int = 1, n_last: int = 1):
+        """Down to `keep` blocks a head by `mass`; table and mass change places with their spares
+        (a captured graph keeps the ones it was captured with)."""
+        table, mass = self._spare
+        self.ctx.kv8_evict(self, n_blocks, keep, n_first, n_last, self.mass, table, mass)
+        self._spare = self.table, self.mass
+        self.table, self.mass = table, mass
+        self._bind()

@@ -107,6 +107,70 @@ class Context:
         self.check(self.lib.mj_attn_block(self.h, C.byref(c), C.byref(w), ptr(h), ptr(kcache),
                                           ptr(vcache), L, par, M))
 
+    # ------------------------------------------------- a KV cache in 8 bits (kv8.py)
+    @staticmethod
+    def _parents(parents, M: int):
+        if parents is None:
+            return None
+        if len(parents) != M:
+            raise ValueError(f"{len(parents)} parents of {M} rows")
+        return (C.c_int32 * M)(*[int(p) for p in parents])
+
+    def qkv_append(self, cfg: dict, qkv, q_norm_w, k_norm_w, ring, L: int, parents, M: int, q_out):
+        """Queries and keys normed and rotated, keys and values appended to the ring; qkv rows may
+        be a slice of wider ones."""
+        c = self.attn_config(cfg)
+        ld = qkv.stride(0) if M > 1 else 0
+        self.check(self.lib.mj_qkv_append(self.h, C.byref(c), ptr(qkv), ld, ptr(q_norm_w),
+                                          ptr(k_norm_w), C.byref(ring.struct), L,
+                                          self._parents(parents, M), M, ptr(q_out)))
+
+    def kv8_seal(self, cache, ring, pos: int, count: int, at: int):
+        self.check(self.lib.mj_kv8_seal(self.h, C.byref(cache.struct), C.byref(ring.struct), pos,
+                                        count, at))
+
+    def kv8_unseal(self, cache, at: int, count: int, ring, pos: int):
+        self.check(self.lib.mj_kv8_unseal(self.h, C.byref(cache.struct), at, count,
+                                          C.byref(ring.struct), pos))
+
+    def kv8_select(self, cache, q, M: int, n_heads: int, n_blocks: int, n_sel: int, n_first: int,
+                   n_last: int, sel, ws=None):
+        self.check(self.lib.mj_kv8_select(self.h, C.byref(cache.struct), n_heads, ptr(q),
+                                          q.stride(0) if M > 1 else 0, M, n_blocks, n_sel, n_first,
+                                          n_last, ptr(sel), ptr(ws),
+                                          0 if ws is None else ws.numel() * ws.element_size()))
+
+    def kv8_attn(self, cache, ring, q, M: int, n_heads: int, n_blocks: int, start: int, L: int,
+                 parents, out, sel=None, mass_in=None, mass_out=None, ws=None):
+        """sel int32 [M][n_kv_heads][n_sel] (kv8_select's) or None: every block."""
+        self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.struct), C.byref(ring.struct), n_heads,
+                                        ptr(q), q.stride(0) if M > 1 else 0, M, n_blocks, ptr(sel),
+                                        0 if sel is None else sel.shape[-1], start, L,
+                                        self._parents(parents, M), ptr(out),
+                                        out.stride(0) if M > 1 else 0, ptr(mass_in), ptr(mass_out),
+                                        ptr(ws), 0 if ws is None else ws.numel() * ws.element_size()))
+
+    def kv8_evict(self, cache, n_blocks: int, keep: int, n_first: int, n_last: int, mass_in,
+                  table_out, mass_out):
+        self.check(self.lib.mj_kv8_evict(self.h, C.byref(cache.struct), n_blocks, keep, n_first,
+                                         n_last, ptr(mass_in), ptr(table_out), ptr(mass_out)))
+
+    def kv8_workspace(self, n_heads: int, n_kv_heads: int, M: int, n_blocks: int, n_sel: int,
+                      ring_rows: int, mass: bool = False) -> int:
+        return int(self.lib.mj_kv8_workspace(n_heads, n_kv_heads, M, n_blocks, n_sel, ring_rows,
+                                             int(mass)))
+
+    def attn_block_kv8(self, cfg: dict, aw: dict, cache, ring, h, n_blocks: int, start: int, L: int,
+                       parents, M: int, n_sel: int = 0, n_first: int = 0, n_last: int = 0,
+                       mass_in=None, mass_out=None):
+        c = self.attn_config(cfg)
+        w = self.attn_struct(aw)
+        self.check(self.lib.mj_attn_block_kv8(self.h, C.byref(c), C.byref(w),
+                                              C.byref(cache.struct), C.byref(ring.struct), ptr(h),
+                                              n_blocks, n_sel, n_first, n_last, start, L,
+                                              self._parents(parents, M), M, ptr(mass_in),
+                                              ptr(mass_out)))
+
     def lm_head_verify(self, x, w, M, K, V, out_argmax, out_max=None, out_logits=None,
                        banned=None, n_banned=0, temperature=1.0, out_lse=None):
         self.check(self.lib.mj_lm_head_verify(self.h, ptr(x), ptr(w), M, K, V, ptr(banned),
