@@ -66,77 +66,66 @@ __device__ __forceinline__ int unit_page(const Kv8AttnArgs& a, int g, int row, i
 struct Tile {
     float m, l;
     f4 o[8];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
 };
 
-// One unit's scores of a tile: D lane (ln, lq) of K Q^T = vector ln against tokens 16 kt + 4 lq + r.
-// K operand s holds dims 64 (s / 2) + 16 lq + 8 (s % 2) + 0 .. 7, as Q's does.
-template <bool RING>
-__device__ __forceinline__ void tile_unit(Tile& T, const u4v q[4], const u4v* Kf, const u4v* Vf,
-                                          int lane, float ksc, float vsc, uint64_t committed,
-                                          uint64_t own, float2* rec) {
-    const int ln = lane & 15, lq = lane >> 4;
-    f4 S[4];
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+// Softmax of one unit's scores against the running state.  S: lane (ln, lq) holds vector ln against
+// tokens 16 kt + 4 lq + r, without the scale ksc >= 0; masked ones -inf.  Returns the weights rounded
+// to fp16, as the two A operands of the product with V (their k slot 8 lq + u is token 32 j + 4 lq +
+// u, then 32 j + 16 + 4 lq + u - 4): a weight carries half a step, 2^-11, into the output's mean,
+// and the sum that divides it adds up the same rounded weights.  lu: the unit's sum, this lane's
+// share.  The state's outputs are rescaled where some vector's maximum moved.
+__device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], float ksc, u4v pa[2], float& lu) {
+    const int lq = (threadIdx.x & 63) >> 4;
+    float m = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-        S[kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            S[kt] = mfma16x16x32(as_h8(Kf[(4 * kt + s) * 64 + lane]), as_h8(q[s]), S[kt]);
+        m = fmaxf(fmaxf(m, S[kt][0]), S[kt][1]);
+        m = fmaxf(fmaxf(m, S[kt][2]), S[kt][3]);
     }
-    float m = -INFINITY;
-    const uint64_t ok = committed | own;
+    m = fmaxf(T.m, x4_max(m) * ksc);
+    // nothing seen yet: any finite reference (a masked score still gives 0, a NaN stays one)
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const bool moved = T.m != m;
+    const float alpha = __builtin_amdgcn_exp2f(T.m - ref);
+    T.m = m;
+    lu = 0.0f;
+    const h2v one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float s = S[kt][r] * ksc;
-            if (RING) s = (ok >> (16 * kt + 4 * lq + r)) & 1 ? s : -INFINITY;
-            S[kt][r] = s;
-            m = fmaxf(m, s);
+        for (int h = 0; h < 2; ++h) {
+            const f2v p = {__builtin_amdgcn_exp2f(fmaf(S[kt][2 * h], ksc, -ref)),
+                           __builtin_amdgcn_exp2f(fmaf(S[kt][2 * h + 1], ksc, -ref))};
+            const h2v ph = __builtin_convertvector(p, h2v);
+            lu = __builtin_amdgcn_fdot2(ph, one, lu, false);
+            pa[kt >> 1][2 * (kt & 1) + h] = __builtin_bit_cast(uint32_t, ph);
         }
-    m = fmaxf(T.m, x4_max(m));
-    // nothing seen yet: any finite reference (a masked score still gives 0, a NaN stays one)
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const float alpha = __builtin_amdgcn_exp2f(T.m - ref);
-    T.m = m;
-    float l = 0.0f;
-    u4v pa[2];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        float p[4];
+    if (__any(moved)) {
+        T.l *= alpha;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(S[kt][r] - ref);
-            l += p[r];
+            const float al = __shfl(alpha, 4 * lq + r, MJ_WAVE);
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) T.o[dt][r] *= al;
         }
-        pa[kt >> 1][2 * (kt & 1)] = pack2(f2h(p[0]), f2h(p[1]));
-        pa[kt >> 1][2 * (kt & 1) + 1] = pack2(f2h(p[2]), f2h(p[3]));
     }
-    T.l = fmaf(T.l, alpha, l);
-    if (rec) {
-        const float lu = x4_sum(l);
-        if (lq == 0) rec[ln] = make_float2(m, lu);
-    }
-    float al[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) al[r] = __shfl(alpha, 4 * lq + r, MJ_WAVE);
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-        f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            o = mfma16x16x32(as_h8(pa[j]), as_h8(Vf[(2 * dt + j) * 64 + lane]), o);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) T.o[dt][r] = fmaf(o[r], vsc, T.o[dt][r] * al[r]);
-    }
+    T.l += lu;
 }
 
 // Infinities and NaN among the V rows of the pass (a tree row's siblings must not see them: 0 times
 // an infinity is a NaN) are left out of the products (staged as 0) and added here, for the rows that
-// do attend to them; bad: the ring rows that hold any.
-__device__ __forceinline__ void add_bad_rows(Tile& T, const u4v q[4], const u4v* Kf, int lane, float ksc,
-                                          uint64_t ok, uint64_t bad, const uint16_t* vrow0,
-                                          int slot0, int C) {
+// do attend to them; bad: the ring rows that hold any, ok: those that vector ln attends.
+__device__ __forceinline__ void add_bad_rows(Tile& T, const u4v q[4], const u4v* Kf, int lane,
+                                             float ksc, uint64_t ok, uint64_t bad,
+                                             const uint16_t* vrow0, int slot0, int C) {
     const int ln = lane & 15, lq = lane >> 4;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
@@ -150,7 +139,7 @@ __device__ __forceinline__ void add_bad_rows(Tile& T, const u4v q[4], const u4v*
         for (int r = 0; r < 4; ++r) {
             const int key = 16 * kt + 4 * lq + r;
             // -1: not attended
-            const float p = (ok >> key) & 1 ? __builtin_amdgcn_exp2f(S[r] * ksc - ref) : -1.0f;
+            const float p = (ok >> key) & 1 ? __builtin_amdgcn_exp2f(fmaf(S[r], ksc, -ref)) : -1.0f;
             for (int kq = 0; kq < 4; ++kq) {
                 const int k = 16 * kt + 4 * kq + r;
                 if (!((bad >> k) & 1)) continue;  // uniform
@@ -181,197 +170,513 @@ __device__ __forceinline__ u4v finite8(u4v v, bool& bad) {
     return v;
 }
 
-// A 256-thread block takes part blockIdx.x of KV head blockIdx.z for 4 T tiles of query vectors
-// (vector r * G + j: head j of the group, row r; where rows list their own blocks, the vectors of row
-// blockIdx.y), T a wave.  Units are staged in LDS as the halves the matrix instructions take: K
-// operand (kt, s) and V operand (dt, j), 1 KB each, a lane's 16 bytes at 16 * lane.
-template <int T>
-__global__ __launch_bounds__(256) void k_kv8_attn(Kv8AttnArgs a) {
-    __shared__ __align__(16) u4v Kf[16 * 64];
-    __shared__ __align__(16) u4v Vf[16 * 64];
+// Query vectors tv + ln of KV head g (vector r * G + j: head j of the group, row r) as the B operand:
+// operand s holds dims 64 (s / 2) + 16 lq + 8 (s % 2) + 0 .. 7, as the K operands do.
+__device__ __forceinline__ void load_q(const Kv8AttnArgs& a, int g, int v, bool on, u4v q[4],
+                                       uint64_t& anc) {
+    const int lq = (threadIdx.x & 63) >> 4;
+    const int r = on ? v / a.G : 0, h = on ? g * a.G + v - r * a.G : 0;
+    const uint16_t* qp = a.q + (size_t)r * a.ldq + (size_t)h * HD;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        q[s] = *(const u4v*)(qp + 64 * (s >> 1) + 16 * lq + 8 * (s & 1));
+        if (!on) q[s] = (u4v){0u, 0u, 0u, 0u};
+    }
+    anc = on ? a.anc[r] : 0;
+}
+
+// 64 rows of the ring, base .. base + 63 of the call's open rows, as the operands of a unit in LDS: K
+// operand (kt, s) and V operand (dt, j), 1 KB each, a lane's 16 bytes at 16 * lane.  V is turned four
+// tokens by eight dims at a time.  Rows past the last are zeros; bad: the rows with an infinity or
+// NaN in V (set here, cleared before).
+template <int NT>
+__device__ __forceinline__ void stage_ring(const Kv8AttnArgs& a, int g, int base, u4v* Kf, u4v* Vf,
+                                           uint32_t* bad) {
+    const int t = threadIdx.x, rows = a.R + a.M, C = (int)a.ring.C;
+    auto slot = [&](int k) {  // of row `base + k`, a row past the last taken as the last
+        int s = a.slot0 + min(base + k, rows - 1);
+        s -= s >= C ? C : 0;
+        return ((size_t)g * C + s) * HD;
+    };
+    constexpr int NK = 1024 / NT, NV = 256 / NT > 0 ? 256 / NT : 1;
+    u4v kr[NK], vr[NV][4];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        const int c = t + NT * i;
+        kr[i] = *(const u4v*)(a.ring.k + slot(c >> 4) + 8 * (c & 15));
+    }
+    const bool vt = NT <= 256 || t < 256;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = (t + NT * n) & 255;
+            vr[n][i] = *(const u4v*)(a.ring.v + slot(4 * (c & 15) + i) + 8 * (c >> 4));
+        }
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+        const int c = t + NT * i, k = c >> 4, dg = c & 15;
+        Kf[(4 * (k >> 4) + 2 * (dg >> 3) + (dg & 1)) * 64 + 16 * ((dg >> 1) & 3) + (k & 15)] =
+            base + k < rows ? kr[i] : (u4v){0u, 0u, 0u, 0u};
+    }
+    if (!vt) return;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int c = t + NT * n, kg = c & 15, vd = c >> 4, aa = kg >> 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (base + 4 * kg + i >= rows) vr[n][i] = (u4v){0u, 0u, 0u, 0u};
+            bool b = false;
+            vr[n][i] = finite8(vr[n][i], b);
+            if (b) atomicOr(&bad[kg >> 3], 1u << ((4 * kg + i) & 31));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int sh = 16 * (e & 1), d = 8 * vd + e;
+            const uint32_t x = pack2(vr[n][0][e >> 1] >> sh, vr[n][1][e >> 1] >> sh);
+            const uint32_t y = pack2(vr[n][2][e >> 1] >> sh, vr[n][3][e >> 1] >> sh);
+            uint2* p = (uint2*)&Vf[(2 * (d >> 4) + (aa >> 1)) * 64 + 16 * (kg & 3) + (d & 15)];
+            p[aa & 1] = make_uint2(x, y);
+        }
+    }
+}
+
+// The rows of a ring unit that a vector with ancestor mask anc attends.
+__device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, uint64_t anc, bool on) {
+    uint64_t committed = 0;
+    if (a.R > base) committed = a.R - base >= 64 ? ~0ull : (1ull << (a.R - base)) - 1;
+    const int d0 = base - a.R;  // own row of the unit's first token
+    const uint64_t own = d0 >= 64 ? 0 : d0 >= 0 ? anc >> d0 : d0 > -64 ? anc << -d0 : 0;
+    return on ? committed | own : 0;
+}
+
+// T tiles against one unit staged in LDS; each operand is read once for all of them.
+template <int T, bool RING>
+__device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u4v* Kf, const u4v* Vf,
+                                            int lane, float ksc, float vsc, const uint64_t* ok,
+                                            float2* const* rec) {
+    const int ln = lane & 15, lq = lane >> 4;
+    f4 S[T][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int i = 0; i < T; ++i) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const h8 k = as_h8(Kf[(4 * kt + s) * 64 + lane]);
+#pragma unroll
+            for (int i = 0; i < T; ++i) S[i][kt] = mfma16x16x32(k, as_h8(q[i][s]), S[i][kt]);
+        }
+    }
+    u4v pa[T][2];
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        if constexpr (RING)
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    S[i][kt][r] = (ok[i] >> (16 * kt + 4 * lq + r)) & 1 ? S[i][kt][r] : -INFINITY;
+        float lu;
+        softmax_unit(tl[i], S[i], ksc, pa[i], lu);
+        if (!RING && rec && rec[i]) {
+            lu = x4_sum(lu);
+            if (lq == 0) *rec[i] = make_float2(tl[i].m, lu);
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+        const h8 v0 = as_h8(Vf[(2 * dt) * 64 + lane]), v1 = as_h8(Vf[(2 * dt + 1) * 64 + lane]);
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            o = mfma16x16x32(as_h8(pa[i][0]), v0, o);
+            o = mfma16x16x32(as_h8(pa[i][1]), v1, o);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tl[i].o[dt][r] = fmaf(o[r], vsc, tl[i].o[dt][r]);
+        }
+    }
+}
+
+__device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g, int tv, int vend,
+                                           const Tile& T) {
+    const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4, nv = a.M * a.G;
+    const float l = x4_sum(T.l);
+    const size_t pb = ((size_t)part * a.p.nKV + g) * nv + tv;
+    if (lq == 0 && tv + ln < vend) a.ml[pb + ln] = make_float2(T.m, l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (tv + 4 * lq + r < vend) {
+            float* op = a.opart + (pb + 4 * lq + r) * HD + ln;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) op[16 * dt] = T.o[dt][r];
+        }
+}
+
+// Many rows: a block of NW waves takes a run of units of KV head blockIdx.z for NW T tiles of query
+// vectors, T a wave.  A unit is turned to halves once, by the whole block, and read from LDS by its
+// waves; two units are in LDS and one in registers on its way, one barrier a unit.
+template <int T, int NW>
+__global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
+    constexpr int NT = 64 * NW, NR = 512 / NT;
+    extern __shared__ __align__(16) u4v lds[];  // two units: K operands, V operands
     __shared__ int s_abort;
-    __shared__ uint32_t s_bad[2][2];  // ring rows with an infinity or NaN in V, units in turn
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15, lq = lane >> 4;
+    __shared__ uint32_t s_bad[3][2];  // ring rows with an infinity or NaN in V, of unit u % 3
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15;
     const int part = blockIdx.x, g = blockIdx.z;
-    const int row_y = a.sel ? blockIdx.y : 0;
-    const int v0 = a.sel ? row_y * a.G : (int)blockIdx.y * 64 * T;    // first vector of the block
-    const int vend = a.sel ? v0 + a.G : a.M * a.G;
-    const int nv = a.M * a.G, nQ = a.p.nKV * a.G, C = (int)a.ring.C;
+    const int v0 = (int)blockIdx.y * 16 * NW * T, vend = a.M * a.G;  // the block's vectors
+    const int nv = a.M * a.G, C = (int)a.ring.C;
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_abort = ab;
-    if (t < 4) s_bad[t >> 1][t & 1] = 0;
     Tile tl[T];
     u4v q[T][4];
     uint64_t anc[T];
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int v = v0 + 16 * (wv * T + i) + ln;
-        const bool on = v < vend;
-        const int r = on ? v / a.G : 0, h = on ? g * a.G + v - r * a.G : 0;
-        const uint16_t* qp = a.q + (size_t)r * a.ldq + (size_t)h * HD;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            q[i][s] = *(const u4v*)(qp + 64 * (s >> 1) + 16 * lq + 8 * (s & 1));
-            if (!on) q[i][s] = (u4v){0u, 0u, 0u, 0u};
-        }
-        anc[i] = on ? a.anc[r] : 0;
-        tl[i].m = -INFINITY;
-        tl[i].l = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) tl[i].o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+        load_q(a, g, v, v < vend, q[i], anc[i]);
+        tl[i].clear();
     }
+    const bool idle = v0 + 16 * wv * T >= vend;  // the wave has no vector: it stages only
+    const int u0 = part * a.upp, u1 = min(u0 + a.upp, a.units);
+    const float sc2 = LOG2E * 0.08838834764831845f;  // log2 e / sqrt(128)
+    u4v kr[NR], vr[NR];
+    auto page = [&](int u) {  // of unit u, -1: none (a ring unit, or no block)
+        return u < u1 && u < a.n_list ? unit_page(a, g, 0, u) : -1;
+    };
+    auto request = [&](int pg) {
+        const u4v* kp = (const u4v*)(a.p.k + (size_t)max(pg, 0) * KV8_PAGE_BYTES);
+        const u4v* vp = (const u4v*)(a.p.v + (size_t)max(pg, 0) * KV8_PAGE_BYTES);
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+            kr[c] = kp[t + NT * c];
+            vr[c] = vp[t + NT * c];
+        }
+    };
+    auto stage = [&](int u, int pg) {
+        u4v* Kf = lds + (u & 1) * 2048;
+        u4v* Vf = Kf + 1024;
+        if (u >= a.n_list) {
+            stage_ring<NT>(a, g, 64 * (u - a.n_list), Kf, Vf, s_bad[u % 3]);
+            return;
+        }
+        if (pg < 0) return;
+#pragma unroll
+        for (int c = 0; c < NR; ++c) {
+            const int f = (t + NT * c) >> 6;
+            codes16(kr[c], Kf[(2 * f) * 64 + lane], Kf[(2 * f + 1) * 64 + lane]);
+            codes16(vr[c], Vf[(2 * f) * 64 + lane], Vf[(2 * f + 1) * 64 + lane]);
+        }
+    };
+    int pg = page(u0), pn = page(u0 + 1);
+    request(pg);
+    if (t < 6) s_bad[t >> 1][t & 1] = 0;
     __syncthreads();
     if (s_abort) return;
-    const float sc2 = LOG2E * 0.08838834764831845f;  // log2 e / sqrt(128)
-    const int u1 = min((part + 1) * a.upp, a.units);
-    for (int u = part * a.upp; u < u1; ++u) {
+    stage(u0, pg);
+    request(pn);
+    for (int u = u0; u < u1; ++u) {
+        const int p2 = page(u + 2);
+        __syncthreads();  // unit u is staged; everyone is done with unit u - 1
         const bool ringu = u >= a.n_list;
-        float ksc = sc2, vsc = 1.0f;
-        int pg = 0;
-        uint64_t committed = 0;
-        int base = 0, slot_b = 0;  // ring row of the unit's first token, its slot
-        if (!ringu) {
-            pg = unit_page(a, g, row_y, u);
-            if (pg < 0) continue;  // whole block
-            ksc = a.p.ks[pg] * sc2;
-            vsc = a.p.vs[pg];
-            const u4v* kp = (const u4v*)(a.p.k + (size_t)pg * KV8_PAGE_BYTES);
-            const u4v* vp = (const u4v*)(a.p.v + (size_t)pg * KV8_PAGE_BYTES);
-            u4v kr[2], vr[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                kr[c] = kp[t + 256 * c];
-                vr[c] = vp[t + 256 * c];
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int ch = t + 256 * c, f = ch >> 6;
-                codes16(kr[c], Kf[(2 * f) * 64 + lane], Kf[(2 * f + 1) * 64 + lane]);
-                codes16(vr[c], Vf[(2 * f) * 64 + lane], Vf[(2 * f + 1) * 64 + lane]);
-            }
-        } else {
-            base = 64 * (u - a.n_list);
-            const int rows = a.R + a.M;
-            slot_b = a.slot0 + base;
-            slot_b -= slot_b >= C ? C : 0;
-            auto slot = [&](int k) {  // of row `base + k`, a row past the last taken as the last
-                int s = a.slot0 + min(base + k, rows - 1);
-                s -= s >= C ? C : 0;
-                return ((size_t)g * C + s) * HD;
-            };
-            if (t < 2) s_bad[(u & 1) ^ 1][t] = 0;  // nobody reads or sets the other one's now
-            if (a.R > base) committed = a.R - base >= 64 ? ~0ull : (1ull << (a.R - base)) - 1;
-            u4v kr[4], vr[4];
-            const int kg = t & 15, vd = t >> 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = t + 256 * i;
-                kr[i] = *(const u4v*)(a.ring.k + slot(c >> 4) + 8 * (c & 15));
-                vr[i] = *(const u4v*)(a.ring.v + slot(4 * kg + i) + 8 * vd);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = t + 256 * i, k = c >> 4, dg = c & 15;
-                const bool on = base + k < rows;
-                Kf[(4 * (k >> 4) + 2 * (dg >> 3) + (dg & 1)) * 64 + 16 * ((dg >> 1) & 3) + (k & 15)] =
-                    on ? kr[i] : (u4v){0u, 0u, 0u, 0u};
-                if (base + 4 * kg + i >= rows) vr[i] = (u4v){0u, 0u, 0u, 0u};
-                bool bad = false;
-                vr[i] = finite8(vr[i], bad);
-                if (bad) atomicOr(&s_bad[u & 1][kg >> 3], 1u << ((4 * kg + i) & 31));
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int sh = 16 * (e & 1);
-                const uint32_t x = pack2(vr[0][e >> 1] >> sh, vr[1][e >> 1] >> sh);
-                const uint32_t y = pack2(vr[2][e >> 1] >> sh, vr[3][e >> 1] >> sh);
-                const int d = 8 * vd + e, aa = kg >> 2;
-                uint2* p = (uint2*)&Vf[(2 * (d >> 4) + (aa >> 1)) * 64 + 16 * (kg & 3) + (d & 15)];
-                p[aa & 1] = make_uint2(x, y);
-            }
+        uint64_t bad = 0;
+        if (ringu) bad = s_bad[u % 3][0] | ((uint64_t)s_bad[u % 3][1] << 32);
+        if (t < 2) s_bad[(u + 2) % 3][t] = 0;  // read before this barrier, set after the next
+        const float ks = pg >= 0 ? a.p.ks[pg] : 1.0f, vs = pg >= 0 ? a.p.vs[pg] : 1.0f;
+        if (u + 1 < u1) {
+            stage(u + 1, pn);
+            request(p2);
         }
-        __syncthreads();
+        const u4v* Kf = lds + (u & 1) * 2048;
+        const u4v* Vf = Kf + 1024;
+        if (!idle && ringu) {
+            const int base = 64 * (u - a.n_list);
+            uint64_t ok[T];
 #pragma unroll
-        for (int i = 0; i < T; ++i) {
-            const int tv = v0 + 16 * (wv * T + i);
-            if (tv >= vend) continue;  // uniform
-            if (!ringu) {
-                float2* rec = a.rec ? a.rec + ((size_t)g * a.n + u) * nv + tv : nullptr;
-                if (rec && tv + ln >= vend) rec = a.rec + (size_t)a.p.nKV * a.n * nv;  // (spare row)
-                tile_unit<false>(tl[i], q[i], Kf, Vf, lane, ksc, vsc, 0, 0, rec);
-            } else {
-                const int d0 = base - a.R;  // own row of the unit's first token
-                const uint64_t own = d0 >= 64 ? 0 : d0 >= 0 ? anc[i] >> d0 : d0 > -64 ? anc[i] << -d0 : 0;
-                const bool on = tv + ln < vend;
-                const uint64_t ok = on ? committed | own : 0;
-                tile_unit<true>(tl[i], q[i], Kf, Vf, lane, ksc, vsc, ok, 0, nullptr);
-                const uint64_t bad = s_bad[u & 1][0] | ((uint64_t)s_bad[u & 1][1] << 32);
-                if (bad)
-                    add_bad_rows(tl[i], q[i], Kf, lane, ksc, ok, bad,
-                                 a.ring.v + (size_t)g * C * HD, slot_b, C);
+            for (int i = 0; i < T; ++i)
+                ok[i] = ring_mask(a, base, anc[i], v0 + 16 * (wv * T + i) + ln < vend);
+            staged_unit<T, true>(tl, q, Kf, Vf, lane, sc2, 1.0f, ok, nullptr);
+            if (bad) {
+                int sb = a.slot0 + base;
+                sb -= sb >= C ? C : 0;
+#pragma unroll
+                for (int i = 0; i < T; ++i)
+                    add_bad_rows(tl[i], q[i], Kf, lane, sc2, ok[i], bad,
+                                 a.ring.v + (size_t)g * C * HD, sb, C);
             }
+        } else if (!idle && pg >= 0) {
+            float2* rec[T];
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                const int v = v0 + 16 * (wv * T + i) + ln;
+                rec[i] = !a.rec ? nullptr
+                         : v < vend ? a.rec + ((size_t)g * a.n + u) * nv + v
+                                    : a.rec + (size_t)a.p.nKV * a.n * nv + ln;  // a spare row
+            }
+            staged_unit<T, false>(tl, q, Kf, Vf, lane, ks * sc2, vs, nullptr, rec);
         }
-        __syncthreads();
+        pg = pn;
+        pn = p2;
     }
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int tv = v0 + 16 * (wv * T + i);
-        if (tv >= vend) continue;
-        const float l = x4_sum(tl[i].l);
-        const size_t pb = ((size_t)part * a.p.nKV + g) * nv + tv;
-        if (lq == 0 && tv + ln < vend) a.ml[pb + ln] = make_float2(tl[i].m, l);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (tv + 4 * lq + r < vend) {
-                float* op = a.opart + (pb + 4 * lq + r) * HD + ln;
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) op[16 * dt] = tl[i].o[dt][r];
-            }
+        if (tv < vend) write_part(a, part, g, tv, vend, tl[i]);
     }
 }
 
-// One 256-thread block a row and head: wave w takes parts w, w + 4, .. in turn (lane = two dims), the
-// four sums are added in wave order.  A part that saw no key has maximum -inf and weight 0.
+// Few rows: T tiles of query vectors, and every wave takes pages of its own, straight into registers:
+// a page's bytes lie in the order of the operands, so a lane's 16 bytes are two of them.  A wave's
+// next K goes out behind its scores, its next V behind its output product; the page numbers and
+// scales of 64 pages come with one request a lane each.  The block's NW waves are joined in LDS.
+// Blocks past the pages' parts take one ring unit each, all waves staging it.  Where rows list their
+// own blocks (a.sel), blockIdx.y is a row and a share of its heads.
+template <int T, int NW>
+__global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
+    constexpr int NT = 64 * NW, RS = HD + 4;
+    extern __shared__ __align__(16) u4v lds[];
+    __shared__ int s_abort;
+    __shared__ uint32_t s_bad[2];
+    __shared__ float s_m[NW][16], s_l[NW][16];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15, lq = lane >> 4;
+    const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
+    int row = 0, v0 = (int)blockIdx.y * 16 * T, vend = nv;
+    if (a.sel) {
+        const int cols = (a.G + 16 * T - 1) / (16 * T);
+        row = blockIdx.y / cols;
+        v0 = row * a.G + 16 * T * (blockIdx.y % cols);
+        vend = row * a.G + a.G;
+    }
+    const int ab = a.abort ? *a.abort : 0;
+    if (t == 0) s_abort = ab;
+    const float sc2 = LOG2E * 0.08838834764831845f;  // log2 e / sqrt(128)
+    if (part >= a.page_parts) {
+        // ---- one ring unit, a tile a wave
+        if (t < 2) s_bad[t] = 0;
+        __syncthreads();
+        if (s_abort) return;
+        const int base = 64 * (part - a.page_parts), C = (int)a.ring.C;
+        u4v* Kf = lds;
+        u4v* Vf = Kf + 1024;
+        stage_ring<NT>(a, g, base, Kf, Vf, s_bad);
+        const int tv = v0 + 16 * wv;
+        u4v q[1][4];
+        uint64_t anc;
+        load_q(a, g, tv + ln, tv + ln < vend, q[0], anc);
+        __syncthreads();
+        if (wv >= T || tv >= vend) return;
+        Tile tl[1];
+        tl[0].clear();
+        const uint64_t ok = ring_mask(a, base, anc, tv + ln < vend);
+        staged_unit<1, true>(tl, q, Kf, Vf, lane, sc2, 1.0f, &ok, nullptr);
+        const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
+        if (bad) {
+            int sb = a.slot0 + base;
+            sb -= sb >= C ? C : 0;
+            add_bad_rows(tl[0], q[0], Kf, lane, sc2, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
+        }
+        write_part(a, part, g, tv, vend, tl[0]);
+        return;
+    }
+    Tile tl[T];
+    u4v q[T][4];
+    const int u0 = part * a.upp + wv, u1 = min((part + 1) * a.upp, a.n_list);
+    for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NW) {
+        const int ul = ub + NW * lane;  // lane's unit
+        const int pl = ul < u1 ? unit_page(a, g, row, ul) : -1;
+        uint64_t todo = __ballot(pl >= 0);
+        u4v kr[8], vr[8];
+        auto request_k = [&](int i) {
+            const u4v* p = (const u4v*)(a.p.k + (size_t)__builtin_amdgcn_readlane(pl, i) * KV8_PAGE_BYTES);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) kr[f] = p[64 * f + lane];
+        };
+        auto request_v = [&](int i) {
+            const u4v* p = (const u4v*)(a.p.v + (size_t)__builtin_amdgcn_readlane(pl, i) * KV8_PAGE_BYTES);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) vr[f] = p[64 * f + lane];
+        };
+        int i0 = todo ? __builtin_ctzll(todo) : -1;
+        if (i0 >= 0) {
+            request_k(i0);
+            request_v(i0);
+        }
+        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * sc2, vsl = pl >= 0 ? a.p.vs[pl] : 0.0f;
+        if (ub == u0) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                uint64_t anc;
+                load_q(a, g, v0 + 16 * i + ln, v0 + 16 * i + ln < vend, q[i], anc);
+                tl[i].clear();
+            }
+        }
+        while (todo) {
+            const int i = i0;
+            todo &= todo - 1;
+            i0 = todo ? __builtin_ctzll(todo) : i;  // the last page is requested again, unused
+            const float ksc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ksl), i));
+            const float vsc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vsl), i));
+            f4 S[T][4];
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+                for (int x = 0; x < T; ++x) S[x][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    u4v k0, k1;
+                    codes16(kr[2 * kt + j], k0, k1);
+#pragma unroll
+                    for (int x = 0; x < T; ++x) {
+                        S[x][kt] = mfma16x16x32(as_h8(k0), as_h8(q[x][2 * j]), S[x][kt]);
+                        S[x][kt] = mfma16x16x32(as_h8(k1), as_h8(q[x][2 * j + 1]), S[x][kt]);
+                    }
+                }
+            }
+            request_k(i0);
+            u4v pa[T][2];
+#pragma unroll
+            for (int x = 0; x < T; ++x) {
+                float lu;
+                softmax_unit(tl[x], S[x], ksc, pa[x], lu);
+                if (a.rec) {
+                    const int v = v0 + 16 * x + ln;
+                    lu = x4_sum(lu);
+                    if (lq == 0 && v < vend)
+                        a.rec[((size_t)g * a.n + ub + NW * i) * nv + v] = make_float2(tl[x].m, lu);
+                }
+            }
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) {
+                u4v w0, w1;
+                codes16(vr[dt], w0, w1);
+#pragma unroll
+                for (int x = 0; x < T; ++x) {
+                    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                    o = mfma16x16x32(as_h8(pa[x][0]), as_h8(w0), o);
+                    o = mfma16x16x32(as_h8(pa[x][1]), as_h8(w1), o);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) tl[x].o[dt][r] = fmaf(o[r], vsc, tl[x].o[dt][r]);
+                }
+            }
+            request_v(i0);
+        }
+    }
+    // ---- the waves joined, a tile at a time: all to the block's maximum, then summed in wave order
+    float* so = (float*)lds;  // [NW][16][RS]
+#pragma unroll
+    for (int x = 0; x < T; ++x) {
+        const int tv = v0 + 16 * x;
+        const float l = x4_sum(tl[x].l);
+        __syncthreads();
+        if (s_abort) return;
+        if (lq == 0) s_m[wv][ln] = tl[x].m;
+        __syncthreads();
+        float m = s_m[0][ln];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][ln]);
+        const float sc = __builtin_amdgcn_exp2f(tl[x].m - (m == -INFINITY ? 0.0f : m));
+        if (lq == 0) s_l[wv][ln] = l * sc;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float sr = __shfl(sc, 4 * lq + r, MJ_WAVE);
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt)
+                so[(wv * 16 + 4 * lq + r) * RS + 16 * dt + ln] = tl[x].o[dt][r] * sr;
+        }
+        __syncthreads();
+        const size_t pb = ((size_t)part * a.p.nKV + g) * nv + tv;
+        if (wv == 0 && lq == 0 && tv + ln < vend) {
+            float ls = s_l[0][ln];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) ls += s_l[w][ln];
+            a.ml[pb + ln] = make_float2(m, ls);
+        }
+        for (int e = t; e < 16 * 32; e += NT) {
+            const int vec = e >> 5, d = 4 * (e & 31);
+            if (tv + vec >= vend) continue;
+            f4 o = *(const f4*)(so + vec * RS + d);
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                const f4 y = *(const f4*)(so + (w * 16 + vec) * RS + d);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] += y[k];
+            }
+            *(f4*)(a.opart + (pb + vec) * HD + d) = o;
+        }
+    }
+}
+
+// One 256-thread block a row and head.  Eight groups of 32 lanes (a lane four dims) take every eighth
+// part, eight requested at a time, each to its own running maximum; the groups are then joined in
+// order.  A part that saw no key has maximum -inf and weight 0.
 __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
-    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    const int t = threadIdx.x, gr = t >> 5, d4 = t & 31;
     const int nQ = a.p.nKV * a.G, nv = a.M * a.G;
     const int r = blockIdx.x / nQ, h = blockIdx.x % nQ, g = h / a.G, v = r * a.G + h % a.G;
-    __shared__ float s_o[4][HD];
-    __shared__ float s_l[4];
+    __shared__ f4 s_o[8][32];
+    __shared__ float s_m[8], s_l[8];
     __shared__ int s_abort;
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_abort = ab;
     const size_t step = (size_t)a.p.nKV * nv, at = (size_t)g * nv + v;
-    float mx = -INFINITY;
-    for (int c = lane; c < a.parts; c += 64) mx = fmaxf(mx, a.ml[at + c * step].x);
-    mx = wave_max(mx);
-    const float ref = mx == -INFINITY ? 0.0f : mx;
-    float o0 = 0.0f, o1 = 0.0f, l = 0.0f;
-    for (int c = wv; c < a.parts; c += 4) {
-        const float2 ml = a.ml[at + c * step];
-        const float2 o = *(const float2*)(a.opart + (at + c * step) * HD + 2 * lane);
-        const float w = __builtin_amdgcn_exp2f(ml.x - ref);
-        l = fmaf(ml.y, w, l);
-        o0 = fmaf(o.x, w, o0);
-        o1 = fmaf(o.y, w, o1);
+    float m = -INFINITY, l = 0.0f;
+    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = gr; c0 < a.parts; c0 += 64) {
+        float2 ml[8];
+        f4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const size_t c = at + (size_t)min(c0 + 8 * j, a.parts - 1) * step;
+            ml[j] = a.ml[c];
+            x[j] = *(const f4*)(a.opart + c * HD + 4 * d4);
+        }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mn = fmaxf(mn, ml[j].x);  // (a repeated last part changes nothing)
+        const float ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (c0 + 8 * j >= a.parts) break;
+            const float w = __builtin_amdgcn_exp2f(ml[j].x - ref);
+            l = fmaf(ml[j].y, w, l);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = fmaf(x[j][k], w, o[k]);
+        }
+        m = mn;
     }
-    s_o[wv][2 * lane] = o0;
-    s_o[wv][2 * lane + 1] = o1;
-    if (lane == 0) s_l[wv] = l;
+    s_o[gr][d4] = o;
+    if (d4 == 0) {
+        s_m[gr] = m;
+        s_l[gr] = l;
+    }
     __syncthreads();
-    if (s_abort) return;
-    if (t >= 16) return;
-    l = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
+    if (s_abort || t >= 16) return;
+    float mx = s_m[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s_m[j]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float y[8] = {};
+    l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float w = __builtin_amdgcn_exp2f(s_m[j] - ref);
+        l = fmaf(s_l[j], w, l);
+        const f4 p0 = s_o[j][2 * t], p1 = s_o[j][2 * t + 1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            y[k] = fmaf(p0[k], w, y[k]);
+            y[4 + k] = fmaf(p1[k], w, y[4 + k]);
+        }
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key at all: zeros
     if (t == 0 && a.stat) a.stat[at] = make_float2(ref, inv);
     u4v ov;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int d = 8 * t + 2 * j;
-        const float x = (((s_o[0][d] + s_o[1][d]) + s_o[2][d]) + s_o[3][d]) * inv;
-        const float y = (((s_o[0][d + 1] + s_o[1][d + 1]) + s_o[2][d + 1]) + s_o[3][d + 1]) * inv;
-        ov[j] = pack2(f2h(x), f2h(y));
-    }
+    for (int j = 0; j < 4; ++j) ov[j] = pack2(f2h(y[2 * j] * inv), f2h(y[2 * j + 1] * inv));
     if (a.out) *(u4v*)(a.out + (size_t)r * a.ldo + (size_t)h * HD + 8 * t) = ov;
     if (a.out_perm) {
         const int K = nQ * HD;
@@ -397,17 +702,34 @@ __global__ __launch_bounds__(256) void k_kv8_mass(Kv8AttnArgs a) {
     if (lane == 0) a.mass_out[at] = (a.mass_in ? a.mass_in[at] : 0.0f) + s;
 }
 
+// Shapes of the two kernels: few<T, 8> for up to FEW_TILES tiles and for listed blocks, else many.
+#define FEW_WAVES 8
+#define FEW_TILES 2
+#define MANY_WAVES 8
+#define MANY_T 2
+
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.n_list = a.n_sel > 0 ? a.n_sel : a.n;
-    a.units = a.n_list + (a.R + a.M + KV8_B - 1) / KV8_B;
+    const int ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
+    a.units = a.n_list + ring_units;
     const int nv = a.M * a.G;
-    const int vb = a.n_sel > 0 ? a.G : nv;           // vectors a block column takes
-    a.tiles = (vb + 15) / 16 > 4 ? 2 : 1;  // tiles a wave
-    const int cols = a.n_sel > 0 ? a.M : (vb + 64 * a.tiles - 1) / (64 * a.tiles);
-    int parts = std::max(1, 512 / (cols * a.p.nKV));
-    parts = std::min(parts, a.units);
-    a.upp = (a.units + parts - 1) / parts;
-    a.parts = (a.units + a.upp - 1) / a.upp;
+    const int tiles = ((a.n_sel > 0 ? a.G : nv) + 15) / 16;  // that share their units
+    a.few = a.n_sel > 0 || tiles <= FEW_TILES;
+    a.tiles = a.few ? std::min(tiles, FEW_TILES) : MANY_T;  // a wave
+    const int per = a.few ? a.tiles : MANY_T * MANY_WAVES;
+    a.cols = (a.n_sel > 0 ? a.M : 1) * ((tiles + per - 1) / per);
+    // one block a CU
+    int parts = std::max(1, 256 / (a.cols * a.p.nKV));
+    if (a.few) {
+        parts = std::min(parts, (a.n_list + FEW_WAVES - 1) / FEW_WAVES);
+        a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
+        a.page_parts = parts ? (a.n_list + a.upp - 1) / a.upp : 0;
+        a.parts = a.page_parts + ring_units;
+    } else {
+        parts = std::min(parts, a.units);
+        a.upp = (a.units + parts - 1) / parts;
+        a.parts = a.page_parts = (a.units + a.upp - 1) / a.upp;
+    }
     size_t off = 0;
     auto take = [&](size_t bytes) {
         off = (off + 255) & ~(size_t)255;
@@ -423,15 +745,38 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     return off;
 }
 
+#define FEW_LDS (FEW_WAVES * 16 * (HD + 4) * 4)  // the waves' outputs side by side (a ring unit: 32 KB)
+#define MANY_LDS 65536                           // two units
+
+static hipError_t attn_attributes() {
+    static const hipError_t done = [] {
+        const int most = hipFuncAttributeMaxDynamicSharedMemorySize;
+        hipError_t e = hipSuccess;
+        const void* few[] = {(const void*)k_kv8_attn_few<1, FEW_WAVES>,
+                             (const void*)k_kv8_attn_few<2, FEW_WAVES>};
+        for (const void* k : few)
+            if (e == hipSuccess) e = hipFuncSetAttribute(k, (hipFuncAttribute)most, FEW_LDS);
+        if (e == hipSuccess)
+            e = hipFuncSetAttribute((const void*)k_kv8_attn_many<MANY_T, MANY_WAVES>,
+                                    (hipFuncAttribute)most, MANY_LDS);
+        return e;
+    }();
+    return done;
+}
+
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t st) {
-    if (a.M < 1 || a.M > MJ_ROWS || a.ring.C >= ((int64_t)1 << 30) || a.units < 1)
+    if (a.M < 1 || a.M > MJ_ROWS || a.ring.C >= ((int64_t)1 << 30) || a.units < 1 || a.parts < 1)
         return hipErrorInvalidValue;
-    const int nv = a.M * a.G, vb = a.n_sel > 0 ? a.G : nv;
-    const int cols = a.n_sel > 0 ? a.M : (vb + 64 * a.tiles - 1) / (64 * a.tiles);
-    const dim3 grid(a.parts, cols, a.p.nKV);
-    if (a.tiles == 1) hipLaunchKernelGGL(k_kv8_attn<1>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_kv8_attn<2>, grid, dim3(256), 0, st, a);
-    hipError_t e = hipGetLastError();
+    const dim3 grid(a.parts, a.cols, a.p.nKV);
+    hipError_t e = attn_attributes();
+    if (e != hipSuccess) return e;
+    auto go = [&](auto kernel, int waves, size_t lds) {
+        hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), lds, st, a);
+        return hipGetLastError();
+    };
+    if (!a.few) e = go(k_kv8_attn_many<MANY_T, MANY_WAVES>, MANY_WAVES, MANY_LDS);
+    else if (a.tiles == 1) e = go(k_kv8_attn_few<1, FEW_WAVES>, FEW_WAVES, FEW_LDS);
+    else e = go(k_kv8_attn_few<2, FEW_WAVES>, FEW_WAVES, FEW_LDS);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(k_kv8_combine, dim3(a.M * a.p.nKV * a.G), dim3(256), 0, st, a);
     e = hipGetLastError();

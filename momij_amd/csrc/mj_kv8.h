@@ -73,9 +73,11 @@ struct Kv8AttnArgs {
     float2* out_sum;
     const float* mass_in;
     float* mass_out;
-    // set by kv8_attn_plan: units (listed blocks, then 64-row chunks of the ring) a part, parts,
-    // tiles of 16 query vectors a block, and the workspace
-    int n_list, units, upp, parts, tiles;
+    // set by kv8_attn_plan: units are the listed blocks, then 64-row chunks of the ring.  few: parts
+    // of upp blocks each (page_parts), then one a ring unit; else parts of upp units.  tiles: of 16
+    // query vectors, a wave; cols: block columns (groups of tiles, rows with lists of their own)
+    int n_list, units, upp, parts, page_parts, tiles, cols;
+    bool few;
     float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
     float2* ml;     // [parts][nKV][nv] {m, sum}
     float2* rec;    // [nKV][n][nv] {m, sum} of each block where masses are wanted
