@@ -9,7 +9,7 @@
 #include "mj_kv8.h"
 
 #define HD 128
-#define LOG2E 1.44269504088896341f
+#define SC2 (1.44269504088896341f * 0.08838834764831845f)  // log2 e / sqrt(128)
 
 // max / sum over lanes i, i ^ 16, i ^ 32, i ^ 48 (the same bits in every lane)
 __device__ __forceinline__ float x4_max(float v) {
@@ -51,6 +51,10 @@ __device__ __forceinline__ void codes16(const u4v w, u4v& a, u4v& b) {
     b.w = y;
 }
 
+__device__ __forceinline__ float lane_of(float v, int i) {  // lane i's value (i uniform)
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+
 __device__ __forceinline__ int unit_page(const Kv8AttnArgs& a, int g, int row, int u) {
     int i = u;
     if (a.sel) {
@@ -76,13 +80,30 @@ struct Tile {
 
 typedef float f2v __attribute__((ext_vector_type(2)));
 
+// What a unit's codes stand for: ksc, the factor of its raw scores to log2 units; lv, log2 of its V
+// scale (at least LV_MIN, that of a block of the least fp16 number; a block of zeros has none), and
+// 2^-lv.
+struct Scales {
+    float ksc, lv, ilv;
+};
+#define LV_MIN -31.0f
+__device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
+    const float l = __builtin_amdgcn_logf(vs);
+    return l < LV_MIN ? LV_MIN : l;
+}
+
 // Softmax of one unit's scores against the running state.  S: lane (ln, lq) holds vector ln against
-// tokens 16 kt + 4 lq + r, without the scale ksc >= 0; masked ones -inf.  Returns the weights rounded
-// to fp16, as the two A operands of the product with V (their k slot 8 lq + u is token 32 j + 4 lq +
-// u, then 32 j + 16 + 4 lq + u - 4): a weight carries half a step, 2^-11, into the output's mean,
-// and the sum that divides it adds up the same rounded weights.  lu: the unit's sum, this lane's
-// share.  The state's outputs are rescaled where some vector's maximum moved.
-__device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], float ksc, u4v pa[2], float& lu) {
+// tokens 16 kt + 4 lq + r, without the scale ksc >= 0; masked ones -inf.  The weights come out times
+// the unit's V scale, w = exp2(s + lv - m), so the products with V accumulate in the state without a
+// step between; m is the running reference of s + lv.  It follows the maximum only where that is more
+// than 2^SLACK above it: outputs are rescaled once or twice a part, not at every unit, and w stays
+// below 2^(SLACK + 1).  w is rounded to fp16, as the two A operands of the product with V (their k
+// slot 8 lq + u is token 32 j + 4 lq + u, then 32 j + 16 + 4 lq + u - 4): half a step, 2^-11 of a
+// weight, averaged over the keys; the sum takes the weights before that rounding (a small V scale may
+// put them below fp16's normal range where they still count in the sum).  lu: the unit's sum of
+// exp2(s - m), this lane's share.
+#define SLACK 6.0f
+__device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], Scales u, u4v pa[2], float& lu) {
     const int lq = (threadIdx.x & 63) >> 4;
     float m = -INFINITY;
 #pragma unroll
@@ -90,25 +111,12 @@ __device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], float ksc, u4v pa
         m = fmaxf(fmaxf(m, S[kt][0]), S[kt][1]);
         m = fmaxf(fmaxf(m, S[kt][2]), S[kt][3]);
     }
-    m = fmaxf(T.m, x4_max(m) * ksc);
-    // nothing seen yet: any finite reference (a masked score still gives 0, a NaN stays one)
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const bool moved = T.m != m;
-    const float alpha = __builtin_amdgcn_exp2f(T.m - ref);
-    T.m = m;
-    lu = 0.0f;
-    const h2v one = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const f2v p = {__builtin_amdgcn_exp2f(fmaf(S[kt][2 * h], ksc, -ref)),
-                           __builtin_amdgcn_exp2f(fmaf(S[kt][2 * h + 1], ksc, -ref))};
-            const h2v ph = __builtin_convertvector(p, h2v);
-            lu = __builtin_amdgcn_fdot2(ph, one, lu, false);
-            pa[kt >> 1][2 * (kt & 1) + h] = __builtin_bit_cast(uint32_t, ph);
-        }
+    m = fmaf(x4_max(m), u.ksc, u.lv);
+    const bool moved = m > T.m + SLACK;
     if (__any(moved)) {
+        const float mn = fmaxf(T.m, m);
+        const float alpha = T.m == mn ? 1.0f : __builtin_amdgcn_exp2f(T.m - mn);  // (both may be -inf)
+        T.m = mn;
         T.l *= alpha;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -117,45 +125,44 @@ __device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], float ksc, u4v pa
             for (int dt = 0; dt < 8; ++dt) T.o[dt][r] *= al;
         }
     }
+    // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
+    const float c = u.lv - (T.m == -INFINITY ? 0.0f : T.m);
+    lu = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const f2v p = {__builtin_amdgcn_exp2f(fmaf(S[kt][2 * h], u.ksc, c)),
+                           __builtin_amdgcn_exp2f(fmaf(S[kt][2 * h + 1], u.ksc, c))};
+            lu += p.x;
+            lu += p.y;
+            pa[kt >> 1][2 * (kt & 1) + h] =
+                __builtin_bit_cast(uint32_t, __builtin_convertvector(p, h2v));
+        }
+    lu *= u.ilv;
     T.l += lu;
 }
 
 // Infinities and NaN among the V rows of the pass (a tree row's siblings must not see them: 0 times
-// an infinity is a NaN) are left out of the products (staged as 0) and added here, for the rows that
-// do attend to them; bad: the ring rows that hold any, ok: those that vector ln attends.
-__device__ __forceinline__ void add_bad_rows(Tile& T, const u4v q[4], const u4v* Kf, int lane,
-                                             float ksc, uint64_t ok, uint64_t bad,
+// an infinity is a NaN) are left out of the products (staged as 0) and added here to the outputs of
+// the vectors that attend to them, whatever their weights (which are above 0, if not in fp32).  bad:
+// the unit's rows that hold any, ok: those that vector ln attends.
+__device__ __forceinline__ void add_bad_rows(Tile& T, int lane, uint64_t ok, uint64_t bad,
                                              const uint16_t* vrow0, int slot0, int C) {
     const int ln = lane & 15, lq = lane >> 4;
+#pragma unroll 1
+    for (; bad; bad &= bad - 1) {
+        const int k = __builtin_ctzll(bad);
+        const uint32_t att = (uint32_t)__ballot((ok >> k) & 1) >> (4 * lq);  // of vectors 4 lq + x
+        int sl = slot0 + k;
+        sl -= sl >= C ? C : 0;
+        const uint16_t* vr = vrow0 + (size_t)sl * HD + ln;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        if (!((bad >> (16 * kt)) & 0xFFFFu)) continue;
-        f4 S = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int dt = 0; dt < 8; ++dt) {
+            const float v = h2f(vr[16 * dt]);
+            const float e = fabsf(v) < INFINITY ? 0.0f : v;
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-            S = mfma16x16x32(as_h8(Kf[(4 * kt + s) * 64 + lane]), as_h8(q[s]), S);
-        const float ref = T.m == -INFINITY ? 0.0f : T.m;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int key = 16 * kt + 4 * lq + r;
-            // -1: not attended
-            const float p = (ok >> key) & 1 ? __builtin_amdgcn_exp2f(fmaf(S[r], ksc, -ref)) : -1.0f;
-            for (int kq = 0; kq < 4; ++kq) {
-                const int k = 16 * kt + 4 * kq + r;
-                if (!((bad >> k) & 1)) continue;  // uniform
-                int sl = slot0 + k;
-                sl -= sl >= C ? C : 0;
-                const uint16_t* vr = vrow0 + (size_t)sl * HD + ln;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const float pv = __shfl(p, 16 * kq + 4 * lq + x, MJ_WAVE);
-#pragma unroll
-                    for (int dt = 0; dt < 8; ++dt) {
-                        const float v = h2f(vr[16 * dt]);
-                        if (!(fabsf(v) < INFINITY) && !(pv < 0.0f)) T.o[dt][x] += pv * v;
-                    }
-                }
-            }
+            for (int x = 0; x < 4; ++x) T.o[dt][x] += (att >> x) & 1 ? e : 0.0f;
         }
     }
 }
@@ -250,24 +257,37 @@ __device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, ui
     return on ? committed | own : 0;
 }
 
-// T tiles against one unit staged in LDS; each operand is read once for all of them.
+// T tiles against one unit staged in LDS; each operand is read once for all of them.  All K operands
+// are requested before the first product and all V operands before the softmax: left to itself the
+// compiler waits for each read in turn, some 30 LDS latencies a unit (64 rows at 65000 tokens: 61 ->
+// %s us).
 template <int T, bool RING>
 __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u4v* Kf, const u4v* Vf,
-                                            int lane, float ksc, float vsc, const uint64_t* ok,
+                                            int lane, Scales u, const uint64_t* ok,
                                             float2* const* rec) {
     const int ln = lane & 15, lq = lane >> 4;
     f4 S[T][4];
+    {
+        u4v k[16];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+        for (int f = 0; f < 16; ++f) k[f] = Kf[f * 64 + lane];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < T; ++i) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < T; ++i)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const h8 k = as_h8(Kf[(4 * kt + s) * 64 + lane]);
+            for (int kt = 0; kt < 4; ++kt) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < T; ++i) S[i][kt] = mfma16x16x32(k, as_h8(q[i][s]), S[i][kt]);
-        }
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < T; ++i)
+                    S[i][kt] = mfma16x16x32(as_h8(k[4 * kt + s]), as_h8(q[i][s]), S[i][kt]);
     }
+    u4v v[16];
+#pragma unroll
+    for (int f = 0; f < 16; ++f) v[f] = Vf[f * 64 + lane];
+    __builtin_amdgcn_sched_barrier(0);
     u4v pa[T][2];
 #pragma unroll
     for (int i = 0; i < T; ++i) {
@@ -278,24 +298,19 @@ __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u
                 for (int r = 0; r < 4; ++r)
                     S[i][kt][r] = (ok[i] >> (16 * kt + 4 * lq + r)) & 1 ? S[i][kt][r] : -INFINITY;
         float lu;
-        softmax_unit(tl[i], S[i], ksc, pa[i], lu);
+        softmax_unit(tl[i], S[i], u, pa[i], lu);
         if (!RING && rec && rec[i]) {
             lu = x4_sum(lu);
             if (lq == 0) *rec[i] = make_float2(tl[i].m, lu);
         }
     }
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) {
-        const h8 v0 = as_h8(Vf[(2 * dt) * 64 + lane]), v1 = as_h8(Vf[(2 * dt + 1) * 64 + lane]);
+    for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
         for (int i = 0; i < T; ++i) {
-            f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-            o = mfma16x16x32(as_h8(pa[i][0]), v0, o);
-            o = mfma16x16x32(as_h8(pa[i][1]), v1, o);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) tl[i].o[dt][r] = fmaf(o[r], vsc, tl[i].o[dt][r]);
+            tl[i].o[dt] = mfma16x16x32(as_h8(pa[i][0]), as_h8(v[2 * dt]), tl[i].o[dt]);
+            tl[i].o[dt] = mfma16x16x32(as_h8(pa[i][1]), as_h8(v[2 * dt + 1]), tl[i].o[dt]);
         }
-    }
 }
 
 __device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g, int tv, int vend,
@@ -313,54 +328,80 @@ __device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g
         }
 }
 
-// Many rows: a block of NW waves takes a run of units of KV head blockIdx.z for NW T tiles of query
-// vectors, T a wave.  A unit is turned to halves once, by the whole block, and read from LDS by its
-// waves; two units are in LDS and one in registers on its way, one barrier a unit.
+// One ring unit (rows base .. of the call's open ones) as a part of its own: the block of NW waves
+// stages it and takes the query vectors v0 .. vend - 1 a tile a wave at a time.  lds: 32 KB.
+template <int NW>
+__device__ __forceinline__ void ring_part(const Kv8AttnArgs& a, int part, int g, int base, int v0,
+                                          int vend, u4v* lds, uint32_t* s_bad, const int* s_abort) {
+    const int t = threadIdx.x, lane = t & 63, ln = lane & 15, C = (int)a.ring.C;
+    if (t < 2) s_bad[t] = 0;
+    __syncthreads();
+    if (*s_abort) return;
+    u4v* Kf = lds;
+    u4v* Vf = Kf + 1024;
+    stage_ring<64 * NW>(a, g, base, Kf, Vf, s_bad);
+    __syncthreads();
+    const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
+    for (int tv = v0 + 16 * (t >> 6); tv < vend; tv += 16 * NW) {
+        u4v q[1][4];
+        uint64_t anc;
+        load_q(a, g, tv + ln, tv + ln < vend, q[0], anc);
+        Tile tl[1];
+        tl[0].clear();
+        const uint64_t ok = ring_mask(a, base, anc, tv + ln < vend);
+        staged_unit<1, true>(tl, q, Kf, Vf, lane, Scales{SC2, 0.0f, 1.0f}, &ok, nullptr);
+        if (bad) {
+            int sb = a.slot0 + base;
+            sb -= sb >= C ? C : 0;
+            add_bad_rows(tl[0], lane, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
+        }
+        write_part(a, part, g, tv, vend, tl[0]);
+    }
+}
+
+// Many rows: a block of NW waves takes a run of pages of KV head blockIdx.z for NW T tiles of query
+// vectors, T a wave.  A page is turned to halves once, by the whole block, and read from LDS by its
+// waves; two pages are in LDS and one in registers on its way, one barrier a page.  The first blocks take a
+// ring unit each.
 template <int T, int NW>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NR = 512 / NT;
-    extern __shared__ __align__(16) u4v lds[];  // two units: K operands, V operands
+    extern __shared__ __align__(16) u4v lds[];  // two pages: K operands, V operands
     __shared__ int s_abort;
-    __shared__ uint32_t s_bad[3][2];  // ring rows with an infinity or NaN in V, of unit u % 3
+    __shared__ uint32_t s_bad[2];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15;
-    const int part = blockIdx.x, g = blockIdx.z;
-    const int v0 = (int)blockIdx.y * 16 * NW * T, vend = a.M * a.G;  // the block's vectors
-    const int nv = a.M * a.G, C = (int)a.ring.C;
+    const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
+    const int v0 = (int)blockIdx.y * 16 * NW * T, vend = min(nv, v0 + 16 * NW * T);
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_abort = ab;
+    if (part < a.ring_units) {
+        ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
+        return;
+    }
     Tile tl[T];
     u4v q[T][4];
-    uint64_t anc[T];
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         const int v = v0 + 16 * (wv * T + i) + ln;
-        load_q(a, g, v, v < vend, q[i], anc[i]);
+        uint64_t anc;
+        load_q(a, g, v, v < vend, q[i], anc);
         tl[i].clear();
     }
     const bool idle = v0 + 16 * wv * T >= vend;  // the wave has no vector: it stages only
-    const int u0 = part * a.upp, u1 = min(u0 + a.upp, a.units);
-    const float sc2 = LOG2E * 0.08838834764831845f;  // log2 e / sqrt(128)
+    const int u0 = (part - a.ring_units) * a.upp, u1 = min(u0 + a.upp, a.n_list);
     u4v kr[NR], vr[NR];
-    auto page = [&](int u) {  // of unit u, -1: none (a ring unit, or no block)
-        return u < u1 && u < a.n_list ? unit_page(a, g, 0, u) : -1;
-    };
     auto request = [&](int pg) {
-        const u4v* kp = (const u4v*)(a.p.k + (size_t)max(pg, 0) * KV8_PAGE_BYTES);
-        const u4v* vp = (const u4v*)(a.p.v + (size_t)max(pg, 0) * KV8_PAGE_BYTES);
+        const u4v* kp = (const u4v*)(a.p.k + (size_t)pg * KV8_PAGE_BYTES);
+        const u4v* vp = (const u4v*)(a.p.v + (size_t)pg * KV8_PAGE_BYTES);
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
             kr[c] = kp[t + NT * c];
             vr[c] = vp[t + NT * c];
         }
     };
-    auto stage = [&](int u, int pg) {
-        u4v* Kf = lds + (u & 1) * 2048;
+    auto stage = [&](int b) {
+        u4v* Kf = lds + b * 2048;
         u4v* Vf = Kf + 1024;
-        if (u >= a.n_list) {
-            stage_ring<NT>(a, g, 64 * (u - a.n_list), Kf, Vf, s_bad[u % 3]);
-            return;
-        }
-        if (pg < 0) return;
 #pragma unroll
         for (int c = 0; c < NR; ++c) {
             const int f = (t + NT * c) >> 6;
@@ -368,55 +409,49 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
             codes16(vr[c], Vf[(2 * f) * 64 + lane], Vf[(2 * f + 1) * 64 + lane]);
         }
     };
-    int pg = page(u0), pn = page(u0 + 1);
-    request(pg);
-    if (t < 6) s_bad[t >> 1][t & 1] = 0;
-    __syncthreads();
-    if (s_abort) return;
-    stage(u0, pg);
-    request(pn);
-    for (int u = u0; u < u1; ++u) {
-        const int p2 = page(u + 2);
-        __syncthreads();  // unit u is staged; everyone is done with unit u - 1
-        const bool ringu = u >= a.n_list;
-        uint64_t bad = 0;
-        if (ringu) bad = s_bad[u % 3][0] | ((uint64_t)s_bad[u % 3][1] << 32);
-        if (t < 2) s_bad[(u + 2) % 3][t] = 0;  // read before this barrier, set after the next
-        const float ks = pg >= 0 ? a.p.ks[pg] : 1.0f, vs = pg >= 0 ? a.p.vs[pg] : 1.0f;
-        if (u + 1 < u1) {
-            stage(u + 1, pn);
-            request(p2);
+    // 64 pages' numbers and scales at a time, one a lane (a page at a time they are two dependent
+    // round trips before its request goes out)
+    for (int ub = u0; ub < u1; ub += 64) {
+        const int pl = ub + lane < u1 ? unit_page(a, g, 0, ub + lane) : -1;
+        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
+        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
+        uint64_t todo = __ballot(pl >= 0);  // the same in every wave
+        int cur = todo ? __builtin_ctzll(todo) : -1, nxt = -1, b = 0;
+        if (cur >= 0) {
+            request(__builtin_amdgcn_readlane(pl, cur));
+            todo &= todo - 1;
+            nxt = todo ? __builtin_ctzll(todo) : -1;
         }
-        const u4v* Kf = lds + (u & 1) * 2048;
-        const u4v* Vf = Kf + 1024;
-        if (!idle && ringu) {
-            const int base = 64 * (u - a.n_list);
-            uint64_t ok[T];
-#pragma unroll
-            for (int i = 0; i < T; ++i)
-                ok[i] = ring_mask(a, base, anc[i], v0 + 16 * (wv * T + i) + ln < vend);
-            staged_unit<T, true>(tl, q, Kf, Vf, lane, sc2, 1.0f, ok, nullptr);
-            if (bad) {
-                int sb = a.slot0 + base;
-                sb -= sb >= C ? C : 0;
-#pragma unroll
-                for (int i = 0; i < T; ++i)
-                    add_bad_rows(tl[i], q[i], Kf, lane, sc2, ok[i], bad,
-                                 a.ring.v + (size_t)g * C * HD, sb, C);
+        __syncthreads();  // (the last batch's pages are done with)
+        if (s_abort) return;
+        if (cur >= 0) stage(0);
+        if (nxt >= 0) request(__builtin_amdgcn_readlane(pl, nxt));
+        while (cur >= 0) {
+            todo &= todo - 1;
+            const int n2 = todo ? __builtin_ctzll(todo) : -1;
+            __syncthreads();  // page cur is staged; everyone is done with the one before
+            if (nxt >= 0) {
+                stage(b ^ 1);
+                request(__builtin_amdgcn_readlane(pl, n2 >= 0 ? n2 : nxt));
             }
-        } else if (!idle && pg >= 0) {
-            float2* rec[T];
+            if (!idle) {
+                const u4v* Kf = lds + b * 2048;
+                float2* rec[T];
 #pragma unroll
-            for (int i = 0; i < T; ++i) {
-                const int v = v0 + 16 * (wv * T + i) + ln;
-                rec[i] = !a.rec ? nullptr
-                         : v < vend ? a.rec + ((size_t)g * a.n + u) * nv + v
-                                    : a.rec + (size_t)a.p.nKV * a.n * nv + ln;  // a spare row
+                for (int i = 0; i < T; ++i) {
+                    const int v = v0 + 16 * (wv * T + i) + ln;
+                    rec[i] = !a.rec ? nullptr
+                             : v < vend ? a.rec + ((size_t)g * a.n + ub + cur) * nv + v
+                                        : a.rec + (size_t)a.p.nKV * a.n * nv + ln;  // a spare row
+                }
+                staged_unit<T, false>(tl, q, Kf, Kf + 1024, lane,
+                                      Scales{lane_of(ksl, cur), lane_of(lvl, cur), lane_of(ill, cur)},
+                                      nullptr, rec);
             }
-            staged_unit<T, false>(tl, q, Kf, Vf, lane, ks * sc2, vs, nullptr, rec);
+            cur = nxt;
+            nxt = n2;
+            b ^= 1;
         }
-        pg = pn;
-        pn = p2;
     }
 #pragma unroll
     for (int i = 0; i < T; ++i) {
@@ -429,8 +464,8 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
 // a page's bytes lie in the order of the operands, so a lane's 16 bytes are two of them.  A wave's
 // next K goes out behind its scores, its next V behind its output product; the page numbers and
 // scales of 64 pages come with one request a lane each.  The block's NW waves are joined in LDS.
-// Blocks past the pages' parts take one ring unit each, all waves staging it.  Where rows list their
-// own blocks (a.sel), blockIdx.y is a row and a share of its heads.
+// The first blocks take a ring unit each.  Where rows list their own blocks (a.sel),
+// blockIdx.y is a row and a share of its heads.
 template <int T, int NW>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, RS = HD + 4;
@@ -449,38 +484,15 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
     }
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_abort = ab;
-    const float sc2 = LOG2E * 0.08838834764831845f;  // log2 e / sqrt(128)
-    if (part >= a.page_parts) {
-        // ---- one ring unit, a tile a wave
-        if (t < 2) s_bad[t] = 0;
-        __syncthreads();
-        if (s_abort) return;
-        const int base = 64 * (part - a.page_parts), C = (int)a.ring.C;
-        u4v* Kf = lds;
-        u4v* Vf = Kf + 1024;
-        stage_ring<NT>(a, g, base, Kf, Vf, s_bad);
-        const int tv = v0 + 16 * wv;
-        u4v q[1][4];
-        uint64_t anc;
-        load_q(a, g, tv + ln, tv + ln < vend, q[0], anc);
-        __syncthreads();
-        if (wv >= T || tv >= vend) return;
-        Tile tl[1];
-        tl[0].clear();
-        const uint64_t ok = ring_mask(a, base, anc, tv + ln < vend);
-        staged_unit<1, true>(tl, q, Kf, Vf, lane, sc2, 1.0f, &ok, nullptr);
-        const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
-        if (bad) {
-            int sb = a.slot0 + base;
-            sb -= sb >= C ? C : 0;
-            add_bad_rows(tl[0], q[0], Kf, lane, sc2, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
-        }
-        write_part(a, part, g, tv, vend, tl[0]);
+    if (part < a.ring_units) {
+        ring_part<NW>(a, part, g, 64 * part, v0, min(vend, v0 + 16 * T), lds, s_bad,
+                      &s_abort);
         return;
     }
     Tile tl[T];
     u4v q[T][4];
-    const int u0 = part * a.upp + wv, u1 = min((part + 1) * a.upp, a.n_list);
+    const int up = (part - a.ring_units) * a.upp;
+    const int u0 = up + wv, u1 = min(up + a.upp, a.n_list);
     for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NW) {
         const int ul = ub + NW * lane;  // lane's unit
         const int pl = ul < u1 ? unit_page(a, g, row, ul) : -1;
@@ -501,7 +513,8 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
             request_k(i0);
             request_v(i0);
         }
-        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * sc2, vsl = pl >= 0 ? a.p.vs[pl] : 0.0f;
+        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
+        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
         if (ub == u0) {
 #pragma unroll
             for (int i = 0; i < T; ++i) {
@@ -514,8 +527,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
             const int i = i0;
             todo &= todo - 1;
             i0 = todo ? __builtin_ctzll(todo) : i;  // the last page is requested again, unused
-            const float ksc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ksl), i));
-            const float vsc = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vsl), i));
+            const Scales sc{lane_of(ksl, i), lane_of(lvl, i), lane_of(ill, i)};
             f4 S[T][4];
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
@@ -537,7 +549,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
 #pragma unroll
             for (int x = 0; x < T; ++x) {
                 float lu;
-                softmax_unit(tl[x], S[x], ksc, pa[x], lu);
+                softmax_unit(tl[x], S[x], sc, pa[x], lu);
                 if (a.rec) {
                     const int v = v0 + 16 * x + ln;
                     lu = x4_sum(lu);
@@ -551,11 +563,8 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
                 codes16(vr[dt], w0, w1);
 #pragma unroll
                 for (int x = 0; x < T; ++x) {
-                    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-                    o = mfma16x16x32(as_h8(pa[x][0]), as_h8(w0), o);
-                    o = mfma16x16x32(as_h8(pa[x][1]), as_h8(w1), o);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) tl[x].o[dt][r] = fmaf(o[r], vsc, tl[x].o[dt][r]);
+                    tl[x].o[dt] = mfma16x16x32(as_h8(pa[x][0]), as_h8(w0), tl[x].o[dt]);
+                    tl[x].o[dt] = mfma16x16x32(as_h8(pa[x][1]), as_h8(w1), tl[x].o[dt]);
                 }
             }
             request_v(i0);
@@ -704,32 +713,31 @@ __global__ __launch_bounds__(256) void k_kv8_mass(Kv8AttnArgs a) {
 
 // Shapes of the two kernels: few<T, 8> for up to FEW_TILES tiles and for listed blocks, else many.
 #define FEW_WAVES 8
+#ifndef FEW_TILES
 #define FEW_TILES 2
+#endif
+#ifndef MANY_WAVES
 #define MANY_WAVES 8
+#endif
+#ifndef MANY_T
 #define MANY_T 2
+#endif
 
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.n_list = a.n_sel > 0 ? a.n_sel : a.n;
-    const int ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
-    a.units = a.n_list + ring_units;
+    a.ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
     const int nv = a.M * a.G;
     const int tiles = ((a.n_sel > 0 ? a.G : nv) + 15) / 16;  // that share their units
     a.few = a.n_sel > 0 || tiles <= FEW_TILES;
     a.tiles = a.few ? std::min(tiles, FEW_TILES) : MANY_T;  // a wave
     const int per = a.few ? a.tiles : MANY_T * MANY_WAVES;
     a.cols = (a.n_sel > 0 ? a.M : 1) * ((tiles + per - 1) / per);
-    // one block a CU
-    int parts = std::max(1, 256 / (a.cols * a.p.nKV));
-    if (a.few) {
-        parts = std::min(parts, (a.n_list + FEW_WAVES - 1) / FEW_WAVES);
-        a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
-        a.page_parts = parts ? (a.n_list + a.upp - 1) / a.upp : 0;
-        a.parts = a.page_parts + ring_units;
-    } else {
-        parts = std::min(parts, a.units);
-        a.upp = (a.units + parts - 1) / parts;
-        a.parts = a.page_parts = (a.units + a.upp - 1) / a.upp;
-    }
+    // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
+    // chip holds would run alone at the end
+    int parts = std::max(1, 256 / (a.cols * a.p.nKV) - a.ring_units);
+    parts = std::min(parts, a.few ? (a.n_list + FEW_WAVES - 1) / FEW_WAVES : a.n_list);
+    a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
+    a.parts = a.ring_units + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         off = (off + 255) & ~(size_t)255;
@@ -765,7 +773,7 @@ static hipError_t attn_attributes() {
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t st) {
-    if (a.M < 1 || a.M > MJ_ROWS || a.ring.C >= ((int64_t)1 << 30) || a.units < 1 || a.parts < 1)
+    if (a.M < 1 || a.M > MJ_ROWS || a.ring.C >= ((int64_t)1 << 30) || a.parts < 1)
         return hipErrorInvalidValue;
     const dim3 grid(a.parts, a.cols, a.p.nKV);
     hipError_t e = attn_attributes();

@@ -73,10 +73,10 @@ struct Kv8AttnArgs {
     float2* out_sum;
     const float* mass_in;
     float* mass_out;
-    // set by kv8_attn_plan: units are the listed blocks, then 64-row chunks of the ring.  few: parts
-    // of upp blocks each (page_parts), then one a ring unit; else parts of upp units.  tiles: of 16
-    // query vectors, a wave; cols: block columns (groups of tiles, rows with lists of their own)
-    int n_list, units, upp, parts, page_parts, tiles, cols;
+    // set by kv8_attn_plan: a part for every 64 rows of the ring (ring_units), then parts of upp
+    // listed blocks each; few: which kernel; tiles: of 16 query vectors, a wave; cols: block columns
+    // (groups of tiles, rows with lists of their own)
+    int n_list, upp, parts, ring_units, tiles, cols;
     bool few;
     float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
     float2* ml;     // [parts][nKV][nv] {m, sum}
