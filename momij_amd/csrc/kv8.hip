@@ -1,6 +1,8 @@
 // kv8.hip -- the 8-bit KV cache: appending normed and rotated rows to the fp16 ring, sealing blocks
 // into pages and back, choosing blocks by a cheap score, evicting them by accumulated weight.
 // (Attention over the cache: kv8_attn.hip.)
+#include <type_traits>
+
 #include "mj_device.h"
 #include "mj_kv8.h"
 
@@ -103,10 +105,48 @@ __device__ __forceinline__ float absmax_finite(float m, float x) {
     const float ax = fabsf(x);
     return ax < INFINITY && ax > m ? ax : m;  // (a NaN compares false)
 }
-// code of x under 127 / greatest magnitude: nearest whole number, an infinity at +-127, a NaN 0
+// code of x under r = 127 / greatest magnitude (0: all codes 0): nearest whole number, an infinity at
+// +-127, a NaN 0
 __device__ __forceinline__ int code8(float x, float r) {
-    const float c = fminf(fmaxf(rintf(x * r), -127.0f), 127.0f);
-    return x == x && r > 0.0f ? (int)c : 0;
+    float v = x * r;
+    v = v == v ? v : 0.0f;
+    return (int)rintf(__builtin_amdgcn_fmed3f(v, -127.0f, 127.0f));
+}
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {  // the low bytes, a lowest
+    const uint32_t ab = __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0C0C0400u);
+    const uint32_t cd = __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x0C0C0400u);
+    return ab | (cd << 16);
+}
+
+// Wave-wide steps by lane moves (an LDS shuffle costs some 100 cycles a step, and a block that does
+// little else waits for each): inclusive sums, and the least and greatest in every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);  // from 1, 2, 4, 8 lanes below in the row
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row 0's total to row 1, row 2's to row 3
+    return dpp_add<0x143, 0xC>(v);  // rows 0 and 1's to rows 2 and 3
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_mov(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false);
+}
+template <bool MIN>
+__device__ __forceinline__ uint32_t wave_ext(uint32_t v) {
+    auto ext = [](uint32_t a, uint32_t b) { return MIN ? min(a, b) : max(a, b); };
+    v = ext(v, dpp_mov<0xB1>(v));   // xor 1
+    v = ext(v, dpp_mov<0x4E>(v));   // xor 2
+    v = ext(v, dpp_mov<0x141>(v));  // eight lanes mirrored
+    v = ext(v, dpp_mov<0x140>(v));  // sixteen
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = ext(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return ext(b[0], b[1]);
 }
 
 // A 256-thread block seals K (blockIdx.z 0) or V (1) of one block of one head: 16 KB in, 8 KB of
@@ -148,14 +188,15 @@ __global__ __launch_bounds__(256) void k_kv8_seal(Kv8Pool p, Kv8Ring ring, int64
     int hi[8], lo[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        uint32_t w[2] = {0u, 0u};
+        int c[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int c = code8(h2f((uint16_t)(raw[j][e >> 1] >> (16 * (e & 1)))), r);
-            hi[e] = j == 0 ? c : max(hi[e], c);
-            lo[e] = j == 0 ? c : min(lo[e], c);
-            w[e >> 2] |= (uint32_t)(c + 128) << (8 * (e & 3));
+            c[e] = code8(h2f((uint16_t)(raw[j][e >> 1] >> (16 * (e & 1)))), r);
+            hi[e] = j == 0 ? c[e] : max(hi[e], c[e]);
+            lo[e] = j == 0 ? c[e] : min(lo[e], c[e]);
         }
+        const uint32_t w[2] = {bytes4(c[0], c[1], c[2], c[3]) ^ 0x80808080u,
+                               bytes4(c[4], c[5], c[6], c[7]) ^ 0x80808080u};
         const int key = k0 + 16 * j;
         if (!isv) {
             *(uint2*)(dst + 2048 * j + 1024 * (dg >> 3) + 256 * ((dg >> 1) & 3) + 16 * k0 +
@@ -266,6 +307,69 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return f != f ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
+// max over 16 consecutive lanes, in all of them
+__device__ __forceinline__ float max16(float v) {
+    auto step = [](float x, uint32_t y) { return fmaxf(x, __uint_as_float(y)); };
+    v = step(v, dpp_mov<0xB1>(__float_as_uint(v)));
+    v = step(v, dpp_mov<0x4E>(__float_as_uint(v)));
+    v = step(v, dpp_mov<0x141>(__float_as_uint(v)));
+    return step(v, dpp_mov<0x140>(__float_as_uint(v)));
+}
+
+// A query vector's 8-bit codes as operands: lane (ln, lq) holds dims 64 j + 16 lq + 0 .. 15 of column
+// ln's vector q; up = max(c, 0), dn = min(c, 0); returns the scale.
+__device__ __forceinline__ float query_codes(const uint16_t* q, i4v up[2], i4v dn[2]) {
+    u4v raw[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) raw[j] = *(const u4v*)(q + 64 * (j >> 1) + 8 * (j & 1));
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            m = absmax_finite(m, h2f((uint16_t)(raw[j][e >> 1] >> (16 * (e & 1)))));
+    m = fmaxf(m, __shfl_xor(m, 16, MJ_WAVE));
+    m = fmaxf(m, __shfl_xor(m, 32, MJ_WAVE));
+    const float r = m > 0.0f ? 127.0f / m : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            int c[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int e = 4 * w + b;
+                c[b] = code8(h2f((uint16_t)(raw[2 * j + (e >> 3)][(e & 7) >> 1] >> (16 * (e & 1)))), r);
+            }
+            const uint32_t pc = bytes4(c[0], c[1], c[2], c[3]);
+            const uint32_t sign = (pc >> 7) & 0x01010101u, neg = (sign << 8) - sign;  // bytes < 0
+            up[j][w] = (int)(pc & ~neg);
+            dn[j][w] = (int)(pc & neg);
+        }
+    return m / 127.0f;
+}
+
+// u = sum_d max(c_d hi_d, c_d lo_d) = sum_d up_d hi_d + dn_d lo_d of 16 blocks (rows) and 16 query
+// vectors (columns), exact in whole numbers.
+__device__ __forceinline__ i4v bound_sums(const i4v hi[2], const i4v lo[2], const i4v up[2],
+                                          const i4v dn[2]) {
+    i4v u = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        u = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi[j], up[j], u, 0, 0, 0);
+        u = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo[j], dn[j], u, 0, 0, 0);
+    }
+    return u;
+}
+__device__ __forceinline__ void load_bounds(const Kv8Pool& p, int pg, i4v hi[2], i4v lo[2]) {
+    const int8_t* b = p.bounds + (size_t)max(pg, 0) * (2 * HD) + 16 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        hi[j] = *(const i4v*)(b + 64 * j);
+        lo[j] = *(const i4v*)(b + HD + 64 * j);
+    }
+}
+
 // Scores of 64 blocks of one head for the rows of blockIdx.z's share, a wave 16 blocks:
 //   u = sum_d max(c_d hi_d, c_d lo_d) = sum_d c+_d hi_d + c-_d lo_d,  c+ = max(c, 0), c- = min(c, 0),
 // on v_mfma_i32_16x16x64_i8 (blocks as rows, query heads as columns), exact in whole numbers.  A
@@ -278,14 +382,7 @@ __global__ __launch_bounds__(256) void k_kv8_score(Kv8SelectArgs a, int P, int t
     const int pg = idx < a.n ? page_of(a.p, g, idx) : -1;
     if (aborted(a.abort)) return;
     i4v hi[2], lo[2];
-    {
-        const int8_t* b = a.p.bounds + (size_t)(pg < 0 ? 0 : pg) * (2 * HD) + 16 * lq;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            hi[j] = *(const i4v*)(b + 64 * j);
-            lo[j] = *(const i4v*)(b + HD + 64 * j);
-        }
-    }
+    load_bounds(a.p, pg, hi, lo);
     const float ks_l = pg < 0 ? 0.0f : a.p.ks[pg];
     float ks[4];
     bool have[4];
@@ -304,41 +401,9 @@ __global__ __launch_bounds__(256) void k_kv8_score(Kv8SelectArgs a, int P, int t
             const bool on = row < a.M && head < a.G;
             const uint16_t* q = a.q + (size_t)(on ? row : 0) * a.ldq +
                                 (size_t)(g * a.G + (on ? head : 0)) * HD + 16 * lq;
-            u4v raw[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) raw[j] = *(const u4v*)(q + 64 * (j >> 1) + 8 * (j & 1));
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    m = absmax_finite(m, h2f((uint16_t)(raw[j][e >> 1] >> (16 * (e & 1)))));
-            m = fmaxf(m, __shfl_xor(m, 16, MJ_WAVE));
-            m = fmaxf(m, __shfl_xor(m, 32, MJ_WAVE));
-            const float r = m > 0.0f ? 127.0f / m : 0.0f, sq = m / 127.0f;
             i4v up[2], dn[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t pu = 0, pd = 0;
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const int e = 4 * w + b;
-                        const int c = code8(
-                            h2f((uint16_t)(raw[2 * j + (e >> 3)][(e & 7) >> 1] >> (16 * (e & 1)))), r);
-                        pu |= (uint32_t)(max(c, 0) & 255) << (8 * b);
-                        pd |= (uint32_t)(min(c, 0) & 255) << (8 * b);
-                    }
-                    up[j][w] = (int)pu;
-                    dn[j][w] = (int)pd;
-                }
-            i4v u = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                u = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi[j], up[j], u, 0, 0, 0);
-                u = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo[j], dn[j], u, 0, 0, 0);
-            }
+            const float sq = query_codes(q, up, dn);
+            const i4v u = bound_sums(hi, lo, up, dn);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float sc = (float)u[k] * ks[k] * sq;
@@ -357,7 +422,238 @@ __global__ __launch_bounds__(256) void k_kv8_score(Kv8SelectArgs a, int P, int t
     }
 }
 
-// The k greatest of n keys (0 < k <= n), the lower index first among equal ones: the threshold key
+// The k greatest of the keys that a block's threads hold in registers, the lower index first among
+// equal ones: thr and take such that key > thr, or key == thr and among the first `take` of those.
+// Thread (w, lane) holds R keys, of indices (w R + r) 64 + lane; ON marks those that compete (k of
+// them at least, k > 0).  The range of the keys is cut into 1024 equal bins, the bin that holds the
+// k-th found, and so on inside it until it holds 64 keys or fewer, which one wave ranks: one round
+// for scores that spread at all (a radix round of eight bits a time took four, most keys meeting in
+// one bin of the first).
+template <int NT, int R>
+__device__ __forceinline__ void kth_of(const uint32_t key[R], const bool on[R], int k, uint32_t& thr,
+                                       int& take) {
+    constexpr int NW = NT / 64, LB = NT == 1024 ? 10 : 8;  // a thread a bin
+    static_assert(NT == 1 << LB, "");
+    __shared__ int hist[NT], s_tot[NW], s_pick[3], s_n;
+    __shared__ uint32_t s_lo[NW], s_hi[NW], s_cand[64];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, lw = lane & (NW - 1);
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (on[r]) {
+            lo = min(lo, key[r]);
+            hi = max(hi, key[r]);
+        }
+    lo = wave_ext<true>(lo);
+    hi = wave_ext<false>(hi);
+    if (lane == 0) {
+        s_lo[wv] = lo;
+        s_hi[wv] = hi;
+    }
+    hist[t] = 0;
+    if (t == 0) s_n = 0;
+    __syncthreads();
+    lo = wave_ext<true>(s_lo[lw]);
+    hi = wave_ext<false>(s_hi[lw]);
+    for (;;) {
+        const int bits = hi > lo ? 32 - __clz((int)(hi - lo)) : 0, sh = bits > LB ? bits - LB : 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (on[r] && key[r] >= lo && key[r] <= hi) atomicAdd(&hist[(key[r] - lo) >> sh], 1);
+        __syncthreads();
+        const int c = hist[NT - 1 - t];  // bins from the top
+        const int run = wave_scan(c);
+        if (lane == 63) s_tot[wv] = run;
+        __syncthreads();
+        const int tot = wave_scan(lane < NW ? s_tot[lw] : 0);
+        const int before = run - c + (wv ? __builtin_amdgcn_readlane(tot, wv - 1) : 0);
+        if (before < k && before + c >= k) {
+            s_pick[0] = NT - 1 - t;
+            s_pick[1] = before;
+            s_pick[2] = c;
+        }
+        hist[NT - 1 - t] = 0;
+        __syncthreads();
+        lo += (uint32_t)s_pick[0] << sh;
+        hi = min(hi, lo + ((1u << sh) - 1));
+        k -= s_pick[1];
+        const int in = s_pick[2];
+        if (sh == 0) {  // one key is left
+            thr = lo;
+            take = k;
+            return;
+        }
+        if (in == k) {  // the whole bin: the keys from lo on
+            thr = lo > 0 ? lo - 1 : 0;
+            take = lo > 0 ? 0 : 0x7FFFFFFF;
+            return;
+        }
+        if (in > 64) continue;  // (nobody writes s_pick before the next two barriers)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (on[r] && key[r] >= lo && key[r] <= hi) s_cand[atomicAdd(&s_n, 1)] = key[r];
+        __syncthreads();
+        // every wave ranks them for itself
+        const uint32_t mine = lane < in ? s_cand[lane] : 0;
+        int above = 0, same = 0;
+        for (int i = 0; i < in; ++i) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+            above += o > mine;
+            same += o == mine;
+        }
+        const int at = __builtin_ctzll(__ballot(lane < in && above < k && k <= above + same));
+        thr = (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+        take = k - __builtin_amdgcn_readlane(above, at);
+        return;
+    }
+}
+
+// The keys of kth_of's layout split in two, each part in increasing index order: out(i, place, chosen),
+// place among the chosen (sure: without competing) or among the others; n keys in all.
+template <int NT, int R, typename O>
+__device__ __forceinline__ void split_keys(const uint32_t key[R], const bool on[R], const bool sure[R],
+                                           int n, uint32_t thr, int take, O out) {
+    constexpr int NW = NT / 64;
+    __shared__ int s_eq[NW], s_gt[NW];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, lw = lane & (NW - 1);
+    const uint64_t below = (1ull << lane) - 1;
+    int eq = 0, gt = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        eq += __popcll(__ballot(on[r] && key[r] == thr));
+        gt += __popcll(__ballot(sure[r] || (on[r] && key[r] > thr)));
+    }
+    if (lane == 0) {
+        s_eq[wv] = eq;
+        s_gt[wv] = gt;
+    }
+    __syncthreads();
+    eq = wave_scan(lane < NW ? s_eq[lw] : 0);
+    gt = wave_scan(lane < NW ? s_gt[lw] : 0);
+    eq = wv ? __builtin_amdgcn_readlane(eq, wv - 1) : 0;  // those of the waves before
+    gt = wv ? __builtin_amdgcn_readlane(gt, wv - 1) : 0;
+    int in = gt + min(eq, take);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = (wv * R + r) * 64 + lane;
+        const uint64_t e = __ballot(on[r] && key[r] == thr);
+        const bool chosen = sure[r] || (on[r] && (key[r] > thr || (key[r] == thr &&
+                                                                   eq + __popcll(e & below) < take)));
+        const uint64_t b = __ballot(chosen);
+        const int place = in + __popcll(b & below);
+        if (i < n) out(i, r, chosen ? place : i - place, chosen);
+        eq += __popcll(e);
+        in += __popcll(b);
+    }
+}
+
+// k of n keys (0 <= k <= n), those of the first and last indices for certain.  key(i, r) requests the
+// key of index i < n, the thread's r-th (of no keys: -1); abort: thread 0's reading decides for the block, which
+// returns false with nothing done.
+template <int NT, int R, typename F, typename O>
+__device__ __forceinline__ bool pick_keys(F key, int n, int k, int first, int last, int abort, O out) {
+    __shared__ int s_abort;
+    const int t = threadIdx.x;
+    uint32_t kr[R], thr = 0xFFFFFFFFu;  // (no key of a float)
+    bool on[R], sure[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = ((t >> 6) * R + r) * 64 + (t & 63);
+        sure[r] = i < n && (i < first || i >= n - last || k == n);
+        on[r] = i < n && !sure[r];
+        kr[r] = key(min(i, n - 1), r);
+    }
+    if (t == 0) s_abort = abort;
+    __syncthreads();
+    if (s_abort) return false;
+    int take = 0;
+    const int left = k == n ? 0 : k - first - last;  // (first + last <= k < n: they do not overlap)
+    if (left > 0) kth_of<NT, R>(kr, on, left, thr, take);
+    split_keys<NT, R>(kr, on, sure, n, thr, take, out);
+    return true;
+}
+
+// One block a row and head: scores formed in LDS, then the n_sel greatest, for up to CHOOSE_MAX blocks
+// (its 256 bytes a block come through one CU: 500 of them %A against %B us in two launches).
+#define CHOOSE_MAX 1024
+#ifndef CHOOSE_N
+#define CHOOSE_N 1024
+#endif
+__global__ __launch_bounds__(1024) void k_kv8_choose(Kv8SelectArgs a) {
+    __shared__ float s_sc[CHOOSE_MAX];
+    __shared__ __align__(16) i4v s_q[4][4][64];
+    __shared__ float s_sq[4][16];
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15, lq = lane >> 4;
+    const int g = blockIdx.x, row = blockIdx.y, groups = (a.G + 15) / 16;
+    const int ab = a.abort ? *a.abort : 0;
+    constexpr int X = CHOOSE_MAX / 256;
+    int pg[X];
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+        const int idx = 16 * (wv + 16 * x) + ln;
+        pg[x] = idx < a.n ? page_of(a.p, g, idx) : -1;
+    }
+    i4v hi[X][2], lo[X][2];
+    float ksl[X];
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+        if (16 * (wv + 16 * x) >= a.n) break;  // uniform
+        load_bounds(a.p, pg[x], hi[x], lo[x]);
+        ksl[x] = a.p.ks[max(pg[x], 0)];
+    }
+    if (wv < groups) {  // 16 heads a wave; a head past the group's last takes that one again
+        const int head = min(16 * wv + ln, a.G - 1);
+        i4v up[2], dn[2];
+        const float sq =
+            query_codes(a.q + (size_t)row * a.ldq + (size_t)(g * a.G + head) * HD + 16 * lq, up, dn);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            s_q[wv][j][lane] = up[j];
+            s_q[wv][2 + j][lane] = dn[j];
+        }
+        if (lq == 0) s_sq[wv][ln] = sq;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+        const int b0 = 16 * (wv + 16 * x);
+        if (b0 >= a.n) break;
+        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ks[4];
+        bool have[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            ks[k] = __shfl(ksl[x], 4 * lq + k, MJ_WAVE);
+            have[k] = __shfl(pg[x], 4 * lq + k, MJ_WAVE) >= 0;
+        }
+        for (int h = 0; h < groups; ++h) {
+            const i4v up[2] = {s_q[h][0][lane], s_q[h][1][lane]};
+            const i4v dn[2] = {s_q[h][2][lane], s_q[h][3][lane]};
+            const i4v u = bound_sums(hi[x], lo[x], up, dn);
+            const float sq = s_sq[h][ln];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float sc = (float)u[k] * ks[k] * sq;
+                best[k] = have[k] && sc > best[k] ? sc : best[k];  // (not a NaN)
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            best[k] = max16(best[k]);
+            if (ln == 0) s_sc[b0 + 4 * lq + k] = best[k];
+        }
+    }
+    __syncthreads();
+    int32_t* sel = a.sel + ((size_t)row * a.p.nKV + g) * a.n_sel;
+    const int k = min(a.n_sel, a.n);
+    if (!pick_keys<1024, 1>([&](int i, int) { return order_key(s_sc[max(i, 0)]); }, a.n, k, a.first,
+                            a.last, ab, [&](int i, int, int place, bool in) {
+                                if (in) sel[place] = i;
+                            }))
+        return;
+    for (int i = k + t; i < a.n_sel; i += 1024) sel[i] = -1;
+}
+
+// The same over keys in memory, any number of them: the k greatest of n keys (0 < k <= n), the lower index first among equal ones: the threshold key
 // and how many of the keys equal to it belong to them.  Radix selection, eight bits a round from the
 // top; whole block of NT threads, the same in every thread.
 template <int NT, typename F>
@@ -442,18 +738,26 @@ __device__ __forceinline__ void split_by_key(F key, int n, uint32_t thr, int tak
     }
 }
 
-// One block a row and head: the n_sel greatest scores, the first and last blocks above all others.
-template <int NT>
+// One block a row and head: the n_sel greatest scores; R keys a thread in registers, or R = 0: in
+// memory.
+template <int NT, int R>
 __global__ __launch_bounds__(NT) void k_kv8_topk(Kv8SelectArgs a) {
     const size_t rg = blockIdx.x;
-    if (block_aborted(a.abort)) return;
     const float* s = a.scores + rg * a.n;
     int32_t* sel = a.sel + rg * a.n_sel;
-    auto key = [&](int i) -> uint32_t {
-        return i < a.first || i >= a.n - a.last ? 0xFFFFFFFFu : order_key(s[i]);
-    };
     const int k = min(a.n_sel, a.n);
-    if (k > 0) {
+    if constexpr (R > 0) {
+        const int ab = a.abort ? *a.abort : 0;
+        if (!pick_keys<NT, R>([&](int i, int) { return order_key(s[i]); }, a.n, k, a.first, a.last, ab,
+                              [&](int i, int, int place, bool in) {
+                                  if (in) sel[place] = i;
+                              }))
+            return;
+    } else {
+        if (block_aborted(a.abort)) return;
+        auto key = [&](int i) -> uint32_t {
+            return i < a.first || i >= a.n - a.last ? 0xFFFFFFFFu : order_key(s[i]);
+        };
         uint32_t thr;
         int take;
         kth_key<NT>(key, a.n, k, thr, take);
@@ -465,47 +769,71 @@ __global__ __launch_bounds__(NT) void k_kv8_topk(Kv8SelectArgs a) {
 }
 
 hipError_t launch_kv8_select(const Kv8SelectArgs& a, hipStream_t st) {
-    if (a.n > 0) {
-        int P = 1;
-        while (P < a.G && P < 16) P *= 2;
-        const int rpt = 16 / P, tiles = (a.M + rpt - 1) / rpt, nb = (a.n + 63) / 64;
-        // the rows' tiles over further blocks while the launch is small
-        int z = 1;
-        while (z < tiles && nb * a.p.nKV * z < 512) z *= 2;
-        const int per = (tiles + z - 1) / z;
-        hipLaunchKernelGGL(k_kv8_score, dim3(nb, a.p.nKV, (tiles + per - 1) / per), dim3(256), 0, st, a,
-                           P, per);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    if (a.n <= CHOOSE_N) {
+        hipLaunchKernelGGL(k_kv8_choose, dim3(a.p.nKV, a.M), dim3(1024), 0, st, a);
+        return hipGetLastError();
     }
-    hipLaunchKernelGGL(k_kv8_topk<1024>, dim3(a.M * a.p.nKV), dim3(1024), 0, st, a);
+    int P = 1;
+    while (P < a.G && P < 16) P *= 2;
+    const int rpt = 16 / P, tiles = (a.M + rpt - 1) / rpt, nb = (a.n + 63) / 64;
+    // the rows' tiles over further blocks while the launch is small
+    int z = 1;
+    while (z < tiles && nb * a.p.nKV * z < 512) z *= 2;
+    const int per = (tiles + z - 1) / z;
+    hipLaunchKernelGGL(k_kv8_score, dim3(nb, a.p.nKV, (tiles + per - 1) / per), dim3(256), 0, st, a, P,
+                       per);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const dim3 flat(a.M * a.p.nKV);
+    if (a.n <= 1024) hipLaunchKernelGGL((k_kv8_topk<256, 4>), flat, dim3(256), 0, st, a);
+    else if (a.n <= 4096) hipLaunchKernelGGL((k_kv8_topk<1024, 4>), flat, dim3(1024), 0, st, a);
+    else if (a.n <= 16384) hipLaunchKernelGGL((k_kv8_topk<1024, 16>), flat, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((k_kv8_topk<1024, 0>), flat, dim3(1024), 0, st, a);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------- evict
 // One block a head: the `keep` greatest masses, the first and last blocks above all others; the
-// table and the masses split in two, each part in its old order.
-template <int NT>
+// table and the masses split in two, each part in its old order.  R as above.
+template <int NT, int R>
 __global__ __launch_bounds__(NT) void k_kv8_evict(Kv8Pool p, int n, int keep, int first, int last,
                                                   const float* __restrict__ mass_in,
                                                   int32_t* __restrict__ table_out,
                                                   float* __restrict__ mass_out, const int* abort) {
-    if (block_aborted(abort)) return;
     const size_t row = (size_t)blockIdx.x * p.stride;
     const float* m = mass_in + row;
-    auto key = [&](int i) -> uint32_t {
-        return i < first || i >= n - last ? 0xFFFFFFFFu : order_key(m[i]);
-    };
-    uint32_t thr = 0xFFFFFFFFu;  // keep 0: nothing stays
-    int take = 0;
-    if (keep > 0) kth_key<NT>(key, n, keep, thr, take);
-    split_by_key<NT>(key, n, thr, take, [&](int i, int place, bool in) {
-        const int at = in ? place : keep + place;
-        table_out[row + at] = p.table[row + i];
-        mass_out[row + at] = in ? m[i] : 0.0f;
-    });
+    const int32_t* tab = p.table + row;
+    if constexpr (R > 0) {
+        const int ab = abort ? *abort : 0;
+        float mr[R];
+        int32_t tr[R];
+        auto key = [&](int i, int r) {  // (of no blocks: unused)
+            mr[r] = m[max(i, 0)];
+            tr[r] = tab[max(i, 0)];
+            return order_key(mr[r]);
+        };
+        if (!pick_keys<NT, R>(key, n, keep, first, last, ab, [&](int i, int r, int place, bool in) {
+                const int at = in ? place : keep + place;
+                table_out[row + at] = tr[r];
+                mass_out[row + at] = in ? mr[r] : 0.0f;
+            }))
+            return;
+    } else {
+        if (block_aborted(abort)) return;
+        auto key = [&](int i) -> uint32_t {
+            return i < first || i >= n - last ? 0xFFFFFFFFu : order_key(m[i]);
+        };
+        uint32_t thr = 0xFFFFFFFFu;  // keep 0: nothing stays
+        int take = 0;
+        if (keep > 0) kth_key<NT>(key, n, keep, thr, take);
+        split_by_key<NT>(key, n, thr, take, [&](int i, int place, bool in) {
+            const int at = in ? place : keep + place;
+            table_out[row + at] = tab[i];
+            mass_out[row + at] = in ? m[i] : 0.0f;
+        });
+    }
     for (int i = n + threadIdx.x; i < p.stride; i += NT) {
-        table_out[row + i] = p.table[row + i];
+        table_out[row + i] = tab[i];
         mass_out[row + i] = 0.0f;
     }
 }
@@ -513,7 +841,14 @@ __global__ __launch_bounds__(NT) void k_kv8_evict(Kv8Pool p, int n, int keep, in
 hipError_t launch_kv8_evict(const Kv8Pool& p, int n, int keep, int first, int last,
                             const float* mass_in, int32_t* table_out, float* mass_out,
                             const int* abort, hipStream_t st) {
-    hipLaunchKernelGGL(k_kv8_evict<1024>, dim3(p.nKV), dim3(1024), 0, st, p, n, keep, first, last,
-                       mass_in, table_out, mass_out, abort);
+    auto go = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(p.nKV), dim3(threads), 0, st, p, n, keep, first, last, mass_in,
+                           table_out, mass_out, abort);
+    };
+    if (n <= 256) go(k_kv8_evict<256, 1>, 256);
+    else if (n <= 1024) go(k_kv8_evict<256, 4>, 256);
+    else if (n <= 4096) go(k_kv8_evict<1024, 4>, 1024);
+    else if (n <= 16384) go(k_kv8_evict<1024, 16>, 1024);
+    else go(k_kv8_evict<1024, 0>, 1024);
     return hipGetLastError();
 }

@@ -4,6 +4,7 @@
 // one page or 64 rows of the ring; a part is a run of units that one block takes; the parts of a row
 // and head are joined by k_kv8_combine.  Scores are kept in log2 units (scale * log2 e).
 #include <algorithm>
+#include <type_traits>
 
 #include "mj_device.h"
 #include "mj_kv8.h"
@@ -55,14 +56,14 @@ __device__ __forceinline__ float lane_of(float v, int i) {  // lane i's value (i
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
 }
 
-__device__ __forceinline__ int unit_page(const Kv8AttnArgs& a, int g, int row, int u) {
-    int i = u;
-    if (a.sel) {
-        i = a.sel[((size_t)row * a.p.nKV + g) * a.n_sel + u];
-        if ((unsigned)i >= (unsigned)a.n) return -1;
-    }
+__device__ __forceinline__ int page_of_list(const Kv8AttnArgs& a, int g, int i) {
     const int pg = a.p.table[(size_t)g * a.p.stride + i];
     return (unsigned)pg < (unsigned)a.p.n_pages ? pg : -1;
+}
+__device__ __forceinline__ int unit_page(const Kv8AttnArgs& a, int g, int row, int u) {
+    if (!a.sel) return page_of_list(a, g, u);
+    const int i = a.sel[((size_t)row * a.p.nKV + g) * a.n_sel + u];
+    return (unsigned)i < (unsigned)a.n ? page_of_list(a, g, i) : -1;
 }
 
 // The state of one tile of 16 query vectors.  Lane (ln, lq): query vector ln's maximum and sum (lq's
@@ -103,28 +104,40 @@ __device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
 // put them below fp16's normal range where they still count in the sum).  lu: the unit's sum of
 // exp2(s - m), this lane's share.
 #define SLACK 6.0f
-__device__ __forceinline__ void softmax_unit(Tile& T, f4 S[4], Scales u, u4v pa[2], float& lu) {
-    const int lq = (threadIdx.x & 63) >> 4;
-    float m = -INFINITY;
+// The reference moved, for T tiles at once (one branch; the weights of one tile can then be formed
+// under the products of another).
+template <int T>
+__device__ __forceinline__ void move_ref(Tile* tl, const f4 (*S)[4], Scales u) {
+    float m[T];
+    bool moved = false;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        m = fmaxf(fmaxf(m, S[kt][0]), S[kt][1]);
-        m = fmaxf(fmaxf(m, S[kt][2]), S[kt][3]);
+    for (int i = 0; i < T; ++i) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            x = fmaxf(fmaxf(x, S[i][kt][0]), S[i][kt][1]);
+            x = fmaxf(fmaxf(x, S[i][kt][2]), S[i][kt][3]);
+        }
+        m[i] = fmaf(x4_max(x), u.ksc, u.lv);
+        moved |= m[i] > tl[i].m + SLACK;
     }
-    m = fmaf(x4_max(m), u.ksc, u.lv);
-    const bool moved = m > T.m + SLACK;
-    if (__any(moved)) {
-        const float mn = fmaxf(T.m, m);
-        const float alpha = T.m == mn ? 1.0f : __builtin_amdgcn_exp2f(T.m - mn);  // (both may be -inf)
-        T.m = mn;
-        T.l *= alpha;
+    if (!__any(moved)) return;
+    const int lq = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        const float mn = fmaxf(tl[i].m, m[i]);
+        const float alpha = tl[i].m == mn ? 1.0f : __builtin_amdgcn_exp2f(tl[i].m - mn);  // (both may be -inf)
+        tl[i].m = mn;
+        tl[i].l *= alpha;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float al = __shfl(alpha, 4 * lq + r, MJ_WAVE);
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) T.o[dt][r] *= al;
+            for (int dt = 0; dt < 8; ++dt) tl[i].o[dt][r] *= al;
         }
     }
+}
+__device__ __forceinline__ void weights(Tile& T, const f4 S[4], Scales u, u4v pa[2], float& lu) {
     // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
     const float c = u.lv - (T.m == -INFINITY ? 0.0f : T.m);
     lu = 0.0f;
@@ -177,19 +190,15 @@ __device__ __forceinline__ u4v finite8(u4v v, bool& bad) {
     return v;
 }
 
-// Query vectors tv + ln of KV head g (vector r * G + j: head j of the group, row r) as the B operand:
-// operand s holds dims 64 (s / 2) + 16 lq + 8 (s % 2) + 0 .. 7, as the K operands do.
-__device__ __forceinline__ void load_q(const Kv8AttnArgs& a, int g, int v, bool on, u4v q[4],
-                                       uint64_t& anc) {
+// Query vector v of KV head g (head j of the group, row r: v = r * G + j) as the B operand: operand s
+// holds dims 64 (s / 2) + 16 lq + 8 (s % 2) + 0 .. 7, as the K operands do.  Lanes without a vector
+// (on false) take the head's first, unused.
+__device__ __forceinline__ void load_q(const Kv8AttnArgs& a, int g, int v, bool on, u4v q[4]) {
     const int lq = (threadIdx.x & 63) >> 4;
-    const int r = on ? v / a.G : 0, h = on ? g * a.G + v - r * a.G : 0;
+    const int r = on ? v / a.G : 0, h = on ? g * a.G + v - r * a.G : g * a.G;
     const uint16_t* qp = a.q + (size_t)r * a.ldq + (size_t)h * HD;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-        q[s] = *(const u4v*)(qp + 64 * (s >> 1) + 16 * lq + 8 * (s & 1));
-        if (!on) q[s] = (u4v){0u, 0u, 0u, 0u};
-    }
-    anc = on ? a.anc[r] : 0;
+    for (int s = 0; s < 4; ++s) q[s] = *(const u4v*)(qp + 64 * (s >> 1) + 16 * lq + 8 * (s & 1));
 }
 
 // 64 rows of the ring, base .. base + 63 of the call's open rows, as the operands of a unit in LDS: K
@@ -248,8 +257,9 @@ __device__ __forceinline__ void stage_ring(const Kv8AttnArgs& a, int g, int base
     }
 }
 
-// The rows of a ring unit that a vector with ancestor mask anc attends.
-__device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, uint64_t anc, bool on) {
+// The rows of a ring unit that vector v attends.
+__device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, int v, bool on) {
+    const uint64_t anc = a.anc[on ? v / a.G : 0];
     uint64_t committed = 0;
     if (a.R > base) committed = a.R - base >= 64 ? ~0ull : (1ull << (a.R - base)) - 1;
     const int d0 = base - a.R;  // own row of the unit's first token
@@ -257,60 +267,31 @@ __device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, ui
     return on ? committed | own : 0;
 }
 
-// T tiles against one unit staged in LDS; each operand is read once for all of them.  All K operands
-// are requested before the first product and all V operands before the softmax: left to itself the
-// compiler waits for each read in turn, some 30 LDS latencies a unit (64 rows at 65000 tokens: 61 ->
-// %s us).
-template <int T, bool RING>
-__device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u4v* Kf, const u4v* Vf,
-                                            int lane, Scales u, const uint64_t* ok,
-                                            float2* const* rec) {
-    const int ln = lane & 15, lq = lane >> 4;
-    f4 S[T][4];
-    {
-        u4v k[16];
+// A tile against a ring unit staged in LDS; ok: the rows that vector ln attends.
+__device__ __forceinline__ void ring_unit(Tile& tl, const u4v q[4], const u4v* Kf, const u4v* Vf,
+                                          int lane, uint64_t ok) {
+    const int lq = lane >> 4;
+    f4 S[1][4];
 #pragma unroll
-        for (int f = 0; f < 16; ++f) k[f] = Kf[f * 64 + lane];
-        __builtin_amdgcn_sched_barrier(0);
+    for (int kt = 0; kt < 4; ++kt) {
+        S[0][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < T; ++i)
+        for (int s = 0; s < 4; ++s)
+            S[0][kt] = mfma16x16x32(as_h8(Kf[(4 * kt + s) * 64 + lane]), as_h8(q[s]), S[0][kt]);
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < T; ++i)
-                    S[i][kt] = mfma16x16x32(as_h8(k[4 * kt + s]), as_h8(q[i][s]), S[i][kt]);
+        for (int r = 0; r < 4; ++r)
+            S[0][kt][r] = (ok >> (16 * kt + 4 * lq + r)) & 1 ? S[0][kt][r] : -INFINITY;
     }
-    u4v v[16];
+    const Scales u{SC2, 0.0f, 1.0f};
+    u4v pa[2];
+    float lu;
+    move_ref<1>(&tl, S, u);
+    weights(tl, S[0], u, pa, lu);
 #pragma unroll
-    for (int f = 0; f < 16; ++f) v[f] = Vf[f * 64 + lane];
-    __builtin_amdgcn_sched_barrier(0);
-    u4v pa[T][2];
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < T; ++i) {
-        if constexpr (RING)
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    S[i][kt][r] = (ok[i] >> (16 * kt + 4 * lq + r)) & 1 ? S[i][kt][r] : -INFINITY;
-        float lu;
-        softmax_unit(tl[i], S[i], u, pa[i], lu);
-        if (!RING && rec && rec[i]) {
-            lu = x4_sum(lu);
-            if (lq == 0) *rec[i] = make_float2(tl[i].m, lu);
-        }
-    }
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-        for (int i = 0; i < T; ++i) {
-            tl[i].o[dt] = mfma16x16x32(as_h8(pa[i][0]), as_h8(v[2 * dt]), tl[i].o[dt]);
-            tl[i].o[dt] = mfma16x16x32(as_h8(pa[i][1]), as_h8(v[2 * dt + 1]), tl[i].o[dt]);
-        }
+        for (int dt = 0; dt < 8; ++dt)
+            tl.o[dt] = mfma16x16x32(as_h8(pa[j]), as_h8(Vf[(2 * dt + j) * 64 + lane]), tl.o[dt]);
 }
 
 __device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g, int tv, int vend,
@@ -328,65 +309,116 @@ __device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g
         }
 }
 
+// The query vectors v0 .. vend - 1 of a block of `per` at most, column blockIdx.y; with lists of their
+// own, of one row.
+__device__ __forceinline__ void block_vectors(const Kv8AttnArgs& a, int per, int& row, int& v0,
+                                              int& vend) {
+    const int cols = a.sel ? (a.G + per - 1) / per : 1;
+    row = a.sel ? blockIdx.y / cols : 0;
+    v0 = a.sel ? row * a.G + per * (blockIdx.y % cols) : per * (int)blockIdx.y;
+    vend = min(a.sel ? row * a.G + a.G : a.M * a.G, v0 + per);
+}
+
 // One ring unit (rows base .. of the call's open ones) as a part of its own: the block of NW waves
 // stages it and takes the query vectors v0 .. vend - 1 a tile a wave at a time.  lds: 32 KB.
 template <int NW>
 __device__ __forceinline__ void ring_part(const Kv8AttnArgs& a, int part, int g, int base, int v0,
-                                          int vend, u4v* lds, uint32_t* s_bad, const int* s_abort) {
+                                          int vend, u4v* lds, uint32_t* s_bad, int* s_abort) {
     const int t = threadIdx.x, lane = t & 63, ln = lane & 15, C = (int)a.ring.C;
+    const int ab = a.abort ? *a.abort : 0;  // thread 0's reading decides for the block
     if (t < 2) s_bad[t] = 0;
     __syncthreads();
-    if (*s_abort) return;
     u4v* Kf = lds;
     u4v* Vf = Kf + 1024;
     stage_ring<64 * NW>(a, g, base, Kf, Vf, s_bad);
+    if (t == 0) *s_abort = ab;
     __syncthreads();
+    if (*s_abort) return;
     const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
     for (int tv = v0 + 16 * (t >> 6); tv < vend; tv += 16 * NW) {
-        u4v q[1][4];
-        uint64_t anc;
-        load_q(a, g, tv + ln, tv + ln < vend, q[0], anc);
-        Tile tl[1];
-        tl[0].clear();
-        const uint64_t ok = ring_mask(a, base, anc, tv + ln < vend);
-        staged_unit<1, true>(tl, q, Kf, Vf, lane, Scales{SC2, 0.0f, 1.0f}, &ok, nullptr);
+        u4v q[4];
+        load_q(a, g, tv + ln, tv + ln < vend, q);
+        Tile tl;
+        tl.clear();
+        const uint64_t ok = ring_mask(a, base, tv + ln, tv + ln < vend);
+        ring_unit(tl, q, Kf, Vf, lane, ok);
         if (bad) {
             int sb = a.slot0 + base;
             sb -= sb >= C ? C : 0;
-            add_bad_rows(tl[0], lane, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
+            add_bad_rows(tl, lane, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
         }
-        write_part(a, part, g, tv, vend, tl[0]);
+        write_part(a, part, g, tv, vend, tl);
     }
 }
 
-// Many rows: a block of NW waves takes a run of pages of KV head blockIdx.z for NW T tiles of query
-// vectors, T a wave.  A page is turned to halves once, by the whole block, and read from LDS by its
-// waves; two pages are in LDS and one in registers on its way, one barrier a page.  The first blocks take a
-// ring unit each.
-template <int T, int NW>
-__global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
+// A tile's products with a unit in LDS: all K operands are requested before the first product and all V
+// operands before the softmax (left to itself the compiler waits for each read in turn).
+template <int T>
+__device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u4v* Kf, const u4v* Vf,
+                                            int lane, Scales u, float2* const* rec) {
+    f4 S[T][4];
+    {
+        u4v k[16];
+#pragma unroll
+        for (int f = 0; f < 16; ++f) k[f] = Kf[f * 64 + lane];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int i = 0; i < T; ++i)
+                    S[i][kt] = mfma16x16x32(as_h8(k[4 * kt + s]), as_h8(q[i][s]), S[i][kt]);
+    }
+    u4v v[16];
+#pragma unroll
+    for (int f = 0; f < 16; ++f) v[f] = Vf[f * 64 + lane];
+    __builtin_amdgcn_sched_barrier(0);
+    move_ref<T>(tl, S, u);
+    u4v pa[T][2];
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        float lu;
+        weights(tl[i], S[i], u, pa[i], lu);
+        if (rec[i]) {
+            lu = x4_sum(lu);
+            if (lane < 16) *rec[i] = make_float2(tl[i].m, lu);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+                tl[i].o[dt] = mfma16x16x32(as_h8(pa[i][j]), as_h8(v[2 * dt + j]), tl[i].o[dt]);
+}
+
+// Pages shared: a block of NW waves takes a run of pages for NW T tiles of query vectors, T a wave.  A
+// page is turned to halves once, by the whole block, and read from LDS by its waves; two pages are in
+// LDS and one in registers on its way, one barrier a page.  The first blocks take a ring unit each;
+// rows with lists of their own (a.sel) as below.
+template <int T, int NW, bool MASS>
+__global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NR = 512 / NT;
     extern __shared__ __align__(16) u4v lds[];  // two pages: K operands, V operands
     __shared__ int s_abort;
     __shared__ uint32_t s_bad[2];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15;
     const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
-    const int v0 = (int)blockIdx.y * 16 * NW * T, vend = min(nv, v0 + 16 * NW * T);
-    const int ab = a.abort ? *a.abort : 0;
-    if (t == 0) s_abort = ab;
+    int row, v0, vend;
+    block_vectors(a, 16 * NW * T, row, v0, vend);
     if (part < a.ring_units) {
         ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
         return;
     }
+    const int ab = a.abort ? *a.abort : 0;
     Tile tl[T];
     u4v q[T][4];
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-        const int v = v0 + 16 * (wv * T + i) + ln;
-        uint64_t anc;
-        load_q(a, g, v, v < vend, q[i], anc);
-        tl[i].clear();
-    }
     const bool idle = v0 + 16 * wv * T >= vend;  // the wave has no vector: it stages only
     const int u0 = (part - a.ring_units) * a.upp, u1 = min(u0 + a.upp, a.n_list);
     u4v kr[NR], vr[NR];
@@ -409,12 +441,16 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
             codes16(vr[c], Vf[(2 * f) * 64 + lane], Vf[(2 * f + 1) * 64 + lane]);
         }
     };
-    // 64 pages' numbers and scales at a time, one a lane (a page at a time they are two dependent
-    // round trips before its request goes out)
     for (int ub = u0; ub < u1; ub += 64) {
-        const int pl = ub + lane < u1 ? unit_page(a, g, 0, ub + lane) : -1;
-        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
-        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
+        const int pl = ub + lane < u1 ? unit_page(a, g, row, ub + lane) : -1;
+        if (ub == u0) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                const int v = v0 + 16 * (wv * T + i) + ln;
+                load_q(a, g, v, v < vend, q[i]);
+                tl[i].clear();
+            }
+        }
         uint64_t todo = __ballot(pl >= 0);  // the same in every wave
         int cur = todo ? __builtin_ctzll(todo) : -1, nxt = -1, b = 0;
         if (cur >= 0) {
@@ -422,17 +458,20 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
             todo &= todo - 1;
             nxt = todo ? __builtin_ctzll(todo) : -1;
         }
-        __syncthreads();  // (the last batch's pages are done with)
-        if (s_abort) return;
+        const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
+        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
+        if (t == 0) s_abort = ab;
+        if (ub != u0) __syncthreads();  // the batch before is done with
         if (cur >= 0) stage(0);
         if (nxt >= 0) request(__builtin_amdgcn_readlane(pl, nxt));
-        while (cur >= 0) {
+        for (bool first = true; cur >= 0; first = false) {
             todo &= todo - 1;
             const int n2 = todo ? __builtin_ctzll(todo) : -1;
             __syncthreads();  // page cur is staged; everyone is done with the one before
+            if (first && s_abort) return;
             if (nxt >= 0) {
                 stage(b ^ 1);
-                request(__builtin_amdgcn_readlane(pl, n2 >= 0 ? n2 : nxt));
+                if (n2 >= 0) request(__builtin_amdgcn_readlane(pl, n2));
             }
             if (!idle) {
                 const u4v* Kf = lds + b * 2048;
@@ -440,13 +479,12 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < T; ++i) {
                     const int v = v0 + 16 * (wv * T + i) + ln;
-                    rec[i] = !a.rec ? nullptr
+                    rec[i] = !MASS      ? nullptr
                              : v < vend ? a.rec + ((size_t)g * a.n + ub + cur) * nv + v
                                         : a.rec + (size_t)a.p.nKV * a.n * nv + ln;  // a spare row
                 }
-                staged_unit<T, false>(tl, q, Kf, Kf + 1024, lane,
-                                      Scales{lane_of(ksl, cur), lane_of(lvl, cur), lane_of(ill, cur)},
-                                      nullptr, rec);
+                staged_unit<T>(tl, q, Kf, Kf + 1024, lane,
+                               Scales{lane_of(ksl, cur), lane_of(lvl, cur), lane_of(ill, cur)}, rec);
             }
             cur = nxt;
             nxt = n2;
@@ -460,35 +498,28 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_many(Kv8AttnArgs a) {
     }
 }
 
-// Few rows: T tiles of query vectors, and every wave takes pages of its own, straight into registers:
-// a page's bytes lie in the order of the operands, so a lane's 16 bytes are two of them.  A wave's
-// next K goes out behind its scores, its next V behind its output product; the page numbers and
-// scales of 64 pages come with one request a lane each.  The block's NW waves are joined in LDS.
-// The first blocks take a ring unit each.  Where rows list their own blocks (a.sel),
-// blockIdx.y is a row and a share of its heads.
-template <int T, int NW>
-__global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
-    constexpr int NT = 64 * NW, RS = HD + 4;
+// A wave's own pages: T tiles of query vectors a block, the same for all of its NW waves, and every
+// wave takes pages of its own, straight into registers: a page's bytes lie in the order of the operands, so a lane's 16 bytes
+// are two of them, turned to halves once for all T tiles.  A wave's next K goes out behind its scores,
+// its next V behind its output products; the page numbers and scales of 64 pages come with one
+// request a lane each.  The waves are joined in LDS.  The first blocks take a ring unit each.  Where
+// rows list their own blocks (a.sel), blockIdx.y is a row and a share of its heads.
+template <int T, int NW, bool MASS>
+__global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
+    constexpr int NT = 64 * NW;
     extern __shared__ __align__(16) u4v lds[];
     __shared__ int s_abort;
     __shared__ uint32_t s_bad[2];
-    __shared__ float s_m[NW][16], s_l[NW][16];
+    __shared__ float s_m[T][NW][16], s_l[NW][16];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15, lq = lane >> 4;
     const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
-    int row = 0, v0 = (int)blockIdx.y * 16 * T, vend = nv;
-    if (a.sel) {
-        const int cols = (a.G + 16 * T - 1) / (16 * T);
-        row = blockIdx.y / cols;
-        v0 = row * a.G + 16 * T * (blockIdx.y % cols);
-        vend = row * a.G + a.G;
-    }
-    const int ab = a.abort ? *a.abort : 0;
-    if (t == 0) s_abort = ab;
+    int row, v0, vend;
+    block_vectors(a, 16 * T, row, v0, vend);
     if (part < a.ring_units) {
-        ring_part<NW>(a, part, g, 64 * part, v0, min(vend, v0 + 16 * T), lds, s_bad,
-                      &s_abort);
+        ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
         return;
     }
+    const int ab = a.abort ? *a.abort : 0;
     Tile tl[T];
     u4v q[T][4];
     const int up = (part - a.ring_units) * a.upp;
@@ -496,6 +527,13 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
     for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NW) {
         const int ul = ub + NW * lane;  // lane's unit
         const int pl = ul < u1 ? unit_page(a, g, row, ul) : -1;
+        if (ub == u0) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                load_q(a, g, v0 + 16 * i + ln, v0 + 16 * i + ln < vend, q[i]);
+                tl[i].clear();
+            }
+        }
         uint64_t todo = __ballot(pl >= 0);
         u4v kr[8], vr[8];
         auto request_k = [&](int i) {
@@ -515,18 +553,7 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
         }
         const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
         const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
-        if (ub == u0) {
-#pragma unroll
-            for (int i = 0; i < T; ++i) {
-                uint64_t anc;
-                load_q(a, g, v0 + 16 * i + ln, v0 + 16 * i + ln < vend, q[i], anc);
-                tl[i].clear();
-            }
-        }
-        while (todo) {
-            const int i = i0;
-            todo &= todo - 1;
-            i0 = todo ? __builtin_ctzll(todo) : i;  // the last page is requested again, unused
+        auto step = [&](int i, int nx, auto more) {  // page i; page nx requested behind it
             const Scales sc{lane_of(ksl, i), lane_of(lvl, i), lane_of(ill, i)};
             f4 S[T][4];
 #pragma unroll
@@ -538,19 +565,21 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
                     u4v k0, k1;
                     codes16(kr[2 * kt + j], k0, k1);
 #pragma unroll
-                    for (int x = 0; x < T; ++x) {
+                    for (int x = 0; x < T; ++x)
                         S[x][kt] = mfma16x16x32(as_h8(k0), as_h8(q[x][2 * j]), S[x][kt]);
+#pragma unroll
+                    for (int x = 0; x < T; ++x)
                         S[x][kt] = mfma16x16x32(as_h8(k1), as_h8(q[x][2 * j + 1]), S[x][kt]);
-                    }
                 }
             }
-            request_k(i0);
+            if constexpr (more.value) request_k(nx);
+            move_ref<T>(tl, S, sc);
             u4v pa[T][2];
 #pragma unroll
             for (int x = 0; x < T; ++x) {
                 float lu;
-                softmax_unit(tl[x], S[x], sc, pa[x], lu);
-                if (a.rec) {
+                weights(tl[x], S[x], sc, pa[x], lu);
+                if constexpr (MASS) {
                     const int v = v0 + 16 * x + ln;
                     lu = x4_sum(lu);
                     if (lq == 0 && v < vend)
@@ -562,65 +591,158 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_few(Kv8AttnArgs a) {
                 u4v w0, w1;
                 codes16(vr[dt], w0, w1);
 #pragma unroll
-                for (int x = 0; x < T; ++x) {
+                for (int x = 0; x < T; ++x)
                     tl[x].o[dt] = mfma16x16x32(as_h8(pa[x][0]), as_h8(w0), tl[x].o[dt]);
+#pragma unroll
+                for (int x = 0; x < T; ++x)
                     tl[x].o[dt] = mfma16x16x32(as_h8(pa[x][1]), as_h8(w1), tl[x].o[dt]);
-                }
             }
-            request_v(i0);
+            if constexpr (more.value) request_v(nx);
+        };
+        // the last page apart: a request that is not used would be waited for at the join
+        while (todo) {
+            const int i = i0;
+            todo &= todo - 1;
+            if (!todo) break;
+            i0 = __builtin_ctzll(todo);
+            step(i, i0, std::true_type{});
         }
+        if (i0 >= 0) step(i0, 0, std::false_type{});
     }
-    // ---- the waves joined, a tile at a time: all to the block's maximum, then summed in wave order
-    float* so = (float*)lds;  // [NW][16][RS]
+    // ---- the waves joined, a tile at a time: each scales its outputs to the block's maximum and puts
+    // those of the tile's vectors side by side in LDS (a lane's four vectors of a dim in 16 bytes), then
+    // a thread adds up one dim of four vectors, wave by wave.  (Every thread weighing every wave's
+    // outputs read three times as much LDS: 1.7 us a tile.)
+    f4* so = (f4*)lds;  // [NW][4][128]: vectors 4 y .. + 3 of dim d
 #pragma unroll
+    for (int x = 0; x < T; ++x)
+        if (lq == 0) s_m[x][wv][ln] = tl[x].m;
+    if (t == 0) s_abort = ab;
+    __syncthreads();
+    if (s_abort) return;
+    auto put = [&](Tile& tt, int x, int rows) {
+        const float l = x4_sum(tt.l);
+        float m = s_m[x][0][ln];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[x][w][ln]);
+        const float f = __builtin_amdgcn_exp2f(tt.m - (m == -INFINITY ? 0.0f : m));
+        if (lq == 0) s_l[wv][ln] = l * f;
+        f4 fr;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * lq + r, MJ_WAVE);
+        if (4 * lq < rows)
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) {
+                f4 o = tt.o[dt];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] *= fr[r];
+                so[(wv * 4 + lq) * 128 + 16 * dt + ln] = o;
+            }
+    };
+#pragma unroll 1
     for (int x = 0; x < T; ++x) {
-        const int tv = v0 + 16 * x;
-        const float l = x4_sum(tl[x].l);
-        __syncthreads();
-        if (s_abort) return;
-        if (lq == 0) s_m[wv][ln] = tl[x].m;
-        __syncthreads();
-        float m = s_m[0][ln];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[w][ln]);
-        const float sc = __builtin_amdgcn_exp2f(tl[x].m - (m == -INFINITY ? 0.0f : m));
-        if (lq == 0) s_l[wv][ln] = l * sc;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float sr = __shfl(sc, 4 * lq + r, MJ_WAVE);
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt)
-                so[(wv * 16 + 4 * lq + r) * RS + 16 * dt + ln] = tl[x].o[dt][r] * sr;
-        }
+        const int tv = v0 + 16 * x, rows = min(vend - tv, 16);
+        if (rows <= 0) break;  // whole block
+        if (x) __syncthreads();
+        if (x == 0) put(tl[0], 0, rows);
+        if constexpr (T > 1)
+            if (x == 1) put(tl[1], 1, rows);
         __syncthreads();
         const size_t pb = ((size_t)part * a.p.nKV + g) * nv + tv;
-        if (wv == 0 && lq == 0 && tv + ln < vend) {
-            float ls = s_l[0][ln];
+        if (t < rows) {
+            float l = 0.0f, m = s_m[x][0][t];
 #pragma unroll
-            for (int w = 1; w < NW; ++w) ls += s_l[w][ln];
-            a.ml[pb + ln] = make_float2(m, ls);
+            for (int w = 0; w < NW; ++w) {
+                l += s_l[w][t];
+                m = fmaxf(m, s_m[x][w][t]);
+            }
+            a.ml[pb + t] = make_float2(m, l);
         }
-        for (int e = t; e < 16 * 32; e += NT) {
-            const int vec = e >> 5, d = 4 * (e & 31);
-            if (tv + vec >= vend) continue;
-            f4 o = *(const f4*)(so + vec * RS + d);
+        for (int e = t; e < 128 * ((rows + 3) / 4); e += NT) {
+            f4 o = so[e];
 #pragma unroll
             for (int w = 1; w < NW; ++w) {
-                const f4 y = *(const f4*)(so + (w * 16 + vec) * RS + d);
+                const f4 y = so[w * 512 + e];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[k] += y[k];
             }
-            *(f4*)(a.opart + (pb + vec) * HD + d) = o;
+            const int vec = 4 * (e >> 7), d = e & 127;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (vec + k < rows) a.opart[(pb + vec + k) * HD + d] = o[k];
         }
+    }
+}
+
+// mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax: a
+// 256-thread block takes MASS_B of a head's blocks, a wave one at a time.  The vectors' final maxima
+// and sums are formed again here from the parts' (a launch that waited for them took 4 us more).
+#define MASS_B 4
+__device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
+    __shared__ float2 s_stat[MJ_ROWS * 64], s_w[2][4][64];
+    __shared__ int s_stop;
+    const int t = threadIdx.x, lane = t & 63, nv = a.M * a.G, per = (a.n + MASS_B - 1) / MASS_B;
+    const int g = blk / per, i0 = (blk - g * per) * MASS_B;
+    const int ab = a.abort ? *a.abort : 0;
+    if (t == 0) s_stop = ab;
+    const size_t step = (size_t)a.p.nKV * nv;
+    const int wv = t >> 6;
+    for (int v0 = 0; v0 < nv; v0 += 64) {  // a lane a vector, a wave every fourth part
+        const float2* ml = a.ml + (size_t)g * nv + min(v0 + lane, nv - 1);
+        float m = -INFINITY, l = 0.0f;
+        for (int c0 = wv; c0 < a.parts; c0 += 64) {
+            float2 x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = ml[(size_t)min(c0 + 4 * j, a.parts - 1) * step];
+            float mn = m;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mn = fmaxf(mn, x[j].x);
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            l *= __builtin_amdgcn_exp2f(m - ref);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                l = c0 + 4 * j < a.parts ? fmaf(x[j].y, __builtin_amdgcn_exp2f(x[j].x - ref), l) : l;
+            m = mn;
+        }
+        s_w[v0 / 64 & 1][wv][lane] = make_float2(m, l);
+        __syncthreads();
+        if (wv == 0 && v0 + lane < nv) {
+            const float2* w = &s_w[v0 / 64 & 1][0][lane];
+            float mx = fmaxf(fmaxf(w[0].x, w[64].x), fmaxf(w[128].x, w[192].x));
+            mx = mx == -INFINITY ? 0.0f : mx;
+            float ls = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ls = fmaf(w[64 * k].y, __builtin_amdgcn_exp2f(w[64 * k].x - mx), ls);
+            s_stat[v0 + lane] = make_float2(mx, ls == 0.0f ? 0.0f : 1.0f / ls);
+        }
+    }
+    __syncthreads();
+    if (s_stop) return;
+    for (int i = i0 + (t >> 6); i < min(i0 + MASS_B, a.n); i += 4) {
+        const size_t at = (size_t)g * a.p.stride + i;
+        float s = 0.0f;
+        if (page_of_list(a, g, i) >= 0)
+            for (int v = lane; v < nv; v += 64) {
+                const float2 rc = a.rec[((size_t)g * a.n + i) * nv + v], st = s_stat[v];
+                s = fmaf(rc.y * st.y,
+                         __builtin_amdgcn_exp2f((rc.x == -INFINITY ? 0.0f : rc.x) - st.x), s);
+            }
+        s = wave_sum(s);
+        if (lane == 0) a.mass_out[at] = (a.mass_in ? a.mass_in[at] : 0.0f) + s;
     }
 }
 
 // One 256-thread block a row and head.  Eight groups of 32 lanes (a lane four dims) take every eighth
 // part, eight requested at a time, each to its own running maximum; the groups are then joined in
-// order.  A part that saw no key has maximum -inf and weight 0.
+// order.  A part that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.
+template <bool MASS>
 __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
     const int t = threadIdx.x, gr = t >> 5, d4 = t & 31;
     const int nQ = a.p.nKV * a.G, nv = a.M * a.G;
+    if (MASS && (int)blockIdx.x >= a.M * nQ) {
+        if constexpr (MASS) mass_blocks(a, blockIdx.x - a.M * nQ);
+        return;
+    }
     const int r = blockIdx.x / nQ, h = blockIdx.x % nQ, g = h / a.G, v = r * a.G + h % a.G;
     __shared__ f4 s_o[8][32];
     __shared__ float s_m[8], s_l[8];
@@ -682,7 +804,6 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
         }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key at all: zeros
-    if (t == 0 && a.stat) a.stat[at] = make_float2(ref, inv);
     u4v ov;
 #pragma unroll
     for (int j = 0; j < 4; ++j) ov[j] = pack2(f2h(y[2 * j] * inv), f2h(y[2 * j + 1] * inv));
@@ -693,34 +814,12 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
     }
 }
 
-// mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax, a wave
-// a block.
-__global__ __launch_bounds__(256) void k_kv8_mass(Kv8AttnArgs a) {
-    const int lane = threadIdx.x & 63, g = blockIdx.y, nv = a.M * a.G;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.n || aborted(a.abort)) return;
-    const size_t at = (size_t)g * a.p.stride + i;
-    const int pg = a.p.table[at];
-    float s = 0.0f;
-    if ((unsigned)pg < (unsigned)a.p.n_pages)
-        for (int v = lane; v < nv; v += 64) {
-            const float2 rc = a.rec[((size_t)g * a.n + i) * nv + v], st = a.stat[(size_t)g * nv + v];
-            s = fmaf(rc.y * st.y, __builtin_amdgcn_exp2f((rc.x == -INFINITY ? 0.0f : rc.x) - st.x), s);
-        }
-    s = wave_sum(s);
-    if (lane == 0) a.mass_out[at] = (a.mass_in ? a.mass_in[at] : 0.0f) + s;
-}
-
-// Shapes of the two kernels: few<T, 8> for up to FEW_TILES tiles and for listed blocks, else many.
-#define FEW_WAVES 8
-#ifndef FEW_TILES
-#define FEW_TILES 2
+#define NWAVES 8
+#ifndef SHARE_MAX
+#define SHARE_MAX (tiles == 1 ? 300 : 2500)
 #endif
-#ifndef MANY_WAVES
-#define MANY_WAVES 8
-#endif
-#ifndef MANY_T
-#define MANY_T 2
+#ifndef T2_MIN
+#define T2_MIN 1400
 #endif
 
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
@@ -728,14 +827,21 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
     const int nv = a.M * a.G;
     const int tiles = ((a.n_sel > 0 ? a.G : nv) + 15) / 16;  // that share their units
-    a.few = a.n_sel > 0 || tiles <= FEW_TILES;
-    a.tiles = a.few ? std::min(tiles, FEW_TILES) : MANY_T;  // a wave
-    const int per = a.few ? a.tiles : MANY_T * MANY_WAVES;
-    a.cols = (a.n_sel > 0 ? a.M : 1) * ((tiles + per - 1) / per);
+    const int rows = a.n_sel > 0 ? a.M : 1;
+    // Blocks for one page each: the whole block turns it to halves (one row at 2500 tokens %s us a
+    // launch, %s where a wave takes it alone); pages beyond that for one or two tiles: waves with
+    // pages of their own (one row at 131000 tokens 23 us, %s shared); for more tiles shared again (9
+    // rows at 32000 14.4, 17.3 with three tiles a wave), two tiles a wave past eight (64 rows at 65000
+    // 48 us, 60 with one; at 2500 17 and 13).
+    const int col1 = rows * ((tiles + NWAVES - 1) / NWAVES);
+    a.shared = tiles > 2 || (int64_t)a.n_list * col1 * a.p.nKV <= SHARE_MAX;
+    a.tiles = !a.shared ? tiles : tiles > NWAVES && (int64_t)a.n_list * a.p.nKV > T2_MIN ? 2 : 1;
+    const int per = a.shared ? a.tiles * NWAVES : a.tiles;
+    a.cols = rows * ((tiles + per - 1) / per);
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
     // chip holds would run alone at the end
     int parts = std::max(1, 256 / (a.cols * a.p.nKV) - a.ring_units);
-    parts = std::min(parts, a.few ? (a.n_list + FEW_WAVES - 1) / FEW_WAVES : a.n_list);
+    parts = std::min(parts, a.shared ? a.n_list : (a.n_list + NWAVES - 1) / NWAVES);
     a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
     a.parts = a.ring_units + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);
     size_t off = 0;
@@ -749,46 +855,40 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.opart = (float*)take(vecs * a.parts * HD * 4);
     a.ml = (float2*)take(vecs * a.parts * 8);
     a.rec = mass ? (float2*)take((vecs * a.n + 16) * 8) : nullptr;
-    a.stat = mass ? (float2*)take(vecs * 8) : nullptr;
     return off;
 }
 
-#define FEW_LDS (FEW_WAVES * 16 * (HD + 4) * 4)  // the waves' outputs side by side (a ring unit: 32 KB)
-#define MANY_LDS 65536                           // two units
+#define ATTN_LDS 65536  // two pages as halves; the waves' outputs side by side; a ring unit
 
-static hipError_t attn_attributes() {
-    static const hipError_t done = [] {
-        const int most = hipFuncAttributeMaxDynamicSharedMemorySize;
-        hipError_t e = hipSuccess;
-        const void* few[] = {(const void*)k_kv8_attn_few<1, FEW_WAVES>,
-                             (const void*)k_kv8_attn_few<2, FEW_WAVES>};
-        for (const void* k : few)
-            if (e == hipSuccess) e = hipFuncSetAttribute(k, (hipFuncAttribute)most, FEW_LDS);
-        if (e == hipSuccess)
-            e = hipFuncSetAttribute((const void*)k_kv8_attn_many<MANY_T, MANY_WAVES>,
-                                    (hipFuncAttribute)most, MANY_LDS);
-        return e;
-    }();
-    return done;
+template <typename K>
+static hipError_t launch_one(K kernel, const hipError_t& attr, const Kv8AttnArgs& a, hipStream_t st) {
+    if (attr != hipSuccess) return attr;
+    hipLaunchKernelGGL(kernel, dim3(a.parts, a.cols, a.p.nKV), dim3(64 * NWAVES), ATTN_LDS, st, a);
+    return hipGetLastError();
+}
+template <int T, bool MASS>
+static hipError_t launch_tiles(const Kv8AttnArgs& a, hipStream_t st) {
+    auto raise = [](const void* k) {
+        return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, ATTN_LDS);
+    };
+    static const hipError_t s = raise((const void*)k_kv8_attn_shared<T, NWAVES, MASS>);
+    static const hipError_t o = raise((const void*)k_kv8_attn_own<T, NWAVES, MASS>);
+    return a.shared ? launch_one(k_kv8_attn_shared<T, NWAVES, MASS>, s, a, st)
+                    : launch_one(k_kv8_attn_own<T, NWAVES, MASS>, o, a, st);
+}
+
+template <bool MASS>
+static hipError_t launch_attn_pass(const Kv8AttnArgs& a, hipStream_t st) {
+    const hipError_t e = a.tiles == 1 ? launch_tiles<1, MASS>(a, st) : launch_tiles<2, MASS>(a, st);
+    if (e != hipSuccess) return e;
+    // the join: a block a row and head, then (masses) one for every MASS_B blocks of a head
+    const int heads = a.M * a.p.nKV * a.G, masses = (a.n + MASS_B - 1) / MASS_B * a.p.nKV;
+    hipLaunchKernelGGL(k_kv8_combine<MASS>, dim3(heads + (MASS ? masses : 0)), dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t st) {
     if (a.M < 1 || a.M > MJ_ROWS || a.ring.C >= ((int64_t)1 << 30) || a.parts < 1)
         return hipErrorInvalidValue;
-    const dim3 grid(a.parts, a.cols, a.p.nKV);
-    hipError_t e = attn_attributes();
-    if (e != hipSuccess) return e;
-    auto go = [&](auto kernel, int waves, size_t lds) {
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), lds, st, a);
-        return hipGetLastError();
-    };
-    if (!a.few) e = go(k_kv8_attn_many<MANY_T, MANY_WAVES>, MANY_WAVES, MANY_LDS);
-    else if (a.tiles == 1) e = go(k_kv8_attn_few<1, FEW_WAVES>, FEW_WAVES, FEW_LDS);
-    else e = go(k_kv8_attn_few<2, FEW_WAVES>, FEW_WAVES, FEW_LDS);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_kv8_combine, dim3(a.M * a.p.nKV * a.G), dim3(256), 0, st, a);
-    e = hipGetLastError();
-    if (e != hipSuccess || !a.rec) return e;
-    hipLaunchKernelGGL(k_kv8_mass, dim3((a.n + 3) / 4, a.p.nKV), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return a.rec ? launch_attn_pass<true>(a, st) : launch_attn_pass<false>(a, st);
 }

@@ -74,14 +74,13 @@ struct Kv8AttnArgs {
     const float* mass_in;
     float* mass_out;
     // set by kv8_attn_plan: a part for every 64 rows of the ring (ring_units), then parts of upp
-    // listed blocks each; few: which kernel; tiles: of 16 query vectors, a wave; cols: block columns
+    // listed blocks each; shared: which kernel; tiles: of 16 query vectors, a wave; cols: block columns
     // (groups of tiles, rows with lists of their own)
     int n_list, upp, parts, ring_units, tiles, cols;
-    bool few;
+    bool shared;
     float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
     float2* ml;     // [parts][nKV][nv] {m, sum}
     float2* rec;    // [nKV][n][nv] {m, sum} of each block where masses are wanted
-    float2* stat;   // [nKV][nv] final {m, 1 / sum}
     const int* abort;
     uint64_t anc[MJ_ROWS];  // of pass row r: bit a set for its ancestors and itself
 };

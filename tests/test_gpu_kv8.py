@@ -474,3 +474,55 @@ def test_evict(ctx, nKV, n, keep, first, last, stride):
         want = torch.zeros(stride)
         want[:keep] = mass[g, kept].cpu()
         assert torch.equal(m1[g].cpu().nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
+
+
+@pytest.mark.parametrize("n", [1, 64, 1023, 1024, 1025, 2048, 2049, 4096, 4097, 16384, 16385])
+@pytest.mark.parametrize("pages,nQ", [(40, 4), (1000, 16), (300, 48)])
+def test_select_long_lists(ctx, n, pages, nQ):
+    """Lists of every length class; blocks listed again and again tie."""
+    import torch
+
+    from momij_amd.kv8 import Kv8Cache
+
+    rnd = gen(n + pages)
+    M, n_sel, first, last = 3, min(n, 57), 1, 0
+    cache = Kv8Cache(ctx, 1, max(n, pages))
+    hi = (rnd(pages, D) * 30 + 40).round().clamp(-127, 127)
+    lo = torch.minimum(hi, (rnd(pages, D) * 30 - 40).round().clamp(-127, 127))
+    cache.k_bounds[:pages] = torch.stack([hi, lo], 1).to(torch.int8)
+    cache.k_scale[:pages] = torch.exp(0.5 * rnd(pages)) * 0.01
+    at = torch.randint(0, pages, (n,), device="cuda", dtype=torch.int32)
+    cache.table[0, :n] = at
+    q = rnd(M, nQ * D).half()
+    sel = torch.empty((M, 1, n_sel), dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    ctx.kv8_select(cache, q, M, nQ, n, n_sel, first, last, sel)
+    ctx.sync()
+    sc = ref.scores(q.reshape(M, 1, nQ, D), hi[None].double(), lo[None].double(),
+                    cache.k_scale[None, :pages])[:, 0, at.long()].cpu()
+    for r in range(M):
+        assert sel[r, 0].tolist() == ref.choose(sc[r].tolist(), first, last, n_sel)
+
+
+@pytest.mark.parametrize("n", [1024, 1025, 4096, 4097, 16384, 16385])
+@pytest.mark.parametrize("kind", ["wide", "equal", "two", "near", "negative"])
+def test_evict_long_lists(ctx, n, kind):
+    import torch
+
+    from momij_amd.kv8 import Kv8Cache
+
+    rnd = gen(n)
+    cache = Kv8Cache(ctx, 2, n)
+    x = rnd(2, n)
+    mass = dict(wide=torch.exp(20 * x), equal=torch.full_like(x, 3.0), two=(x > 0.5).float(),
+                near=1.0 + x.abs() * 1e-6, negative=x * torch.exp(30 * rnd(2, n)))[kind]
+    for keep in (1, n // 3, n - 1):
+        table, m1 = torch.empty_like(cache.table), torch.empty_like(mass)
+        torch.cuda.synchronize()
+        ctx.kv8_evict(cache, n, keep, 0, 1, mass, table, m1)
+        ctx.sync()
+        for g in range(2):
+            kept = ref.choose(mass[g].tolist(), 0, 1, keep)
+            order = kept + sorted(set(range(n)) - set(kept))
+            assert table[g].tolist() == cache.table[g, order].tolist(), (keep, g)
+            assert torch.equal(m1[g, :keep], mass[g, kept]) and not m1[g, keep:].any()
