@@ -380,10 +380,10 @@ __global__ __launch_bounds__(256) void k_kv8_score(Kv8SelectArgs a, int P, int t
     const int g = blockIdx.y, b0 = blockIdx.x * 64 + 16 * (t >> 6);
     const int idx = b0 + ln, nQ = a.p.nKV * a.G;
     const int pg = idx < a.n ? page_of(a.p, g, idx) : -1;
-    if (aborted(a.abort)) return;
+    const int ab = a.abort ? *a.abort : 0;  // decides at the end, off the chain table -> bounds
     i4v hi[2], lo[2];
     load_bounds(a.p, pg, hi, lo);
-    const float ks_l = pg < 0 ? 0.0f : a.p.ks[pg];
+    const float ks_l = a.p.ks[max(pg, 0)];
     float ks[4];
     bool have[4];
 #pragma unroll
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256) void k_kv8_score(Kv8SelectArgs a, int P, int t
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             for (int o = 1; o < P; o <<= 1) best[k] = fmaxf(best[k], __shfl_xor(best[k], o, MJ_WAVE));
-        if (ln % P == 0 && row < a.M) {
+        if (ab == 0 && ln % P == 0 && row < a.M) {
             float* s = a.scores + ((size_t)row * a.p.nKV + g) * a.n;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -548,8 +548,8 @@ __device__ __forceinline__ void split_keys(const uint32_t key[R], const bool on[
 }
 
 // k of n keys (0 <= k <= n), those of the first and last indices for certain.  key(i, r) requests the
-// key of index i < n, the thread's r-th (of no keys: -1); abort: thread 0's reading decides for the block, which
-// returns false with nothing done.
+// key of index i < n, the thread's r-th (of no keys: -1); abort: thread 0's reading decides for the
+// block, which returns false with nothing done.
 template <int NT, int R, typename F, typename O>
 __device__ __forceinline__ bool pick_keys(F key, int n, int k, int first, int last, int abort, O out) {
     __shared__ int s_abort;
@@ -574,11 +574,9 @@ __device__ __forceinline__ bool pick_keys(F key, int n, int k, int first, int la
 }
 
 // One block a row and head: scores formed in LDS, then the n_sel greatest, for up to CHOOSE_MAX blocks
-// (its 256 bytes a block come through one CU: 500 of them %A against %B us in two launches).
+// (256 bytes a block come through one CU: 500 of them for 8 rows take 10.4 us, in two launches 6.2 and
+// 4.4 us and the gap between them; 2047 of one row 26 us, 15 in two).
 #define CHOOSE_MAX 1024
-#ifndef CHOOSE_N
-#define CHOOSE_N 1024
-#endif
 __global__ __launch_bounds__(1024) void k_kv8_choose(Kv8SelectArgs a) {
     __shared__ float s_sc[CHOOSE_MAX];
     __shared__ __align__(16) i4v s_q[4][4][64];
@@ -653,9 +651,8 @@ __global__ __launch_bounds__(1024) void k_kv8_choose(Kv8SelectArgs a) {
     for (int i = k + t; i < a.n_sel; i += 1024) sel[i] = -1;
 }
 
-// The same over keys in memory, any number of them: the k greatest of n keys (0 < k <= n), the lower index first among equal ones: the threshold key
-// and how many of the keys equal to it belong to them.  Radix selection, eight bits a round from the
-// top; whole block of NT threads, the same in every thread.
+// The same over keys in memory, any number of them (0 < k <= n), by radix selection, eight bits a round
+// from the top; whole block of NT threads, thr and take the same in every thread.
 template <int NT, typename F>
 __device__ __forceinline__ void kth_key(F key, int n, int k, uint32_t& thr, int& take) {
     __shared__ int hist[256];
@@ -769,7 +766,7 @@ __global__ __launch_bounds__(NT) void k_kv8_topk(Kv8SelectArgs a) {
 }
 
 hipError_t launch_kv8_select(const Kv8SelectArgs& a, hipStream_t st) {
-    if (a.n <= CHOOSE_N) {
+    if (a.n <= CHOOSE_MAX) {
         hipLaunchKernelGGL(k_kv8_choose, dim3(a.p.nKV, a.M), dim3(1024), 0, st, a);
         return hipGetLastError();
     }

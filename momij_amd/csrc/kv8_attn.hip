@@ -270,17 +270,19 @@ __device__ __forceinline__ uint64_t ring_mask(const Kv8AttnArgs& a, int base, in
 // A tile against a ring unit staged in LDS; ok: the rows that vector ln attends.
 __device__ __forceinline__ void ring_unit(Tile& tl, const u4v q[4], const u4v* Kf, const u4v* Vf,
                                           int lane, uint64_t ok) {
-    const int lq = lane >> 4;
+    const uint64_t okl = ok >> (4 * (lane >> 4));  // token 16 kt + 4 lq + r: bit 16 kt + r
     f4 S[1][4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
+        const uint32_t w = (uint32_t)(okl >> (32 * (kt >> 1))) >> (16 * (kt & 1));
         S[0][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             S[0][kt] = mfma16x16x32(as_h8(Kf[(4 * kt + s) * 64 + lane]), as_h8(q[s]), S[0][kt]);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            S[0][kt][r] = (ok >> (16 * kt + 4 * lq + r)) & 1 ? S[0][kt][r] : -INFINITY;
+            S[0][kt][r] = (w >> r) & 1 ? S[0][kt][r] : -INFINITY;
+        __builtin_amdgcn_sched_barrier(0);  // (all operands ahead of the products: 100 registers more)
     }
     const Scales u{SC2, 0.0f, 1.0f};
     u4v pa[2];
@@ -290,8 +292,10 @@ __device__ __forceinline__ void ring_unit(Tile& tl, const u4v q[4], const u4v* K
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
+        for (int dt = 0; dt < 8; ++dt) {
             tl.o[dt] = mfma16x16x32(as_h8(pa[j]), as_h8(Vf[(2 * dt + j) * 64 + lane]), tl.o[dt]);
+            if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
 }
 
 __device__ __forceinline__ void write_part(const Kv8AttnArgs& a, int part, int g, int tv, int vend,
@@ -357,15 +361,15 @@ template <int T>
 __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u4v* Kf, const u4v* Vf,
                                             int lane, Scales u, float2* const* rec) {
     f4 S[T][4];
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     {
         u4v k[16];
 #pragma unroll
         for (int f = 0; f < 16; ++f) k[f] = Kf[f * 64 + lane];
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < T; ++i)
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) S[i][kt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -815,27 +819,21 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 #define NWAVES 8
-#ifndef SHARE_MAX
-#define SHARE_MAX (tiles == 1 ? 300 : 2500)
-#endif
-#ifndef T2_MIN
-#define T2_MIN 1400
-#endif
-
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.n_list = a.n_sel > 0 ? a.n_sel : a.n;
     a.ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
     const int nv = a.M * a.G;
     const int tiles = ((a.n_sel > 0 ? a.G : nv) + 15) / 16;  // that share their units
     const int rows = a.n_sel > 0 ? a.M : 1;
-    // Blocks for one page each: the whole block turns it to halves (one row at 2500 tokens %s us a
-    // launch, %s where a wave takes it alone); pages beyond that for one or two tiles: waves with
-    // pages of their own (one row at 131000 tokens 23 us, %s shared); for more tiles shared again (9
-    // rows at 32000 14.4, 17.3 with three tiles a wave), two tiles a wave past eight (64 rows at 65000
-    // 48 us, 60 with one; at 2500 17 and 13).
+    // Shared pages: each is turned to halves by a whole block, a page a block where there are few (one
+    // row at 2000 tokens 5.3 us, 7.2 where a wave takes a page alone; 8 rows at 9600 8.0 and 11.8).
+    // Pages of a wave's own, for one or two tiles: they stream (one row at 131000 tokens 23 us; 8 rows
+    // at 65000 17.4, 19.9 shared).  More tiles share (9 rows at 32000 14, 17 with three tiles a wave).
+    // Two tiles a wave past eight in all, where the block's LDS reads bound it (64 rows at 65000 tokens
+    // 46 us, 60 with one; at 9600 20.6 and 18.8).
     const int col1 = rows * ((tiles + NWAVES - 1) / NWAVES);
-    a.shared = tiles > 2 || (int64_t)a.n_list * col1 * a.p.nKV <= SHARE_MAX;
-    a.tiles = !a.shared ? tiles : tiles > NWAVES && (int64_t)a.n_list * a.p.nKV > T2_MIN ? 2 : 1;
+    a.shared = tiles > 2 || (int64_t)a.n_list * col1 * a.p.nKV <= (tiles == 1 ? 300 : 2500);
+    a.tiles = !a.shared ? tiles : tiles > NWAVES && (int64_t)a.n_list * a.p.nKV > 1400 ? 2 : 1;
     const int per = a.shared ? a.tiles * NWAVES : a.tiles;
     a.cols = rows * ((tiles + per - 1) / per);
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
