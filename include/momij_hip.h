@@ -249,7 +249,8 @@ mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv,
 /* Positions [pos, pos + 64 count) of the ring sealed into the pages of table entries at .. at +
  * count - 1 of every head: scale = m / 127 and code = round(x * (127 / m)) to the nearest whole
  * number, ties to even, each operation in fp32, m the block's greatest finite magnitude (0: all
- * codes 0).  An infinity takes the code +-127, a NaN 0.  64 count <= capacity. */
+ * codes 0).  An infinity takes the code +-127, a NaN 0.  64 count <= capacity.
+ * A page that two of the entries name holds parts of either block. */
 mj_status mj_kv8_seal(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int64_t pos,
                       int count, int at);
 /* The way back, for a rewind into sealed blocks: entries at .. at + count - 1 to positions
@@ -291,8 +292,8 @@ mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, 
  * others, those of the greatest mass stay (the lower index on ties; a NaN counts as the least; each
  * head by its own masses).  table_out [n_kv_heads][table_stride] lists the kept blocks in their
  * order, then the evicted ones' pages (free now) in theirs, then the rest of the row unchanged;
- * mass_out likewise, 0 from `keep` on.  n_first + n_last <= keep <= n_blocks.  table_out must not be
- * cache->table, nor mass_out be mass_in. */
+ * mass_out likewise, 0 from `keep` on.  n_first + n_last <= keep <= n_blocks.  table_out must not
+ * lie over cache->table, nor mass_out over mass_in. */
 mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep, int n_first,
                        int n_last, const float* mass_in, int32_t* table_out, float* mass_out);
 

@@ -29,6 +29,11 @@ bool aligned16(std::initializer_list<const void*> ps) {
     return (bits & 15) == 0;
 }
 
+bool overlap(const void* a, const void* b, size_t bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y ? y - x < bytes : x - y < bytes;
+}
+
 constexpr int kMaxGroup = 64;              // query heads a KV head
 constexpr int kMaxBlocks = 1 << 20;        // blocks a head lists
 constexpr int64_t kMaxRing = 1ll << 30;    // slots (slots are counted in 32 bits)
@@ -173,8 +178,11 @@ mj_status fill_append(mj_ctx* ctx, Kv8AppendArgs& a, const mj_attn_config& c, co
     a.half = c.rope_dim / 2;
     a.eps = c.eps;
     a.abort = ctx->abort_dev;
-    for (int i = 0; i < a.half; ++i)
-        a.turns[i] = std::pow((double)c.rope_base, -(double)i / a.half) / (2.0 * M_PI);
+    // base^(-i / half) / 2 pi by products of 64 bits' mantissa (a power each takes longer than the
+    // rest of the call)
+    const long double step = a.half ? std::pow((long double)c.rope_base, -1.0L / a.half) : 1.0L;
+    long double turn = 0.5L / 3.14159265358979323846264338327950288L;
+    for (int i = 0; i < a.half; ++i, turn *= step) a.turns[i] = (double)turn;
     for (int i = 0; i < M; ++i) a.depth[i] = (uint8_t)sd.depth[i];
     return MJ_OK;
 }
@@ -327,8 +335,10 @@ mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep,
     Kv8Pool p;
     mj_status s = check_pool(ctx, cache, what, p);
     if (s != MJ_OK) return s;
-    if (!mass_in || !table_out || !mass_out || table_out == cache->table || mass_out == mass_in)
-        return mj_fail(ctx, MJ_INVALID_ARG, "%s: null pointer, or an output that is its input", what);
+    const size_t bytes = (size_t)p.nKV * p.stride * 4;
+    if (!mass_in || !table_out || !mass_out || overlap(table_out, cache->table, bytes) ||
+        overlap(mass_out, mass_in, bytes))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: null pointer, or an output over its input", what);
     if (n_blocks < 0 || n_blocks > p.stride || keep < 0 || keep > n_blocks || n_first < 0 ||
         n_last < 0 || (int64_t)n_first + n_last > keep)
         return mj_fail(ctx, MJ_INVALID_ARG,

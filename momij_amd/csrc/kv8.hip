@@ -574,9 +574,10 @@ __device__ __forceinline__ bool pick_keys(F key, int n, int k, int first, int la
 }
 
 // One block a row and head: scores formed in LDS, then the n_sel greatest, for up to CHOOSE_MAX blocks
-// (256 bytes a block come through one CU: 500 of them for 8 rows take 10.4 us, in two launches 6.2 and
-// 4.4 us and the gap between them; 2047 of one row 26 us, 15 in two).
-#define CHOOSE_MAX 1024
+// (their 256 bytes each come through one CU, which has only so many lines under way: of 8 rows 250
+// blocks take 10 us and 500 13, in two launches 12.5 and 12.5 and the gap between them; 1000 19 and
+// 13.5).
+#define CHOOSE_MAX 512
 __global__ __launch_bounds__(1024) void k_kv8_choose(Kv8SelectArgs a) {
     __shared__ float s_sc[CHOOSE_MAX];
     __shared__ __align__(16) i4v s_q[4][4][64];

@@ -837,8 +837,9 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     const int per = a.shared ? a.tiles * NWAVES : a.tiles;
     a.cols = rows * ((tiles + per - 1) / per);
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
-    // chip holds would run alone at the end
-    int parts = std::max(1, 256 / (a.cols * a.p.nKV) - a.ring_units);
+    // chip holds would run alone at the end.  A ring of many units leaves the pages half the chip.
+    const int share = 256 / (a.cols * a.p.nKV);
+    int parts = std::max({1, share / 2, share - a.ring_units});
     parts = std::min(parts, a.shared ? a.n_list : (a.n_list + NWAVES - 1) / NWAVES);
     a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
     a.parts = a.ring_units + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);

@@ -42,8 +42,10 @@ class Kv8Cache:
     """A pool for `blocks` blocks of each head, head g's pages g * blocks .. at first; `mass`
     [n_kv_heads][blocks] holds the blocks' accumulated attention weight."""
 
-    def __init__(self, ctx, n_kv_heads: int, blocks: int, device: str = "cuda"):
+    def __init__(self, ctx, n_kv_heads: int, blocks: int):
         import torch
+
+        device = torch.device("cuda", ctx.device)
 
         self.ctx, self.n_kv_heads, self.blocks = ctx, n_kv_heads, blocks
         pages = n_kv_heads * blocks
@@ -57,6 +59,7 @@ class Kv8Cache:
         self.table = torch.arange(pages, dtype=torch.int32, device=device).reshape(n_kv_heads, blocks)
         self.mass = zeros((n_kv_heads, blocks), torch.float32)
         self._spare = torch.empty_like(self.table), torch.empty_like(self.mass)
+        torch.cuda.synchronize(device)  # the zeros are in place for the context's stream
         self._bind()
 
     def _bind(self):

@@ -8,6 +8,7 @@ before handing freshly written tensors to it, and `ctx.sync()` before reading re
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 from . import _lib
 from ._lib import AttnConfig, AttnWeights, LayerWeights, MoeWeights, ModelConfig, MomijError
@@ -114,7 +115,7 @@ class Context:
             return None
         if len(parents) != M:
             raise ValueError(f"{len(parents)} parents of {M} rows")
-        return (C.c_int32 * M)(*[int(p) for p in parents])
+        return (C.c_int32 * M).from_buffer(array("i", parents))
 
     def qkv_append(self, cfg: dict, qkv, q_norm_w, k_norm_w, ring, L: int, parents, M: int, q_out):
         """Queries and keys normed and rotated, keys and values appended to the ring; qkv rows may
