@@ -502,39 +502,41 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     }
 }
 
-// A wave's own pages: T tiles of query vectors a block, the same for all of its NW waves, and every
-// wave takes pages of its own, straight into registers: a page's bytes lie in the order of the operands, so a lane's 16 bytes
-// are two of them, turned to halves once for all T tiles.  A wave's next K goes out behind its scores,
-// its next V behind its output products; the page numbers and scales of 64 pages come with one
-// request a lane each.  The waves are joined in LDS.  The first blocks take a ring unit each.  Where
-// rows list their own blocks (a.sel), blockIdx.y is a row and a share of its heads.
-template <int T, int NW, bool MASS>
+// Pages of P waves' own: every P waves of the block take pages for themselves, T tiles of query vectors
+// each, straight into registers: a page's bytes lie in the order of the operands, so a lane's 16 bytes
+// are two of them, turned to halves once for all T tiles.  (The P waves ask for a page at about the
+// same time; it comes from memory once.)  A wave's next K goes out behind its scores, its next V behind
+// its output products; the page numbers and scales of 64 pages come with one request a lane each.  The
+// waves are joined in LDS.  The first blocks take a ring unit each.  Where rows list their own blocks
+// (a.sel), blockIdx.y is a row and a share of its heads.
+template <int T, int P, int NW, bool MASS>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
-    constexpr int NT = 64 * NW;
+    constexpr int NT = 64 * NW, NG = NW / P;
     extern __shared__ __align__(16) u4v lds[];
     __shared__ int s_abort;
     __shared__ uint32_t s_bad[2];
     __shared__ float s_m[T][NW][16], s_l[NW][16];
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6, ln = lane & 15, lq = lane >> 4;
-    const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
+    const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G, pr = wv % P;
     int row, v0, vend;
-    block_vectors(a, 16 * T, row, v0, vend);
+    block_vectors(a, 16 * T * P, row, v0, vend);
     if (part < a.ring_units) {
         ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
         return;
     }
+    const int vw = v0 + 16 * T * pr;  // the wave's vectors
     const int ab = a.abort ? *a.abort : 0;
     Tile tl[T];
     u4v q[T][4];
     const int up = (part - a.ring_units) * a.upp;
-    const int u0 = up + wv, u1 = min(up + a.upp, a.n_list);
-    for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NW) {
-        const int ul = ub + NW * lane;  // lane's unit
+    const int u0 = up + wv / P, u1 = P > 1 && vw >= vend ? 0 : min(up + a.upp, a.n_list);
+    for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NG) {
+        const int ul = ub + NG * lane;  // lane's unit
         const int pl = ul < u1 ? unit_page(a, g, row, ul) : -1;
         if (ub == u0) {
 #pragma unroll
             for (int i = 0; i < T; ++i) {
-                load_q(a, g, v0 + 16 * i + ln, v0 + 16 * i + ln < vend, q[i]);
+                load_q(a, g, vw + 16 * i + ln, vw + 16 * i + ln < vend, q[i]);
                 tl[i].clear();
             }
         }
@@ -584,10 +586,10 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
                 float lu;
                 weights(tl[x], S[x], sc, pa[x], lu);
                 if constexpr (MASS) {
-                    const int v = v0 + 16 * x + ln;
+                    const int v = vw + 16 * x + ln;
                     lu = x4_sum(lu);
                     if (lq == 0 && v < vend)
-                        a.rec[((size_t)g * a.n + ub + NW * i) * nv + v] = make_float2(tl[x].m, lu);
+                        a.rec[((size_t)g * a.n + ub + NG * i) * nv + v] = make_float2(tl[x].m, lu);
                 }
             }
 #pragma unroll
@@ -613,10 +615,10 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
         }
         if (i0 >= 0) step(i0, 0, std::false_type{});
     }
-    // ---- the waves joined, a tile at a time: each scales its outputs to the block's maximum and puts
-    // those of the tile's vectors side by side in LDS (a lane's four vectors of a dim in 16 bytes), then
-    // a thread adds up one dim of four vectors, wave by wave.  (Every thread weighing every wave's
-    // outputs read three times as much LDS: 1.7 us a tile.)
+    // ---- the waves joined, a tile of each of the P together at a time: each wave scales its outputs to
+    // its tile's maximum and puts them side by side in LDS (a lane's four vectors of a dim in 16
+    // bytes), then a thread adds up one dim of four vectors, wave by wave.  (Every thread weighing
+    // every wave's outputs read three times as much LDS: 1.7 us a tile.)
     f4* so = (f4*)lds;  // [NW][4][128]: vectors 4 y .. + 3 of dim d
 #pragma unroll
     for (int x = 0; x < T; ++x)
@@ -624,17 +626,17 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
     if (t == 0) s_abort = ab;
     __syncthreads();
     if (s_abort) return;
-    auto put = [&](Tile& tt, int x, int rows) {
+    auto put = [&](Tile& tt, int x) {
         const float l = x4_sum(tt.l);
-        float m = s_m[x][0][ln];
+        float m = s_m[x][pr][ln];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) m = fmaxf(m, s_m[x][w][ln]);
+        for (int w = 1; w < NG; ++w) m = fmaxf(m, s_m[x][w * P + pr][ln]);
         const float f = __builtin_amdgcn_exp2f(tt.m - (m == -INFINITY ? 0.0f : m));
         if (lq == 0) s_l[wv][ln] = l * f;
         f4 fr;
 #pragma unroll
         for (int r = 0; r < 4; ++r) fr[r] = __shfl(f, 4 * lq + r, MJ_WAVE);
-        if (4 * lq < rows)
+        if (vw + 16 * x + 4 * lq < vend)
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) {
                 f4 o = tt.o[dt];
@@ -645,59 +647,66 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
     };
 #pragma unroll 1
     for (int x = 0; x < T; ++x) {
-        const int tv = v0 + 16 * x, rows = min(vend - tv, 16);
-        if (rows <= 0) break;  // whole block
+        if (v0 + 16 * x >= vend) break;  // whole block
         if (x) __syncthreads();
-        if (x == 0) put(tl[0], 0, rows);
+        if (x == 0) put(tl[0], 0);
         if constexpr (T > 1)
-            if (x == 1) put(tl[1], 1, rows);
+            if (x == 1) put(tl[1], 1);
         __syncthreads();
-        const size_t pb = ((size_t)part * a.p.nKV + g) * nv + tv;
-        if (t < rows) {
-            float l = 0.0f, m = s_m[x][0][t];
+        const size_t pb = ((size_t)part * a.p.nKV + g) * nv;
+        if (t < 16 * P) {
+            const int p = t >> 4, v = v0 + 16 * (T * p + x) + (t & 15);
+            float l = 0.0f, m = s_m[x][p][t & 15];
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                l += s_l[w][t];
-                m = fmaxf(m, s_m[x][w][t]);
+            for (int w = 0; w < NG; ++w) {
+                l += s_l[w * P + p][t & 15];
+                m = fmaxf(m, s_m[x][w * P + p][t & 15]);
             }
-            a.ml[pb + t] = make_float2(m, l);
+            if (v < vend) a.ml[pb + v] = make_float2(m, l);
         }
-        for (int e = t; e < 128 * ((rows + 3) / 4); e += NT) {
-            f4 o = so[e];
 #pragma unroll
-            for (int w = 1; w < NW; ++w) {
-                const f4 y = so[w * 512 + e];
+        for (int e0 = 0; e0 < 512 * P; e0 += NT) {
+            const int e = e0 + t, p = e >> 9, v = v0 + 16 * (T * p + x) + 4 * ((e >> 7) & 3), d = e & 127;
+            if (v >= vend) continue;
+            const f4* src = so + p * 512 + (e & 511);
+            f4 o = src[0];
+#pragma unroll
+            for (int w = 1; w < NG; ++w) {
+                const f4 y = src[w * P * 512];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[k] += y[k];
             }
-            const int vec = 4 * (e >> 7), d = e & 127;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (vec + k < rows) a.opart[(pb + vec + k) * HD + d] = o[k];
+                if (v + k < vend) a.opart[(pb + v + k) * HD + d] = o[k];
         }
     }
 }
 
-// mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax: a
-// 256-thread block takes MASS_B of a head's blocks, a wave one at a time.  The vectors' final maxima
+// mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax: a wave
+// takes one of a head's blocks.  The vectors' final maxima
 // and sums are formed again here from the parts' (a launch that waited for them took 4 us more).
-#define MASS_B 4
+template <int NW>
 __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
-    __shared__ float2 s_stat[MJ_ROWS * 64], s_w[2][4][64];
+    __shared__ float2 s_w[2][NW][64];
     __shared__ int s_stop;
-    const int t = threadIdx.x, lane = t & 63, nv = a.M * a.G, per = (a.n + MASS_B - 1) / MASS_B;
-    const int g = blk / per, i0 = (blk - g * per) * MASS_B;
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, nv = a.M * a.G, per = (a.n + NW - 1) / NW;
+    const int g = blk / per, i = (blk - g * per) * NW + wv, ic = min(i, a.n - 1);
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_stop = ab;
-    const size_t step = (size_t)a.p.nKV * nv;
-    const int wv = t >> 6;
-    for (int v0 = 0; v0 < nv; v0 += 64) {  // a lane a vector, a wave every fourth part
-        const float2* ml = a.ml + (size_t)g * nv + min(v0 + lane, nv - 1);
+    const size_t step = (size_t)a.p.nKV * nv, at = (size_t)g * a.p.stride + ic;
+    const bool there = page_of_list(a, g, ic) >= 0;
+    const float before = a.mass_in ? a.mass_in[at] : 0.0f;
+    float s = 0.0f;
+    for (int v0 = 0; v0 < nv; v0 += 64) {  // a lane a vector, a wave every NW-th part
+        const int vc = min(v0 + lane, nv - 1);
+        const float2 rc = a.rec[((size_t)g * a.n + ic) * nv + vc];
+        const float2* ml = a.ml + (size_t)g * nv + vc;
         float m = -INFINITY, l = 0.0f;
-        for (int c0 = wv; c0 < a.parts; c0 += 64) {
+        for (int c0 = wv; c0 < a.parts; c0 += 16 * NW) {
             float2 x[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = ml[(size_t)min(c0 + 4 * j, a.parts - 1) * step];
+            for (int j = 0; j < 16; ++j) x[j] = ml[(size_t)min(c0 + NW * j, a.parts - 1) * step];
             float mn = m;
 #pragma unroll
             for (int j = 0; j < 16; ++j) mn = fmaxf(mn, x[j].x);
@@ -705,63 +714,55 @@ __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
             l *= __builtin_amdgcn_exp2f(m - ref);
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                l = c0 + 4 * j < a.parts ? fmaf(x[j].y, __builtin_amdgcn_exp2f(x[j].x - ref), l) : l;
+                l = c0 + NW * j < a.parts ? fmaf(x[j].y, __builtin_amdgcn_exp2f(x[j].x - ref), l) : l;
             m = mn;
         }
         s_w[v0 / 64 & 1][wv][lane] = make_float2(m, l);
-        __syncthreads();
-        if (wv == 0 && v0 + lane < nv) {
-            const float2* w = &s_w[v0 / 64 & 1][0][lane];
-            float mx = fmaxf(fmaxf(w[0].x, w[64].x), fmaxf(w[128].x, w[192].x));
-            mx = mx == -INFINITY ? 0.0f : mx;
-            float ls = 0.0f;
+        __syncthreads();  // (the next write of this buffer is behind the next barrier)
+        const float2* w = &s_w[v0 / 64 & 1][0][lane];
+        float mx = w[0].x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) ls = fmaf(w[64 * k].y, __builtin_amdgcn_exp2f(w[64 * k].x - mx), ls);
-            s_stat[v0 + lane] = make_float2(mx, ls == 0.0f ? 0.0f : 1.0f / ls);
-        }
+        for (int k = 1; k < NW; ++k) mx = fmaxf(mx, w[64 * k].x);
+        mx = mx == -INFINITY ? 0.0f : mx;
+        float ls = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) ls = fmaf(w[64 * k].y, __builtin_amdgcn_exp2f(w[64 * k].x - mx), ls);
+        const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+        const float share =
+            rc.y * inv * __builtin_amdgcn_exp2f((rc.x == -INFINITY ? 0.0f : rc.x) - mx);
+        s += v0 + lane < nv ? share : 0.0f;
     }
-    __syncthreads();
     if (s_stop) return;
-    for (int i = i0 + (t >> 6); i < min(i0 + MASS_B, a.n); i += 4) {
-        const size_t at = (size_t)g * a.p.stride + i;
-        float s = 0.0f;
-        if (page_of_list(a, g, i) >= 0)
-            for (int v = lane; v < nv; v += 64) {
-                const float2 rc = a.rec[((size_t)g * a.n + i) * nv + v], st = s_stat[v];
-                s = fmaf(rc.y * st.y,
-                         __builtin_amdgcn_exp2f((rc.x == -INFINITY ? 0.0f : rc.x) - st.x), s);
-            }
-        s = wave_sum(s);
-        if (lane == 0) a.mass_out[at] = (a.mass_in ? a.mass_in[at] : 0.0f) + s;
-    }
+    s = wave_sum(there ? s : 0.0f);
+    if (lane == 0 && i < a.n) a.mass_out[at] = before + s;
 }
 
-// One 256-thread block a row and head.  Eight groups of 32 lanes (a lane four dims) take every eighth
-// part, eight requested at a time, each to its own running maximum; the groups are then joined in
-// order.  A part that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.
-template <bool MASS>
-__global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
+// One block a row and head.  NG groups of 32 lanes (a lane four dims) take every NG-th part, eight
+// requested at a time, each to its own running maximum; the groups are then joined in order.  A part
+// that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.
+template <int NG, bool MASS>
+__global__ __launch_bounds__(32 * NG) void k_kv8_combine(Kv8AttnArgs a) {
     const int t = threadIdx.x, gr = t >> 5, d4 = t & 31;
     const int nQ = a.p.nKV * a.G, nv = a.M * a.G;
     if (MASS && (int)blockIdx.x >= a.M * nQ) {
-        if constexpr (MASS) mass_blocks(a, blockIdx.x - a.M * nQ);
+        if constexpr (MASS) mass_blocks<NG / 2>(a, blockIdx.x - a.M * nQ);
         return;
     }
     const int r = blockIdx.x / nQ, h = blockIdx.x % nQ, g = h / a.G, v = r * a.G + h % a.G;
-    __shared__ f4 s_o[8][32];
-    __shared__ float s_m[8], s_l[8];
+    __shared__ f4 s_o[NG][32];
+    __shared__ float s_m[NG], s_l[NG];
     __shared__ int s_abort;
     const int ab = a.abort ? *a.abort : 0;
     if (t == 0) s_abort = ab;
     const size_t step = (size_t)a.p.nKV * nv, at = (size_t)g * nv + v;
     float m = -INFINITY, l = 0.0f;
     f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = gr; c0 < a.parts; c0 += 64) {
+    for (int c0 = gr; c0 < a.parts; c0 += 8 * NG) {
         float2 ml[8];
         f4 x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const size_t c = at + (size_t)min(c0 + 8 * j, a.parts - 1) * step;
+            const size_t c = at + (size_t)min(c0 + NG * j, a.parts - 1) * step;
             ml[j] = a.ml[c];
             x[j] = *(const f4*)(a.opart + c * HD + 4 * d4);
         }
@@ -775,7 +776,7 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
         for (int k = 0; k < 4; ++k) o[k] *= f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (c0 + 8 * j >= a.parts) break;
+            if (c0 + NG * j >= a.parts) break;
             const float w = __builtin_amdgcn_exp2f(ml[j].x - ref);
             l = fmaf(ml[j].y, w, l);
 #pragma unroll
@@ -792,12 +793,12 @@ __global__ __launch_bounds__(256) void k_kv8_combine(Kv8AttnArgs a) {
     if (s_abort || t >= 16) return;
     float mx = s_m[0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) mx = fmaxf(mx, s_m[j]);
+    for (int j = 1; j < NG; ++j) mx = fmaxf(mx, s_m[j]);
     const float ref = mx == -INFINITY ? 0.0f : mx;
     float y[8] = {};
     l = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < NG; ++j) {
         const float w = __builtin_amdgcn_exp2f(s_m[j] - ref);
         l = fmaf(s_l[j], w, l);
         const f4 p0 = s_o[j][2 * t], p1 = s_o[j][2 * t + 1];
@@ -828,19 +829,22 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     // Shared pages: each is turned to halves by a whole block, a page a block where there are few (one
     // row at 2000 tokens 5.3 us, 7.2 where a wave takes a page alone; 8 rows at 9600 8.0 and 11.8).
     // Pages of a wave's own, for one or two tiles: they stream (one row at 131000 tokens 23 us; 8 rows
-    // at 65000 17.4, 19.9 shared).  More tiles share (9 rows at 32000 14, 17 with three tiles a wave).
-    // Two tiles a wave past eight in all, where the block's LDS reads bound it (64 rows at 65000 tokens
-    // 46 us, 60 with one; at 9600 20.6 and 18.8).
-    const int col1 = rows * ((tiles + NWAVES - 1) / NWAVES);
-    a.shared = tiles > 2 || (int64_t)a.n_list * col1 * a.p.nKV <= (tiles == 1 ? 300 : 2500);
-    a.tiles = !a.shared ? tiles : tiles > NWAVES && (int64_t)a.n_list * a.p.nKV > 1400 ? 2 : 1;
-    const int per = a.shared ? a.tiles * NWAVES : a.tiles;
+    // at 65000 17.4, 19.9 shared); of two waves together, for three or four, later (9 rows at 131000
+    // tokens 31.6 us, 35.9 shared; at 65000 19.7 and 20.6; at 32000 14.8 and 14.3).  More share (17
+    // rows at 131000 47 us, 51 by four waves together).  Two tiles a wave past eight in all, where the
+    // block's LDS reads bound it (64 rows at 65000 tokens 46 us, 60 with one; at 9600 20.6 and 18.8).
+    const int64_t visits = (int64_t)a.n_list * a.p.nKV;
+    const int64_t most = tiles == 1 ? 300 : tiles == 2 ? 2500 : tiles <= 4 ? 3500 : INT64_MAX;
+    a.shared = visits * rows * ((tiles + NWAVES - 1) / NWAVES) <= most;
+    a.pair = !a.shared && tiles > 2 ? 2 : 1;
+    a.tiles = a.shared ? (tiles > NWAVES && visits > 1400 ? 2 : 1) : std::min(tiles, 2);
+    const int per = a.shared ? a.tiles * NWAVES : a.tiles * a.pair;
     a.cols = rows * ((tiles + per - 1) / per);
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
     // chip holds would run alone at the end.  A ring of many units leaves the pages half the chip.
     const int share = 256 / (a.cols * a.p.nKV);
     int parts = std::max({1, share / 2, share - a.ring_units});
-    parts = std::min(parts, a.shared ? a.n_list : (a.n_list + NWAVES - 1) / NWAVES);
+    parts = std::min(parts, a.shared ? a.n_list : (a.n_list + NWAVES / a.pair - 1) / (NWAVES / a.pair));
     a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
     a.parts = a.ring_units + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);
     size_t off = 0;
@@ -865,24 +869,39 @@ static hipError_t launch_one(K kernel, const hipError_t& attr, const Kv8AttnArgs
     hipLaunchKernelGGL(kernel, dim3(a.parts, a.cols, a.p.nKV), dim3(64 * NWAVES), ATTN_LDS, st, a);
     return hipGetLastError();
 }
+static hipError_t raise_lds(const void* kernel) {
+    return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, ATTN_LDS);
+}
 template <int T, bool MASS>
-static hipError_t launch_tiles(const Kv8AttnArgs& a, hipStream_t st) {
-    auto raise = [](const void* k) {
-        return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, ATTN_LDS);
-    };
-    static const hipError_t s = raise((const void*)k_kv8_attn_shared<T, NWAVES, MASS>);
-    static const hipError_t o = raise((const void*)k_kv8_attn_own<T, NWAVES, MASS>);
-    return a.shared ? launch_one(k_kv8_attn_shared<T, NWAVES, MASS>, s, a, st)
-                    : launch_one(k_kv8_attn_own<T, NWAVES, MASS>, o, a, st);
+static hipError_t launch_shared(const Kv8AttnArgs& a, hipStream_t st) {
+    static const hipError_t s = raise_lds((const void*)k_kv8_attn_shared<T, NWAVES, MASS>);
+    return launch_one(k_kv8_attn_shared<T, NWAVES, MASS>, s, a, st);
+}
+template <int T, int P, bool MASS>
+static hipError_t launch_own(const Kv8AttnArgs& a, hipStream_t st) {
+    static const hipError_t s = raise_lds((const void*)k_kv8_attn_own<T, P, NWAVES, MASS>);
+    return launch_one(k_kv8_attn_own<T, P, NWAVES, MASS>, s, a, st);
+}
+template <bool MASS>
+static hipError_t launch_pages(const Kv8AttnArgs& a, hipStream_t st) {
+    if (a.shared) return a.tiles == 1 ? launch_shared<1, MASS>(a, st) : launch_shared<2, MASS>(a, st);
+    if (a.pair == 2) return launch_own<2, 2, MASS>(a, st);
+    return a.tiles == 1 ? launch_own<1, 1, MASS>(a, st) : launch_own<2, 1, MASS>(a, st);
 }
 
 template <bool MASS>
 static hipError_t launch_attn_pass(const Kv8AttnArgs& a, hipStream_t st) {
-    const hipError_t e = a.tiles == 1 ? launch_tiles<1, MASS>(a, st) : launch_tiles<2, MASS>(a, st);
+    const hipError_t e = launch_pages<MASS>(a, st);
     if (e != hipSuccess) return e;
-    // the join: a block a row and head, then (masses) one for every MASS_B blocks of a head
-    const int heads = a.M * a.p.nKV * a.G, masses = (a.n + MASS_B - 1) / MASS_B * a.p.nKV;
-    hipLaunchKernelGGL(k_kv8_combine<MASS>, dim3(heads + (MASS ? masses : 0)), dim3(256), 0, st, a);
+    // the join: a block a row and head, then (masses) one for every NG / 2 blocks of a head
+    auto join = [&](auto kernel, int ng) {
+        const int masses = MASS ? (a.n + ng / 2 - 1) / (ng / 2) * a.p.nKV : 0;
+        hipLaunchKernelGGL(kernel, dim3(a.M * a.p.nKV * a.G + masses), dim3(32 * ng), 0, st, a);
+    };
+    // more than 64 parts, a round of 8 groups' requests: 32 groups (4 rows of 8 heads over 250 parts 6.3
+    // us, 11.8 by 8 groups; 1 row of 16 heads over 60 parts 4.9 us, 4.0 by 8)
+    if (a.parts > 64) join(k_kv8_combine<32, MASS>, 32);
+    else join(k_kv8_combine<8, MASS>, 8);
     return hipGetLastError();
 }
 

@@ -74,9 +74,9 @@ struct Kv8AttnArgs {
     const float* mass_in;
     float* mass_out;
     // set by kv8_attn_plan: a part for every 64 rows of the ring (ring_units), then parts of upp
-    // listed blocks each; shared: which kernel; tiles: of 16 query vectors, a wave; cols: block columns
-    // (groups of tiles, rows with lists of their own)
-    int n_list, upp, parts, ring_units, tiles, cols;
+    // listed blocks each; shared: which kernel; tiles: of 16 query vectors, a wave; pair: waves that
+    // take their pages together; cols: block columns (groups of tiles, rows with lists of their own)
+    int n_list, upp, parts, ring_units, tiles, pair, cols;
     bool shared;
     float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
     float2* ml;     // [parts][nKV][nv] {m, sum}

@@ -647,3 +647,61 @@ def test_select_either_way(ctx, M, n):
     for r in range(M):
         for g in range(nKV):
             assert sel[r, g].tolist() == ref.choose(sc[r, g].tolist(), 3, 5, n_sel), (r, g)
+
+
+LONG = [
+    # M, nQ, nKV, blocks, open rows, tree: sizes on the far side of each rule
+    (1, 16, 4, 100, 5, False), (3, 16, 4, 321, 0, True),             # a tile, pages of each wave's own
+    (5, 128, 32, 81, 3, True), (8, 64, 16, 161, 64, False),          # two tiles
+    (9, 128, 32, 115, 50, False), (13, 128, 32, 111, 1, True),       # three, four: pages of two waves
+    (12, 16, 4, 900, 17, True), (16, 16, 4, 877, 9, False),
+    (64, 16, 4, 360, 10, True), (33, 64, 16, 91, 0, False),          # two tiles a wave, pages shared
+    (2, 16, 1, 300, 66, False)]                                      # parts past one round of the join
+
+
+@pytest.mark.parametrize("M,nQ,nKV,n,open_,tree", LONG)
+@pytest.mark.parametrize("mass", [False, True])
+def test_long_contexts(ctx, M, nQ, nKV, n, open_, tree, mass):
+    import torch
+
+    from tests.test_gpu_kv8 import Ctx8, gen, run_attn
+
+    rnd = gen(M + n)
+    c = Ctx8(ctx, rnd, nKV, n, open_, M)
+    parents = ref.tree(M, np.random.default_rng(n)) if tree else None
+    c.cache.table[nKV - 1, n // 2] = -1  # one head lacks a block
+    q = rnd(M, nQ * D).half()
+    m0 = torch.rand((nKV, n + 2), device="cuda") if mass else None
+    out, m1 = run_attn(ctx, c, q, nQ, nKV, parents, mass=m0)
+    again, m2 = run_attn(ctx, c, q, nQ, nKV, parents, mass=m0)
+    assert torch.equal(out, again) and (not mass or torch.equal(m1, m2))
+    G, seen = nQ // nKV, c.mask(parents)
+    for g in range(nKV):
+        ok = seen.clone()
+        if g == nKV - 1:
+            ok[:, n // 2 * B:(n // 2 + 1) * B] = False
+        want, p, tol, rel = attend(q.reshape(M, nKV, G, D)[:, g], *c.keys(g), ok, G)
+        err = (out.double().reshape(M, nKV, G, D)[:, g].reshape(M * G, D) - want).abs()
+        assert (err <= tol).all(), (g, float((err / tol).max()))
+        if mass:
+            add = p[:, :n * B].reshape(M * G, n, B).sum(2)
+            want = m0[g, :n].double() + add.sum(0)
+            tol = (add * (rel + 2.0 ** -20)).sum(0) + want * (M * G + 4) * ref.E32 + 1e-30
+            assert ((m1[g, :n].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M,nQ,nKV,n,n_sel", [(8, 384, 8, 90, 64), (40, 80, 4, 30, 20), (5, 64, 1, 700, 9)])
+def test_long_lists_of_rows(ctx, M, nQ, nKV, n, n_sel):
+    """Rows with lists of their own and more than a tile of heads."""
+    import torch
+
+    from tests.test_gpu_kv8 import Ctx8, check_rows, gen, run_attn
+
+    rnd = gen(nQ)
+    c = Ctx8(ctx, rnd, nKV, n, 20, M)
+    rng = np.random.default_rng(n)
+    sel = np.stack([[np.sort(rng.permutation(n)[:n_sel]) for _ in range(nKV)] for _ in range(M)])
+    blocks = torch.zeros((M, nKV, n), dtype=torch.bool).scatter_(2, torch.from_numpy(sel), True)
+    q = rnd(M, nQ * D).half()
+    out, _ = run_attn(ctx, c, q, nQ, nKV, None, sel=torch.from_numpy(sel.astype(np.int32)).cuda())
+    check_rows(c, q, out, nQ, nKV, torch.stack([c.mask(None, blocks[:, g]) for g in range(nKV)]))
