@@ -323,35 +323,59 @@ __device__ __forceinline__ void block_vectors(const Kv8AttnArgs& a, int per, int
     vend = min(a.sel ? row * a.G + a.G : a.M * a.G, v0 + per);
 }
 
-// One ring unit (rows base .. of the call's open ones) as a part of its own: the block of NW waves
-// stages it and takes the query vectors v0 .. vend - 1 a tile a wave at a time.  lds: 32 KB.
+// A part of the ring: units part * upr on, upr of them (64 rows each of the call's open ones), one at a
+// time; the block of NW waves stages a unit and takes the query vectors v0 .. vend - 1 a tile a wave,
+// in further rounds where they are more.  lds: 32 KB.
 template <int NW>
-__device__ __forceinline__ void ring_part(const Kv8AttnArgs& a, int part, int g, int base, int v0,
-                                          int vend, u4v* lds, uint32_t* s_bad, int* s_abort) {
+__device__ __forceinline__ void ring_part(const Kv8AttnArgs& a, int part, int g, int v0, int vend,
+                                          u4v* lds, uint32_t* s_bad, int* s_abort) {
     const int t = threadIdx.x, lane = t & 63, ln = lane & 15, C = (int)a.ring.C;
+    const int u0 = part * a.upr, u1 = min(u0 + a.upr, a.ring_units);
     const int ab = a.abort ? *a.abort : 0;  // thread 0's reading decides for the block
-    if (t < 2) s_bad[t] = 0;
-    __syncthreads();
     u4v* Kf = lds;
     u4v* Vf = Kf + 1024;
-    stage_ring<64 * NW>(a, g, base, Kf, Vf, s_bad);
-    if (t == 0) *s_abort = ab;
-    __syncthreads();
-    if (*s_abort) return;
-    const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
-    for (int tv = v0 + 16 * (t >> 6); tv < vend; tv += 16 * NW) {
+    auto stage = [&](int u) {
+        if (t < 2) s_bad[t] = 0;
+        __syncthreads();
+        stage_ring<64 * NW>(a, g, KV8_B * u, Kf, Vf, s_bad);
+        if (t == 0) *s_abort = ab;
+        __syncthreads();
+        return *s_abort != 0;
+    };
+    auto take = [&](int u, int tv, const u4v* q, Tile& tl) {
+        const uint64_t bad = s_bad[0] | ((uint64_t)s_bad[1] << 32);
+        const uint64_t ok = ring_mask(a, KV8_B * u, tv + ln, tv + ln < vend);
+        ring_unit(tl, q, Kf, Vf, lane, ok);
+        if (bad) {
+            int sb = a.slot0 + KV8_B * u;
+            sb -= sb >= C ? C : 0;
+            add_bad_rows(tl, lane, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
+        }
+    };
+    if (a.upr == 1) {  // staged once (one loop for both forms cost a short context 0.8 us)
+        if (stage(u0)) return;
+        for (int tv = v0 + 16 * (t >> 6); tv < vend; tv += 16 * NW) {
+            u4v q[4];
+            load_q(a, g, tv + ln, tv + ln < vend, q);
+            Tile tl;
+            tl.clear();
+            take(u0, tv, q, tl);
+            write_part(a, part, g, tv, vend, tl);
+        }
+        return;
+    }
+    for (int r0 = v0; r0 < vend; r0 += 16 * NW) {
+        const int tv = r0 + 16 * (t >> 6);
         u4v q[4];
         load_q(a, g, tv + ln, tv + ln < vend, q);
         Tile tl;
         tl.clear();
-        const uint64_t ok = ring_mask(a, base, tv + ln, tv + ln < vend);
-        ring_unit(tl, q, Kf, Vf, lane, ok);
-        if (bad) {
-            int sb = a.slot0 + base;
-            sb -= sb >= C ? C : 0;
-            add_bad_rows(tl, lane, ok, bad, a.ring.v + (size_t)g * C * HD, sb, C);
+        for (int u = u0; u < u1; ++u) {
+            __syncthreads();  // everyone is done with the unit before
+            if (stage(u)) return;
+            if (tv < vend) take(u, tv, q, tl);
         }
-        write_part(a, part, g, tv, vend, tl);
+        if (tv < vend) write_part(a, part, g, tv, vend, tl);
     }
 }
 
@@ -404,8 +428,12 @@ __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u
 
 // Pages shared: a block of NW waves takes a run of pages for NW T tiles of query vectors, T a wave.  A
 // page is turned to halves once, by the whole block, and read from LDS by its waves; two pages are in
-// LDS and one in registers on its way, one barrier a page.  The first blocks take a ring unit each;
-// rows with lists of their own (a.sel) as below.
+// LDS and one in registers on its way, one barrier a page.  The first blocks take the ring's
+// parts; rows with lists of their own (a.sel) as below.  64 rows of 16 heads over 65500 tokens: 46 us, 0.74
+// PFLOP/s, the matrix units busy 39% of the time and the VALU 50% (the softmax, the codes).  17 rows
+// over 32000 tokens with masses 17.5 us: eight pages a block, each a barrier and a chain of products,
+// softmax and products that its few waves do not cover (a second page on its way, or half the LDS
+// reads, change nothing).
 template <int T, int NW, bool MASS>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NR = 512 / NT;
@@ -416,15 +444,15 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G;
     int row, v0, vend;
     block_vectors(a, 16 * NW * T, row, v0, vend);
-    if (part < a.ring_units) {
-        ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
+    if (part < a.ring_parts) {
+        ring_part<NW>(a, part, g, v0, vend, lds, s_bad, &s_abort);
         return;
     }
     const int ab = a.abort ? *a.abort : 0;
     Tile tl[T];
     u4v q[T][4];
     const bool idle = v0 + 16 * wv * T >= vend;  // the wave has no vector: it stages only
-    const int u0 = (part - a.ring_units) * a.upp, u1 = min(u0 + a.upp, a.n_list);
+    const int u0 = (part - a.ring_parts) * a.upp, u1 = min(u0 + a.upp, a.n_list);
     u4v kr[NR], vr[NR];
     auto request = [&](int pg) {
         const u4v* kp = (const u4v*)(a.p.k + (size_t)pg * KV8_PAGE_BYTES);
@@ -507,8 +535,9 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
 // are two of them, turned to halves once for all T tiles.  (The P waves ask for a page at about the
 // same time; it comes from memory once.)  A wave's next K goes out behind its scores, its next V behind
 // its output products; the page numbers and scales of 64 pages come with one request a lane each.  The
-// waves are joined in LDS.  The first blocks take a ring unit each.  Where rows list their own blocks
-// (a.sel), blockIdx.y is a row and a share of its heads.
+// waves are joined in LDS.  The first blocks take the ring's parts.  Where rows list their own blocks
+// (a.sel), blockIdx.y is a row and a share of its heads.  Bound by memory: one row over 131000 tokens
+// of 4 heads, 134 MB, in 23 us (5.8 TB/s).
 template <int T, int P, int NW, bool MASS>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NG = NW / P;
@@ -520,15 +549,15 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
     const int part = blockIdx.x, g = blockIdx.z, nv = a.M * a.G, pr = wv % P;
     int row, v0, vend;
     block_vectors(a, 16 * T * P, row, v0, vend);
-    if (part < a.ring_units) {
-        ring_part<NW>(a, part, g, 64 * part, v0, vend, lds, s_bad, &s_abort);
+    if (part < a.ring_parts) {
+        ring_part<NW>(a, part, g, v0, vend, lds, s_bad, &s_abort);
         return;
     }
     const int vw = v0 + 16 * T * pr;  // the wave's vectors
     const int ab = a.abort ? *a.abort : 0;
     Tile tl[T];
     u4v q[T][4];
-    const int up = (part - a.ring_units) * a.upp;
+    const int up = (part - a.ring_parts) * a.upp;
     const int u0 = up + wv / P, u1 = P > 1 && vw >= vend ? 0 : min(up + a.upp, a.n_list);
     for (int ub = u0; ub < u1 || ub == u0; ub += 64 * NG) {
         const int ul = ub + NG * lane;  // lane's unit
@@ -684,8 +713,9 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
 }
 
 // mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax: a wave
-// takes one of a head's blocks.  The vectors' final maxima
-// and sums are formed again here from the parts' (a launch that waited for them took 4 us more).
+// takes one of a head's blocks.  The vectors' final maxima and sums are formed again here from the
+// parts' (a launch that waited for them took 4 us more).  17 rows, 500 blocks of 4 heads: with the join
+// 6.1 us.
 template <int NW>
 __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
     __shared__ float2 s_w[2][NW][64];
@@ -739,7 +769,9 @@ __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
 
 // One block a row and head.  NG groups of 32 lanes (a lane four dims) take every NG-th part, eight
 // requested at a time, each to its own running maximum; the groups are then joined in order.  A part
-// that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.
+// that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.  One row of 16
+// heads over 30 to 64 parts 4 to 5 us, a launch and a round of requests; 64 rows over 31 parts (17 MB)
+// 7.6 us.
 template <int NG, bool MASS>
 __global__ __launch_bounds__(32 * NG) void k_kv8_combine(Kv8AttnArgs a) {
     const int t = threadIdx.x, gr = t >> 5, d4 = t & 31;
@@ -841,12 +873,15 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     const int per = a.shared ? a.tiles * NWAVES : a.tiles * a.pair;
     a.cols = rows * ((tiles + per - 1) / per);
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
-    // chip holds would run alone at the end.  A ring of many units leaves the pages half the chip.
-    const int share = 256 / (a.cols * a.p.nKV);
-    int parts = std::max({1, share / 2, share - a.ring_units});
+    // chip holds would run alone at the end.  A ring of many units leaves the pages half the chip, and
+    // one of more than 8192 rows takes several units a part (the parts' outputs grow with them).
+    const int share = 256 / (a.cols * a.p.nKV), ring_most = std::max(share, 128);
+    a.upr = (a.ring_units + ring_most - 1) / ring_most;
+    a.ring_parts = (a.ring_units + a.upr - 1) / a.upr;
+    int parts = std::max({1, share / 2, share - a.ring_parts});
     parts = std::min(parts, a.shared ? a.n_list : (a.n_list + NWAVES / a.pair - 1) / (NWAVES / a.pair));
     a.upp = parts ? (a.n_list + parts - 1) / parts : 0;
-    a.parts = a.ring_units + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);
+    a.parts = a.ring_parts + (parts ? (a.n_list + a.upp - 1) / a.upp : 0);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         off = (off + 255) & ~(size_t)255;

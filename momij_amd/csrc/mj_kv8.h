@@ -73,10 +73,10 @@ struct Kv8AttnArgs {
     float2* out_sum;
     const float* mass_in;
     float* mass_out;
-    // set by kv8_attn_plan: a part for every 64 rows of the ring (ring_units), then parts of upp
-    // listed blocks each; shared: which kernel; tiles: of 16 query vectors, a wave; pair: waves that
+    // set by kv8_attn_plan: ring_parts of upr units (64 rows) of the ring each, then parts of upp
+    // listed blocks each, parts in all; shared: which kernel; tiles: of 16 query vectors, a wave; pair: waves that
     // take their pages together; cols: block columns (groups of tiles, rows with lists of their own)
-    int n_list, upp, parts, ring_units, tiles, pair, cols;
+    int n_list, upp, parts, ring_units, upr, ring_parts, tiles, pair, cols;
     bool shared;
     float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
     float2* ml;     // [parts][nKV][nv] {m, sum}

@@ -705,3 +705,34 @@ def test_long_lists_of_rows(ctx, M, nQ, nKV, n, n_sel):
     q = rnd(M, nQ * D).half()
     out, _ = run_attn(ctx, c, q, nQ, nKV, None, sel=torch.from_numpy(sel.astype(np.int32)).cuda())
     check_rows(c, q, out, nQ, nKV, torch.stack([c.mask(None, blocks[:, g]) for g in range(nKV)]))
+
+
+@pytest.mark.parametrize("M,nQ,nKV,n,open_,tree", [(1, 16, 4, 30, 8192, False), (9, 8, 2, 3, 20001, True),
+                                                   (64, 16, 2, 0, 9000, True), (3, 64, 16, 1, 16500, False)])
+def test_rings_of_several_units_a_part(ctx, M, nQ, nKV, n, open_, tree):
+    """Open rows past 8192, an infinity and a NaN among the values in different units."""
+    import torch
+
+    from tests.test_gpu_kv8 import Ctx8, gen, run_attn
+
+    rnd = gen(open_ + 1)
+    c = Ctx8(ctx, rnd, nKV, n, open_, M, spread=0.5)
+    parents = ref.tree(M, np.random.default_rng(M)) if tree else None
+    q = rnd(M, nQ * D).half()
+    out, _ = run_attn(ctx, c, q, nQ, nKV, parents)
+    G, ok = nQ // nKV, c.mask(parents)
+
+    def check(skip=()):
+        for g in range(nKV):
+            want, _, tol, _ = attend(q.reshape(M, nKV, G, D)[:, g], *c.keys(g), ok, G)
+            err = (out.double().reshape(M, nKV, G, D)[:, g].reshape(M * G, D) - want).abs()
+            keep = [d for d in range(D) if (g, d) not in skip]
+            assert (err <= tol)[:, keep].all(), g
+
+    check()
+    c.rv[0, c.slots[5], 3], c.rv[nKV - 1, c.slots[open_ - 70], 77] = math.inf, math.nan
+    out, _ = run_attn(ctx, c, q, nQ, nKV, parents)
+    o = out.reshape(M, nKV, G, D)
+    assert (o[:, 0, :, 3] == math.inf).all() and o[:, nKV - 1, :, 77].isnan().all()
+    c.rv[0, c.slots[5], 3], c.rv[nKV - 1, c.slots[open_ - 70], 77] = 0.0, 0.0
+    check(skip={(0, 3), (nKV - 1, 77)})
