@@ -153,7 +153,7 @@ __device__ __forceinline__ uint32_t wave_ext(uint32_t v) {
 // A 256-thread block seals K (blockIdx.z 0) or V (1) of one block of one head: 16 KB in, 8 KB of
 // codes out.  Thread t holds dims 8 (t % 16) .. + 7 of tokens t / 16 + 16 i.  K codes go straight to
 // their 8-byte places; V codes are turned by way of LDS, as a page has four tokens of a dim side by
-// side.  Bound by memory: 2048 blocks of 4 heads, 402 MB, in 79 us (5.1 TB/s; a copy reaches 5.2); the
+// side.  Bound by memory: 2048 blocks of 4 heads, 402 MB, in about 80 us (5 TB/s; a copy reaches 5.2); the
 // ring's rows, done with here, pass by the caches (87 us else, the codes' lines pushed out).
 __global__ __launch_bounds__(256) void k_kv8_seal(Kv8Pool p, Kv8Ring ring, int64_t slot0, int at,
                                                   const int* abort) {
