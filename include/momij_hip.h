@@ -208,7 +208,8 @@ mj_status mj_attn_block(mj_ctx* ctx, const mj_attn_config* cfg, const mj_attn_we
 
 /* Pool of pages and the lists of them.  A page holds one block of one KV head: 64 x 128 codes of K
  * and of V, a scale for each, and the greatest and the least K code of every dim.  A value is
- * code * scale.  Page bytes are in the order the matrix instructions take them:
+ * code * scale, scales 0 or more (a V scale below 2^-31, which sealing never writes, counts as 2^-31).
+ * Page bytes are in the order the matrix instructions take them:
  *   K: byte 2048 (t / 16) + 1024 (d / 64) + 256 (d / 16 % 4) + 16 (t % 16) + d % 16
  *   V: byte 1024 (d / 16) + 256 (t / 4 % 4) + 16 (d % 16) + 4 (t / 16) + t % 4
  * of token t, dim d, each byte its code + 128.  table[g * table_stride + i] is the page of the i-th
@@ -249,8 +250,7 @@ mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv,
 /* Positions [pos, pos + 64 count) of the ring sealed into the pages of table entries at .. at +
  * count - 1 of every head: scale = m / 127 and code = round(x * (127 / m)) to the nearest whole
  * number, ties to even, each operation in fp32, m the block's greatest finite magnitude (0: all
- * codes 0).  An infinity takes the code +-127, a NaN 0.  64 count <= capacity.
- * A page that two of the entries name holds parts of either block. */
+ * codes 0).  An infinity takes the code +-127, a NaN 0.  64 count <= capacity. */
 mj_status mj_kv8_seal(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int64_t pos,
                       int count, int at);
 /* The way back, for a rewind into sealed blocks: entries at .. at + count - 1 to positions

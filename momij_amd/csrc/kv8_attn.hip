@@ -4,6 +4,7 @@
 // one page or 64 rows of the ring; a part is a run of units that one block takes; the parts of a row
 // and head are joined by k_kv8_combine.  Scores are kept in log2 units (scale * log2 e).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "mj_device.h"
@@ -898,30 +899,30 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
 
 #define ATTN_LDS 65536  // two pages as halves; the waves' outputs side by side; a ring unit
 
-template <typename K>
-static hipError_t launch_one(K kernel, const hipError_t& attr, const Kv8AttnArgs& a, hipStream_t st) {
-    if (attr != hipSuccess) return attr;
-    hipLaunchKernelGGL(kernel, dim3(a.parts, a.cols, a.p.nKV), dim3(64 * NWAVES), ATTN_LDS, st, a);
+// The LDS past 64 KB is asked for once a kernel and device.
+template <auto KERNEL>
+static hipError_t launch_one(const Kv8AttnArgs& a, hipStream_t st) {
+    static std::atomic<uint64_t> raised{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(raised.load(std::memory_order_relaxed) & bit)) {
+        e = hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, ATTN_LDS);
+        if (e != hipSuccess) return e;
+        raised.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(KERNEL, dim3(a.parts, a.cols, a.p.nKV), dim3(64 * NWAVES), ATTN_LDS, st, a);
     return hipGetLastError();
-}
-static hipError_t raise_lds(const void* kernel) {
-    return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, ATTN_LDS);
-}
-template <int T, bool MASS>
-static hipError_t launch_shared(const Kv8AttnArgs& a, hipStream_t st) {
-    static const hipError_t s = raise_lds((const void*)k_kv8_attn_shared<T, NWAVES, MASS>);
-    return launch_one(k_kv8_attn_shared<T, NWAVES, MASS>, s, a, st);
-}
-template <int T, int P, bool MASS>
-static hipError_t launch_own(const Kv8AttnArgs& a, hipStream_t st) {
-    static const hipError_t s = raise_lds((const void*)k_kv8_attn_own<T, P, NWAVES, MASS>);
-    return launch_one(k_kv8_attn_own<T, P, NWAVES, MASS>, s, a, st);
 }
 template <bool MASS>
 static hipError_t launch_pages(const Kv8AttnArgs& a, hipStream_t st) {
-    if (a.shared) return a.tiles == 1 ? launch_shared<1, MASS>(a, st) : launch_shared<2, MASS>(a, st);
-    if (a.pair == 2) return launch_own<2, 2, MASS>(a, st);
-    return a.tiles == 1 ? launch_own<1, 1, MASS>(a, st) : launch_own<2, 1, MASS>(a, st);
+    if (a.shared)
+        return a.tiles == 1 ? launch_one<k_kv8_attn_shared<1, NWAVES, MASS>>(a, st)
+                            : launch_one<k_kv8_attn_shared<2, NWAVES, MASS>>(a, st);
+    if (a.pair == 2) return launch_one<k_kv8_attn_own<2, 2, NWAVES, MASS>>(a, st);
+    return a.tiles == 1 ? launch_one<k_kv8_attn_own<1, 1, NWAVES, MASS>>(a, st)
+                        : launch_one<k_kv8_attn_own<2, 1, NWAVES, MASS>>(a, st);
 }
 
 template <bool MASS>
