@@ -736,3 +736,51 @@ def test_rings_of_several_units_a_part(ctx, M, nQ, nKV, n, open_, tree):
     assert (o[:, 0, :, 3] == math.inf).all() and o[:, nKV - 1, :, 77].isnan().all()
     c.rv[0, c.slots[5], 3], c.rv[nKV - 1, c.slots[open_ - 70], 77] = 0.0, 0.0
     check(skip={(0, 3), (nKV - 1, 77)})
+
+
+# -------------------------------------------------------------------------- scales far apart
+@pytest.mark.parametrize("nQ,lead", [(4, 0.6), (4, 0.2), (32, 0.6), (64, 1.2)])
+def test_v_scales_far_apart(ctx, nQ, lead):
+    """Blocks of V from the least fp16 number to the greatest, one of zeros; each row attends to one block
+    above all.  The weights carry the V scale into fp16, so a block's bound counts the steps of weights
+    below fp16's normal range: 2^-25 of a code, in units of at most the greatest weight times scale."""
+    import torch
+
+    from momij_amd.kv8 import Kv8Cache, KvRing
+
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(nQ)
+
+    def rnd(*s):
+        return torch.randn(s, generator=gen, device="cuda")
+
+    n = M = 21
+    way = rnd(n, 1, D)
+    kk = (0.3 * rnd(n, B, D) + 3 * way).half()
+    amp = 2.0 ** torch.linspace(-24, 13, n, device="cuda")[torch.randperm(n, generator=gen, device="cuda")]
+    vv = (rnd(n, B, D) * amp[:, None, None]).clamp(-65504, 65504).half()
+    vv[4] = 0.0
+    vv[9] = 0.0
+    vv[9, 3, 7] = 2.0 ** -24
+    rk, rv = rnd(1, M + 40, D).half(), rnd(1, M + 40, D).half()
+    q = (0.5 * rnd(M, nQ, D) + lead * way).half().reshape(M, nQ * D)
+    cache, out = Kv8Cache(ctx, 1, n), torch.empty_like(q)
+    torch.cuda.synchronize()
+    ctx.kv8_seal(cache, KvRing(kk.reshape(1, -1, D), vv.reshape(1, -1, D)), 0, n, 0)
+    ctx.kv8_attn(cache, KvRing(rk, rv), q, M, nQ, n, n * B, n * B + 40, None, out, mass_out=cache.mass)
+    ctx.sync()
+    (kc, ks), (vc, vs) = ref.seal(kk), ref.seal(vv)
+    at = [(n * B + i) % (M + 40) for i in range(M + 40)]
+    k = torch.cat([(kc * ks.double()[:, None, None]).reshape(-1, D), rk[0, at].double()])
+    scale = torch.cat([vs.double().repeat_interleave(B), torch.ones(M + 40, device="cuda").double()])
+    code = torch.cat([vc.reshape(-1, D), rv[0, at].double()])
+    ok = torch.cat([torch.ones((M, n * B + 40), dtype=torch.bool), ref.sees(None, M)[0]], 1).cuda()
+    want, p, _, rel = attend(q, k, code * scale[:, None], ok, nQ)
+    unit = (p * scale).amax(1, keepdim=True)
+    tol = (p @ (code * scale[:, None]).abs()) * (ref.E16 + rel + 2.0 ** -20) + want.abs() * ref.E16
+    tol += 2.0 ** -25 * (1 + unit * code.abs().sum(0))
+    err = (out.double().reshape(M * nQ, D) - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+    add = p[:, :n * B].reshape(M * nQ, n, B).sum(2)
+    tol = (add * (rel + 2.0 ** -20)).sum(0) + add.sum(0) * (M * nQ + 4) * ref.E32 + 1e-30
+    assert ((cache.mass[0].double() - add.sum(0)).abs() <= tol).all()
