@@ -433,8 +433,8 @@ __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u
 // parts; rows with lists of their own (a.sel) as below.  64 rows of 16 heads over 65500 tokens: 46 us, 0.74
 // PFLOP/s, the matrix units busy 39% of the time and the VALU 50% (the softmax, the codes).  17 rows
 // over 32000 tokens with masses 17.5 us: eight pages a block, each a barrier and a chain of products,
-// softmax and products that its few waves do not cover (a second page on its way, or half the LDS
-// reads, change nothing).
+// softmax and products that its few waves do not cover (a second page on its way, half the LDS
+// reads, or the next page's scores under a page's softmax change nothing).
 template <int T, int NW, bool MASS>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NR = 512 / NT;
