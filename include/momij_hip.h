@@ -241,7 +241,7 @@ typedef struct mj_kv_ring {
  * first rope_dim dims (0, 32, 64 or 128; halves (i, i + rope_dim / 2) of a head rotate together) at
  * the row's position L + depth(r), angles formed in 64 bits; parents_host as in mj_attn_block.  qkv
  * fp16 [M] rows of ld_qkv halves (0: packed; else a multiple of 8): the q, k and v heads of a raw
- * projection.  q_out fp16 [M][n_heads * 128]; keys and values of row r go to slot (L + r) %
+ * projection.  q_out fp16 [M][n_heads * 128], not over qkv; keys and values of row r go to slot (L + r) %
  * capacity.  Reads n_heads, n_kv_heads, head_dim, rope_dim, rope_base and eps of cfg. */
 mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv, int64_t ld_qkv,
                         const void* q_norm_w, const void* k_norm_w, const mj_kv_ring* ring,
@@ -297,8 +297,9 @@ mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, 
 mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep, int n_first,
                        int n_last, const float* mass_in, int32_t* table_out, float* mass_out);
 
-/* Bytes of workspace that mj_kv8_select and mj_kv8_attn with these sizes (ring_rows = L - start + M;
- * n_sel 0: every block; mass: mass_out given) take at most; 0 where an argument is out of range. */
+/* Bytes of workspace that mj_kv8_select and mj_kv8_attn with these sizes or smaller ones of the same heads
+ * (ring_rows = L - start + M; n_sel 0: every block; mass: mass_out given) take at most; 0 where an
+ * argument is out of range. */
 size_t mj_kv8_workspace(int n_heads, int n_kv_heads, int M, int n_blocks, int n_sel,
                         int64_t ring_rows, int mass);
 

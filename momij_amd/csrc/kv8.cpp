@@ -356,9 +356,8 @@ size_t mj_kv8_workspace(int n_heads, int n_kv_heads, int M, int n_blocks, int n_
         n_blocks > kMaxBlocks || n_sel < 0 || n_sel > kMaxBlocks || ring_rows < M ||
         ring_rows >= kMaxRing)
         return 0;
-    Kv8AttnArgs a{};
-    attn_sizes(a, n_kv_heads, n_heads, M, n_blocks, n_sel, ring_rows);
-    return std::max(kv8_attn_plan(a, mass != 0 && n_sel == 0 && n_blocks > 0, nullptr),
+    return std::max(kv8_attn_bound(n_kv_heads, M * n_heads, n_sel > 0 ? n_sel : n_blocks, ring_rows,
+                                   mass && n_sel == 0 ? n_blocks : 0),
                     select_bytes(M, n_kv_heads, n_blocks));
 }
 

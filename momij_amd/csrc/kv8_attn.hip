@@ -853,6 +853,8 @@ __global__ __launch_bounds__(32 * NG) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 #define NWAVES 8
+#define CHIP 256       // blocks of the attention launch, one a CU
+#define RING_MOST 128  // parts of a ring
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.n_list = a.n_sel > 0 ? a.n_sel : a.n;
     a.ring_units = (a.R + a.M + KV8_B - 1) / KV8_B;
@@ -876,7 +878,7 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     // one block a CU, those of the ring (small, first in the grid) among them: a block more than the
     // chip holds would run alone at the end.  A ring of many units leaves the pages half the chip, and
     // one of more than 8192 rows takes several units a part (the parts' outputs grow with them).
-    const int share = 256 / (a.cols * a.p.nKV), ring_most = std::max(share, 128);
+    const int share = CHIP / (a.cols * a.p.nKV), ring_most = std::max(share, RING_MOST);
     a.upr = (a.ring_units + ring_most - 1) / ring_most;
     a.ring_parts = (a.ring_units + a.upr - 1) / a.upr;
     int parts = std::max({1, share / 2, share - a.ring_parts});
@@ -895,6 +897,16 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     a.ml = (float2*)take(vecs * a.parts * 8);
     a.rec = mass ? (float2*)take((vecs * a.n + 16) * 8) : nullptr;
     return off;
+}
+
+// A plan's parts: at most a list's blocks and CHIP / (cols nKV), and of the ring its units and ring_most.
+// A column has at most 16 tiles, so vectors times page parts stay below 256 CHIP, or one part each.
+size_t kv8_attn_bound(int nKV, int64_t vecs, int n_list, int64_t ring_rows, int n_mass) {
+    const int64_t share = std::max(1, CHIP / nKV);
+    const int64_t units = (ring_rows + KV8_B - 1) / KV8_B;
+    const int64_t pages = std::min(vecs * std::min<int64_t>(n_list, share), std::max<int64_t>(vecs, 256 * CHIP));
+    const int64_t ring = vecs * std::min(units, std::max<int64_t>(share, RING_MOST));
+    return (size_t)(pages + ring) * (HD * 4 + 8) + (n_mass ? ((size_t)vecs * n_mass + 16) * 8 : 0) + 1024;
 }
 
 #define ATTN_LDS 65536  // two pages as halves; the waves' outputs side by side; a ring unit

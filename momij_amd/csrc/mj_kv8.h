@@ -87,4 +87,7 @@ struct Kv8AttnArgs {
 // Fills the plan fields for the sizes given and returns the workspace bytes; base (nullable) is
 // where the workspace lies.
 size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base);
+// Bytes that no plan of up to vecs query vectors (of all heads), n_list blocks a list, ring_rows open
+// and new rows and n_mass blocks with masses passes.
+size_t kv8_attn_bound(int nKV, int64_t vecs, int n_list, int64_t ring_rows, int n_mass);
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t st);

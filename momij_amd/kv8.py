@@ -29,6 +29,8 @@ class KvRing:
     def __init__(self, k, v, capacity: int | None = None):
         self.k, self.v = k, v
         if capacity is None:
+            if isinstance(k, int):
+                raise ValueError("ring addresses need their capacity")
             if k.shape != v.shape or k.dim() != 3 or k.shape[2] != 128 or not (
                     k.is_contiguous() and v.is_contiguous()):
                 raise ValueError("ring tensors: two contiguous [n_kv_heads][capacity][128]")

@@ -223,3 +223,42 @@ def test_workspace():
                  (16, 4, 2, -1, 0, 2, 0), (16, 4, 2, (1 << 20) + 1, 0, 2, 0), (16, 4, 2, 8, -1, 2, 0),
                  (16, 4, 2, 8, (1 << 20) + 1, 2, 0), (16, 4, 2, 8, 0, 1, 0), (16, 4, 2, 8, 0, 1 << 30, 0)):
         assert ws(*args) == 0, args
+
+
+def test_workspace_serves_smaller_calls(call):
+    """What a call asks for (it is refused without) is within the workspace of its sizes and of any
+    greater ones."""
+    import random
+    import re
+
+    ws, rng = _lib.load().mj_kv8_workspace, random.Random(4)
+    big = kv8(stride=1 << 20, n_pages=1 << 30)
+
+    def need(nkv, nq, M, n, n_sel, rows, mass):
+        big.n_kv_heads = nkv
+        st, msg = call("mj_kv8_attn", big, ring(cap=1 << 29), nq, P, 0, M, n, P if n_sel else None, n_sel,
+                       0, rows - M, None, P, 0, None, P if mass else None, P, 0)
+        assert st == BAD, msg
+        return int(re.search(r"needs (\d+)", msg).group(1))
+
+    for nkv, g in ((4, 4), (1, 8), (1, 64), (8, 8), (32, 1), (64, 1), (1024, 1), (2, 64), (300, 3)):
+        for _ in range(40):
+            M, n, rows = rng.choice([1, 2, 9, 17, 33, 64]), rng.choice([0, 1, 75, 76, 2047, 99999]), \
+                rng.choice([0, 1, 80, 8000, 8300, 131000, 2 ** 28])
+            n_sel, mass = rng.choice([0, 0, 5, 64, 3000]), rng.choice([0, 1])
+            mass = 0 if n_sel else mass
+            bound = ws(nkv * g, nkv, M, n, n_sel, rows + M, mass)
+            for k in range(12):
+                m = M if k % 3 == 0 else rng.randint(1, M)
+                s = n_sel and rng.randint(1, n_sel)
+                size = (m, n if k % 2 else rng.randint(0, n), s, m + (rows if k % 4 else rng.randint(0, rows)))
+                assert need(nkv, nkv * g, *size, mass) <= bound, (nkv, g, M, n, n_sel, rows, mass, size)
+                assert ws(nkv * g, nkv, *size, mass) <= bound
+
+
+def test_ring_addresses_need_a_capacity():
+    from momij_amd.kv8 import KvRing
+
+    with pytest.raises(ValueError):
+        KvRing(P, P)
+    assert KvRing(P, P, capacity=7).struct.capacity == 7
