@@ -254,7 +254,8 @@ mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv,
 mj_status mj_kv8_seal(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int64_t pos,
                       int count, int at);
 /* The way back, for a rewind into sealed blocks: entries at .. at + count - 1 to positions
- * [pos, pos + 64 count) of the ring, half(code * scale). */
+ * [pos, pos + 64 count) of the ring, half(code * scale).  Masses are the caller's: those of entries
+ * that will be sealed again want clearing. */
 mj_status mj_kv8_unseal(mj_ctx* ctx, const mj_kv8* cache, int at, int count,
                         const mj_kv_ring* ring, int64_t pos);
 

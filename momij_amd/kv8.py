@@ -15,6 +15,8 @@ A layer's context in use:
     # a bounded cache: the blocks that got the least attention go, their pages are used again
     ctx.kv8_attn(..., mass_in=cache.mass, mass_out=cache.mass)
     cache.evict(n, keep, n_first=1, n_last=4); n = keep
+    # a rewind into sealed blocks: back to the ring, their weight forgotten
+    n, start = n - 1, start - 64; ctx.kv8_unseal(cache, n, 1, ring, start); cache.mass[:, n:] = 0
 """
 from __future__ import annotations
 
