@@ -20,26 +20,47 @@ A layer's context in use:
 """
 from __future__ import annotations
 
+import torch
+
 from . import _lib
 from .ops import ptr
 
 
 class KvRing:
-    """K and V rows fp16 [n_kv_heads][capacity][128]: torch tensors, or device addresses (those of
-    VerifyEngine.kv) with the capacity given."""
+    """K and V rows fp16 [n_kv_heads][capacity][128]: torch tensors (flat ones with the capacity
+    given), or device addresses (those of VerifyEngine.kv) with the capacity given and, for the
+    calls to check, the heads."""
 
-    def __init__(self, k, v, capacity: int | None = None):
-        self.k, self.v = k, v
+    def __init__(self, k, v, capacity: int | None = None, n_kv_heads: int | None = None):
+        self.k, self.v, self.device = k, v, None
+        tensors = [t for t in (k, v) if not isinstance(t, int)]
         if capacity is None:
-            if isinstance(k, int):
+            if len(tensors) < 2:
                 raise ValueError("ring addresses need their capacity")
-            if k.shape != v.shape or k.dim() != 3 or k.shape[2] != 128 or not (
-                    k.is_contiguous() and v.is_contiguous()):
-                raise ValueError("ring tensors: two contiguous [n_kv_heads][capacity][128]")
+            if k.dim() != 3:
+                raise ValueError("ring tensors: two contiguous fp16 [n_kv_heads][capacity][128]")
             capacity = k.shape[1]
-        self.capacity = int(capacity)
+        self.capacity, self.n_kv_heads = int(capacity), n_kv_heads
+        for t in tensors:
+            row = self.capacity * 128
+            heads = t.numel() // row if row > 0 else 0
+            if heads < 1 or t.numel() != heads * row or (
+                    t.dim() > 1 and t.shape != (heads, self.capacity, 128)) or (
+                    t.dtype != torch.float16 or not t.is_contiguous()):
+                raise ValueError("ring tensors: two contiguous fp16 [n_kv_heads][capacity][128]")
+            if self.n_kv_heads not in (heads, None) or self.device not in (t.get_device(), None):
+                raise ValueError("ring tensors: of the same heads on one device")
+            self.n_kv_heads, self.device = heads, t.get_device()
         addr = [t if isinstance(t, int) else ptr(t) for t in (k, v)]
         self.struct = _lib.KvRingStruct(addr[0], addr[1], self.capacity)
+
+    def of(self, n_kv_heads: int, device: int) -> _lib.KvRingStruct:
+        """The struct for a call of n_kv_heads on `device`: a ring of fewer heads would be read and
+        written past its end."""
+        if self.n_kv_heads not in (n_kv_heads, None) or self.device not in (device, None):
+            raise ValueError(f"a ring of {self.n_kv_heads} heads on device {self.device} in a call of "
+                             f"{n_kv_heads} on device {device}")
+        return self.struct
 
 
 class Kv8Cache:
@@ -47,8 +68,6 @@ class Kv8Cache:
     [n_kv_heads][blocks] holds the blocks' accumulated attention weight."""
 
     def __init__(self, ctx, n_kv_heads: int, blocks: int):
-        import torch
-
         device = torch.device("cuda", ctx.device)
 
         self.ctx, self.n_kv_heads, self.blocks = ctx, n_kv_heads, blocks
@@ -70,6 +89,12 @@ class Kv8Cache:
         self.struct = _lib.Kv8(self.n_kv_heads, self.n_kv_heads * self.blocks, ptr(self.k_codes),
                                ptr(self.v_codes), ptr(self.k_scale), ptr(self.v_scale),
                                ptr(self.k_bounds), ptr(self.table), self.blocks)
+
+    def on(self, device: int) -> _lib.Kv8:
+        """The struct for a call on `device`."""
+        if self.ctx.device != device:
+            raise ValueError(f"a cache on device {self.ctx.device} in a call on device {device}")
+        return self.struct
 
     def evict(self, n_blocks: int, keep: int, n_first: int = 1, n_last: int = 1):
         """Down to `keep` blocks a head by `mass`; table and mass change places with their spares

@@ -123,20 +123,21 @@ class Context:
         c = self.attn_config(cfg)
         ld = qkv.stride(0) if M > 1 else 0
         self.check(self.lib.mj_qkv_append(self.h, C.byref(c), ptr(qkv), ld, ptr(q_norm_w),
-                                          ptr(k_norm_w), C.byref(ring.struct), L,
+                                          ptr(k_norm_w), C.byref(ring.of(c.n_kv_heads, self.device)), L,
                                           self._parents(parents, M), M, ptr(q_out)))
 
     def kv8_seal(self, cache, ring, pos: int, count: int, at: int):
-        self.check(self.lib.mj_kv8_seal(self.h, C.byref(cache.struct), C.byref(ring.struct), pos,
-                                        count, at))
+        self.check(self.lib.mj_kv8_seal(self.h, C.byref(cache.on(self.device)),
+                                        C.byref(ring.of(cache.n_kv_heads, self.device)), pos, count,
+                                        at))
 
     def kv8_unseal(self, cache, at: int, count: int, ring, pos: int):
-        self.check(self.lib.mj_kv8_unseal(self.h, C.byref(cache.struct), at, count,
-                                          C.byref(ring.struct), pos))
+        self.check(self.lib.mj_kv8_unseal(self.h, C.byref(cache.on(self.device)), at, count,
+                                          C.byref(ring.of(cache.n_kv_heads, self.device)), pos))
 
     def kv8_select(self, cache, q, M: int, n_heads: int, n_blocks: int, n_sel: int, n_first: int,
                    n_last: int, sel, ws=None):
-        self.check(self.lib.mj_kv8_select(self.h, C.byref(cache.struct), n_heads, ptr(q),
+        self.check(self.lib.mj_kv8_select(self.h, C.byref(cache.on(self.device)), n_heads, ptr(q),
                                           q.stride(0) if M > 1 else 0, M, n_blocks, n_sel, n_first,
                                           n_last, ptr(sel), ptr(ws),
                                           0 if ws is None else ws.numel() * ws.element_size()))
@@ -144,7 +145,8 @@ class Context:
     def kv8_attn(self, cache, ring, q, M: int, n_heads: int, n_blocks: int, start: int, L: int,
                  parents, out, sel=None, mass_in=None, mass_out=None, ws=None):
         """sel int32 [M][n_kv_heads][n_sel] (kv8_select's) or None: every block."""
-        self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.struct), C.byref(ring.struct), n_heads,
+        self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.on(self.device)),
+                                        C.byref(ring.of(cache.n_kv_heads, self.device)), n_heads,
                                         ptr(q), q.stride(0) if M > 1 else 0, M, n_blocks, ptr(sel),
                                         0 if sel is None else sel.shape[-1], start, L,
                                         self._parents(parents, M), ptr(out),
@@ -153,7 +155,7 @@ class Context:
 
     def kv8_evict(self, cache, n_blocks: int, keep: int, n_first: int, n_last: int, mass_in,
                   table_out, mass_out):
-        self.check(self.lib.mj_kv8_evict(self.h, C.byref(cache.struct), n_blocks, keep, n_first,
+        self.check(self.lib.mj_kv8_evict(self.h, C.byref(cache.on(self.device)), n_blocks, keep, n_first,
                                          n_last, ptr(mass_in), ptr(table_out), ptr(mass_out)))
 
     def kv8_workspace(self, n_heads: int, n_kv_heads: int, M: int, n_blocks: int, n_sel: int,
@@ -167,7 +169,8 @@ class Context:
         c = self.attn_config(cfg)
         w = self.attn_struct(aw)
         self.check(self.lib.mj_attn_block_kv8(self.h, C.byref(c), C.byref(w),
-                                              C.byref(cache.struct), C.byref(ring.struct), ptr(h),
+                                              C.byref(cache.on(self.device)),
+                                              C.byref(ring.of(c.n_kv_heads, self.device)), ptr(h),
                                               n_blocks, n_sel, n_first, n_last, start, L,
                                               self._parents(parents, M), M, ptr(mass_in),
                                               ptr(mass_out)))
