@@ -9,6 +9,9 @@ from __future__ import annotations
 
 import ctypes as C
 from array import array
+from operator import itemgetter
+
+import torch
 
 from . import _lib
 from ._lib import AttnConfig, AttnWeights, LayerWeights, MoeWeights, ModelConfig, MomijError
@@ -21,10 +24,44 @@ def ptr(t) -> int | None:
     return t.data_ptr()
 
 
+_F16 = torch.float16
+_CONFIG = itemgetter("H", "nQ", "nKV", "D", "rope_dim", "rope_base", "eps", "window", "C", "gs")
+
+
+def row_stride(t, M: int, width: int, device: int, what: str) -> int:
+    """Halves between M rows of `width` fp16 values side by side, as the library's calls take it (0:
+    one row, or packed ones; hence no row that stands for all M)."""
+    if t.dtype is _F16 and t.get_device() == device:
+        if t.numel() == M * width and t.is_contiguous():
+            return 0
+        shape, step = t.shape, t.stride()
+        if len(shape) == 2 and shape[0] >= M and shape[1] >= width and step[1] == 1:
+            if M <= 1:
+                return 0
+            if step[0] >= width:
+                return step[0]
+        if M == 1 and t.numel() >= width and t.is_contiguous() and (
+                len(shape) == 1 or width % shape[-1] == 0):  # flat, or head by head
+            return 0
+        if len(shape) > 2 and shape[0] >= M and (M == 1 or step[0] >= width):
+            if t[0].numel() >= width and t[0].is_contiguous():
+                return step[0] if M > 1 else 0
+    raise ValueError(f"{what}: {M} rows of {width} fp16 values on device {device}, not {t.dtype} "
+                     f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
+
+
+def packed(t, dtype, rows: int, width: int, device: int, what: str) -> int:
+    """Address of `rows` rows of `width` values of a type without gaps."""
+    if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        n = t.numel()
+        if n == rows * width or n > rows * width and (rows <= 1 or t.stride(0) <= width):
+            return t.data_ptr()
+    raise ValueError(f"{what}: {rows} packed rows of {width} {dtype} on device {device}, not {t.dtype} "
+                     f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
+
+
 class Context:
     def __init__(self, device: int = 0):
-        import torch
-
         self.lib = _lib.load()
         h = C.c_void_p()
         st = self.lib.mj_init(device, C.byref(h))
@@ -96,8 +133,7 @@ class Context:
 
     @staticmethod
     def attn_config(cfg: dict) -> AttnConfig:
-        return AttnConfig(cfg["H"], cfg["nQ"], cfg["nKV"], cfg["D"], cfg["rope_dim"],
-                          cfg["rope_base"], cfg["eps"], cfg["window"], cfg["C"], cfg["gs"])
+        return AttnConfig(*_CONFIG(cfg))
 
     def attn_block(self, cfg: dict, aw: dict, h, kcache, vcache, L: int, parents, M: int):
         c = self.attn_config(cfg)
@@ -120,11 +156,12 @@ class Context:
     def qkv_append(self, cfg: dict, qkv, q_norm_w, k_norm_w, ring, L: int, parents, M: int, q_out):
         """Queries and keys normed and rotated, keys and values appended to the ring; qkv rows may
         be a slice of wider ones."""
-        c = self.attn_config(cfg)
-        ld = qkv.stride(0) if M > 1 else 0
-        self.check(self.lib.mj_qkv_append(self.h, C.byref(c), ptr(qkv), ld, ptr(q_norm_w),
-                                          ptr(k_norm_w), C.byref(ring.of(c.n_kv_heads, self.device)), L,
-                                          self._parents(parents, M), M, ptr(q_out)))
+        c, dev = self.attn_config(cfg), self.device
+        ld = row_stride(qkv, M, (c.n_heads + 2 * c.n_kv_heads) * 128, dev, "qkv")
+        self.check(self.lib.mj_qkv_append(self.h, C.byref(c), qkv.data_ptr(), ld,
+                                          ptr(q_norm_w), ptr(k_norm_w), C.byref(ring.of(c.n_kv_heads, dev)), L,
+                                          self._parents(parents, M), M,
+                                          packed(q_out, _F16, M, c.n_heads * 128, dev, "q_out")))
 
     def kv8_seal(self, cache, ring, pos: int, count: int, at: int):
         self.check(self.lib.mj_kv8_seal(self.h, C.byref(cache.on(self.device)),
@@ -138,19 +175,20 @@ class Context:
     def kv8_select(self, cache, q, M: int, n_heads: int, n_blocks: int, n_sel: int, n_first: int,
                    n_last: int, sel, ws=None):
         self.check(self.lib.mj_kv8_select(self.h, C.byref(cache.on(self.device)), n_heads, ptr(q),
-                                          q.stride(0) if M > 1 else 0, M, n_blocks, n_sel, n_first,
-                                          n_last, ptr(sel), ptr(ws),
+                                          row_stride(q, M, n_heads * 128, self.device, "q"), M,
+                                          n_blocks, n_sel, n_first, n_last, ptr(sel), ptr(ws),
                                           0 if ws is None else ws.numel() * ws.element_size()))
 
     def kv8_attn(self, cache, ring, q, M: int, n_heads: int, n_blocks: int, start: int, L: int,
                  parents, out, sel=None, mass_in=None, mass_out=None, ws=None):
         """sel int32 [M][n_kv_heads][n_sel] (kv8_select's) or None: every block."""
-        self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.on(self.device)),
-                                        C.byref(ring.of(cache.n_kv_heads, self.device)), n_heads,
-                                        ptr(q), q.stride(0) if M > 1 else 0, M, n_blocks, ptr(sel),
+        dev, width = self.device, n_heads * 128
+        self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.on(dev)),
+                                        C.byref(ring.of(cache.n_kv_heads, dev)), n_heads, ptr(q),
+                                        row_stride(q, M, width, dev, "q"), M, n_blocks, ptr(sel),
                                         0 if sel is None else sel.shape[-1], start, L,
                                         self._parents(parents, M), ptr(out),
-                                        out.stride(0) if M > 1 else 0, ptr(mass_in), ptr(mass_out),
+                                        row_stride(out, M, width, dev, "out"), ptr(mass_in), ptr(mass_out),
                                         ptr(ws), 0 if ws is None else ws.numel() * ws.element_size()))
 
     def kv8_evict(self, cache, n_blocks: int, keep: int, n_first: int, n_last: int, mass_in,
@@ -170,7 +208,8 @@ class Context:
         w = self.attn_struct(aw)
         self.check(self.lib.mj_attn_block_kv8(self.h, C.byref(c), C.byref(w),
                                               C.byref(cache.on(self.device)),
-                                              C.byref(ring.of(c.n_kv_heads, self.device)), ptr(h),
+                                              C.byref(ring.of(c.n_kv_heads, self.device)),
+                                              packed(h, _F16, M, c.H, self.device, "h"),
                                               n_blocks, n_sel, n_first, n_last, start, L,
                                               self._parents(parents, M), M, ptr(mass_in),
                                               ptr(mass_out)))

@@ -8,7 +8,7 @@ import torch
 from momij_amd.kv8 import Kv8Cache, KvRing
 from momij_amd.ops import Context
 
-NQ, NKV, D, BLOCKS, C, M = 8, 2, 128, 6, 200, 3
+NQ, NKV, D, BLOCKS, C, M = 10, 2, 128, 6, 200, 3
 F16, F32, I32 = torch.float16, torch.float32, torch.int32
 
 
@@ -132,3 +132,58 @@ def test_rings_and_caches_of_another_device(ctx, f):
     refused(other, f, ring=ring, **({} if f is append else dict(cache=cache_of(other))))
     if f is not append:
         refused(other, f, cache=cache, ring=KvRing(4096, 8192, capacity=C))
+
+
+# -------------------------------------------------------------------------------------- rows
+def bad_rows(width, m=M):
+    """Tensors that do not hold m rows of `width` fp16 values side by side."""
+    return [z(m, width, dtype=F32), z(m, width).bfloat16(), z(m - 1, width), z(m, width - 8),
+            z(1, width).expand(m, width),          # one row for all: a stride of 0 means packed
+            z(width, m).T, z(m, 2 * width)[:, ::2],  # values apart
+            z(m * width).as_strided((m, width), (8, 1)),  # rows over each other
+            z(m, 2, width)[:, :, : width - 8], z(m, 2, width)[:, :, : width // 2], torch.zeros((), dtype=F16)]
+
+
+def good_rows(width, m=M):
+    """[tensor, stride in halves] (0: packed)"""
+    return [(z(m, width), 0), (z(m + 2, width), width), (z(m, width + 64)[:, 8:8 + width], width + 64),
+            (z(m, width // 128, 128), 0), (z(m + 1, width // 128, 128), width),
+            (z(m, 2, width)[:, 1], 2 * width)]
+
+
+@pytest.mark.parametrize("f,name,width,at", [
+    (append, "qkv", (NQ + 2 * NKV) * D, 3), (attn, "q", NQ * D, 5), (attn, "out", NQ * D, 14)])
+def test_strided_rows(ctx, f, name, width, at):
+    """Rows of a stride: the address and the stride come together in the library's arguments."""
+    for t in bad_rows(width):
+        refused(ctx, f, **{name: t})
+    for t, stride in good_rows(width):
+        args = taken(ctx, f, **{name: t})
+        assert args[at - 1] == t.data_ptr() and args[at] == stride
+    # a single row has none: the first of many, a slice, a flat vector, heads by heads
+    for t in (z(1, width), z(5, width + 8)[:, :width], z(width), z(width // 128, 128), z(1, width // 128, 128),
+              z(1, width).expand(4, width)):
+        args = taken(ctx, f, **{name: t, "m": 1})
+        assert args[at - 1] == t.data_ptr() and args[at] == 0
+    for t in (z(width - 8), z(1, 2 * width)[:, ::2], z(2 * width)[::2], z(width, dtype=F32), z(2, width - 8)):
+        refused(ctx, f, **{name: t, "m": 1})
+
+
+def test_query_rows_of_a_selection(ctx):
+    def select(ctx, q, m=M):
+        ctx.kv8_select(cache_of(ctx), q, m, NQ, 4, 2, 0, 0, z(m, NKV, 2, dtype=I32))
+
+    for t in bad_rows(NQ * D):
+        refused(ctx, select, q=t)
+    for t, stride in good_rows(NQ * D):
+        args = taken(ctx, select, q=t)
+        assert args[3] == t.data_ptr() and args[4] == stride
+
+
+@pytest.mark.parametrize("f,name,width", [(append, "q", NQ * D), (block, "h", 2048)])
+def test_packed_rows(ctx, f, name, width):
+    """Rows without a stride in the library's arguments: packed ones only."""
+    for t in bad_rows(width) + [z(M, width + 64)[:, :width], z(M, width + 64)]:
+        refused(ctx, f, **{name: t})
+    for t in (z(M, width), z(M + 1, width), z(M, width // 128, 128), z(M * width)):
+        taken(ctx, f, **{name: t})
