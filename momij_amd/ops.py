@@ -153,13 +153,31 @@ class Context:
             raise ValueError(f"{len(parents)} parents of {M} rows")
         return (C.c_int32 * M).from_buffer(array("i", parents))
 
+    def _list(self, sel, M: int, n_kv_heads: int, n_sel: int) -> int:
+        if (sel.dim() > 1 and sel.shape[-1] != n_sel) or (sel.dim() == 3 and sel.shape[1] != n_kv_heads):
+            raise ValueError(f"sel: {tuple(sel.shape)}, not [{M}][{n_kv_heads}][{n_sel}]")
+        return packed(sel, torch.int32, M, n_kv_heads * n_sel, self.device, "sel")
+
+    def _mass(self, mass, cache) -> int | None:
+        if mass is None:
+            return None
+        return packed(mass, torch.float32, cache.n_kv_heads, cache.blocks, self.device, "mass")
+
+    def _space(self, ws) -> tuple:
+        if ws is None:
+            return None, 0
+        if not ws.is_contiguous() or ws.get_device() != self.device:
+            raise ValueError(f"ws: contiguous memory on device {self.device}")
+        return ws.data_ptr(), ws.numel() * ws.element_size()
+
     def qkv_append(self, cfg: dict, qkv, q_norm_w, k_norm_w, ring, L: int, parents, M: int, q_out):
         """Queries and keys normed and rotated, keys and values appended to the ring; qkv rows may
         be a slice of wider ones."""
         c, dev = self.attn_config(cfg), self.device
         ld = row_stride(qkv, M, (c.n_heads + 2 * c.n_kv_heads) * 128, dev, "qkv")
         self.check(self.lib.mj_qkv_append(self.h, C.byref(c), qkv.data_ptr(), ld,
-                                          ptr(q_norm_w), ptr(k_norm_w), C.byref(ring.of(c.n_kv_heads, dev)), L,
+                                          ptr(q_norm_w), ptr(k_norm_w),
+                                          C.byref(ring.of(c.n_kv_heads, dev)), L,
                                           self._parents(parents, M), M,
                                           packed(q_out, _F16, M, c.n_heads * 128, dev, "q_out")))
 
@@ -176,25 +194,32 @@ class Context:
                    n_last: int, sel, ws=None):
         self.check(self.lib.mj_kv8_select(self.h, C.byref(cache.on(self.device)), n_heads, ptr(q),
                                           row_stride(q, M, n_heads * 128, self.device, "q"), M,
-                                          n_blocks, n_sel, n_first, n_last, ptr(sel), ptr(ws),
-                                          0 if ws is None else ws.numel() * ws.element_size()))
+                                          n_blocks, n_sel, n_first, n_last,
+                                          self._list(sel, M, cache.n_kv_heads, n_sel),
+                                          *self._space(ws)))
 
     def kv8_attn(self, cache, ring, q, M: int, n_heads: int, n_blocks: int, start: int, L: int,
                  parents, out, sel=None, mass_in=None, mass_out=None, ws=None):
         """sel int32 [M][n_kv_heads][n_sel] (kv8_select's) or None: every block."""
-        dev, width = self.device, n_heads * 128
+        dev, width, n_sel, lists = self.device, n_heads * 128, 0, None
+        if sel is not None:
+            n_sel = sel.shape[-1]
+            lists = self._list(sel, M, cache.n_kv_heads, n_sel)
         self.check(self.lib.mj_kv8_attn(self.h, C.byref(cache.on(dev)),
                                         C.byref(ring.of(cache.n_kv_heads, dev)), n_heads, ptr(q),
-                                        row_stride(q, M, width, dev, "q"), M, n_blocks, ptr(sel),
-                                        0 if sel is None else sel.shape[-1], start, L,
-                                        self._parents(parents, M), ptr(out),
-                                        row_stride(out, M, width, dev, "out"), ptr(mass_in), ptr(mass_out),
-                                        ptr(ws), 0 if ws is None else ws.numel() * ws.element_size()))
+                                        row_stride(q, M, width, dev, "q"), M, n_blocks, lists, n_sel,
+                                        start, L, self._parents(parents, M), ptr(out),
+                                        row_stride(out, M, width, dev, "out"),
+                                        self._mass(mass_in, cache), self._mass(mass_out, cache),
+                                        *self._space(ws)))
 
     def kv8_evict(self, cache, n_blocks: int, keep: int, n_first: int, n_last: int, mass_in,
                   table_out, mass_out):
         self.check(self.lib.mj_kv8_evict(self.h, C.byref(cache.on(self.device)), n_blocks, keep, n_first,
-                                         n_last, ptr(mass_in), ptr(table_out), ptr(mass_out)))
+                                         n_last, self._mass(mass_in, cache),
+                                         packed(table_out, torch.int32, cache.n_kv_heads, cache.blocks,
+                                                self.device, "table_out"),
+                                         self._mass(mass_out, cache)))
 
     def kv8_workspace(self, n_heads: int, n_kv_heads: int, M: int, n_blocks: int, n_sel: int,
                       ring_rows: int, mass: bool = False) -> int:
@@ -211,8 +236,8 @@ class Context:
                                               C.byref(ring.of(c.n_kv_heads, self.device)),
                                               packed(h, _F16, M, c.H, self.device, "h"),
                                               n_blocks, n_sel, n_first, n_last, start, L,
-                                              self._parents(parents, M), M, ptr(mass_in),
-                                              ptr(mass_out)))
+                                              self._parents(parents, M), M,
+                                              self._mass(mass_in, cache), self._mass(mass_out, cache)))
 
     def lm_head_verify(self, x, w, M, K, V, out_argmax, out_max=None, out_logits=None,
                        banned=None, n_banned=0, temperature=1.0, out_lse=None):

@@ -161,8 +161,8 @@ def test_strided_rows(ctx, f, name, width, at):
         args = taken(ctx, f, **{name: t})
         assert args[at - 1] == t.data_ptr() and args[at] == stride
     # a single row has none: the first of many, a slice, a flat vector, heads by heads
-    for t in (z(1, width), z(5, width + 8)[:, :width], z(width), z(width // 128, 128), z(1, width // 128, 128),
-              z(1, width).expand(4, width)):
+    for t in (z(1, width), z(5, width + 8)[:, :width], z(width), z(width // 128, 128),
+              z(1, width // 128, 128), z(1, width).expand(4, width)):
         args = taken(ctx, f, **{name: t, "m": 1})
         assert args[at - 1] == t.data_ptr() and args[at] == 0
     for t in (z(width - 8), z(1, 2 * width)[:, ::2], z(2 * width)[::2], z(width, dtype=F32), z(2, width - 8)):
@@ -187,3 +187,77 @@ def test_packed_rows(ctx, f, name, width):
         refused(ctx, f, **{name: t})
     for t in (z(M, width), z(M + 1, width), z(M, width // 128, 128), z(M * width)):
         taken(ctx, f, **{name: t})
+
+
+# ----------------------------------------------------------------- lists, masses, workspaces
+def select(ctx, sel=None, m=M, **kw):
+    ctx.kv8_select(cache_of(ctx), z(m, NQ * D), m, NQ, 4, 3, 0, 0,
+                   z(m, NKV, 3, dtype=I32) if sel is None else sel, **kw)
+
+
+def listed(ctx, sel, m=M):
+    attn(ctx, sel=sel, m=m)
+
+
+@pytest.mark.parametrize("f", [select, listed])
+def test_lists(ctx, f):
+    for t in (z(M, NKV, 3, dtype=torch.int64), z(M, NKV, 3), z(M - 1, NKV, 3, dtype=I32),
+              z(M, NKV, 6, dtype=I32)[..., :3],
+              z(M, NKV, 6, dtype=I32)[..., ::2], z(1, NKV, 3, dtype=I32).expand(M, NKV, 3),
+              z(M, 1, 3, dtype=I32).expand(M, NKV, 3), z(NKV, M, 3, dtype=I32).transpose(0, 1),
+              z(M, NKV + 1, 3, dtype=I32), z(M, 3, dtype=I32), z(3, dtype=I32), z(NKV, M, 3, dtype=I32)):
+        refused(ctx, f, sel=t)
+    for t in (z(M, NKV, 3, dtype=I32), z(M + 2, NKV, 3, dtype=I32), z(M * NKV, 3, dtype=I32)):
+        taken(ctx, f, sel=t)
+    taken(ctx, f, sel=z(1, NKV, 3, dtype=I32), m=1)
+    refused(ctx, f, sel=z(1, NKV, 3, dtype=I32), m=2)
+
+
+def test_lists_of_another_length_than_chosen(ctx):
+    for n in (2, 4):
+        refused(ctx, select, sel=z(M, NKV, n, dtype=I32))
+
+
+def bad_masses(t=F32):
+    """Not [NKV][BLOCKS] values of type t."""
+    return [z(NKV, BLOCKS, dtype=torch.float64), z(NKV, BLOCKS), z(NKV, BLOCKS - 1, dtype=t),
+            z(NKV - 1, BLOCKS, dtype=t), z(NKV, BLOCKS + 1, dtype=t)[:, :BLOCKS],
+            z(NKV, BLOCKS + 1, dtype=t), z(1, BLOCKS, dtype=t).expand(NKV, BLOCKS),
+            z(BLOCKS, NKV, dtype=t).T, z(0, dtype=t)]
+
+
+@pytest.mark.parametrize("f", [attn, block])
+def test_masses(ctx, f):
+    good = z(NKV, BLOCKS, dtype=F32)
+    for t in bad_masses():
+        refused(ctx, f, mass_out=t)
+        refused(ctx, f, mass_in=t, mass_out=good)
+    taken(ctx, f, mass_out=good)
+    taken(ctx, f, mass_in=good, mass_out=z(NKV + 1, BLOCKS, dtype=F32))
+
+
+def test_eviction(ctx):
+    def evict(ctx, mass=z(NKV, BLOCKS, dtype=F32), table=z(NKV, BLOCKS, dtype=I32),
+              out=z(NKV, BLOCKS, dtype=F32)):
+        ctx.kv8_evict(cache_of(ctx), 4, 2, 0, 0, mass, table, out)
+
+    for t in bad_masses():
+        refused(ctx, evict, mass=t)
+        refused(ctx, evict, out=t)
+    for t in bad_masses(I32):
+        refused(ctx, evict, table=t)
+    taken(ctx, evict)
+    cache = cache_of(ctx)
+    table, mass = cache.table, cache.mass
+    cache.evict(4, 2)
+    assert cache.table is not table and cache.mass is not mass and len(ctx.lib.calls) == 1
+
+
+@pytest.mark.parametrize("f", [select, attn])
+def test_workspaces(ctx, f):
+    for t in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 10, dtype=F32)[::2]):
+        refused(ctx, f, ws=t)
+    for t in (torch.zeros(1 << 10, dtype=torch.uint8), torch.zeros(1 << 8, dtype=F32)):
+        args = taken(ctx, f, ws=t)
+        assert args[-2:] == (t.data_ptr(), 1 << 10)
+    assert taken(ctx, f)[-2:] == (None, 0)
