@@ -278,8 +278,8 @@ mj_status mj_kv8_select(mj_ctx* ctx, const mj_kv8* cache, int n_heads, const voi
  * is listed twice counts twice.  q as in mj_kv8_select, out fp16 [M] rows of ld_out halves.  0 <=
  * start <= L, L - start + M <= ring capacity.
  * mass_out (nullable; not with sel) float [n_kv_heads][table_stride]: for every block its entry of
- * mass_in (same layout, NULL: zeros; may be mass_out) plus the softmax weight that all rows and the
- * group's heads gave the block's keys.
+ * mass_in (same layout, NULL: zeros; may be mass_out, not a part of it) plus the softmax weight that
+ * all rows and the group's heads gave the block's keys.
  * Scores, softmax statistics and outputs are summed in fp32; the weights are rounded to fp16 for the
  * product with V.  A call repeats bit for bit; a row's result in a call of other rows may differ by
  * rounding (the keys are split differently). */
@@ -293,8 +293,8 @@ mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, 
  * others, those of the greatest mass stay (the lower index on ties; a NaN counts as the least; each
  * head by its own masses).  table_out [n_kv_heads][table_stride] lists the kept blocks in their
  * order, then the evicted ones' pages (free now) in theirs, then the rest of the row unchanged;
- * mass_out likewise, 0 from `keep` on.  n_first + n_last <= keep <= n_blocks.  table_out must not
- * lie over cache->table, nor mass_out over mass_in. */
+ * mass_out likewise, 0 from `keep` on.  n_first + n_last <= keep <= n_blocks.  table_out and
+ * mass_out must lie over neither cache->table, mass_in nor each other. */
 mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep, int n_first,
                        int n_last, const float* mass_in, int32_t* table_out, float* mass_out);
 

@@ -29,9 +29,9 @@ bool aligned16(std::initializer_list<const void*> ps) {
     return (bits & 15) == 0;
 }
 
-bool overlap(const void* a, const void* b, size_t bytes) {
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y ? y - x < bytes : x - y < bytes;
+    return x < y ? y - x < a_bytes : x - y < b_bytes;
 }
 
 constexpr int kMaxGroup = 64;              // query heads a KV head
@@ -124,7 +124,7 @@ void attn_sizes(Kv8AttnArgs& a, int n_kv, int n_heads, int M, int n_blocks, int 
 
 mj_status fill_attn(mj_ctx* ctx, Kv8AttnArgs& a, const Kv8Pool& p, const Kv8Ring& r, int n_heads,
                     int M, int n_blocks, const int32_t* sel, int n_sel, int64_t start, int64_t L,
-                    const int32_t* parents, bool mass, const char* what) {
+                    const int32_t* parents, const float* mass_in, float* mass_out, const char* what) {
     if (n_blocks < 0 || n_blocks > p.stride)
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: n_blocks=%d (table_stride %d)", what, n_blocks,
                        p.stride);
@@ -136,8 +136,11 @@ mj_status fill_attn(mj_ctx* ctx, Kv8AttnArgs& a, const Kv8Pool& p, const Kv8Ring
                        (long long)r.C, (long long)(L - start), M);
     if (sel ? n_sel < 1 || n_sel > kMaxBlocks : n_sel != 0)
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: n_sel=%d", what, n_sel);
-    if (sel && mass)
+    if (sel && mass_out)
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: masses are of attention over every block", what);
+    const size_t mass_bytes = (size_t)p.nKV * p.stride * 4;
+    if (mass_in && mass_in != mass_out && overlap(mass_in, mass_bytes, mass_out, mass_bytes))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: mass_out over a part of mass_in", what);
     StepDesc sd{};
     mj_status s = fill_tree(ctx, &sd, parents, M);
     if (s != MJ_OK) return s;
@@ -145,6 +148,8 @@ mj_status fill_attn(mj_ctx* ctx, Kv8AttnArgs& a, const Kv8Pool& p, const Kv8Ring
     a.p = p;
     a.ring = r;
     a.sel = sel;
+    a.mass_in = mass_in;
+    a.mass_out = mass_out;
     a.slot0 = (int)(start % r.C);
     std::copy(sd.anc, sd.anc + M, a.anc);
     a.abort = ctx->abort_dev;
@@ -235,6 +240,11 @@ mj_status mj_qkv_append(mj_ctx* ctx, const mj_attn_config* cfg, const void* qkv,
     Kv8AppendArgs a{};
     s = fill_append(ctx, a, *cfg, qkv, ld_qkv, q_norm_w, k_norm_w, r, L, parents_host, M, q_out, what);
     if (s != MJ_OK) return s;
+    // rows are read by several blocks, each when it comes
+    for (int i = 0; i < M; ++i)
+        if (overlap(q_out, (size_t)M * cfg->n_heads * 256, a.qkv + i * ld_qkv,
+                    (size_t)(cfg->n_heads + 2 * cfg->n_kv_heads) * 256))
+            return mj_fail(ctx, MJ_INVALID_ARG, "%s: q_out over qkv", what);
     OnDevice on(ctx->device);
     s = refuse_tree(ctx, parents_host, what);
     if (s != MJ_OK) return s;
@@ -309,14 +319,12 @@ mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, 
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: mass_in without mass_out", what);
     Kv8AttnArgs a{};
     s = fill_attn(ctx, a, p, r, n_heads, M, n_blocks, sel, n_sel, start, L, parents_host,
-                  mass_out != nullptr, what);
+                  mass_in, mass_out, what);
     if (s != MJ_OK) return s;
     a.q = (const uint16_t*)q;
     a.ldq = ld_q;
     a.out = (uint16_t*)out;
     a.ldo = ld_out;
-    a.mass_in = mass_in;
-    a.mass_out = mass_out;
     OnDevice on(ctx->device);
     s = refuse_tree(ctx, parents_host, what);
     if (s != MJ_OK) return s;
@@ -336,9 +344,10 @@ mj_status mj_kv8_evict(mj_ctx* ctx, const mj_kv8* cache, int n_blocks, int keep,
     mj_status s = check_pool(ctx, cache, what, p);
     if (s != MJ_OK) return s;
     const size_t bytes = (size_t)p.nKV * p.stride * 4;
-    if (!mass_in || !table_out || !mass_out || overlap(table_out, cache->table, bytes) ||
-        overlap(mass_out, mass_in, bytes))
-        return mj_fail(ctx, MJ_INVALID_ARG, "%s: null pointer, or an output over its input", what);
+    auto over = [&](const void* a, const void* b) { return overlap(a, bytes, b, bytes); };
+    if (!mass_in || !table_out || !mass_out || over(table_out, cache->table) || over(mass_out, mass_in) ||
+        over(table_out, mass_in) || over(mass_out, cache->table) || over(table_out, mass_out))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: null pointer, or an output over another array", what);
     if (n_blocks < 0 || n_blocks > p.stride || keep < 0 || keep > n_blocks || n_first < 0 ||
         n_last < 0 || (int64_t)n_first + n_last > keep)
         return mj_fail(ctx, MJ_INVALID_ARG,
@@ -398,7 +407,7 @@ mj_status mj_attn_block_kv8(mj_ctx* ctx, const mj_attn_config* cfg, const mj_att
     Kv8AttnArgs a{};
     Kv8AppendArgs ap{};
     s = fill_attn(ctx, a, p, r, nQ, M, n_blocks, pick ? p.table : nullptr, pick ? n_sel : 0, start, L,
-                  parents_host, mass_out != nullptr, what);
+                  parents_host, mass_in, mass_out, what);
     if (s == MJ_OK)
         s = fill_append(ctx, ap, c, nullptr, qkvN, w->q_norm_w, w->k_norm_w, r, L, parents_host, M,
                         nullptr, what);
@@ -464,8 +473,6 @@ mj_status mj_attn_block_kv8(mj_ctx* ctx, const mj_attn_config* cfg, const mj_att
     a.ldq = (int64_t)nQ * 128;
     a.out_perm = (uint16_t*)b[4];
     a.out_sum = (float2*)b[5];
-    a.mass_in = mass_in;
-    a.mass_out = mass_out;
     s = mj_hip(ctx, launch_kv8_attn(a, st), "attention");
     if (s != MJ_OK) return s;
     GatherArgs o{};

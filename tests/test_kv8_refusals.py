@@ -262,3 +262,19 @@ def test_ring_addresses_need_a_capacity():
     with pytest.raises(ValueError):
         KvRing(P, P)
     assert KvRing(P, P, capacity=7).struct.capacity == 7
+
+
+def test_outputs_over_inputs(call):
+    """Arrays that a call would overwrite before it has read them, in whole or in part: refused."""
+    row = 24 * 128 * 2  # bytes of a row of qkv; q_out's rows are packed
+    for q in (2 * P, 2 * P + row - 16, 2 * P + 9 * row + 16 * 256 - 16, 2 * P - 3 * 16 * 256 + 16):
+        append(call, BAD, qkv=2 * P, q=q, ld=9 * 24 * 128, M=2 if q > 2 * P else 3, rg=ring(64 * P, 80 * P))
+    # evict: 4 rows of 16 entries
+    for kw in (dict(to=9 * P, mi=9 * P), dict(to=9 * P + 240, mi=9 * P), dict(to=9 * P, mi=9 * P + 240),
+               dict(mo=P), dict(mo=P + 240), dict(mo=P - 240), dict(to=9 * P, mo=9 * P),
+               dict(to=9 * P, mo=9 * P - 240)):
+        evict(call, BAD, **dict(dict(mi=6 * P), **kw))
+    # attention: masses added in place, or apart
+    for mi in (9 * P + 16, 9 * P - 240):
+        attn(call, BAD, mi=mi, mo=9 * P)
+        block(call, BAD, mi=mi, mo=9 * P)
