@@ -96,15 +96,18 @@ __device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
 
 // Softmax of one unit's scores against the running state.  S: lane (ln, lq) holds vector ln against
 // tokens 16 kt + 4 lq + r, without the scale ksc >= 0; masked ones -inf.  The weights come out times
-// the unit's V scale, w = exp2(s + lv - m), so the products with V accumulate in the state without a
+// the unit's V scale, w = exp2(s + lv - m + LIFT), so the products with V accumulate in the state without a
 // step between; m is the running reference of s + lv.  It follows the maximum only where that is more
-// than 2^SLACK above it: outputs are rescaled once or twice a part, not at every unit, and w stays
-// below 2^(SLACK + 1).  w is rounded to fp16, as the two A operands of the product with V (their k
-// slot 8 lq + u is token 32 j + 4 lq + u, then 32 j + 16 + 4 lq + u - 4): half a step, 2^-11 of a
-// weight, averaged over the keys; the sum takes the weights before that rounding (a small V scale may
-// put them below fp16's normal range where they still count in the sum).  lu: the unit's sum of
-// exp2(s - m), this lane's share.
+// than 2^SLACK above it: outputs are rescaled once or twice a part, not at every unit.  w is rounded to
+// fp16, as the two A operands of the product with V (their k slot 8 lq + u is token 32 j + 4 lq + u,
+// then 32 j + 16 + 4 lq + u - 4): half a step, 2^-11 of a weight.  It is lifted by 2^LIFT before, as
+// high as fp16 goes (SLACK + LIFT = 15): fp16's steps widen below 2^-14, which is 2^-23 of the reference,
+// so a weight times V scale is off by at most 2^-34 of the part's greatest one (unlifted by 2^-25: of
+// pages with V scales 2^26 apart the smaller one's values were lost).  The factor is the same in outputs
+// and sums and leaves with the division.  The sum takes the weights before the rounding.  lu: the unit's
+// sum of exp2(s - m + LIFT), this lane's share.
 #define SLACK 6.0f
+#define LIFT 9.0f
 // The reference moved, for T tiles at once (one branch; the weights of one tile can then be formed
 // under the products of another).
 template <int T>
@@ -140,7 +143,7 @@ __device__ __forceinline__ void move_ref(Tile* tl, const f4 (*S)[4], Scales u) {
 }
 __device__ __forceinline__ void weights(Tile& T, const f4 S[4], Scales u, u4v pa[2], float& lu) {
     // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
-    const float c = u.lv - (T.m == -INFINITY ? 0.0f : T.m);
+    const float c = u.lv + LIFT - (T.m == -INFINITY ? 0.0f : T.m);
     lu = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)

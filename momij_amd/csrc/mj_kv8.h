@@ -78,9 +78,9 @@ struct Kv8AttnArgs {
     // take their pages together; cols: block columns (groups of tiles, rows with lists of their own)
     int n_list, upp, parts, ring_units, upr, ring_parts, tiles, pair, cols;
     bool shared;
-    float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v
-    float2* ml;     // [parts][nKV][nv] {m, sum}
-    float2* rec;    // [nKV][n][nv] {m, sum} of each block where masses are wanted
+    float* opart;   // [parts][nKV][nv][128] sums of exp2(s - m) v, times a constant
+    float2* ml;     // [parts][nKV][nv] {m, sum}: the sum times the same
+    float2* rec;    // [nKV][n][nv] {m, sum} of each block where masses are wanted, likewise
     const int* abort;
     uint64_t anc[MJ_ROWS];  // of pass row r: bit a set for its ancestors and itself
 };
