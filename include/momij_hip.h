@@ -282,8 +282,8 @@ mj_status mj_kv8_select(mj_ctx* ctx, const mj_kv8* cache, int n_heads, const voi
  * all rows and the group's heads gave the block's keys.
  * Scores, softmax statistics and outputs are summed in fp32.  For the product with V a weight is rounded
  * to fp16 together with its block's V scale: off by half a step, 2^-11 of itself, or, where it is less
- * than 2^-23 of a greater one, by up to 2^-34 of that one (times the code).  A call repeats bit for bit; a row's result in a call of other rows may differ by
- * rounding (the keys are split differently). */
+ * than 2^-23 of a greater one, by up to 2^-34 of that one (times the code).  A call repeats bit for
+ * bit; a row's result in a call of other rows may differ by rounding (the keys are split differently). */
 mj_status mj_kv8_attn(mj_ctx* ctx, const mj_kv8* cache, const mj_kv_ring* ring, int n_heads,
                       const void* q, int64_t ld_q, int M, int n_blocks, const int32_t* sel,
                       int n_sel, int64_t start, int64_t L, const int32_t* parents_host, void* out,

@@ -83,12 +83,13 @@ struct Tile {
 typedef float f2v __attribute__((ext_vector_type(2)));
 
 // What a unit's codes stand for: ksc, the factor of its raw scores to log2 units; lv, log2 of its V
-// scale (at least LV_MIN, that of a block of the least fp16 number; a block of zeros has none), and
-// 2^-lv.
+// scale (at least LV_MIN, that of a block of the least fp16 number; a block of zeros has none) less
+// LV_TOP; ilv, 1 / V scale.
 struct Scales {
     float ksc, lv, ilv;
 };
 #define LV_MIN -31.0f
+#define LV_TOP 3.0f
 __device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
     const float l = __builtin_amdgcn_logf(vs);
     return l < LV_MIN ? LV_MIN : l;
@@ -108,42 +109,71 @@ __device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
 // sum of exp2(s - m + LIFT), this lane's share.
 #define SLACK 6.0f
 #define LIFT 9.0f
+// Scores past FAR, whose steps in fp32 are an eighth and more: s + lv would lose lv, and a weight's one
+// fma differs from the rounded s by up to thousands (weights of infinity or 0).  There m is at least the
+// rounded s itself, and move_ref takes it off the rounded scores, exactly for those near it, in the
+// branch that it has for moving.  A weight is then up to 2^(lv + LIFT): below 2^15.1 for a sealed block
+// (scale 65504 / 127 at most), which is what LV_TOP is for.
+#define FAR 1048576.0f
+
+// a * b rounded (the compiler would make one fma of it and a difference)
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 // The reference moved, for T tiles at once (one branch; the weights of one tile can then be formed
-// under the products of another).
+// under the products of another); c: what makes exp2(fma(S, ksc, c)) of vector ln's scores its weights.
 template <int T>
-__device__ __forceinline__ void move_ref(Tile* tl, const f4 (*S)[4], Scales u) {
-    float m[T];
-    bool moved = false;
+__device__ __forceinline__ void move_ref(Tile* tl, f4 (*S)[4], Scales u, float* c) {
+    float x[T], m[T], ref[T];
+    bool rare = false;
 #pragma unroll
     for (int i = 0; i < T; ++i) {
-        float x = -INFINITY;
+        x[i] = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-            x = fmaxf(fmaxf(x, S[i][kt][0]), S[i][kt][1]);
-            x = fmaxf(fmaxf(x, S[i][kt][2]), S[i][kt][3]);
+            x[i] = fmaxf(fmaxf(x[i], S[i][kt][0]), S[i][kt][1]);
+            x[i] = fmaxf(fmaxf(x[i], S[i][kt][2]), S[i][kt][3]);
         }
-        m[i] = fmaf(x4_max(x), u.ksc, u.lv);
-        moved |= m[i] > tl[i].m + SLACK;
+        x[i] = x4_max(x[i]);
+        m[i] = fmaf(x[i], u.ksc, u.lv);
+        rare |= (m[i] > tl[i].m + SLACK) | (fabsf(m[i]) > FAR);
+        ref[i] = tl[i].m;
     }
-    if (!__any(moved)) return;
-    const int lq = (threadIdx.x & 63) >> 4;
+    if (__any(rare)) {
+        const int lq = (threadIdx.x & 63) >> 4;
 #pragma unroll
-    for (int i = 0; i < T; ++i) {
-        const float mn = fmaxf(tl[i].m, m[i]);
-        const float alpha = tl[i].m == mn ? 1.0f : __builtin_amdgcn_exp2f(tl[i].m - mn);  // (both may be -inf)
-        tl[i].m = mn;
-        tl[i].l *= alpha;
+        for (int i = 0; i < T; ++i) {
+            const float s = product(x[i], u.ksc);
+            const bool far = fabsf(m[i]) > FAR && s > -INFINITY;  // (-inf: every score is masked)
+            const float mn = fmaxf(tl[i].m, far ? s : m[i]);
+            // (both may be -inf)
+            const float alpha = tl[i].m == mn ? 1.0f : __builtin_amdgcn_exp2f(tl[i].m - mn);
+            tl[i].m = mn;
+            tl[i].l *= alpha;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float al = __shfl(alpha, 4 * lq + r, MJ_WAVE);
+            for (int r = 0; r < 4; ++r) {
+                const float al = __shfl(alpha, 4 * lq + r, MJ_WAVE);
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) tl[i].o[dt][r] *= al;
+                for (int dt = 0; dt < 8; ++dt) tl[i].o[dt][r] *= al;
+            }
+            ref[i] = far ? 0.0f : mn;
+            if (!__any(far)) continue;
+            const float inv = 1.0f / u.ksc;  // (far scores have no ksc of 0)
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    S[i][kt][r] = far ? (product(S[i][kt][r], u.ksc) - mn) * inv : S[i][kt][r];
         }
     }
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+        // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
+        c[i] = u.lv + LIFT - (ref[i] == -INFINITY ? 0.0f : ref[i]);
 }
-__device__ __forceinline__ void weights(Tile& T, const f4 S[4], Scales u, u4v pa[2], float& lu) {
-    // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
-    const float c = u.lv + LIFT - (T.m == -INFINITY ? 0.0f : T.m);
+__device__ __forceinline__ void weights(Tile& T, const f4 S[4], Scales u, float c, u4v pa[2], float& lu) {
     lu = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
@@ -288,11 +318,11 @@ __device__ __forceinline__ void ring_unit(Tile& tl, const u4v q[4], const u4v* K
             S[0][kt][r] = (w >> r) & 1 ? S[0][kt][r] : -INFINITY;
         __builtin_amdgcn_sched_barrier(0);  // (all operands ahead of the products: 100 registers more)
     }
-    const Scales u{SC2, 0.0f, 1.0f};
+    const Scales u{SC2, -LV_TOP, 1.0f};
     u4v pa[2];
-    float lu;
-    move_ref<1>(&tl, S, u);
-    weights(tl, S[0], u, pa, lu);
+    float c, lu;
+    move_ref<1>(&tl, S, u, &c);
+    weights(tl, S[0], u, c, pa, lu);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -410,12 +440,13 @@ __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u
 #pragma unroll
     for (int f = 0; f < 16; ++f) v[f] = Vf[f * 64 + lane];
     __builtin_amdgcn_sched_barrier(0);
-    move_ref<T>(tl, S, u);
+    float c[T];
+    move_ref<T>(tl, S, u, c);
     u4v pa[T][2];
 #pragma unroll
     for (int i = 0; i < T; ++i) {
         float lu;
-        weights(tl[i], S[i], u, pa[i], lu);
+        weights(tl[i], S[i], u, c[i], pa[i], lu);
         if (rec[i]) {
             lu = x4_sum(lu);
             if (lane < 16) *rec[i] = make_float2(tl[i].m, lu);
@@ -495,7 +526,8 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
             nxt = todo ? __builtin_ctzll(todo) : -1;
         }
         const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
-        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
+        const float lg = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), lvl = lg - LV_TOP;
+        const float ill = __builtin_amdgcn_exp2f(-lg);
         if (t == 0) s_abort = ab;
         if (ub != u0) __syncthreads();  // the batch before is done with
         if (cur >= 0) stage(0);
@@ -591,7 +623,8 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
             request_v(i0);
         }
         const float ksl = (pl >= 0 ? a.p.ks[pl] : 0.0f) * SC2;
-        const float lvl = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), ill = __builtin_amdgcn_exp2f(-lvl);
+        const float lg = log2_scale(pl >= 0 ? a.p.vs[pl] : 0.0f), lvl = lg - LV_TOP;
+        const float ill = __builtin_amdgcn_exp2f(-lg);
         auto step = [&](int i, int nx, auto more) {  // page i; page nx requested behind it
             const Scales sc{lane_of(ksl, i), lane_of(lvl, i), lane_of(ill, i)};
             f4 S[T][4];
@@ -612,12 +645,13 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
                 }
             }
             if constexpr (more.value) request_k(nx);
-            move_ref<T>(tl, S, sc);
+            float c[T];
+            move_ref<T>(tl, S, sc, c);
             u4v pa[T][2];
 #pragma unroll
             for (int x = 0; x < T; ++x) {
                 float lu;
-                weights(tl[x], S[x], sc, pa[x], lu);
+                weights(tl[x], S[x], sc, c[x], pa[x], lu);
                 if constexpr (MASS) {
                     const int v = vw + 16 * x + ln;
                     lu = x4_sum(lu);
