@@ -278,3 +278,27 @@ def test_outputs_over_inputs(call):
     for mi in (9 * P + 16, 9 * P - 240):
         attn(call, BAD, mi=mi, mo=9 * P)
         block(call, BAD, mi=mi, mo=9 * P)
+
+
+def test_plan_restated(call):
+    """The split that the GPU tests name their sizes by gives the workspaces that the calls ask for."""
+    import random
+    import re
+
+    from tests.kv8_plan import plan
+
+    rng, big, seen = random.Random(7), kv8(stride=1 << 20, n_pages=1 << 30), set()
+    for _ in range(3000):
+        nkv, g = rng.choice([(4, 4), (1, 16), (1, 64), (8, 4), (32, 4), (64, 4), (128, 1), (2, 7)])
+        M, n = rng.choice([1, 2, 5, 9, 17, 20, 40, 64]), rng.choice([1, 9, 75, 76, 200, 520, 2047, 20000])
+        n_sel, mass = rng.choice([0, 0, 5, 64, 600]), rng.choice([0, 1])
+        mass = 0 if n_sel else mass
+        rows = M + rng.choice([0, 1, 80, 8000, 16300, 131000])
+        big.n_kv_heads = nkv
+        st, msg = call("mj_kv8_attn", big, ring(cap=1 << 29), nkv * g, P, 0, M, n, P if n_sel else None, n_sel,
+                       0, rows - M, None, P, 0, None, P if mass else None, P, 0)
+        assert st == BAD, msg
+        p = plan(nkv * g, nkv, M, n, n_sel, rows, mass)
+        assert int(re.search(r"needs (\d+)", msg).group(1)) == p["bytes"], (nkv, g, M, n, n_sel, rows, mass, p)
+        seen.add((p["shared"], p["pair"], p["tiles"], p["upp"] > p["batch"], p["parts"] > 256))
+    assert {s[:3] for s in seen} == {(True, 1, 1), (True, 1, 2), (False, 1, 1), (False, 1, 2), (False, 2, 2)}
