@@ -266,7 +266,8 @@ mj_status mj_kv8_unseal(mj_ctx* ctx, const mj_kv8* cache, int at, int count,
  * block: with c the query's 8-bit codes of scale s_q (formed as sealed ones are),
  *   max over the group's heads of  (sum_d max(c_d greatest_d, c_d least_d)) * k_scale * s_q,
  * the sum in whole numbers, the products in fp32 from left to right.  A NaN score counts as the
- * least.  q fp16 [M] rows of ld_q halves (0: packed; else a multiple of 8). */
+ * least.  q fp16 [M] rows of ld_q halves (0: packed; else a multiple of 8).  Takes scratch at every
+ * length, also where a short list's scores stay in the kernel. */
 mj_status mj_kv8_select(mj_ctx* ctx, const mj_kv8* cache, int n_heads, const void* q, int64_t ld_q,
                         int M, int n_blocks, int n_sel, int n_first, int n_last, int32_t* sel,
                         void* ws, size_t ws_bytes);
@@ -279,7 +280,8 @@ mj_status mj_kv8_select(mj_ctx* ctx, const mj_kv8* cache, int n_heads, const voi
  * start <= L, L - start + M <= ring capacity.
  * mass_out (nullable; not with sel) float [n_kv_heads][table_stride]: for every block its entry of
  * mass_in (same layout, NULL: zeros; may be mass_out, not a part of it) plus the softmax weight that
- * all rows and the group's heads gave the block's keys.
+ * all rows and the group's heads gave the block's keys (every row's, whether or not it is kept after the
+ * pass).
  * Scores, softmax statistics and outputs are summed in fp32.  For the product with V a weight is rounded
  * to fp16 together with its block's V scale: off by half a step, 2^-11 of itself, or, where it is less
  * than 2^-23 of a greater one, by up to 2^-34 of that one (times the code).  A call repeats bit for

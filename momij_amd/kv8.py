@@ -12,7 +12,8 @@ A layer's context in use:
     # a long context in part: blocks chosen for every row
     ctx.kv8_select(cache, q, M, n_heads, n, n_sel, 1, 2, sel)
     ctx.kv8_attn(cache, ring, q, M, n_heads, n, start, L, parents, out, sel=sel)
-    # a bounded cache: the blocks that got the least attention go, their pages are used again
+    # a bounded cache (of one block more than `keep`): the blocks that got the least attention, of all
+    # rows of the passes that were given the masses, go; their pages are used again
     ctx.kv8_attn(..., mass_in=cache.mass, mass_out=cache.mass)
     cache.evict(n, keep, n_first=1, n_last=4); n = keep
     # a rewind into sealed blocks: back to the ring, their weight forgotten
