@@ -58,10 +58,11 @@ class KvRing:
     def of(self, n_kv_heads: int, device: int) -> _lib.KvRingStruct:
         """The struct for a call of n_kv_heads on `device`: a ring of fewer heads would be read and
         written past its end."""
-        if self.n_kv_heads not in (n_kv_heads, None) or self.device not in (device, None):
-            raise ValueError(f"a ring of {self.n_kv_heads} heads on device {self.device} in a call of "
-                             f"{n_kv_heads} on device {device}")
-        return self.struct
+        if (self.n_kv_heads == n_kv_heads or self.n_kv_heads is None) and (
+                self.device == device or self.device is None):
+            return self.struct
+        raise ValueError(f"a ring of {self.n_kv_heads} heads on device {self.device} in a call of "
+                         f"{n_kv_heads} on device {device}")
 
 
 class Kv8Cache:
