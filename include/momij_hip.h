@@ -230,7 +230,8 @@ typedef struct mj_kv8 {
 } mj_kv8;
 
 /* fp16 rows [n_kv_heads][capacity][128] of K and V, position p at slot p % capacity (the layout of
- * mj_attn_block's caches and of mj_model_kv). */
+ * mj_attn_block's caches and of mj_model_kv); n_kv_heads is that of the cache or configuration it is used
+ * with (it has no count of its own to check). */
 typedef struct mj_kv_ring {
     void* k;
     void* v;

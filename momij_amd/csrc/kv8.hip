@@ -582,8 +582,8 @@ __device__ __forceinline__ bool pick_keys(F key, int n, int k, int first, int la
 
 // One block a row and head: scores formed in LDS, then the n_sel greatest, for up to CHOOSE_MAX blocks
 // (their 256 bytes each come through one CU, which has only so many lines under way: of 8 rows 250
-// blocks take 10 us and 500 13, in two launches 12.5 and 12.5 and the gap between them; 1000 19 and
-// 13.5).
+// blocks take 10 us and 500 13, in two launches 12.5 and 12.5 and the gap between them, so about there
+// the two meet; 1000 19 and 13.5).
 #define CHOOSE_MAX 512
 __global__ __launch_bounds__(1024) void k_kv8_choose(Kv8SelectArgs a) {
     __shared__ float s_sc[CHOOSE_MAX];

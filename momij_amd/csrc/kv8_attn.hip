@@ -464,11 +464,12 @@ __device__ __forceinline__ void staged_unit(Tile* tl, const u4v (*q)[4], const u
 // Pages shared: a block of NW waves takes a run of pages for NW T tiles of query vectors, T a wave.  A
 // page is turned to halves once, by the whole block, and read from LDS by its waves; two pages are in
 // LDS and one in registers on its way, one barrier a page.  The first blocks take the ring's
-// parts; rows with lists of their own (a.sel) as below.  64 rows of 16 heads over 65500 tokens: 46 us, 0.74
-// PFLOP/s, the matrix units busy 39% of the time and the VALU 50% (the softmax, the codes).  17 rows
-// over 32000 tokens with masses 17.5 us: eight pages a block, each a barrier and a chain of products,
-// softmax and products that its few waves do not cover (a second page on its way, half the LDS
-// reads, or the next page's scores under a page's softmax change nothing).
+// parts; rows with lists of their own (a.sel) as below.  64 rows of 16 heads over 65500 tokens: 47 us,
+// 0.73 PFLOP/s, the matrix units busy 38% of the time and the VALU 51% (the softmax, the codes), one
+// after the other, as all waves run the same phase between two barriers.  17 rows over 32000 tokens with
+// masses 17.6 us: eight pages a block, each a barrier and a chain of products, softmax and products that
+// its few waves do not cover (a second page on its way, half the LDS reads, or the next page's scores
+// under a page's softmax change nothing).
 template <int T, int NW, bool MASS>
 __global__ __launch_bounds__(64 * NW) void k_kv8_attn_shared(Kv8AttnArgs a) {
     constexpr int NT = 64 * NW, NR = 512 / NT;
@@ -752,8 +753,9 @@ __global__ __launch_bounds__(64 * NW) void k_kv8_attn_own(Kv8AttnArgs a) {
 
 // mass_out = mass_in + sum over the head's query vectors of the block's share of their softmax: a wave
 // takes one of a head's blocks.  The vectors' final maxima and sums are formed again here from the
-// parts' (a launch that waited for them took 4 us more).  17 rows, 500 blocks of 4 heads: with the join
-// 6.1 us.
+// parts' (a launch that waited for them took 4 us more), once for NW blocks: vectors x parts x blocks /
+// NW reads.  17 rows, 500 blocks of 4 heads: with the join 6.5 us; 64 rows, 1023 blocks 20.4 us (7.6
+// without masses).
 template <int NW>
 __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
     __shared__ float2 s_w[2][NW][64];
@@ -808,8 +810,8 @@ __device__ __forceinline__ void mass_blocks(const Kv8AttnArgs& a, int blk) {
 // One block a row and head.  NG groups of 32 lanes (a lane four dims) take every NG-th part, eight
 // requested at a time, each to its own running maximum; the groups are then joined in order.  A part
 // that saw no key has maximum -inf and weight 0.  Blocks past the rows' form the masses.  One row of 16
-// heads over 30 to 64 parts 4 to 5 us, a launch and a round of requests; 64 rows over 31 parts (17 MB)
-// 7.6 us.
+// heads over 30 to 64 parts 3.4 to 5.3 us, a launch and a round of requests; 64 rows over 63 parts (33
+// MB) 7.6 us.
 template <int NG, bool MASS>
 __global__ __launch_bounds__(32 * NG) void k_kv8_combine(Kv8AttnArgs a) {
     const int t = threadIdx.x, gr = t >> 5, d4 = t & 31;
@@ -898,13 +900,16 @@ size_t kv8_attn_plan(Kv8AttnArgs& a, bool mass, void* base) {
     const int nv = a.M * a.G;
     const int tiles = ((a.n_sel > 0 ? a.G : nv) + 15) / 16;  // that share their units
     const int rows = a.n_sel > 0 ? a.M : 1;
-    // Shared pages: each is turned to halves by a whole block, a page a block where there are few (one
-    // row at 2000 tokens 5.3 us, 7.2 where a wave takes a page alone; 8 rows at 9600 8.0 and 11.8).
+    // Shared pages: each is turned to halves by a whole block, a page or two a block where there are few
+    // (one row at 2000 tokens 5.3 us, 7.2 where a wave takes a page alone; 8 rows at 9600 8.0 and 11.8).
     // Pages of a wave's own, for one or two tiles: they stream (one row at 131000 tokens 23 us; 8 rows
     // at 65000 17.4, 19.9 shared); of two waves together, for three or four, later (9 rows at 131000
     // tokens 31.6 us, 35.9 shared; at 65000 19.7 and 20.6; at 32000 14.8 and 14.3).  More share (17
     // rows at 131000 47 us, 51 by four waves together).  Two tiles a wave past eight in all, where the
     // block's LDS reads bound it (64 rows at 65000 tokens 46 us, 60 with one; at 9600 20.6 and 18.8).
+    // Rows with lists of their own take pages each (join included: one row of 64 listed blocks 10.6 us
+    // shared and 10.9, of 128 11.7 and 11.2; 9 rows of 8 9.5 and 10.4, of 16 10.4 and 10.6, of 32 13.2
+    // and 10.9; 64 rows of one 19.1 and 17.5).
     const int64_t visits = (int64_t)a.n_list * a.p.nKV;
     const int64_t most = tiles == 1 ? 300 : tiles == 2 ? 2500 : tiles <= 4 ? 3500 : INT64_MAX;
     a.shared = visits * rows * ((tiles + NWAVES - 1) / NWAVES) <= most;
