@@ -32,7 +32,7 @@ def row_stride(t, M: int, width: int, device: int, what: str) -> int:
     """Halves between M rows of `width` fp16 values side by side, as the library's calls take it (0:
     one row, or packed ones; hence no row that stands for all M)."""
     if t.dtype is _F16 and t.get_device() == device:
-        if t.numel() == M * width and t.is_contiguous():
+        if t.numel() == M * width and t.size(0) == M and t.is_contiguous():
             return 0
         shape, step = t.shape, t.stride()
         if len(shape) == 2 and shape[0] >= M and shape[1] >= width and step[1] == 1:
@@ -43,6 +43,8 @@ def row_stride(t, M: int, width: int, device: int, what: str) -> int:
         if M == 1 and t.numel() >= width and t.is_contiguous() and (
                 len(shape) == 1 or width % shape[-1] == 0):  # flat, or head by head
             return 0
+        if len(shape) > 2 and shape[0] == 1 and M > 1:  # a batch of one
+            return row_stride(t[0], M, width, device, what)
         if len(shape) > 2 and shape[0] >= M and (M == 1 or step[0] >= width):
             if t[0].numel() >= width and t[0].is_contiguous():
                 return step[0] if M > 1 else 0
@@ -52,10 +54,12 @@ def row_stride(t, M: int, width: int, device: int, what: str) -> int:
 
 def packed(t, dtype, rows: int, width: int, device: int, what: str) -> int:
     """Address of `rows` rows of `width` values of a type without gaps."""
-    if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
-        n = t.numel()
-        if n == rows * width or n > rows * width and (rows <= 1 or t.stride(0) <= width):
+    if t.dtype is dtype and t.get_device() == device and t.numel() >= rows * width and t.is_contiguous():
+        step = t.stride(0) if rows > 1 else width
+        if step == width or step < width and t.dim() < 3:  # (flat, or head by head)
             return t.data_ptr()
+        if rows > 1 and t.dim() > 2 and t.size(0) == 1:  # a batch of one
+            return packed(t[0], dtype, rows, width, device, what)
     raise ValueError(f"{what}: {rows} packed rows of {width} {dtype} on device {device}, not {t.dtype} "
                      f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
 

@@ -148,7 +148,7 @@ def good_rows(width, m=M):
     """[tensor, stride in halves] (0: packed)"""
     return [(z(m, width), 0), (z(m + 2, width), width), (z(m, width + 64)[:, 8:8 + width], width + 64),
             (z(m, width // 128, 128), 0), (z(m + 1, width // 128, 128), width),
-            (z(m, 2, width)[:, 1], 2 * width)]
+            (z(m, 2, width)[:, 1], 2 * width), (z(1, m, width), 0), (z(1, m, width + 8)[:, :, :width], width + 8)]
 
 
 @pytest.mark.parametrize("f,name,width,at", [
@@ -185,7 +185,7 @@ def test_packed_rows(ctx, f, name, width):
     """Rows without a stride in the library's arguments: packed ones only."""
     for t in bad_rows(width) + [z(M, width + 64)[:, :width], z(M, width + 64)]:
         refused(ctx, f, **{name: t})
-    for t in (z(M, width), z(M + 1, width), z(M, width // 128, 128), z(M * width)):
+    for t in (z(M, width), z(M + 1, width), z(M, width // 128, 128), z(M * width), z(M * width // 128, 128)):
         taken(ctx, f, **{name: t})
 
 
@@ -261,3 +261,19 @@ def test_workspaces(ctx, f):
         args = taken(ctx, f, ws=t)
         assert args[-2:] == (t.data_ptr(), 1 << 10)
     assert taken(ctx, f)[-2:] == (None, 0)
+
+
+@pytest.mark.parametrize("f,name,width", [(append, "qkv", (NQ + 2 * NKV) * D), (attn, "q", NQ * D),
+                                          (attn, "out", NQ * D)])
+def test_heads_before_rows(ctx, f, name, width):
+    """[heads][M][128] is as large as [M][heads][128] and no rows."""
+    for t in (z(width // 128, M, 128), z(width, M), z(M * width // 8, 8), z(1, M * width)):
+        refused(ctx, f, **{name: t})
+
+
+@pytest.mark.parametrize("f,name,width", [(append, "q", NQ * D), (block, "h", 2048)])
+def test_heads_before_packed_rows(ctx, f, name, width):
+    for t in (z(width // 128, M, 128), z(1, M, width + 8), z(1, M - 1, 2 * width), z(2, M, width)):
+        refused(ctx, f, **{name: t})
+    for t in (z(1, M, width), z(1, M + 1, width), z(1, M, width // 128, 128)):
+        taken(ctx, f, **{name: t})
