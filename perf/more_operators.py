@@ -11,6 +11,10 @@ Heads of 128; the head counts are those of the benchmark model and of the tests,
 those of a pass: one (decode), 9 (a K = 8 chain), 17 (a 16-node tree), 64 (a prefill chunk).  Sizes of a
 batch go by the case alone (lengths spread evenly over their logarithm, row counts over 1 .. M);
 which sequence has which goes by the seed.
+
+Pages hold 32, 64, 128 or 256 tokens of a layer, by KV head in units of 32 tokens by 128 dims, 8 KB of K
+and of V each, in the order of the matrix operands.  Of token t (of the unit) and dim d, K is at
+[t / 4 % 2][d / 32][d / 8 % 4][t / 8][t % 4][d % 8] and V at [d / 16][t / 8][d % 16][t % 8].
 """
 from __future__ import annotations
 
@@ -87,7 +91,7 @@ def _log(rng, lo, hi):
 def draw(rng):
     kind = rng.choice(["attn"] * 5 + ["append", "branch", "commit", "accept", "accept"])
     nq, nkv = rng.choice([(16, 4), (16, 4), (16, 4), (8, 8), (16, 2), (32, 4), (12, 4), (16, 1)])
-    page = rng.choice([16, 32, 64, 64, 128, 256])
+    page = rng.choice([32, 64, 64, 128, 256])
     if kind == "attn":
         n, M = _log(rng, 1, 64), _log(rng, 1, 64)
         most = min(131000, 130000 * 4 // (n * max(nkv, 4)), 16 * 64 * 36000 // (n * nq * M))
@@ -103,11 +107,11 @@ def draw(rng):
         n = _log(rng, 2, 64)
         return dict(kind=kind, nkv=nkv if nkv <= 4 else 4, n=n, parents=rng.randint(1, min(8, n - 1)),
                     M=_log(rng, 1, 9), lo=rng.randint(1, 200), hi=_log(rng, 201, 2000),
-                    page=rng.choice([16, 32, 64]), layers=rng.randint(1, 24), go_on=rng.random() < 0.5)
+                    page=rng.choice([32, 64]), layers=rng.randint(1, 24), go_on=rng.random() < 0.5)
     if kind == "commit":
         return dict(kind=kind, nkv=nkv if nkv <= 4 else 4, n=_log(rng, 1, 64), M=_log(rng, 2, 17),
                     ragged=rng.random() < 0.5, tree=rng.random() < 0.8, lo=rng.randint(0, 30),
-                    hi=_log(rng, 31, 120), page=rng.choice([16, 32, 64]), layers=rng.randint(1, 24))
+                    hi=_log(rng, 31, 120), page=rng.choice([32, 64]), layers=rng.randint(1, 24))
     n, tree = _log(rng, 1, 64), rng.random() < 0.3
     return dict(kind=kind, n=n, M=rng.randint(1, min(17, 300 // n)), ragged=rng.random() < 0.5,
                 tree=tree, V=rng.choice([_log(rng, 500, 40000), _log(rng, 40000, VOCAB), VOCAB]),
@@ -213,8 +217,8 @@ def _inputs(case, seed):
     refs = np.zeros(pages, np.int64)
     refs[table[table >= 0]] = 1
     d.update(lens=ints(lens), table=ints(table), refs=ints(refs),
-             k=randn(layers, pages, nkv, page, D, dtype=torch.float16),
-             v=randn(layers, pages, nkv, page // 8, D, 8, dtype=torch.float16))
+             k=randn(layers, pages, nkv, page // 32, 2, 4, 4, 4, 4, 8, dtype=torch.float16),
+             v=randn(layers, pages, nkv, page // 32, 8, 4, 16, 8, dtype=torch.float16))
     if kind == "attn":
         d["q"] = (randn(R, case["nq"] * D) * 2.0).half()
     elif kind == "append":
@@ -318,9 +322,26 @@ def _run_plain(st):
 
 def _rows_of_pages(st, pages):
     """K and V rows of pages [...] in 32 bits, [..., nkv, page, 128], of layer 0."""
-    k, v = st["k"][0][pages].float(), st["v"][0][pages].float()
-    v = v.transpose(-1, -2)
-    return k, v.reshape(k.shape)
+    k, v = st["k"][0][pages], st["v"][0][pages]
+    k = k.movedim((-3, -6, -2), (-6, -5, -4)).float()
+    v = v.movedim((-3, -1), (-4, -3)).float()
+    shape = pages.shape + (st["case"]["nkv"], st["case"]["page"], D)
+    return k.reshape(shape), v.reshape(shape)
+
+
+def _read(st, pages, t):
+    """K and V of tokens t of pages, in all layers, as the pools' rows of them lie."""
+    u, t = t // 32, t % 32
+    return (st["k"][:, pages, :, u, t // 4 % 2, :, :, t // 8, t % 4],
+            st["v"][:, pages, :, u, :, t // 8, :, t % 8])
+
+
+def _write(st, pages, t, k, v):
+    """The same the other way, [rows, nkv, 128] or as they were read."""
+    head = (pages.shape[0], st["k"].shape[0], st["k"].shape[2])
+    u, t = t // 32, t % 32
+    st["k"][:, pages, :, u, t // 4 % 2, :, :, t // 8, t % 4] = k.reshape(head + (4, 4, 8))
+    st["v"][:, pages, :, u, :, t // 8, :, t % 8] = v.reshape(head + (8, 16))
 
 
 def _plain_attn(st):
@@ -367,8 +388,7 @@ def _plain_append(st):
         y, z = qk[..., :half], qk[..., half:rope]
         qk = torch.cat([y * c - z * s, z * c + y * s, qk[..., rope:]], -1)
     pg, t = _slots(st, b.seq, L + b.at)
-    st["k"][0][pg, :, t] = qk[:, nq:].half()
-    st["v"][0][pg, :, t // 8, :, t % 8] = x[:, nq + nkv:].half()
+    _write(st, pg, t, qk[:, nq:].half(), x[:, nq + nkv:].half())
     return dict(q=qk[:, :nq].half().reshape(-1, nq * D), k=st["k"], v=st["v"])
 
 
@@ -426,12 +446,11 @@ def _plain_branch(st):
     here, there = old.gather(1, f)[:, 0], new.gather(1, f)[:, 0]
     res = torch.stack([served.long(), need.sum(1), torch.where(part, here, -1), torch.where(part, there, -1)], 1)
     st["reserved"].copy_(res)
-    # tokens of the block that are committed; the others hold nothing yet
+    # tokens of the block that are committed, in whole groups of eight; the others hold nothing yet
     there, here = torch.where(part, there, 0), torch.where(part, here, 0)
-    fill = (part[:, None] & (torch.arange(page, device=src.device) < (lens % page)[:, None]))
+    fill = (part[:, None] & (torch.arange(page, device=src.device) // 8 * 8 < (lens % page)[:, None]))
     i, t = torch.nonzero(fill, as_tuple=True)
-    st["k"][:, there[i], :, t] = st["k"][:, here[i], :, t]
-    st["v"][:, there[i], :, t // 8, :, t % 8] = st["v"][:, here[i], :, t // 8, :, t % 8]
+    _write(st, there[i], t, *_read(st, here[i], t))
     return {x: st[x] for x in ("table", "lens", "refs", "reserved", "k", "v")}
 
 
@@ -442,9 +461,7 @@ def _plain_commit(st):
     # rows that are not kept stay where they are
     pg, t = _slots(st, b.seq, L + torch.where(kept, path, b.at))
     pg2, t2 = _slots(st, b.seq, L + b.at)
-    k, v = st["k"][:, pg, :, t], st["v"][:, pg, :, t // 8, :, t % 8]
-    st["k"][:, pg2, :, t2] = k
-    st["v"][:, pg2, :, t2 // 8, :, t2 % 8] = v
+    _write(st, pg2, t2, *_read(st, pg, t))
     new = st["lens"] + torch.where(b.count > 0, st["accepted"] + 1, 0).int()
     return dict(k=st["k"], v=st["v"], lens=new)
 
@@ -522,7 +539,7 @@ def work(case):
     if kind == "commit":  # about half of the kept rows move
         return {"bytes": token * R / 4 + 8 * n, "flops": 1.0 * R}
     p = case["parents"]
-    part = sum((lens[i] % page) * (-(-(n - p - i) // p) + case["go_on"]) for i in range(p))
+    part = sum(-(-(lens[i] % page) // 8) * 8 * (-(-(n - p - i) // p) + case["go_on"]) for i in range(p))
     blocks = sum(-(-x // page) for x in lens)
     return {"bytes": 2 * token * part + 8.0 * blocks * n / p + 4.0 * blocks, "flops": 1.0 * n}
 
@@ -533,6 +550,24 @@ def exact(case, seed):
     return globals()["_exact_" + case["kind"]](case, d)
 
 
+def _at(tokens):
+    """Where a head's K and V of tokens [T] lie in a page, each [T, 128]."""
+    u, t = tokens[:, None] // 32 * 4096, tokens[:, None] % 32
+    i = torch.arange(D, device=tokens.device)
+    return (u + 2048 * (t // 4 % 2) + 512 * (i // 32) + 128 * (i // 8 % 4) + 32 * (t // 8) + 8 * (t % 4) + i % 8,
+            u + 512 * (i // 16) + 128 * (t // 8) + 8 * (i % 16) + t % 8)
+
+
+def _flat(d):
+    return (d[x].reshape(d[x].shape[:3] + (-1,)) for x in "kv")
+
+
+def _move(src, dst, p, t, p2, t2):
+    """K and V of tokens t of page p of flat pools to tokens t2 of page p2."""
+    for a, b, i, j in zip(src, dst, _at(t), _at(t2)):
+        b[:, p2, :, j] = a[:, p, :, i]
+
+
 def _host(d, *names):
     return [d[x].cpu().tolist() for x in names]
 
@@ -541,14 +576,15 @@ def _exact_attn(case, d):
     nq, nkv, page, W = case["nq"], case["nkv"], case["page"], case["window"]
     G = nq // nkv
     start, lens, table = _host(d, "row_start", "lens", "table")
+    K, V = _flat(d)
     out = torch.zeros((d["rows"], nq, D), dtype=torch.float64, device="cuda")
     q = d["q"].double().reshape(-1, nq, D)
     for s, L in enumerate(lens):
         m, par = start[s + 1] - start[s], d["parents"][s]
         pos = torch.arange(L + m, device="cuda")
         pg = torch.tensor(table[s], device="cuda")[pos // page]
-        k = d["k"][0, pg, :, pos % page].double()  # [T, nkv, D]
-        v = d["v"][0, pg, :, pos % page // 8, :, pos % 8].double()
+        ik, iv = _at(pos % page)
+        k, v = (x[0][pg[:, None], :, i].double().transpose(1, 2) for x, i in ((K, ik), (V, iv)))  # [T, nkv, D]
         for r in range(m):
             way, a = [], r
             while a >= 0:
@@ -587,9 +623,11 @@ def _exact_append(case, d):
             y[:, h, i] = a * th.cos() - b * th.sin()
             y[:, h, i + rope // 2] = a * th.sin() + b * th.cos()
     k, v = d["k"].double(), d["v"].double()
-    for r, (pg, t) in enumerate(where):
-        k[0, pg, :, t] = y[r, nq:nq + nkv]
-        v[0, pg, :, t // 8, :, t % 8] = y[r, nq + nkv:]
+    K, V = _flat(dict(k=k, v=v))
+    ik, iv = _at(torch.tensor([t for _, t in where], device="cuda"))
+    for r, (pg, _) in enumerate(where):
+        K[0, pg, :, ik[r]] = y[r, nq:nq + nkv]
+        V[0, pg, :, iv[r]] = y[r, nq + nkv:]
     return dict(q=y[:, :nq].reshape(-1, nq * D), k=k, v=v)
 
 
@@ -617,6 +655,7 @@ def _exact_branch(case, d):
                 refs[table[s][j]] += 1
     before, free = list(refs), [p for p, c in enumerate(refs) if c == 0]
     total, out, k, v = 0, [], d["k"].clone(), d["v"].clone()
+    pools, copies = list(_flat(d)), list(_flat(dict(k=k, v=v)))
     for s in range(n):
         m, L = start[s + 1] - start[s], lens[s]
         row = [0, 0, -1, -1]
@@ -634,9 +673,8 @@ def _exact_branch(case, d):
                         refs[o] -= 1
                         if j == L // page and L % page:
                             row[2:] = o, p
-                            t = torch.arange(L % page, device="cuda")
-                            k[:, p, :, t] = d["k"][:, o, :, t]
-                            v[:, p, :, t // 8, :, t % 8] = d["v"][:, o, :, t // 8, :, t % 8]
+                            t = torch.arange(-(-(L % page) // 8) * 8, device="cuda")
+                            _move(pools, copies, o, t, p, t)
         out.append(row)
     res = [torch.tensor(x) for x in (table, lens, refs, out)]
     return dict(zip(("table", "lens", "refs", "reserved"), res), k=k.double(), v=v.double())
@@ -646,13 +684,13 @@ def _exact_commit(case, d):
     page = case["page"]
     start, lens, table, accepted, path = _host(d, "row_start", "lens", "table", "accepted", "path")
     k, v, new = d["k"].clone(), d["v"].clone(), []
+    pools = list(_flat(dict(k=k, v=v)))
     for s, L in enumerate(lens):
         for i in range(accepted[s] + 1):  # (a path goes upwards: nothing is read after it was written)
             a, b = L + path[start[s] + i], L + i
             pa, pb = table[s][a // page], table[s][b // page]
-            a, b = a % page, b % page
-            k[:, pb, :, b] = k[:, pa, :, a]
-            v[:, pb, :, b // 8, :, b % 8] = v[:, pa, :, a // 8, :, a % 8]
+            a, b = (torch.tensor([x % page], device="cuda") for x in (a, b))
+            _move(pools, pools, pa, a, pb, b)
         new.append(L + accepted[s] + 1)
     return dict(k=k.double(), v=v.double(), lens=torch.tensor(new))
 
