@@ -319,6 +319,126 @@ mj_status mj_attn_block_kv8(mj_ctx* ctx, const mj_attn_config* cfg, const mj_att
                             const int32_t* parents_host, int M, const float* mass_in,
                             float* mass_out);
 
+/* ------------------------------------- the verify step of many requests ------ */
+/* A server's requests in one pool of fp16 pages (no counterpart in the reference, whose engine holds one
+ * request): every layer's page p holds the same tokens of that layer, so one table serves all layers.
+ * A step of a batch of sequences:
+ *   mj_pages_reserve   room for the batch's rows (shared pages that they go to are copied first)
+ *   mj_paged_append    in every layer: queries and keys finished, keys and values written
+ *   mj_paged_attn      in every layer: the rows' attention over their sequences' pages
+ *   mj_accept_rows     the drafts checked against the target's probabilities
+ *   mj_pages_commit    the accepted rows' keys and values together, lengths advanced
+ * mj_pages_fork lets sequences share another's pages, mj_pages_truncate gives pages back.
+ *
+ * Lengths, tables, counts and the rows of a batch are device arrays: every call is asynchronous and may be
+ * captured, and a replay goes by what the arrays hold then (calls with workspace, as the 8-bit
+ * cache's: from ws, 16-byte aligned, or, ws NULL, from the context's growable scratch, and then refused while
+ * the stream is being captured; calls that share a ws must be ordered by the caller).  Whatever the
+ * device arrays hold, no call reads or writes outside of the arrays given: lengths count as at most what a table
+ * row can hold, a table entry outside [0, n_pages) names no page (its tokens are neither read nor
+ * written), rows beyond the batch's or beyond max_rows are left out.  Calls on one pool must be ordered
+ * by the caller, except that mj_paged_attn may overlap itself.  Heads of 128 only. */
+typedef struct mj_pages {
+    int n_layers;
+    int n_kv_heads;
+    int n_pages;
+    int page_tokens;  /* 32, 64, 128 or 256 */
+    /* fp16 [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096]: units of 32 tokens by 128 dims in the
+     * order the matrix instructions take them.  Of token t of a unit and dim d,
+     *   K: half 2048 (t / 4 % 2) + 512 (d / 32) + 128 (d / 8 % 4) + 32 (t / 8) + 8 (t % 4) + d % 8
+     *   V: half 512 (d / 16) + 128 (t / 8) + 8 (d % 16) + t % 8 */
+    void* k;
+    void* v;
+    int32_t* table;   /* [n_seqs][table_stride]: page of a sequence's block, -1 none */
+    int n_seqs;       /* at most 1024 */
+    int table_stride; /* blocks a sequence can have; times page_tokens at most 2^30 */
+    int32_t* lens;    /* [n_seqs] committed tokens */
+    int32_t* refs;    /* [n_pages] how many entries name the page; 0: it is free */
+} mj_pages;
+
+/* The rows of a pass: sequence s has rows row_start[s] .. row_start[s + 1] - 1 (none: it takes no
+ * part), at most max_rows <= MJ_MAX_ROWS.  anc [rows]: bit a of a row's mask is set if it sees row a of
+ * its sequence (a tree's: its ancestors and itself); NULL: chains (every row sees those before it and
+ * itself).  Row r of a sequence of L committed tokens is written at token L + r and stands at position L +
+ * depth, depth the count of rows before it that it sees; its parent is the last of those. */
+typedef struct mj_batch {
+    const int32_t* row_start; /* device [n_seqs + 1], not decreasing, from 0 */
+    const uint64_t* anc;      /* device [rows], or NULL */
+    int n_seqs;
+    int rows;                 /* rows of the arrays (those from row_start[n_seqs] on are left as they are) */
+    int max_rows;
+} mj_batch;
+
+/* Room for the batch's rows: every block of a sequence that rows L .. L + rows - 1 go to gets a page of its
+ * own, where it has none or one that others name too (refs other than 1).  The lowest free pages are
+ * taken, in order of the sequences and their blocks.  A sequence is served if its table row has the
+ * entries and the pages that it and all before it lack are there; others stay as they are (a sequence that
+ * lacks nothing is always served).  A shared page loses a reference for each sequence that leaves it, all
+ * counted as before the call; of the block that holds committed tokens these are copied in all layers
+ * (in groups of eight).  out int32 [n_seqs][4]: 1 if served, pages taken, then the page copied from
+ * and to (-1: none). */
+mj_status mj_pages_reserve(mj_ctx* ctx, const mj_pages* pages, const mj_batch* batch, int32_t* out);
+/* Sequence s becomes a branch of from[s]: what it had is given back, the pages of the source's committed
+ * tokens gain a reference, the length is the source's.  from [n_seqs]: outside [0, n_seqs), or s itself:
+ * s stays as it is; so it does if the source has an entry of its own in `from`. */
+mj_status mj_pages_fork(mj_ctx* ctx, const mj_pages* pages, const int32_t* from);
+/* Sequence s cut to len[s] tokens if that is not negative: blocks behind its length lose their pages,
+ * also those that were reserved for rows not kept.  len [n_seqs] (pages->lens itself: only these).
+ * A page whose count comes to 0 is free. */
+mj_status mj_pages_truncate(mj_ctx* ctx, const mj_pages* pages, const int32_t* len);
+/* The accepted rows of a pass kept: rows path[0] .. path[accepted] of a sequence (accepted [n_seqs], path
+ * [rows] at the sequence's first row, as mj_accept_rows gives them) are moved to its tokens L, L + 1, ...
+ * in all layers, and lens_out[s] = L + accepted + 1 (accepted below 0, or no rows: L).  path NULL: the rows
+ * of a chain, in place already.  An entry that names no row of the sequence moves nothing.  lens_out
+ * [n_seqs] may be pages->lens. */
+mj_status mj_pages_commit(mj_ctx* ctx, const mj_pages* pages, const mj_batch* batch,
+                          const int32_t* accepted, const int32_t* path, int32_t* lens_out);
+
+/* mj_qkv_append for a batch: queries and keys normed (a NULL weight: not), rotated at their positions,
+ * keys and values written to layer `layer` of the sequences' pages.  qkv fp16 [rows] rows of ld_qkv halves
+ * (0: packed; else a multiple of 8), q_out fp16 [rows][n_heads * 128], not over qkv.  Reads n_heads,
+ * n_kv_heads, head_dim, rope_dim, rope_base and eps of cfg. */
+mj_status mj_paged_append(mj_ctx* ctx, const mj_attn_config* cfg, const mj_pages* pages, int layer,
+                          const mj_batch* batch, const void* qkv, int64_t ld_qkv,
+                          const void* q_norm_w, const void* k_norm_w, void* q_out);
+
+/* Attention of the batch's rows: softmax(q k^T / sqrt(128)) v over the sequence's committed tokens (window >
+ * 0: those less than window before the row's position) and over the rows that the row sees, where they were
+ * written.  A row that sees nothing gives zeros.  q fp16 [rows] rows of ld_q halves (0: packed; else a
+ * multiple of 8), out likewise, not over q; at most 64 query heads a KV head.
+ * Scores, softmax statistics and outputs are summed in fp32; a weight is rounded to fp16 for the product with V
+ * (half a step, or at most 2^-34 of the row's greatest weight).  A call repeats bit for bit; a row's result
+ * in a batch of other sequences may differ by rounding (the keys are split differently). */
+mj_status mj_paged_attn(mj_ctx* ctx, const mj_pages* pages, int layer, const mj_batch* batch,
+                        int n_heads, int window, const void* q, int64_t ld_q, void* out,
+                        int64_t ld_out, void* ws, size_t ws_bytes);
+/* Bytes of workspace that mj_paged_attn takes with these heads and at most max_rows rows a sequence; 0
+ * where an argument is out of range. */
+size_t mj_paged_workspace(int n_heads, int n_kv_heads, int max_rows);
+
+/* The drafts of a batch checked from given random numbers.  logits fp32 [rows] rows of ld_logits (0: V):
+ * row r's are of the token after it; tokens int32 [rows]: the token fed there (a sequence's first row: not a
+ * draft).  p = softmax(logits / T) of the sequence's temperature T [n_seqs]; up to 1e-5 (or NaN): all on the
+ * greatest logit, the lowest id of equal ones.  A NaN logit counts as -inf; several +inf share the row.
+ * From the first row on, the current row's drafts (its children, in order) are tested: draft x with the
+ * uniform u = u_accept[its row] is accepted if q(x) > 0, p(x) > 0 and u q(x) rest <= p(x); q the
+ * distribution it was drawn from (q fp32 [rows] rows of ld_q, the parent's row; chains only; negative
+ * and NaN count as 0) or 1 (q NULL: drafts that are certain), rest 1 less p of the drafts of the row refused
+ * before it (one whose token was refused before has nothing left).  The last row reached samples its token: from p
+ * if it has no drafts, else from max(p - q, 0), or (q NULL) from p without the refused tokens; from p
+ * where that leaves nothing.  It is the lowest id where the running sum passes u_sample[s] times the whole.
+ * accepted int32 [n_seqs]: drafts accepted; path int32 [rows]: the rows kept, the first one included, then
+ * -1; token int32 [n_seqs]: the token sampled (-1: a row without any probability; a sequence without
+ * rows: accepted 0, token -1).  u in [0, 1).  Sums are held in 64 bits in a fixed order: a call repeats bit
+ * for bit.  V at most 2^23. */
+mj_status mj_accept_rows(mj_ctx* ctx, const mj_batch* batch, const float* logits, int64_t ld_logits,
+                         int V, const int32_t* tokens, const float* q, int64_t ld_q,
+                         const float* temperature, const float* u_accept, const float* u_sample,
+                         int32_t* accepted, int32_t* path, int32_t* token, void* ws,
+                         size_t ws_bytes);
+/* Bytes of workspace that mj_accept_rows takes with these sizes; 0 where one is out of range. */
+size_t mj_accept_workspace(int n_seqs, int rows, int V);
+
 /* lm_head verify -- encodeMetalHead -> maple_lm_head_argmax/reduce
  * (SeedlessDecodeEngine.swift:481-498, SeedlessMetal.swift:3005-3111) for an fp16 head:
  * logits[m][v] = sum_k w[v][k] * x[m][k] (fp32), argmax per row with the lowest id winning

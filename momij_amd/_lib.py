@@ -111,6 +111,15 @@ class KvRingStruct(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("capacity", i64)]
 
 
+class Pages(C.Structure):
+    _fields_ = [("n_layers", i32), ("n_kv_heads", i32), ("n_pages", i32), ("page_tokens", i32), ("k", vp),
+                ("v", vp), ("table", vp), ("n_seqs", i32), ("table_stride", i32), ("lens", vp), ("refs", vp)]
+
+
+class Batch(C.Structure):
+    _fields_ = [("row_start", vp), ("anc", vp), ("n_seqs", i32), ("rows", i32), ("max_rows", i32)]
+
+
 class Capture(C.Structure):
     _fields_ = [("h", vp), ("inds", vp), ("logits", vp), ("attn_out", vp), ("moe_in", vp),
                 ("router_logits", vp), ("head_in", vp), ("kv_rows", vp)]
@@ -170,6 +179,18 @@ _SIGS = {
     "mj_attn_block_kv8": (i32, [vp, C.POINTER(AttnConfig), C.POINTER(AttnWeights), C.POINTER(Kv8),
                                 C.POINTER(KvRingStruct), vp, i32, i32, i32, i32, i64, i64, vp, i32,
                                 vp, vp]),
+    "mj_pages_reserve": (i32, [vp, C.POINTER(Pages), C.POINTER(Batch), vp]),
+    "mj_pages_fork": (i32, [vp, C.POINTER(Pages), vp]),
+    "mj_pages_truncate": (i32, [vp, C.POINTER(Pages), vp]),
+    "mj_pages_commit": (i32, [vp, C.POINTER(Pages), C.POINTER(Batch), vp, vp, vp]),
+    "mj_paged_append": (i32, [vp, C.POINTER(AttnConfig), C.POINTER(Pages), i32, C.POINTER(Batch), vp, i64,
+                              vp, vp, vp]),
+    "mj_paged_attn": (i32, [vp, C.POINTER(Pages), i32, C.POINTER(Batch), i32, i32, vp, i64, vp, i64, vp,
+                            C.c_size_t]),
+    "mj_paged_workspace": (C.c_size_t, [i32, i32, i32]),
+    "mj_accept_rows": (i32, [vp, C.POINTER(Batch), vp, i64, i32, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp,
+                             C.c_size_t]),
+    "mj_accept_workspace": (C.c_size_t, [i32, i32, i32]),
     "mj_accept_greedy": (i32, [vp, vp, vp, vp, i32, vp]),
     "mj_accept_sampled": (i32, [vp, vp, i32, i32, vp, f32, i32, vp, u64, u64, vp]),
     "mj_accept_sampled_ex": (i32, [vp, vp, i32, i32, vp, C.POINTER(Sampling), i32, vp, u64, u64,

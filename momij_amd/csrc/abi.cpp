@@ -93,6 +93,21 @@ mj_status mj_refuse_capture(mj_ctx* ctx, const char* what) {
     return s;
 }
 
+// Device scratch of one call: the caller's, or the context's (not while its stream is captured).
+mj_status take_ws(mj_ctx* ctx, void* ws, size_t ws_bytes, size_t need, const char* what, void** out) {
+    if (!ws) {
+        mj_status s = mj_refuse_capture(ctx, what);
+        if (s == MJ_OK) s = mj_scratch_reserve(ctx, need);
+        *out = ctx->scratch;
+        return s;
+    }
+    if (!aligned16({ws}) || ws_bytes < need)
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: workspace of %zu bytes (needs %zu, 16-byte aligned)",
+                       what, ws_bytes, need);
+    *out = ws;
+    return MJ_OK;
+}
+
 void* Arena::take(size_t bytes) {
     off = (off + 255) & ~(size_t)255;
     void* p = base ? (char*)base + off : nullptr;

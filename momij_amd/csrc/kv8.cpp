@@ -10,30 +10,6 @@
 
 namespace {
 
-// The context's device for the time of one call.
-struct OnDevice {
-    int prev = -1;
-    explicit OnDevice(int dev) {
-        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-        if (prev != dev) (void)hipSetDevice(dev);
-        else prev = -1;
-    }
-    ~OnDevice() {
-        if (prev >= 0) (void)hipSetDevice(prev);
-    }
-};
-
-bool aligned16(std::initializer_list<const void*> ps) {
-    uintptr_t bits = 0;
-    for (const void* p : ps) bits |= (uintptr_t)p;
-    return (bits & 15) == 0;
-}
-
-bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y ? y - x < a_bytes : x - y < b_bytes;
-}
-
 constexpr int kMaxGroup = 64;              // query heads a KV head
 constexpr int kMaxBlocks = 1 << 20;        // blocks a head lists
 constexpr int64_t kMaxRing = 1ll << 30;    // slots (slots are counted in 32 bits)
@@ -89,21 +65,6 @@ mj_status check_rows(mj_ctx* ctx, int n_heads, int n_kv, int M, const void* q, i
         return mj_fail(ctx, MJ_INVALID_ARG,
                        "%s: rows of %lld halves in a stride of %lld (a multiple of 8, 16-byte aligned)",
                        what, (long long)width, (long long)ld);
-    return MJ_OK;
-}
-
-// Device scratch of one call: the caller's, or the context's (not while its stream is captured).
-mj_status take_ws(mj_ctx* ctx, void* ws, size_t ws_bytes, size_t need, const char* what, void** out) {
-    if (!ws) {
-        mj_status s = mj_refuse_capture(ctx, what);
-        if (s == MJ_OK) s = mj_scratch_reserve(ctx, need);
-        *out = ctx->scratch;
-        return s;
-    }
-    if (!aligned16({ws}) || ws_bytes < need)
-        return mj_fail(ctx, MJ_INVALID_ARG, "%s: workspace of %zu bytes (needs %zu, 16-byte aligned)",
-                       what, ws_bytes, need);
-    *out = ws;
     return MJ_OK;
 }
 

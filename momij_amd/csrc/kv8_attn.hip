@@ -13,20 +13,6 @@
 #define HD 128
 #define SC2 (1.44269504088896341f * 0.08838834764831845f)  // log2 e / sqrt(128)
 
-// max / sum over lanes i, i ^ 16, i ^ 32, i ^ 48 (the same bits in every lane)
-__device__ __forceinline__ float x4_max(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float x4_sum(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // Four codes (bytes, code + 128) to four halves, exactly: a byte under the exponent of 1024 is 1024 +
 // code + 128, and 1152 is taken off.
 __device__ __forceinline__ void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -115,12 +101,6 @@ __device__ __forceinline__ float log2_scale(float vs) {  // (a NaN stays one)
 // branch that it has for moving.  A weight is then up to 2^(lv + LIFT): below 2^15.1 for a sealed block
 // (scale 65504 / 127 at most), which is what LV_TOP is for.
 #define FAR 1048576.0f
-
-// a * b rounded (the compiler would make one fma of it and a difference)
-__device__ __forceinline__ float product(float a, float b) {
-#pragma clang fp contract(off)
-    return a * b;
-}
 
 // The reference moved, for T tiles at once (one branch; the weights of one tile can then be formed
 // under the products of another); c: what makes exp2(fma(S, ksc, c)) of vector ln's scores its weights.
@@ -212,16 +192,6 @@ __device__ __forceinline__ void add_bad_rows(Tile& T, int lane, uint64_t ok, uin
             for (int x = 0; x < 4; ++x) T.o[dt][x] += (att >> x) & 1 ? e : 0.0f;
         }
     }
-}
-
-__device__ __forceinline__ u4v finite8(u4v v, bool& bad) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool b0 = (v[j] & 0x7C00u) == 0x7C00u, b1 = (v[j] & 0x7C000000u) == 0x7C000000u;
-        bad |= b0 | b1;
-        v[j] = (b0 ? 0u : v[j] & 0xFFFFu) | (b1 ? 0u : v[j] & 0xFFFF0000u);
-    }
-    return v;
 }
 
 // Query vector v of KV head g (head j of the group, row r: v = r * G + j) as the B operand: operand s

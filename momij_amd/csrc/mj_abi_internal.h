@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -114,3 +115,30 @@ bool moe_wide_supported(int H, int I, int E, int k, int gs);
 mj_status run_moe(mj_ctx* ctx, const mj_moe_weights* w, const uint16_t* x, uint16_t* y, int M,
                   int flags, const MoeScratch& ms, int32_t* inds, float* scores, hipStream_t st,
                   Prof* prof = nullptr, const NormOut* next = nullptr);
+
+// The context's device for the time of one call.
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(int dev) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev != dev) (void)hipSetDevice(dev);
+        else prev = -1;
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+inline bool aligned16(std::initializer_list<const void*> ps) {
+    uintptr_t bits = 0;
+    for (const void* p : ps) bits |= (uintptr_t)p;
+    return (bits & 15) == 0;
+}
+
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
+
+// Device scratch of one call: the caller's, or the context's (not while its stream is captured).
+mj_status take_ws(mj_ctx* ctx, void* ws, size_t ws_bytes, size_t need, const char* what, void** out);

@@ -208,6 +208,37 @@ __device__ __forceinline__ void wave_argmax(float& v, int& i) {
     }
 }
 
+// max / sum over lanes i, i ^ 16, i ^ 32, i ^ 48 (the same bits in every lane)
+__device__ __forceinline__ float x4_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float x4_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// a * b rounded (the compiler would make one fma of it and a difference)
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
+// Infinities and NaN among eight halves taken as 0 (bad set where there are any).
+__device__ __forceinline__ u4v finite8(u4v v, bool& bad) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool b0 = (v[j] & 0x7C00u) == 0x7C00u, b1 = (v[j] & 0x7C000000u) == 0x7C000000u;
+        bad |= b0 | b1;
+        v[j] = (b0 ? 0u : v[j] & 0xFFFFu) | (b1 ? 0u : v[j] & 0xFFFF0000u);
+    }
+    return v;
+}
+
 // Running log-sum-exp in log2 units: (m, s) stands for s * 2^m.  (-inf, 0) is empty.
 __device__ __forceinline__ void lse_merge(float& m, float& s, float om, float os) {
     const float mn = fmaxf(m, om);

@@ -243,6 +243,87 @@ class Context:
                                               self._parents(parents, M), M,
                                               self._mass(mass_in, cache), self._mass(mass_out, cache)))
 
+    # ------------------------------------------- the verify step of many requests (paged.py)
+    def _ids(self, t, n: int, what: str, dtype=torch.int32) -> int:
+        if t.dtype is dtype and t.get_device() == self.device and t.numel() >= n and t.is_contiguous():
+            return t.data_ptr()
+        raise ValueError(f"{what}: {n} contiguous {dtype} on device {self.device}, not {t.dtype} "
+                         f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
+
+    def _logits(self, t, rows: int, what: str) -> tuple:
+        """Address, row stride and width of fp32 rows [rows][V]."""
+        if (t.dtype is torch.float32 and t.get_device() == self.device and t.dim() == 2 and
+                t.size(0) >= rows and (t.stride(1) == 1 or t.size(1) == 1) and
+                (rows <= 1 or t.stride(0) >= t.size(1))):
+            return t.data_ptr(), t.stride(0) if rows > 1 else 0, t.size(1)
+        raise ValueError(f"{what}: {rows} rows of fp32 values on device {self.device}, not {t.dtype} "
+                         f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
+
+    def pages_reserve(self, cache, batch, out):
+        """Room for the batch's rows; out int32 [n_seqs][4]: served, pages taken, page copied from, to."""
+        self.check(self.lib.mj_pages_reserve(self.h, cache.on(self.device), batch.on(self.device),
+                                             self._ids(out, 4 * cache.n_seqs, "out")))
+
+    def pages_fork(self, cache, source):
+        """source int32 [n_seqs]: the sequence that each becomes a branch of (-1: it stays)."""
+        self.check(self.lib.mj_pages_fork(self.h, cache.on(self.device),
+                                          self._ids(source, cache.n_seqs, "source")))
+
+    def pages_truncate(self, cache, lengths):
+        """lengths int32 [n_seqs]: tokens that a sequence keeps at most (-1: it stays)."""
+        self.check(self.lib.mj_pages_truncate(self.h, cache.on(self.device),
+                                              self._ids(lengths, cache.n_seqs, "lengths")))
+
+    def pages_commit(self, cache, batch, accepted, path=None, lens_out=None):
+        """The accepted rows kept (path None: chains, in place already); lens_out None: cache.lens."""
+        lens = cache.lens if lens_out is None else lens_out
+        self.check(self.lib.mj_pages_commit(
+            self.h, cache.on(self.device), batch.on(self.device),
+            self._ids(accepted, cache.n_seqs, "accepted"),
+            None if path is None else self._ids(path, batch.rows, "path"),
+            self._ids(lens, cache.n_seqs, "lens_out")))
+
+    def paged_append(self, cfg: dict, cache, layer: int, batch, qkv, q_norm_w, k_norm_w, q_out):
+        c, dev, M = self.attn_config(cfg), self.device, batch.rows
+        if M == 0:
+            return
+        for w in (q_norm_w, k_norm_w):
+            if w is not None:
+                packed(w, _F16, 1, 128, dev, "norm weight")
+        ld = row_stride(qkv, M, (c.n_heads + 2 * c.n_kv_heads) * 128, dev, "qkv")
+        self.check(self.lib.mj_paged_append(self.h, C.byref(c), cache.on(dev), layer, batch.on(dev),
+                                            qkv.data_ptr(), ld, ptr(q_norm_w), ptr(k_norm_w),
+                                            packed(q_out, _F16, M, c.n_heads * 128, dev, "q_out")))
+
+    def paged_attn(self, cache, layer: int, batch, q, n_heads: int, out, window: int = 0, ws=None):
+        dev, M, width = self.device, batch.rows, n_heads * 128
+        if M == 0:
+            return
+        self.check(self.lib.mj_paged_attn(self.h, cache.on(dev), layer, batch.on(dev), n_heads, window,
+                                          q.data_ptr(), row_stride(q, M, width, dev, "q"), out.data_ptr(),
+                                          row_stride(out, M, width, dev, "out"), *self._space(ws)))
+
+    def paged_workspace(self, n_heads: int, n_kv_heads: int, max_rows: int) -> int:
+        return int(self.lib.mj_paged_workspace(n_heads, n_kv_heads, max_rows))
+
+    def accept_rows(self, batch, logits, tokens, temperature, u_accept, u_sample, accepted, path, token,
+                    q=None, ws=None):
+        """Drafts of a batch checked from given random numbers; q fp32 [rows][V]: the distributions that
+        the drafts below a row were drawn from (None: drafts that are certain)."""
+        R, n, f32 = batch.rows, batch.n_seqs, torch.float32
+        x, ld, V = self._logits(logits, R, "logits")
+        y, ldq, Vq = (None, 0, V) if q is None else self._logits(q, R, "q")
+        if Vq != V:
+            raise ValueError(f"q: {Vq} ids, the logits: {V}")
+        self.check(self.lib.mj_accept_rows(
+            self.h, batch.on(self.device), x, ld, V, self._ids(tokens, R, "tokens"), y, ldq,
+            self._ids(temperature, n, "temperature", f32), self._ids(u_accept, R, "u_accept", f32),
+            self._ids(u_sample, n, "u_sample", f32), self._ids(accepted, n, "accepted"),
+            self._ids(path, R, "path"), self._ids(token, n, "token"), *self._space(ws)))
+
+    def accept_workspace(self, n_seqs: int, rows: int, V: int) -> int:
+        return int(self.lib.mj_accept_workspace(n_seqs, rows, V))
+
     def lm_head_verify(self, x, w, M, K, V, out_argmax, out_max=None, out_logits=None,
                        banned=None, n_banned=0, temperature=1.0, out_lse=None):
         self.check(self.lib.mj_lm_head_verify(self.h, ptr(x), ptr(w), M, K, V, ptr(banned),
