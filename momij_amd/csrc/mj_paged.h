@@ -80,13 +80,6 @@ struct AcceptPart {
     float m;
     int at;
 };
-// What is left to do for a sequence after its drafts were checked: row (-1: nothing) to sample, how
-// (the row's probabilities, without n_out tokens, or less the draft's), Z and m of the row.
-struct AcceptLast {
-    double Z;
-    float m;
-    int row, mode, n_out;
-};
 struct AcceptArgs {
     PgRows b;
     const float* logits;
@@ -103,9 +96,8 @@ struct AcceptArgs {
     int32_t* token;
     // workspace
     AcceptPart* part;  // [rows][chunks]
-    AcceptLast* last;  // [n_seqs]
-    int32_t* out_ids;  // [n_seqs][MJ_ROWS] refused drafts of the last row
-    double* csum;      // [n_seqs][chunks]
+    double* csum;      // [n_seqs][chunks] what is left of the last row's probabilities
+    int32_t* count;    // [n_seqs] blocks that have stored theirs
     int chunks;
     const int* abort;
 };
