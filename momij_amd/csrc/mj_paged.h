@@ -55,6 +55,7 @@ hipError_t launch_pages_commit(const PgPool& p, const PgRows& b, const int32_t* 
                                const int32_t* path, int32_t* lens_out, const int* abort,
                                hipStream_t st);
 
+#define PG_MAX_BLOCKS 512  // of an attention launch
 struct PgAttnArgs {
     PgPool p;
     PgRows b;
@@ -63,8 +64,9 @@ struct PgAttnArgs {
     uint16_t* out;
     int64_t ldo;
     int layer, G, window;
-    // set by paged_attn_plan: blocks of the launch, query vectors a column group, and the workspace
-    int blocks, cols;
+    // set by paged_attn_plan: blocks of the launch, query vectors a column group, units
+    // a block at least, and the workspace
+    int blocks, cols, least;
     int64_t* off;   // [n_seqs + 2]: units before each sequence, units in all, units a block
     float* po;      // [blocks][2][cols][128] partial outputs of a block's first and last segment
     float2* pml;    // [blocks][2][cols] {reference, sum}

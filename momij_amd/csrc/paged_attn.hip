@@ -6,6 +6,8 @@
 // ones and its work does not depend on how long which sequence is.  A run is cut where a sequence, head or
 // column group ends; a segment that is all of its group's keys is finished by its block, others leave a
 // partial result, and k_paged_join puts these together.  Scores are kept in log2 units.
+#include <type_traits>
+
 #include "mj_abi_internal.h"
 #include "mj_device.h"
 #include "mj_paged.h"
@@ -110,6 +112,12 @@ struct PgCol {
     }
 };
 
+// Bits 0 and 16: of two halves, those that are infinities or NaN (an exponent of all ones carries into the
+// sign's place).  In whole numbers: as comparisons they would take a scalar mask each.
+__device__ __forceinline__ uint32_t bad_halves(uint32_t y) {
+    return ((y & 0x7C007C00u) + 0x04000400u) >> 15 & 0x00010001u;
+}
+
 // Infinities and NaN of V in a unit that not every row sees whole (0 times an infinity is a NaN): they are
 // left out of the product and added here to the outputs of the vectors that attend to them, whatever
 // their weights (which are above 0, if not in fp32).  ok: the unit's tokens that vector ln sees.
@@ -118,192 +126,323 @@ __device__ __forceinline__ void add_bad(PgTile& T, const uint16_t* vu, uint32_t 
 #pragma unroll 1
     for (; bad; bad &= bad - 1) {
         const int t = __builtin_ctz(bad);
-        const bool sees = (ok >> t) & 1;
+        const uint32_t sees = 0u - ((ok >> t) & 1u);
+        const uint16_t* row = vu + pg_v_at(t, 4 * lq);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
+        for (int dt = 0; dt < 8; ++dt) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float v = h2f(vu[pg_v_at(t, 16 * dt + 4 * lq + r)]);
-                T.o[dt][r] += sees && !(fabsf(v) < INFINITY) ? v : 0.0f;
+                const uint32_t v = row[512 * dt + 8 * r];
+                T.o[dt][r] += h2f((uint16_t)(v & sees & (0u - bad_halves(v))));
             }
+            __builtin_amdgcn_sched_barrier(0);  // (32 requests at once take 40 registers from the main loop)
+        }
     }
 }
 
-// A block of four waves takes its run of units, a segment at a time; a wave takes every fourth unit of
-// it, straight from the pages into registers, and the four states meet in LDS.
-__global__ __launch_bounds__(256) void k_paged_attn(PgAttnArgs a) {
-    __shared__ int64_t s_off[PG_MAX_SEQS + 1];
-    __shared__ int64_t s_wsum[4];
-    __shared__ float s_o[4][16][HD + 4];
-    __shared__ float2 s_ml[4][16];
-    if (block_aborted(a.abort)) return;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, ln = lane & 15, lq = lane >> 4;
-    {
-        int64_t u[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            u[i] = 0;
-            if (4 * t + i < a.b.n_seqs) {
-                const SeqUnits q = seq_units(a, 4 * t + i);
-                u[i] = (int64_t)q.nu * q.ncg * a.p.nKV;
-            }
-            sum += u[i];
+// Units before each sequence (s_off[0 .. n]) and the run of this block, by one round of requests and a scan
+// for every NT sequences; a.off gets them for the join.  False: the call was aborted.
+struct PgRun {
+    int64_t b0, b1, per;
+    int s;  // the sequence that the run begins in
+};
+template <int NT>
+__device__ __forceinline__ bool plan_run(const PgAttnArgs& a, int64_t* s_off, int64_t* s_wsum, int* s_abort,
+                                         PgRun& run) {
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = a.b.n_seqs;
+    const int ab = a.abort ? *a.abort : 0;
+    int64_t before = 0;
+    for (int c = 0; c < n; c += NT) {
+        int64_t u = 0;
+        if (c + t < n) {
+            const SeqUnits q = seq_units(a, c + t);
+            u = (int64_t)q.nu * q.ncg * a.p.nKV;
         }
-        int64_t inc = sum;
+        int64_t inc = u;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int64_t x = __shfl_up(inc, o, MJ_WAVE);
             inc += lane >= o ? x : 0;
         }
+        if (c) __syncthreads();
         if (lane == 63) s_wsum[w] = inc;
+        if (t == 0 && c == 0) *s_abort = ab;
         __syncthreads();
-        int64_t at = inc - sum;
-        for (int i = 0; i < w; ++i) at += s_wsum[i];
+        int64_t at = before, all = before;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (4 * t + i <= a.b.n_seqs) s_off[4 * t + i] = at;
-            at += u[i];
+        for (int i = 0; i < NT / 64; ++i) {
+            at += i < w ? s_wsum[i] : 0;
+            all += s_wsum[i];
         }
-        if (t == 255 && a.b.n_seqs == PG_MAX_SEQS) s_off[PG_MAX_SEQS] = at;
-        __syncthreads();
+        if (c + t <= n) s_off[c + t] = at + inc - u;
+        if (c + t + 1 == n) s_off[n] = at + inc;
+        before = all;
     }
-    const int n = a.b.n_seqs;
-    const int64_t total = s_off[n];
-    const int64_t per = max((total + a.blocks - 1) / a.blocks, (int64_t)4);
+    __syncthreads();
+    if (*s_abort) return false;
+    run.per = max((before + a.blocks - 1) / a.blocks, (int64_t)a.least);
     if (blockIdx.x == 0)
-        for (int i = t; i <= n + 1; i += 256) a.off[i] = i <= n ? s_off[i] : per;
-    const int64_t b0 = blockIdx.x * per, b1 = min(total, b0 + per);
-    int64_t x = b0;
-    int s = 0;
-    if (x < b1) {  // the last sequence that begins at or before the run
+        for (int i = t; i <= n + 1; i += NT) a.off[i] = i <= n ? s_off[i] : run.per;
+    run.b0 = blockIdx.x * run.per;
+    run.b1 = min(before, run.b0 + run.per);
+    run.s = 0;
+    if (run.b0 < run.b1) {  // the last sequence that begins at or before the run
         int hi = n;
-        while (hi - s > 1) {
-            const int mid = (s + hi) >> 1;
-            if (s_off[mid] <= x) s = mid;
+        while (hi - run.s > 1) {
+            const int mid = (run.s + hi) >> 1;
+            if (s_off[mid] <= run.b0) run.s = mid;
             else hi = mid;
         }
     }
-    while (x < b1) {
-        while (s_off[s + 1] <= x) ++s;
-        const SeqUnits su = seq_units(a, s);
-        const int64_t rel = x - s_off[s];
-        const int gc = (int)(rel / su.nu), i0 = (int)(rel - (int64_t)gc * su.nu);
-        const int i1 = (int)min((int64_t)su.nu, i0 + (b1 - x));
-        const int g = gc / su.ncg, c = gc - g * su.ncg;
-        const int v0 = c * a.cols, nv = su.m * a.G;
-        // the vectors
-        PgCol col;
-        const int v = v0 + ln;
-        col.on = v < nv;
-        const int vr = col.on ? v / a.G : 0, vh = g * a.G + (col.on ? v - vr * a.G : 0);
-        col.anc = pg_anc(a.b, su.r0 + vr, vr);
-        if (su.m < 64) col.anc &= (1ull << su.m) - 1;  // (a row that there is not is nobody's ancestor)
-        col.first = a.window > 0 ? max(0, su.L + pg_depth(col.anc, vr) - a.window + 1) : 0;
-        u4v q[4];
-        const uint16_t* qp = a.q + (su.r0 + vr) * a.ldq + vh * HD + 8 * lq;
+    return true;
+}
+
+// A segment: units lo + i0 .. lo + i1 - 1 of a sequence, head and column group.
+struct PgSeg {
+    SeqUnits su;
+    int s, g, i0, i1, v0, vend;  // query vectors v0 .. vend - 1 of the sequence's rows and the group's heads
+    int clean0, clean1;          // units that every row sees whole
+    bool whole;                  // all of the group's units
+    int64_t slot;                // where a partial result goes
+};
+__device__ __forceinline__ PgSeg next_seg(const PgAttnArgs& a, const int64_t* s_off, PgRun& run, int64_t x) {
+    while (s_off[run.s + 1] <= x) ++run.s;
+    PgSeg S;
+    S.s = run.s;
+    S.su = seq_units(a, S.s);
+    const int64_t rel = x - s_off[S.s];
+    const int gc = (int)(rel / S.su.nu);
+    S.i0 = (int)(rel - (int64_t)gc * S.su.nu);
+    S.i1 = (int)min((int64_t)S.su.nu, S.i0 + (run.b1 - x));
+    S.g = gc / S.su.ncg;
+    S.v0 = (gc - S.g * S.su.ncg) * a.cols;
+    S.vend = min(S.su.m * a.G, S.v0 + a.cols);
+    S.clean0 = a.window > 0 ? (max(0, S.su.L + MJ_ROWS - a.window + 1) + PG_UNIT - 1) / PG_UNIT : 0;
+    S.clean1 = S.su.L / PG_UNIT;
+    S.whole = S.i0 == 0 && S.i1 == S.su.nu;
+    S.slot = (int64_t)blockIdx.x * 2 + (x == run.b0 ? 0 : 1);
+    return S;
+}
+// The page of the segment's unit i, or -1.
+__device__ __forceinline__ int seg_page(const PgAttnArgs& a, const PgSeg& S, int i) {
+    return pg_page(a.p, S.s, ((S.su.lo + i) * PG_UNIT) >> a.p.shift);
+}
+// Halves from a layer's first to the segment's unit i in page pg.
+__device__ __forceinline__ size_t seg_at(const PgAttnArgs& a, const PgSeg& S, int i, int pg) {
+    const int in = ((S.su.lo + i) * PG_UNIT) & (a.p.page - 1);
+    return ((size_t)pg * a.p.nKV + S.g) * a.p.head_halves() + (size_t)(in >> 5) * PG_UNIT_HALVES;
+}
+
+// Query vector v (lanes without one take the group's first, unused) and what its row sees.
+__device__ __forceinline__ void load_vector(const PgAttnArgs& a, const PgSeg& S, int v, u4v q[4], PgCol& col) {
+    const int lq = (threadIdx.x & 63) >> 4;
+    col.on = v < S.vend;
+    const int r = col.on ? v / a.G : 0, h = S.g * a.G + (col.on ? v - r * a.G : 0);
+    const uint16_t* qp = a.q + (S.su.r0 + r) * a.ldq + h * HD + 8 * lq;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = *(const u4v*)(qp + 32 * k);
-        // units before `clean` (of those behind the window's first whole one) are seen whole by every row
-        const int clean0 = a.window > 0 ? (max(0, su.L + MJ_ROWS - a.window + 1) + PG_UNIT - 1) / PG_UNIT : 0;
-        const int clean1 = su.L / PG_UNIT;
-        PgTile T;
-        T.clear();
-        for (int i = i0 + w; i < i1; i += 4) {
-            const int unit = su.lo + i, pos = unit * PG_UNIT;
-            const int pg = pg_page(a.p, s, pos >> a.p.shift);
-            if (pg < 0) continue;
-            const size_t at = a.layer * a.p.layer_halves() + ((size_t)pg * a.p.nKV + g) * a.p.head_halves() +
-                              (size_t)((pos & (a.p.page - 1)) >> 5) * PG_UNIT_HALVES;
-            const u4v* ku = (const u4v*)(a.p.k + at) + lane;
-            const u4v* vu = (const u4v*)(a.p.v + at) + lane;
-            u4v kr[8], vr8[8];
+    for (int k = 0; k < 4; ++k) q[k] = *(const u4v*)(qp + 32 * k);
+    col.anc = pg_anc(a.b, S.su.r0 + r, r);
+    const int depth = pg_depth(col.anc, r);
+    if (S.su.m < 64) col.anc &= (1ull << S.su.m) - 1;  // (a row that there is not is nobody's ancestor)
+    col.first = a.window > 0 ? max(0, S.su.L + depth - a.window + 1) : 0;
+}
+
+// Scores of tokens that vector ln does not see taken out (ok: those that it sees).
+__device__ __forceinline__ void mask_scores(f4 S[2], uint32_t ok) {
+    const uint32_t mine = ok >> (8 * ((threadIdx.x & 63) >> 4));
 #pragma unroll
-            for (int k = 0; k < 8; ++k) kr[k] = ku[64 * k];
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) vr8[k] = vu[64 * k];
-            f4 S[2];
+        for (int r = 0; r < 4; ++r) S[t][r] = (mine >> (4 * t + r)) & 1 ? S[t][r] : -INFINITY;
+}
+// Infinities and NaN of a unit's V operands taken as 0; which tokens hold any, the same in every lane.
+// Lane (ln, lq) has tokens 8 lq + j of dims 16 k + ln.
+__device__ __forceinline__ uint32_t clear_bad(u4v v[8]) {
+    uint32_t my = 0;
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
-                S[tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < 4; ++j) {
+        uint32_t any = 0;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) S[tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[k]), S[tt]);
-            }
-            uint32_t bad = 0, ok = ~0u;
-            if (unit < clean0 || unit >= clean1) {
-                ok = col.mask(pos, su.L);
-                const uint32_t mine = ok >> (8 * lq);
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t b = bad_halves(v[k][j]);
+            any |= b;
+            v[k][j] &= ~(b * 0xFFFFu);
+        }
+        my |= (any & 1u) << (2 * j) | (any >> 16) << (2 * j + 1);
+    }
+    if (!__any(my != 0)) return 0;
+    my <<= 8 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
+    for (int o = 1; o < 64; o <<= 1) my |= __shfl_xor(my, o, MJ_WAVE);
+    return my;
+}
+
+// A tile's state out: its vectors v .. v + 15 finished, or as a partial result.
+__device__ __forceinline__ void write_tile(const PgAttnArgs& a, const PgSeg& S, int v, const PgTile& T, float l) {
+    const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
+    if (v + ln >= S.vend) return;
+    if (S.whole) {
+        const int r = (v + ln) / a.G, h = S.g * a.G + (v + ln) - r * a.G;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
+        uint16_t* o = a.out + (S.su.r0 + r) * a.ldo + h * HD + 4 * lq;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        S[tt][r] = (mine >> (4 * tt + r)) & 1 ? S[tt][r] : -INFINITY;
-                // which tokens hold an infinity or a NaN: lane (ln, lq) has tokens 8 lq + j of dims 16 dt + ln
-                uint32_t my = 0;
+        for (int dt = 0; dt < 8; ++dt)
+            *(uint2*)(o + 16 * dt) = make_uint2(pack2(f2h(T.o[dt][0] * inv), f2h(T.o[dt][1] * inv)),
+                                                pack2(f2h(T.o[dt][2] * inv), f2h(T.o[dt][3] * inv)));
+        return;
+    }
+    const size_t at = (size_t)S.slot * a.cols + (v - S.v0) + ln;
+    if (lq == 0) a.pml[at] = make_float2(T.m, l);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+    for (int dt = 0; dt < 8; ++dt) *(f4*)(a.po + at * HD + 16 * dt + 4 * lq) = T.o[dt];
+}
+
+// Several waves' states of the same vectors brought together: the others leave theirs in LDS (put), the
+// first takes them up (add).
+struct PgLeft {
+    f4 o[8][64];
+    float m[64], l[64];
+};
+__device__ __forceinline__ void put_tile(PgLeft& p, const PgTile& T) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t y = vr8[k][j];
-                        const bool h0 = (y & 0x7C00u) == 0x7C00u, h1 = (y & 0x7C000000u) == 0x7C000000u;
-                        my |= (h0 ? 1u : 0u) << (2 * j) | (h1 ? 2u : 0u) << (2 * j);
-                        vr8[k][j] = (h0 ? 0u : y & 0xFFFFu) | (h1 ? 0u : y & 0xFFFF0000u);
-                    }
-                if (__any(my != 0)) {
-                    my <<= 8 * lq;
+    for (int dt = 0; dt < 8; ++dt) p.o[dt][lane] = T.o[dt];
+    p.m[lane] = T.m;
+    p.l[lane] = T.l;
+}
+__device__ __forceinline__ void add_tile(const PgLeft& p, PgTile& T) {
+    const int lane = threadIdx.x & 63;
+    const float om = p.m[lane], mn = fmaxf(T.m, om);
+    const float f0 = T.m == mn ? 1.0f : __builtin_amdgcn_exp2f(T.m - mn);  // (both may be -inf)
+    const float f1 = om == mn ? 1.0f : __builtin_amdgcn_exp2f(om - mn);
+    T.m = mn;
+    T.l = T.l * f0 + p.l[lane] * f1;
 #pragma unroll
-                    for (int o = 1; o < 64; o <<= 1) my |= __shfl_xor(my, o, MJ_WAVE);
-                    bad = my;
+    for (int dt = 0; dt < 8; ++dt) T.o[dt] = T.o[dt] * f0 + p.o[dt][lane] * f1;
+}
+
+// Up to 16 T query vectors a sequence and head.  A block of four waves takes its run of units, a segment at a
+// time; a wave takes every fourth unit of it, straight from the pages into registers: a unit's bytes lie in
+// the order of the operands.  The next unit's K goes out behind a unit's scores, its V behind the output
+// products.  Page numbers of 64 units come with one request a lane.  The states meet in LDS.
+template <int T>
+__global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
+    __shared__ int64_t s_off[PG_MAX_SEQS + 1], s_wsum[4];
+    __shared__ int s_abort;
+    __shared__ PgLeft s_left[3][T];
+    PgRun run;
+    if (!plan_run<256>(a, s_off, s_wsum, &s_abort, run)) return;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, ln = lane & 15;
+    const uint16_t* kl = a.p.k + a.layer * a.p.layer_halves();
+    const uint16_t* vl = a.p.v + a.layer * a.p.layer_halves();
+    for (int64_t x = run.b0; x < run.b1;) {
+        const PgSeg S = next_seg(a, s_off, run, x);
+        PgTile tl[T];
+        PgCol col[T];
+        u4v q[T][4], kr[8], vr[8];
+        bool fresh = true;
+        for (int ub = S.i0 + w; ub < S.i1 || fresh; ub += 256) {
+            const int mine = ub + 4 * lane;
+            const int pl = mine < S.i1 ? seg_page(a, S, mine) : -1;
+            if (fresh) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) {
+                    load_vector(a, S, S.v0 + 16 * i + ln, q[i], col[i]);
+                    tl[i].clear();
                 }
+                fresh = false;
             }
-            const u4v p = unit_weights(T, S);
+            const int first = S.su.lo + mine;
+            const uint64_t edge = __ballot(pl >= 0 && (first < S.clean0 || first >= S.clean1));
+            uint64_t todo = __ballot(pl >= 0) & ~edge;
+            auto request = [&](u4v* r, const uint16_t* base, int i) {
+                const u4v* p =
+                    (const u4v*)(base + seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i))) + lane;
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) T.o[dt] = mfma16x16x32(as_h8(vr8[dt]), as_h8(p), T.o[dt]);
-            if (bad) add_bad(T, a.p.v + at, bad, ok);
+                for (int k = 0; k < 8; ++k) r[k] = p[64 * k];
+            };
+            // unit i; MORE: unit nx requested behind it; EDGE: not every row sees all of it
+            auto step = [&](int i, int nx, auto more, auto masked) {
+                f4 sc[T][2];
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+                    for (int j = 0; j < T; ++j) sc[j][tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < T; ++j)
+                            sc[j][tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[j][k]), sc[j][tt]);
+                }
+                if constexpr (more.value) request(kr, kl, nx);
+                uint32_t bad = 0;
+                const int pos = (S.su.lo + ub + 4 * i) * PG_UNIT;
+                if constexpr (masked.value) {
+#pragma unroll
+                    for (int j = 0; j < T; ++j) mask_scores(sc[j], col[j].mask(pos, S.su.L));
+                    bad = clear_bad(vr);
+                }
+                u4v pw[T];
+#pragma unroll
+                for (int j = 0; j < T; ++j) pw[j] = unit_weights(tl[j], sc[j]);
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                    for (int j = 0; j < T; ++j)
+                        tl[j].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[j]), tl[j].o[dt]);
+                if constexpr (more.value) request(vr, vl, nx);
+                if constexpr (masked.value)
+                    if (bad) {
+                        const uint16_t* vu = vl + seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i));
+#pragma unroll
+                        for (int j = 0; j < T; ++j) add_bad(tl[j], vu, bad, col[j].mask(pos, S.su.L));
+                    }
+            };
+            int i0 = todo ? __builtin_ctzll(todo) : -1;
+            if (i0 >= 0) {
+                request(kr, kl, i0);
+                request(vr, vl, i0);
+            }
+            // (the last unit apart: a request that is not used would be waited for)
+            while (todo) {
+                const int i = i0;
+                todo &= todo - 1;
+                if (!todo) break;
+                i0 = __builtin_ctzll(todo);
+                step(i, i0, std::true_type{}, std::false_type{});
+            }
+            if (i0 >= 0) step(i0, 0, std::false_type{}, std::false_type{});
+#pragma unroll 1
+            for (uint64_t e = edge; e; e &= e - 1) {
+                i0 = __builtin_ctzll(e);
+                request(kr, kl, i0);
+                request(vr, vl, i0);
+                step(i0, 0, std::false_type{}, std::true_type{});
+            }
         }
-        // the four waves' states
-        T.l = x4_sum(T.l);
-        __syncthreads();  // (the segment before has been read)
-        if (lq == 0) s_ml[w][ln] = make_float2(T.m, T.l);
+        if (x != run.b0) __syncthreads();  // (the states of the segment before have been read)
+        if (w > 0)
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) *(f4*)&s_o[w][ln][16 * dt + 4 * lq] = T.o[dt];
+            for (int i = 0; i < T; ++i) put_tile(s_left[w - 1][i], tl[i]);
         __syncthreads();
-        const int cc = t >> 4, d0 = 8 * (t & 15);
-        float M = -INFINITY, l = 0.0f, o[8] = {};
+        if (w == 0)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) M = fmaxf(M, s_ml[k][cc].x);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 ml = s_ml[k][cc];
-            const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-            l = fmaf(f, ml.y, l);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) o[d] = fmaf(f, s_o[k][cc][d0 + d], o[d]);
-        }
-        if (v0 + cc < nv) {
-            if (i0 == 0 && i1 == su.nu) {
-                const int r = (v0 + cc) / a.G, h = g * a.G + (v0 + cc) - r * a.G;
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
-                u4v y;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) y[d] = pack2(f2h(o[2 * d] * inv), f2h(o[2 * d + 1] * inv));
-                *(u4v*)(a.out + (su.r0 + r) * a.ldo + h * HD + d0) = y;
-            } else {
-                const size_t slot = (size_t)blockIdx.x * 2 + (x == b0 ? 0 : 1);
-                const size_t at = slot * a.cols + cc;
-                if ((t & 15) == 0) a.pml[at] = make_float2(M, l);
-                *(f4*)(a.po + at * HD + d0) = (f4){o[0], o[1], o[2], o[3]};
-                *(f4*)(a.po + at * HD + d0 + 4) = (f4){o[4], o[5], o[6], o[7]};
+            for (int i = 0; i < T; ++i) {
+#pragma unroll 1
+                for (int k = 0; k < 3; ++k) add_tile(s_left[k][i], tl[i]);
+                write_tile(a, S, S.v0 + 16 * i, tl[i], x4_sum(tl[i].l));
             }
-        }
-        x += i1 - i0;
+        x += S.i1 - S.i0;
     }
 }
 
-// The partial results of one row and head, where its keys went to several blocks: eight groups of 32
-// lanes take every eighth block, four dims a lane, and the groups meet in LDS.
-__global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
-    __shared__ f4 s_o[8][32];
-    __shared__ float2 s_ml[8];
+// The partial results of one row and head, where its keys went to several blocks: their references and sums
+// first, then sixteen groups of 32 lanes take every sixteenth block's outputs, four dims a lane, with several
+// on their way (one at a time, each waited for, 128 blocks took 10 us), and the groups meet in LDS.
+#define PG_JOIN 512
+__global__ __launch_bounds__(PG_JOIN) void k_paged_join(PgAttnArgs a) {
+    __shared__ f4 s_o[PG_JOIN / 32][32];
+    __shared__ float s_f[PG_MAX_BLOCKS], s_w[2][PG_JOIN / 64];
     if (block_aborted(a.abort)) return;
     const int t = threadIdx.x, r = blockIdx.x, h = blockIdx.y, s = pg_seq(a.b, r);
     if (s >= a.b.n_seqs) return;
@@ -318,46 +457,61 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
         if (t < 16) *(u4v*)(out + 8 * t) = (u4v){0u, 0u, 0u, 0u};
         return;
     }
-    const int bA = (int)(S / per), bB = (int)((E - 1) / per);
-    if (bA == bB) return;
-    const int k = t >> 5, d = t & 31;
+    const int bA = (int)(S / per), n = (int)((E - 1) / per) - bA + 1;
+    if (n == 1) return;
+    // (blocks before the last one of a run begin it: their first slot; the first block's last segment is this one)
+    auto place = [&](int i) {
+        const int64_t b = bA + i;
+        return ((size_t)b * 2 + (S <= b * per ? 0 : 1)) * a.cols + cc;
+    };
     float M = -INFINITY, l = 0.0f;
-    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = bA + k; b <= bB; b += 8) {
-        const size_t at = ((size_t)b * 2 + (S <= b * per ? 0 : 1)) * a.cols + cc;
-        const float2 ml = a.pml[at];
-        const f4 y = *(const f4*)(a.po + at * HD + 4 * d);
-        const float mn = fmaxf(M, ml.x);
-        const float f0 = M == mn ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
-        const float f1 = ml.x == mn ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-        M = mn;
-        l = l * f0 + ml.y * f1;
-        o = o * f0 + y * f1;
+    for (int i = t; i < n; i += PG_JOIN) M = fmaxf(M, a.pml[place(i)].x);
+    M = wave_max(M);
+    if ((t & 63) == 0) s_w[0][t >> 6] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PG_JOIN / 64; ++i) M = fmaxf(M, s_w[0][i]);
+    for (int i = t; i < n; i += PG_JOIN) {
+        const float2 ml = a.pml[place(i)];
+        const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        s_f[i] = f;
+        l = fmaf(ml.y, f, l);
     }
-    if (d == 0) s_ml[k] = make_float2(M, l);
+    l = wave_sum(l);
+    if ((t & 63) == 0) s_w[1][t >> 6] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PG_JOIN / 64; ++i) l += s_w[1][i];
+    const int k = t >> 5, d = t & 31;
+    f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = k; i < n; i += 4 * (PG_JOIN / 32)) {
+        f4 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = min(i + j * (PG_JOIN / 32), n - 1);
+            y[j] = *(const f4*)(a.po + place(b) * HD + 4 * d);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * (PG_JOIN / 32) < n) o += y[j] * s_f[i + j * (PG_JOIN / 32)];
+    }
     s_o[k][d] = o;
     __syncthreads();
     if (t >= 32) return;
-    M = -INFINITY;
-    for (int i = 0; i < 8; ++i) M = fmaxf(M, s_ml[i].x);
-    l = 0.0f;
-    o = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < 8; ++i) {
-        const float2 ml = s_ml[i];
-        const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        l += ml.y * f;
-        o += s_o[i][d] * f;
-    }
+    o = s_o[0][d];
+#pragma unroll
+    for (int i = 1; i < PG_JOIN / 32; ++i) o += s_o[i][d];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
     *(uint2*)(out + 4 * d) = make_uint2(pack2(f2h(o[0] * inv), f2h(o[1] * inv)),
                                         pack2(f2h(o[2] * inv), f2h(o[3] * inv)));
 }
 
-#define PG_BLOCKS 512  // two blocks a CU
-
 size_t paged_attn_plan(PgAttnArgs& a, void* base) {
-    a.cols = 16;
-    a.blocks = PG_BLOCKS;
+    const int nv = a.b.max_rows * a.G;
+    a.cols = nv <= 16 ? 16 : 32;
+    a.blocks = 512;  // two a CU
+    a.least = 4;
     Arena ar{base, 0};
     a.off = (int64_t*)ar.take((PG_MAX_SEQS + 2) * sizeof(int64_t));
     a.pml = (float2*)ar.take((size_t)a.blocks * 2 * a.cols * sizeof(float2));
@@ -368,7 +522,10 @@ size_t paged_attn_plan(PgAttnArgs& a, void* base) {
 hipError_t launch_paged_attn(const PgAttnArgs& a, hipStream_t st) {
     if (a.b.n_seqs > PG_MAX_SEQS || a.b.rows < 1 || a.b.max_rows > MJ_ROWS || a.p.page < PG_UNIT)
         return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_paged_attn, dim3(a.blocks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_paged_join, dim3(a.b.rows, a.p.nKV * a.G), dim3(256), 0, st, a);
+    if (a.cols == 16)
+        hipLaunchKernelGGL(k_paged_attn_own<1>, dim3(a.blocks), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL(k_paged_attn_own<2>, dim3(a.blocks), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(k_paged_join, dim3(a.b.rows, a.p.nKV * a.G), dim3(PG_JOIN), 0, st, a);
     return hipGetLastError();
 }
