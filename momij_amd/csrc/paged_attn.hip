@@ -6,6 +6,8 @@
 // ones and its work does not depend on how long which sequence is.  A run is cut where a sequence, head or
 // column group ends; a segment that is all of its group's keys is finished by its block, others leave a
 // partial result, and k_paged_join puts these together.  Scores are kept in log2 units.
+#include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "mj_abi_internal.h"
@@ -34,6 +36,8 @@ __device__ __forceinline__ SeqUnits seq_units(const PgAttnArgs& a, int s) {
 
 // A tile of 16 query vectors, outputs turned: lane (ln, lq) holds vector ln's reference, its share of the
 // sum, and dims 16 dt + 4 lq + r of its output.
+typedef float f2v __attribute__((ext_vector_type(2)));
+
 struct PgTile {
     float m, l;
     f4 o[8];
@@ -56,11 +60,13 @@ struct PgTile {
 // the reference is taken off the rounded scores, in the branch that moves it.
 #define FAR 1048576.0f
 
-// Softmax of a unit's scores against the running state.  S[t]: vector ln against tokens 8 lq + 4 t + r,
-// without the scale; masked ones -inf.  p: the weights as the B operand of the product with V.
-__device__ __forceinline__ u4v unit_weights(PgTile& T, f4 S[2]) {
-    float x = fmaxf(fmaxf(fmaxf(S[0][0], S[0][1]), fmaxf(S[0][2], S[0][3])),
-                    fmaxf(fmaxf(S[1][0], S[1][1]), fmaxf(S[1][2], S[1][3])));
+// Softmax of U units' scores against the running state.  S[2 u + t]: vector ln against tokens 8 lq + 4 t + r of
+// unit u, without the scale; masked ones -inf.  p[u]: the weights as the B operand of the product with V.
+template <int U>
+__device__ __forceinline__ void unit_weights(PgTile& T, f4* S, u4v* p) {
+    float x = fmaxf(S[0][0], S[0][1]);
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) x = fmaxf(fmaxf(x, S[i >> 1][2 * (i & 1)]), S[i >> 1][2 * (i & 1) + 1]);
     x = x4_max(x);
     const float s = product(x, SC2);
     float ref = T.m;
@@ -75,7 +81,7 @@ __device__ __forceinline__ u4v unit_weights(PgTile& T, f4 S[2]) {
         ref = far ? 0.0f : mn;
         if (__any(far)) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2 * U; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     S[t][r] = far ? (product(S[t][r], SC2) - mn) * (1.0f / SC2) : S[t][r];
@@ -83,18 +89,16 @@ __device__ __forceinline__ u4v unit_weights(PgTile& T, f4 S[2]) {
     }
     // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
     const float c = LIFT - (ref == -INFINITY ? 0.0f : ref);
-    u4v p;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float w0 = __builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1)], SC2, c));
-        const float w1 = __builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1) + 1], SC2, c));
-        sum += w0;
-        sum += w1;
-        p[i] = pack2(f2h(w0), f2h(w1));
+    for (int i = 0; i < 4 * U; ++i) {
+        const f2v w = {__builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1)], SC2, c)),
+                       __builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1) + 1], SC2, c))};
+        sum += w.x;
+        sum += w.y;
+        p[i >> 2][i & 3] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, h2v));
     }
     T.l += sum;
-    return p;
 }
 
 // The query vectors of a tile.
@@ -274,7 +278,7 @@ __device__ __forceinline__ uint32_t clear_bad(u4v v[8]) {
     my <<= 8 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) my |= __shfl_xor(my, o, MJ_WAVE);
-    return my;
+    return __builtin_amdgcn_readfirstlane(my);
 }
 
 // A tile's state out: its vectors v .. v + 15 finished, or as a partial result.
@@ -321,6 +325,37 @@ __device__ __forceinline__ void add_tile(const PgLeft& p, PgTile& T) {
     for (int dt = 0; dt < 8; ++dt) T.o[dt] = T.o[dt] * f0 + p.o[dt][lane] * f1;
 }
 
+// A unit that not every row sees whole, straight from the page, a tile at a time.
+template <int T>
+__device__ __forceinline__ void edge_unit(PgTile* tl, const u4v (*q)[4], const PgCol* col, const uint16_t* ku,
+                                          const uint16_t* vu, int pos, int L) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int y = 0; y < T; ++y) {
+        f4 sc[2];
+        u4v r[8], pw;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r[k] = ((const u4v*)ku)[64 * k + lane];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            sc[tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sc[tt] = mfma16x16x32(as_h8(r[4 * tt + k]), as_h8(q[y][k]), sc[tt]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t ok = col[y].mask(pos, L);
+        mask_scores(sc, ok);
+        unit_weights<1>(tl[y], sc, &pw);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) r[dt] = ((const u4v*)vu)[64 * dt + lane];
+        const uint32_t bad = clear_bad(r);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] = mfma16x16x32(as_h8(r[dt]), as_h8(pw), tl[y].o[dt]);
+        if (bad) add_bad(tl[y], vu, bad, ok);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // Up to 16 T query vectors a sequence and head.  A block of four waves takes its run of units, a segment at a
 // time; a wave takes every fourth unit of it, straight from the pages into registers: a unit's bytes lie in
 // the order of the operands.  The next unit's K goes out behind a unit's scores, its V behind the output
@@ -361,8 +396,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) r[k] = p[64 * k];
             };
-            // unit i; MORE: unit nx requested behind it; EDGE: not every row sees all of it
-            auto step = [&](int i, int nx, auto more, auto masked) {
+            auto step = [&](int nx, auto more) {  // the unit in registers; unit nx requested behind it
                 f4 sc[T][2];
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
@@ -375,28 +409,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                             sc[j][tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[j][k]), sc[j][tt]);
                 }
                 if constexpr (more.value) request(kr, kl, nx);
-                uint32_t bad = 0;
-                const int pos = (S.su.lo + ub + 4 * i) * PG_UNIT;
-                if constexpr (masked.value) {
-#pragma unroll
-                    for (int j = 0; j < T; ++j) mask_scores(sc[j], col[j].mask(pos, S.su.L));
-                    bad = clear_bad(vr);
-                }
                 u4v pw[T];
 #pragma unroll
-                for (int j = 0; j < T; ++j) pw[j] = unit_weights(tl[j], sc[j]);
+                for (int j = 0; j < T; ++j) unit_weights<1>(tl[j], sc[j], &pw[j]);
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
                     for (int j = 0; j < T; ++j)
                         tl[j].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[j]), tl[j].o[dt]);
                 if constexpr (more.value) request(vr, vl, nx);
-                if constexpr (masked.value)
-                    if (bad) {
-                        const uint16_t* vu = vl + seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i));
-#pragma unroll
-                        for (int j = 0; j < T; ++j) add_bad(tl[j], vu, bad, col[j].mask(pos, S.su.L));
-                    }
             };
             int i0 = todo ? __builtin_ctzll(todo) : -1;
             if (i0 >= 0) {
@@ -405,19 +426,17 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
             }
             // (the last unit apart: a request that is not used would be waited for)
             while (todo) {
-                const int i = i0;
                 todo &= todo - 1;
                 if (!todo) break;
                 i0 = __builtin_ctzll(todo);
-                step(i, i0, std::true_type{}, std::false_type{});
+                step(i0, std::true_type{});
             }
-            if (i0 >= 0) step(i0, 0, std::false_type{}, std::false_type{});
+            if (i0 >= 0) step(0, std::false_type{});
 #pragma unroll 1
             for (uint64_t e = edge; e; e &= e - 1) {
-                i0 = __builtin_ctzll(e);
-                request(kr, kl, i0);
-                request(vr, vl, i0);
-                step(i0, 0, std::false_type{}, std::true_type{});
+                const int i = __builtin_ctzll(e);
+                const size_t at = seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i));
+                edge_unit<T>(tl, q, col, kl + at, vl + at, (S.su.lo + ub + 4 * i) * PG_UNIT, S.su.L);
             }
         }
         if (x != run.b0) __syncthreads();  // (the states of the segment before have been read)
@@ -436,72 +455,266 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
     }
 }
 
-// The partial results of one row and head, where its keys went to several blocks: their references and sums
-// first, then sixteen groups of 32 lanes take every sixteenth block's outputs, four dims a lane, with several
-// on their way (one at a time, each waited for, 128 blocks took 10 us), and the groups meet in LDS.
-#define PG_JOIN 512
-__global__ __launch_bounds__(PG_JOIN) void k_paged_join(PgAttnArgs a) {
-    __shared__ f4 s_o[PG_JOIN / 32][32];
-    __shared__ float s_f[PG_MAX_BLOCKS], s_w[2][PG_JOIN / 64];
-    if (block_aborted(a.abort)) return;
-    const int t = threadIdx.x, r = blockIdx.x, h = blockIdx.y, s = pg_seq(a.b, r);
-    if (s >= a.b.n_seqs) return;
+// More query vectors: a block of eight waves takes its run for up to 256 of them, two tiles a wave.  Units
+// go from the pages to LDS by direct loads into a ring of eight, as far ahead as it holds, and the waves
+// read their operands from there: one barrier a step, which counts the wave's own requests.  Of few tiles
+// the waves split the keys: `ks` groups of waves have all tiles each, and the groups' states meet in LDS at a
+// segment's end.  A group takes two units a step (one where ks is 4 and the ring holds two steps of one):
+// the softmax's own steps (the maximum over the lanes, the test of the reference) come once for both.
+#define PG_SLOTS 8
+#define PG_SLOT_BYTES (4 * PG_UNIT_HALVES)
+#define PG_CHUNK 1024  // page numbers in LDS
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// At most N of the wave's requests under way, its LDS reads done, then the barrier.
+template <int N>
+__device__ __forceinline__ void ring_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// U units of LDS against a wave's T tiles.  Four operands are on their way while the four before them are
+// multiplied (left to itself the compiler requests them all at once, and spills).
+template <int T, int U>
+__device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const char* slot) {
+    const u4v* base = (const u4v*)slot + (threadIdx.x & 63);
+    f4 sc[T][2 * U];
+    u4v r[2][4];
+    auto k_at = [&](int i, u4v* x) {  // K operands 4 i .. 4 i + 3
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = base[1024 * (i >> 1) + 256 * (i & 1) + 64 * k];
+    };
+    auto v_at = [&](int i, u4v* x) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = base[1024 * (i >> 1) + 512 + 256 * (i & 1) + 64 * k];
+    };
+    k_at(0, r[0]);
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+        if (i + 1 < 2 * U) k_at(i + 1, r[(i + 1) & 1]);
+        else v_at(0, r[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < T; ++y) sc[y][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int y = 0; y < T; ++y) sc[y][i] = mfma16x16x32(as_h8(r[i & 1][k]), as_h8(q[y][k]), sc[y][i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    u4v pw[T][U];
+#pragma unroll
+    for (int y = 0; y < T; ++y) unit_weights<U>(tl[y], sc[y], pw[y]);
+#pragma unroll
+    for (int i = 0; i < 2 * U; ++i) {
+        if (i + 1 < 2 * U) v_at(i + 1, r[(i + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int y = 0; y < T; ++y) {
+                f4& o = tl[y].o[4 * (i & 1) + k];
+                o = mfma16x16x32(as_h8(r[i & 1][k]), as_h8(pw[y][i >> 1]), o);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
+    constexpr int T = 2;
+    extern __shared__ __align__(16) char ring[];  // [PG_SLOTS][K 8 KB, V 8 KB]; then the states
+    __shared__ int64_t s_off[PG_MAX_SEQS + 1], s_wsum[8];
+    __shared__ int s_abort, s_pg[PG_CHUNK];
+    static_assert(12 * sizeof(PgLeft) <= PG_SLOTS * PG_SLOT_BYTES, "states");
+    PgRun run;
+    if (!plan_run<512>(a, s_off, s_wsum, &s_abort, run)) return;
+    const int t = threadIdx.x, lane = t & 63, ln = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint16_t* kl0 = a.p.k + a.layer * a.p.layer_halves();
+    const uint16_t* vl0 = a.p.v + a.layer * a.p.layer_halves();
+    // a wave moves two of a unit's sixteen KB: waves 0 to 3 K, the others V
+    const uint16_t* mover = (w < 4 ? kl0 : vl0) + 1024 * (w & 3) + 8 * lane;
+    for (int64_t x = run.b0; x < run.b1;) {
+        const PgSeg S = next_seg(a, s_off, run, x);
+        const int tg = (S.vend - S.v0 + 31) >> 5, ks = tg <= 2 ? 4 : tg <= 4 ? 2 : 1;
+        const int kl = w / tg, tw = S.v0 + 32 * (w - kl * tg);  // the wave's share of the keys, its first vector
+        const bool works = kl < ks;
+        PgTile tl[T];
+        PgCol col[T];
+        u4v q[T][4];
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            load_vector(a, S, tw + 16 * i + ln, q[i], col[i]);
+            tl[i].clear();
+        }
+        // units i0 .. e0 - 1 and e1 .. i1 - 1 are not seen whole by every row
+        const int e0 = min(max(S.clean0 - S.su.lo, S.i0), S.i1), e1 = min(max(S.clean1 - S.su.lo, e0), S.i1);
+        auto go_round = [&](auto us_) {
+            constexpr int US = us_.value;  // units a group of waves takes a step
+            const int per = US * ks, ahead = PG_SLOTS / per;
+            for (int c0 = e0; c0 < e1; c0 += PG_CHUNK) {
+                const int n = min(e1 - c0, PG_CHUNK), steps = (n + per - 1) / per;
+                for (int i = t; i < n; i += 512) s_pg[i] = seg_page(a, S, c0 + i);
+                __syncthreads();  // (and the ring is free)
+                auto request = [&](int step) {
+#pragma unroll 1
+                    for (int u = 0; u < per; ++u) {
+                        const int i = min(step * per + u, n - 1), pg = __builtin_amdgcn_readfirstlane(s_pg[i]);
+                        const uint16_t* src = mover + seg_at(a, S, c0 + i, max(pg, 0));  // (page 0 for none: unread)
+                        char* dst = ring + ((step & (ahead - 1)) * per + u) * PG_SLOT_BYTES + 2048 * w;
+                        __builtin_amdgcn_global_load_lds(src, (lds_ptr_t)dst, 16, 0, 0);
+                        __builtin_amdgcn_global_load_lds(src + 512, (lds_ptr_t)(dst + 1024), 16, 0, 0);
+                    }
+                };
+                for (int j = 0; j < min(ahead - 1, steps); ++j) request(j);
+#pragma unroll 1
+                for (int j = 0; j < steps; ++j) {
+                    // step j is there for all, and everyone is done with the one before
+                    if (ahead == 2 || steps - 1 - j < ahead - 2) ring_barrier<0>();
+                    else ring_barrier<2 * US * (PG_SLOTS / US - 2)>();  // (ks 1)
+                    if (j + ahead - 1 < steps) request(j + ahead - 1);
+                    const int i = per * j + US * kl;
+                    if (!works || i >= n) continue;
+                    const char* slots = ring + ((j & (ahead - 1)) * per + US * kl) * PG_SLOT_BYTES;
+                    bool all = true;
+#pragma unroll
+                    for (int u = 0; u < US; ++u)
+                        all &= i + u < n && __builtin_amdgcn_readfirstlane(s_pg[min(i + u, n - 1)]) >= 0;
+                    if (all) {
+                        ring_units<T, US>(tl, q, slots);
+                        continue;
+                    }
+                    if constexpr (US > 1)
+#pragma unroll 1
+                        for (int u = 0; u < US; ++u)
+                            if (i + u < n && __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0)
+                                ring_units<T, 1>(tl, q, slots + u * PG_SLOT_BYTES);
+                }
+                __syncthreads();  // (the page numbers and the ring have been read)
+            }
+        };
+        if (ks == 4) go_round(std::integral_constant<int, 1>{});
+        else go_round(std::integral_constant<int, 2>{});
+        if (works)
+#pragma unroll 1
+            for (int e = kl; e < e0 - S.i0 + S.i1 - e1; e += ks) {
+                const int i = e < e0 - S.i0 ? S.i0 + e : e1 + e - (e0 - S.i0);
+                const int pg = __builtin_amdgcn_readfirstlane(seg_page(a, S, i));
+                if (pg < 0) continue;
+                const size_t at = seg_at(a, S, i, pg);
+                edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
+            }
+        PgLeft* left = (PgLeft*)ring;
+        if (ks > 1) {
+            if (x != run.b0) __syncthreads();  // (where no ring came between: the states before have been read)
+            if (works && kl > 0)
+#pragma unroll
+                for (int i = 0; i < T; ++i) put_tile(left[(w - tg) * T + i], tl[i]);
+            __syncthreads();
+        }
+        if (kl == 0) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+#pragma unroll 1
+                for (int k = 1; k < ks; ++k) add_tile(left[(w + (k - 1) * tg) * T + i], tl[i]);
+                if (tw + 16 * i < S.vend) write_tile(a, S, tw + 16 * i, tl[i], x4_sum(tl[i].l));
+            }
+        }
+        x += S.i1 - S.i0;
+    }
+}
+
+// The partial results of a row's heads, where their keys went to several blocks: a block of four waves takes
+// one head together, or, of many rows, four heads, a wave each.  A group of 32 lanes has a share of the
+// blocks, four dims a lane; references, sums and outputs are requested together, eight blocks a group and
+// round.  (References first, then outputs against the greatest: 10 us for 128 blocks; sixteen groups for
+// every head: 22 us for 4096 of them.)
+template <int WAVES>
+__global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
+    constexpr int GR = 2 * WAVES;
+    __shared__ f4 s_o[WAVES == 1 ? 1 : GR][32];
+    __shared__ float2 s_ml[GR];
+    __shared__ int s_abort;
+    const int t = threadIdx.x, lane = t & 63, d = t & 31, r = blockIdx.x;
+    const int h = WAVES == 1 ? 4 * blockIdx.y + (t >> 6) : blockIdx.y;
+    const int ab = a.abort ? *a.abort : 0;
+    const int64_t per = a.off[a.b.n_seqs + 1];
+    const int s = pg_seq(a.b, r);
+    if (t == 0) s_abort = ab;
+    __syncthreads();
+    if (s_abort || s >= a.b.n_seqs || h >= a.p.nKV * a.G) return;  // (h: a whole wave, and the block has no barrier then)
     const SeqUnits su = seq_units(a, s);
     const int local = r - su.r0;
     if (local < 0 || local >= su.m) return;
     uint16_t* out = a.out + r * a.ldo + h * HD;
     const int g = h / a.G, v = local * a.G + h - g * a.G, c = v / a.cols, cc = v - c * a.cols;
-    const int64_t per = a.off[a.b.n_seqs + 1];
     const int64_t S = a.off[s] + ((int64_t)g * su.ncg + c) * su.nu, E = S + su.nu;
     if (su.nu == 0) {
-        if (t < 16) *(u4v*)(out + 8 * t) = (u4v){0u, 0u, 0u, 0u};
+        if (WAVES == 1 ? lane < 32 : t < 32) *(uint2*)(out + 4 * d) = make_uint2(0u, 0u);
         return;
     }
     const int bA = (int)(S / per), n = (int)((E - 1) / per) - bA + 1;
     if (n == 1) return;
-    // (blocks before the last one of a run begin it: their first slot; the first block's last segment is this one)
-    auto place = [&](int i) {
-        const int64_t b = bA + i;
-        return ((size_t)b * 2 + (S <= b * per ? 0 : 1)) * a.cols + cc;
-    };
+    const int k = WAVES == 1 ? lane >> 5 : t >> 5;
     float M = -INFINITY, l = 0.0f;
-    for (int i = t; i < n; i += PG_JOIN) M = fmaxf(M, a.pml[place(i)].x);
-    M = wave_max(M);
-    if ((t & 63) == 0) s_w[0][t >> 6] = M;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PG_JOIN / 64; ++i) M = fmaxf(M, s_w[0][i]);
-    for (int i = t; i < n; i += PG_JOIN) {
-        const float2 ml = a.pml[place(i)];
-        const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        s_f[i] = f;
-        l = fmaf(ml.y, f, l);
-    }
-    l = wave_sum(l);
-    if ((t & 63) == 0) s_w[1][t >> 6] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PG_JOIN / 64; ++i) l += s_w[1][i];
-    const int k = t >> 5, d = t & 31;
     f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = k; i < n; i += 4 * (PG_JOIN / 32)) {
-        f4 y[4];
+#pragma unroll 1
+    for (int i = k; i < n; i += 8 * GR) {
+        f4 y[8];
+        float2 ml[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // (a block before the run's last begins with this segment, or its last segment is this one)
+            const int64_t b = bA + min(i + j * GR, n - 1);
+            const size_t at = ((size_t)b * 2 + (S <= b * per ? 0 : 1)) * a.cols + cc;
+            ml[j] = a.pml[at];
+            y[j] = *(const f4*)(a.po + at * HD + 4 * d);
+        }
+        float mn = M;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mn = i + j * GR < n ? fmaxf(mn, ml[j].x) : mn;
+        const float f0 = M == mn ? 1.0f : __builtin_amdgcn_exp2f(M - mn);  // (both may be -inf)
+        M = mn;
+        l *= f0;
+        o *= f0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = i + j * GR >= n ? 0.0f : ml[j].x == mn ? 1.0f : __builtin_amdgcn_exp2f(ml[j].x - mn);
+            if (i + j * GR < n) {
+                l = fmaf(ml[j].y, f, l);
+                o += y[j] * f;
+            }
+        }
+    }
+    // the groups: two of a wave by lane moves, or all through LDS
+    if constexpr (WAVES == 1) {
+        const float om = __shfl_xor(M, 32, MJ_WAVE), ol = __shfl_xor(l, 32, MJ_WAVE), mn = fmaxf(M, om);
+        const float f0 = M == mn ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+        const float f1 = om == mn ? 1.0f : __builtin_amdgcn_exp2f(om - mn);
+        // (the lower group's share first in both, so that both have the same bits)
+        l = k == 0 ? l * f0 + ol * f1 : ol * f1 + l * f0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int b = min(i + j * (PG_JOIN / 32), n - 1);
-            y[j] = *(const f4*)(a.po + place(b) * HD + 4 * d);
+            const float oo = __shfl_xor(o[j], 32, MJ_WAVE);
+            o[j] = o[j] * f0 + oo * f1;
         }
+        if (k) return;
+    } else {
+        if (d == 0) s_ml[k] = make_float2(M, l);
+        s_o[k][d] = o;
+        __syncthreads();
+        if (t >= 32) return;
+        M = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (i + j * (PG_JOIN / 32) < n) o += y[j] * s_f[i + j * (PG_JOIN / 32)];
+        for (int i = 0; i < GR; ++i) M = fmaxf(M, s_ml[i].x);
+        l = 0.0f;
+        o = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < GR; ++i) {
+            const float2 ml = s_ml[i];
+            const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            l += ml.y * f;
+            o += s_o[i][d] * f;
+        }
     }
-    s_o[k][d] = o;
-    __syncthreads();
-    if (t >= 32) return;
-    o = s_o[0][d];
-#pragma unroll
-    for (int i = 1; i < PG_JOIN / 32; ++i) o += s_o[i][d];
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
     *(uint2*)(out + 4 * d) = make_uint2(pack2(f2h(o[0] * inv), f2h(o[1] * inv)),
                                         pack2(f2h(o[2] * inv), f2h(o[3] * inv)));
@@ -509,8 +722,8 @@ __global__ __launch_bounds__(PG_JOIN) void k_paged_join(PgAttnArgs a) {
 
 size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     const int nv = a.b.max_rows * a.G;
-    a.cols = nv <= 16 ? 16 : 32;
-    a.blocks = 512;  // two a CU
+    a.cols = nv <= 16 ? 16 : nv <= 32 ? 32 : std::min((nv + 31) / 32 * 32, 256);
+    a.blocks = a.cols <= 32 ? 512 : 256;  // two a CU, or one
     a.least = 4;
     Arena ar{base, 0};
     a.off = (int64_t*)ar.take((PG_MAX_SEQS + 2) * sizeof(int64_t));
@@ -519,13 +732,38 @@ size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     return ar.off;
 }
 
+static hipError_t launch_shared(const PgAttnArgs& a, hipStream_t st) {
+    static std::atomic<uint64_t> raised{0};  // the devices whose LDS limit is raised
+    constexpr int lds = PG_SLOTS * PG_SLOT_BYTES;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(raised.load(std::memory_order_relaxed) & bit)) {
+        e = hipFuncSetAttribute((const void*)k_paged_attn_shared, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        raised.fetch_or(bit, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(k_paged_attn_shared, dim3(a.blocks), dim3(512), lds, st, a);
+    return hipSuccess;
+}
+
 hipError_t launch_paged_attn(const PgAttnArgs& a, hipStream_t st) {
-    if (a.b.n_seqs > PG_MAX_SEQS || a.b.rows < 1 || a.b.max_rows > MJ_ROWS || a.p.page < PG_UNIT)
+    if (a.b.n_seqs > PG_MAX_SEQS || a.b.rows < 1 || a.b.max_rows > MJ_ROWS || a.p.page < PG_UNIT ||
+        a.blocks > PG_MAX_BLOCKS)
         return hipErrorInvalidValue;
-    if (a.cols == 16)
+    if (a.cols == 16) {
         hipLaunchKernelGGL(k_paged_attn_own<1>, dim3(a.blocks), dim3(256), 0, st, a);
-    else
+    } else if (a.cols == 32) {
         hipLaunchKernelGGL(k_paged_attn_own<2>, dim3(a.blocks), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(k_paged_join, dim3(a.b.rows, a.p.nKV * a.G), dim3(PG_JOIN), 0, st, a);
+    } else {
+        const hipError_t e = launch_shared(a, st);
+        if (e != hipSuccess) return e;
+    }
+    const int heads = a.p.nKV * a.G;
+    if ((int64_t)a.b.rows * heads >= 2048)
+        hipLaunchKernelGGL(k_paged_join<1>, dim3(a.b.rows, (heads + 3) / 4), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL(k_paged_join<4>, dim3(a.b.rows, heads), dim3(256), 0, st, a);
     return hipGetLastError();
 }
