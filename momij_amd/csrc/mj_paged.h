@@ -66,7 +66,7 @@ struct PgAttnArgs {
     int layer, G, window;
     // set by paged_attn_plan: blocks of the launch, query vectors a column group, units
     // a block at least, and the workspace
-    int blocks, cols, least;
+    int blocks, cols, least, extra;
     int64_t* off;   // [n_seqs + 2]: units before each sequence, units in all, units a block
     float* po;      // [blocks][2][cols][128] partial outputs of a block's first and last segment
     float2* pml;    // [blocks][2][cols] {reference, sum}

@@ -23,10 +23,11 @@ struct SeqUnits {
     int lo, nu;     // first unit, units
     int ncg;        // column groups
 };
-__device__ __forceinline__ SeqUnits seq_units(const PgAttnArgs& a, int s) {
+__device__ __forceinline__ SeqUnits seq_units(const PgAttnArgs& a, int m, int r0, int L) {
     SeqUnits u;
-    u.m = pg_rows(a.b, s, u.r0);
-    u.L = pg_len(a.p, s);
+    u.m = m;
+    u.r0 = r0;
+    u.L = L;
     const int end = min(u.L + u.m, a.p.room());
     u.lo = (a.window > 0 ? max(0, u.L - a.window + 1) : 0) / PG_UNIT;
     u.nu = u.m > 0 ? max(0, (end + PG_UNIT - 1) / PG_UNIT - u.lo) : 0;
@@ -60,35 +61,50 @@ struct PgTile {
 // the reference is taken off the rounded scores, in the branch that moves it.
 #define FAR 1048576.0f
 
-// Softmax of U units' scores against the running state.  S[2 u + t]: vector ln against tokens 8 lq + 4 t + r of
-// unit u, without the scale; masked ones -inf.  p[u]: the weights as the B operand of the product with V.
-template <int U>
-__device__ __forceinline__ void unit_weights(PgTile& T, f4* S, u4v* p) {
-    float x = fmaxf(S[0][0], S[0][1]);
+// Softmax of U units' scores of T tiles against the running states, in two parts.  S[y][2 u + t]: tile y's
+// vector ln against tokens 8 lq + 4 t + r of unit u, without the scale; masked ones -inf.
+// The references moved, for all tiles in one branch; c: what makes exp2(fma(S, SC2, c)) the weights.
+template <int T, int U>
+__device__ __forceinline__ void move_refs(PgTile* tl, f4 (*S)[2 * U], float* c) {
+    float s[T], ref[T];
+    bool rare = false;
 #pragma unroll
-    for (int i = 1; i < 4 * U; ++i) x = fmaxf(fmaxf(x, S[i >> 1][2 * (i & 1)]), S[i >> 1][2 * (i & 1) + 1]);
-    x = x4_max(x);
-    const float s = product(x, SC2);
-    float ref = T.m;
-    if (__any((s > T.m + SLACK) | (fabsf(s) > FAR))) {
-        const bool far = fabsf(s) > FAR && s > -INFINITY;  // (-inf: every score is masked)
-        const float mn = fmaxf(T.m, s);
-        const float alpha = T.m == mn ? 1.0f : __builtin_amdgcn_exp2f(T.m - mn);  // (both may be -inf)
-        T.m = mn;
-        T.l *= alpha;
+    for (int y = 0; y < T; ++y) {
+        float x = fmaxf(S[y][0][0], S[y][0][1]);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) T.o[dt] *= alpha;
-        ref = far ? 0.0f : mn;
-        if (__any(far)) {
+        for (int i = 1; i < 4 * U; ++i)
+            x = fmaxf(fmaxf(x, S[y][i >> 1][2 * (i & 1)]), S[y][i >> 1][2 * (i & 1) + 1]);
+        s[y] = product(x4_max(x), SC2);
+        rare |= (s[y] > tl[y].m + SLACK) | (fabsf(s[y]) > FAR);
+        ref[y] = tl[y].m;
+    }
+    if (__any(rare)) {
+#pragma unroll
+        for (int y = 0; y < T; ++y) {
+            const bool far = fabsf(s[y]) > FAR && s[y] > -INFINITY;  // (-inf: every score is masked)
+            const float mn = fmaxf(tl[y].m, s[y]);
+            const float alpha = tl[y].m == mn ? 1.0f : __builtin_amdgcn_exp2f(tl[y].m - mn);  // (both may be -inf)
+            tl[y].m = mn;
+            tl[y].l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] *= alpha;
+            ref[y] = far ? 0.0f : mn;
+            if (!__any(far)) continue;
 #pragma unroll
             for (int t = 0; t < 2 * U; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    S[t][r] = far ? (product(S[t][r], SC2) - mn) * (1.0f / SC2) : S[t][r];
+                    S[y][t][r] = far ? (product(S[y][t][r], SC2) - mn) * (1.0f / SC2) : S[y][t][r];
         }
     }
-    // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
-    const float c = LIFT - (ref == -INFINITY ? 0.0f : ref);
+#pragma unroll
+    for (int y = 0; y < T; ++y)
+        // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
+        c[y] = LIFT - (ref[y] == -INFINITY ? 0.0f : ref[y]);
+}
+// p[u]: unit u's weights as the B operand of the product with V.
+template <int U>
+__device__ __forceinline__ void unit_weights(PgTile& T, const f4* S, float c, u4v* p) {
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4 * U; ++i) {
@@ -144,23 +160,34 @@ __device__ __forceinline__ void add_bad(PgTile& T, const uint16_t* vu, uint32_t 
     }
 }
 
-// Units before each sequence (s_off[0 .. n]) and the run of this block, by one round of requests and a scan
-// for every NT sequences; a.off gets them for the join.  False: the call was aborted.
+// The batch as a block needs it: units before each sequence, and its rows and length as they were read.
+struct PgPlan {
+    int64_t off[PG_MAX_SEQS + 1], wsum[8];
+    int rows[PG_MAX_SEQS], len[PG_MAX_SEQS];  // first row, and count << 16
+    int abort;
+};
+// The run of this block.  Every segment counts `extra` units more than it has, at its beginning: what it
+// costs a block to begin one, so that blocks with several have less keys to read.
 struct PgRun {
     int64_t b0, b1, per;
     int s;  // the sequence that the run begins in
 };
+// One round of requests and a scan for every NT sequences; a.off gets the units for the join.  False: the
+// call was aborted.
 template <int NT>
-__device__ __forceinline__ bool plan_run(const PgAttnArgs& a, int64_t* s_off, int64_t* s_wsum, int* s_abort,
-                                         PgRun& run) {
+__device__ __forceinline__ bool plan_run(const PgAttnArgs& a, PgPlan& P, PgRun& run) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = a.b.n_seqs;
     const int ab = a.abort ? *a.abort : 0;
     int64_t before = 0;
     for (int c = 0; c < n; c += NT) {
         int64_t u = 0;
         if (c + t < n) {
-            const SeqUnits q = seq_units(a, c + t);
-            u = (int64_t)q.nu * q.ncg * a.p.nKV;
+            int r0;
+            const int m = pg_rows(a.b, c + t, r0), L = pg_len(a.p, c + t);
+            const SeqUnits q = seq_units(a, m, r0, L);
+            u = q.nu > 0 ? (int64_t)(q.nu + a.extra) * q.ncg * a.p.nKV : 0;
+            P.rows[c + t] = r0 | m << 16;
+            P.len[c + t] = L;
         }
         int64_t inc = u;
 #pragma unroll
@@ -169,24 +196,24 @@ __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, int64_t* s_off, in
             inc += lane >= o ? x : 0;
         }
         if (c) __syncthreads();
-        if (lane == 63) s_wsum[w] = inc;
-        if (t == 0 && c == 0) *s_abort = ab;
+        if (lane == 63) P.wsum[w] = inc;
+        if (t == 0 && c == 0) P.abort = ab;
         __syncthreads();
         int64_t at = before, all = before;
 #pragma unroll
         for (int i = 0; i < NT / 64; ++i) {
-            at += i < w ? s_wsum[i] : 0;
-            all += s_wsum[i];
+            at += i < w ? P.wsum[i] : 0;
+            all += P.wsum[i];
         }
-        if (c + t <= n) s_off[c + t] = at + inc - u;
-        if (c + t + 1 == n) s_off[n] = at + inc;
+        if (c + t <= n) P.off[c + t] = at + inc - u;
+        if (c + t + 1 == n) P.off[n] = at + inc;
         before = all;
     }
     __syncthreads();
-    if (*s_abort) return false;
+    if (P.abort) return false;
     run.per = max((before + a.blocks - 1) / a.blocks, (int64_t)a.least);
     if (blockIdx.x == 0)
-        for (int i = t; i <= n + 1; i += NT) a.off[i] = i <= n ? s_off[i] : run.per;
+        for (int i = t; i <= n + 1; i += NT) a.off[i] = i <= n ? P.off[i] : run.per;
     run.b0 = blockIdx.x * run.per;
     run.b1 = min(before, run.b0 + run.per);
     run.s = 0;
@@ -194,7 +221,7 @@ __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, int64_t* s_off, in
         int hi = n;
         while (hi - run.s > 1) {
             const int mid = (run.s + hi) >> 1;
-            if (s_off[mid] <= run.b0) run.s = mid;
+            if (P.off[mid] <= run.b0) run.s = mid;
             else hi = mid;
         }
     }
@@ -209,22 +236,36 @@ struct PgSeg {
     bool whole;                  // all of the group's units
     int64_t slot;                // where a partial result goes
 };
-__device__ __forceinline__ PgSeg next_seg(const PgAttnArgs& a, const int64_t* s_off, PgRun& run, int64_t x) {
-    while (s_off[run.s + 1] <= x) ++run.s;
+// The segment at x, which moves past it; i1 <= i0: only its beginning lies in the run.
+__device__ __forceinline__ PgSeg next_seg(const PgAttnArgs& a, const PgPlan& P, PgRun& run, int64_t& x) {
+    while (P.off[run.s + 1] <= x) ++run.s;
     PgSeg S;
-    S.s = run.s;
-    S.su = seq_units(a, S.s);
-    const int64_t rel = x - s_off[S.s];
-    const int gc = (int)(rel / S.su.nu);
-    S.i0 = (int)(rel - (int64_t)gc * S.su.nu);
-    S.i1 = (int)min((int64_t)S.su.nu, S.i0 + (run.b1 - x));
+    S.s = __builtin_amdgcn_readfirstlane(run.s);
+    const int rw = __builtin_amdgcn_readfirstlane(P.rows[S.s]);
+    S.su = seq_units(a, rw >> 16, rw & 0xFFFF, __builtin_amdgcn_readfirstlane(P.len[S.s]));
+    const int64_t rel = x - P.off[S.s];
+    const int len = S.su.nu + a.extra;
+    int gc, at;
+    if (rel >> 31) {
+        gc = (int)(rel / len);
+        at = (int)(rel - (int64_t)gc * len);
+    } else {  // (a division of 64 bits takes half a microsecond)
+        gc = (int)((uint32_t)rel / (uint32_t)len);
+        at = (int)rel - gc * len;
+    }
+    gc = __builtin_amdgcn_readfirstlane(gc);
+    at = __builtin_amdgcn_readfirstlane(at);
+    const int take = (int)min((int64_t)(len - at), run.b1 - x);
+    S.slot = (int64_t)blockIdx.x * 2 + (x == run.b0 ? 0 : 1);
+    x += take;
+    S.i0 = max(at - a.extra, 0);
+    S.i1 = __builtin_amdgcn_readfirstlane(at - a.extra + take);
     S.g = gc / S.su.ncg;
     S.v0 = (gc - S.g * S.su.ncg) * a.cols;
     S.vend = min(S.su.m * a.G, S.v0 + a.cols);
     S.clean0 = a.window > 0 ? (max(0, S.su.L + MJ_ROWS - a.window + 1) + PG_UNIT - 1) / PG_UNIT : 0;
     S.clean1 = S.su.L / PG_UNIT;
     S.whole = S.i0 == 0 && S.i1 == S.su.nu;
-    S.slot = (int64_t)blockIdx.x * 2 + (x == run.b0 ? 0 : 1);
     return S;
 }
 // The page of the segment's unit i, or -1.
@@ -325,32 +366,36 @@ __device__ __forceinline__ void add_tile(const PgLeft& p, PgTile& T) {
     for (int dt = 0; dt < 8; ++dt) T.o[dt] = T.o[dt] * f0 + p.o[dt][lane] * f1;
 }
 
-// A unit that not every row sees whole, straight from the page, a tile at a time.
+// A unit that not every row sees whole, straight from the page.
 template <int T>
 __device__ __forceinline__ void edge_unit(PgTile* tl, const u4v (*q)[4], const PgCol* col, const uint16_t* ku,
                                           const uint16_t* vu, int pos, int L) {
     const int lane = threadIdx.x & 63;
+    u4v kr[8], vr[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) kr[k] = ((const u4v*)ku)[64 * k + lane];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) vr[k] = ((const u4v*)vu)[64 * k + lane];
+    __builtin_amdgcn_sched_barrier(0);
+    const uint32_t bad = clear_bad(vr);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int y = 0; y < T; ++y) {
-        f4 sc[2];
-        u4v r[8], pw;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r[k] = ((const u4v*)ku)[64 * k + lane];
+        f4 sc[1][2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
-            sc[tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+            sc[0][tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sc[tt] = mfma16x16x32(as_h8(r[4 * tt + k]), as_h8(q[y][k]), sc[tt]);
+            for (int k = 0; k < 4; ++k) sc[0][tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[y][k]), sc[0][tt]);
         }
-        __builtin_amdgcn_sched_barrier(0);
         const uint32_t ok = col[y].mask(pos, L);
-        mask_scores(sc, ok);
-        unit_weights<1>(tl[y], sc, &pw);
+        mask_scores(sc[0], ok);
+        float c;
+        u4v pw;
+        move_refs<1, 1>(&tl[y], sc, &c);
+        unit_weights<1>(tl[y], sc[0], c, &pw);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) r[dt] = ((const u4v*)vu)[64 * dt + lane];
-        const uint32_t bad = clear_bad(r);
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] = mfma16x16x32(as_h8(r[dt]), as_h8(pw), tl[y].o[dt]);
+        for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw), tl[y].o[dt]);
         if (bad) add_bad(tl[y], vu, bad, ok);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -362,19 +407,20 @@ __device__ __forceinline__ void edge_unit(PgTile* tl, const u4v (*q)[4], const P
 // products.  Page numbers of 64 units come with one request a lane.  The states meet in LDS.
 template <int T>
 __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
-    __shared__ int64_t s_off[PG_MAX_SEQS + 1], s_wsum[4];
-    __shared__ int s_abort;
+    __shared__ PgPlan plan;
     __shared__ PgLeft s_left[3][T];
     PgRun run;
-    if (!plan_run<256>(a, s_off, s_wsum, &s_abort, run)) return;
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6, ln = lane & 15;
+    if (!plan_run<256>(a, plan, run)) return;
+    const int t = threadIdx.x, lane = t & 63, ln = lane & 15, w = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint16_t* kl = a.p.k + a.layer * a.p.layer_halves();
     const uint16_t* vl = a.p.v + a.layer * a.p.layer_halves();
+    bool fresh_block = true;
     for (int64_t x = run.b0; x < run.b1;) {
-        const PgSeg S = next_seg(a, s_off, run, x);
+        const PgSeg S = next_seg(a, plan, run, x);
+        if (S.i1 <= S.i0) continue;
         PgTile tl[T];
         PgCol col[T];
-        u4v q[T][4], kr[8], vr[8];
+        u4v q[T][4];
         bool fresh = true;
         for (int ub = S.i0 + w; ub < S.i1 || fresh; ub += 256) {
             const int mine = ub + 4 * lane;
@@ -390,6 +436,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
             const int first = S.su.lo + mine;
             const uint64_t edge = __ballot(pl >= 0 && (first < S.clean0 || first >= S.clean1));
             uint64_t todo = __ballot(pl >= 0) & ~edge;
+            u4v kr[8], vr[8];
             auto request = [&](u4v* r, const uint16_t* base, int i) {
                 const u4v* p =
                     (const u4v*)(base + seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i))) + lane;
@@ -398,6 +445,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
             };
             auto step = [&](int nx, auto more) {  // the unit in registers; unit nx requested behind it
                 f4 sc[T][2];
+                float c[T];
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
@@ -410,8 +458,9 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                 }
                 if constexpr (more.value) request(kr, kl, nx);
                 u4v pw[T];
+                move_refs<T, 1>(tl, sc, c);
 #pragma unroll
-                for (int j = 0; j < T; ++j) unit_weights<1>(tl[j], sc[j], &pw[j]);
+                for (int j = 0; j < T; ++j) unit_weights<1>(tl[j], sc[j], c[j], &pw[j]);
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
@@ -419,19 +468,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                         tl[j].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[j]), tl[j].o[dt]);
                 if constexpr (more.value) request(vr, vl, nx);
             };
-            int i0 = todo ? __builtin_ctzll(todo) : -1;
-            if (i0 >= 0) {
+            if (todo) {
+                int i0 = __builtin_ctzll(todo);
                 request(kr, kl, i0);
                 request(vr, vl, i0);
+                // (the last unit apart: a request that is not used would be waited for)
+                for (todo &= todo - 1; todo; todo &= todo - 1) step(__builtin_ctzll(todo), std::true_type{});
+                step(0, std::false_type{});
             }
-            // (the last unit apart: a request that is not used would be waited for)
-            while (todo) {
-                todo &= todo - 1;
-                if (!todo) break;
-                i0 = __builtin_ctzll(todo);
-                step(i0, std::true_type{});
-            }
-            if (i0 >= 0) step(0, std::false_type{});
 #pragma unroll 1
             for (uint64_t e = edge; e; e &= e - 1) {
                 const int i = __builtin_ctzll(e);
@@ -439,7 +483,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                 edge_unit<T>(tl, q, col, kl + at, vl + at, (S.su.lo + ub + 4 * i) * PG_UNIT, S.su.L);
             }
         }
-        if (x != run.b0) __syncthreads();  // (the states of the segment before have been read)
+        if (!fresh_block) __syncthreads();  // (the states of the segment before have been read)
+        fresh_block = false;
         if (w > 0)
 #pragma unroll
             for (int i = 0; i < T; ++i) put_tile(s_left[w - 1][i], tl[i]);
@@ -451,7 +496,6 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                 for (int k = 0; k < 3; ++k) add_tile(s_left[k][i], tl[i]);
                 write_tile(a, S, S.v0 + 16 * i, tl[i], x4_sum(tl[i].l));
             }
-        x += S.i1 - S.i0;
     }
 }
 
@@ -501,9 +545,11 @@ __device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const 
             for (int y = 0; y < T; ++y) sc[y][i] = mfma16x16x32(as_h8(r[i & 1][k]), as_h8(q[y][k]), sc[y][i]);
         __builtin_amdgcn_sched_barrier(0);
     }
+    float c[T];
     u4v pw[T][U];
+    move_refs<T, U>(tl, sc, c);
 #pragma unroll
-    for (int y = 0; y < T; ++y) unit_weights<U>(tl[y], sc[y], pw[y]);
+    for (int y = 0; y < T; ++y) unit_weights<U>(tl[y], sc[y], c[y], pw[y]);
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
         if (i + 1 < 2 * U) v_at(i + 1, r[(i + 1) & 1]);
@@ -518,24 +564,30 @@ __device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const 
         __builtin_amdgcn_sched_barrier(0);
     }
 }
-__global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
-    constexpr int T = 2;
+
+template <int T, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void k_paged_attn_shared(PgAttnArgs a) {
+    constexpr int NT = 64 * NW, MV = 16 / NW;  // KB of a unit that a wave moves
+    constexpr int U = T > 2 ? 1 : 2;           // units a softmax takes together
     extern __shared__ __align__(16) char ring[];  // [PG_SLOTS][K 8 KB, V 8 KB]; then the states
-    __shared__ int64_t s_off[PG_MAX_SEQS + 1], s_wsum[8];
-    __shared__ int s_abort, s_pg[PG_CHUNK];
-    static_assert(12 * sizeof(PgLeft) <= PG_SLOTS * PG_SLOT_BYTES, "states");
+    __shared__ PgPlan plan;
+    __shared__ int s_pg[PG_CHUNK];
+    static_assert(3 * NW / 4 * T * sizeof(PgLeft) <= PG_SLOTS * PG_SLOT_BYTES, "states");
     PgRun run;
-    if (!plan_run<512>(a, s_off, s_wsum, &s_abort, run)) return;
+    if (!plan_run<NT>(a, plan, run)) return;
     const int t = threadIdx.x, lane = t & 63, ln = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint16_t* kl0 = a.p.k + a.layer * a.p.layer_halves();
     const uint16_t* vl0 = a.p.v + a.layer * a.p.layer_halves();
-    // a wave moves two of a unit's sixteen KB: waves 0 to 3 K, the others V
-    const uint16_t* mover = (w < 4 ? kl0 : vl0) + 1024 * (w & 3) + 8 * lane;
+    // the first half of the waves moves K, the other V
+    const uint16_t* mover = (w < NW / 2 ? kl0 : vl0) + 512 * MV * (w % (NW / 2)) + 8 * lane;
+    bool states = false;  // the ring holds states of the segment before
     for (int64_t x = run.b0; x < run.b1;) {
-        const PgSeg S = next_seg(a, s_off, run, x);
-        const int tg = (S.vend - S.v0 + 31) >> 5, ks = tg <= 2 ? 4 : tg <= 4 ? 2 : 1;
-        const int kl = w / tg, tw = S.v0 + 32 * (w - kl * tg);  // the wave's share of the keys, its first vector
+        const PgSeg S = next_seg(a, plan, run, x);
+        if (S.i1 <= S.i0) continue;
+        const int tg = (S.vend - S.v0 + 16 * T - 1) / (16 * T);  // waves that have all tiles
+        const int ks = NW / tg >= 4 ? 4 : NW / tg >= 2 ? 2 : 1;
+        const int kl = w / tg, tw = S.v0 + 16 * T * (w - kl * tg);  // the wave's share of the keys, its first vector
         const bool works = kl < ks;
         PgTile tl[T];
         PgCol col[T];
@@ -547,29 +599,42 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
         }
         // units i0 .. e0 - 1 and e1 .. i1 - 1 are not seen whole by every row
         const int e0 = min(max(S.clean0 - S.su.lo, S.i0), S.i1), e1 = min(max(S.clean1 - S.su.lo, e0), S.i1);
-        auto go_round = [&](auto us_) {
+        auto edges = [&]() __attribute__((always_inline)) {
+            if (works)
+#pragma unroll 1
+                for (int e = kl; e < e0 - S.i0 + S.i1 - e1; e += ks) {
+                    const int i = e < e0 - S.i0 ? S.i0 + e : e1 + e - (e0 - S.i0);
+                    const int pg = __builtin_amdgcn_readfirstlane(seg_page(a, S, i));
+                    if (pg < 0) continue;
+                    const size_t at = seg_at(a, S, i, pg);
+                    edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
+                }
+        };
+        auto go_round = [&](auto us_) __attribute__((always_inline)) {
             constexpr int US = us_.value;  // units a group of waves takes a step
             const int per = US * ks, ahead = PG_SLOTS / per;
             for (int c0 = e0; c0 < e1; c0 += PG_CHUNK) {
                 const int n = min(e1 - c0, PG_CHUNK), steps = (n + per - 1) / per;
-                for (int i = t; i < n; i += 512) s_pg[i] = seg_page(a, S, c0 + i);
+                for (int i = t; i < n; i += NT) s_pg[i] = seg_page(a, S, c0 + i);
                 __syncthreads();  // (and the ring is free)
                 auto request = [&](int step) {
 #pragma unroll 1
                     for (int u = 0; u < per; ++u) {
                         const int i = min(step * per + u, n - 1), pg = __builtin_amdgcn_readfirstlane(s_pg[i]);
                         const uint16_t* src = mover + seg_at(a, S, c0 + i, max(pg, 0));  // (page 0 for none: unread)
-                        char* dst = ring + ((step & (ahead - 1)) * per + u) * PG_SLOT_BYTES + 2048 * w;
-                        __builtin_amdgcn_global_load_lds(src, (lds_ptr_t)dst, 16, 0, 0);
-                        __builtin_amdgcn_global_load_lds(src + 512, (lds_ptr_t)(dst + 1024), 16, 0, 0);
+                        char* dst = ring + ((step & (ahead - 1)) * per + u) * PG_SLOT_BYTES + 1024 * MV * w;
+#pragma unroll
+                        for (int k = 0; k < MV; ++k)
+                            __builtin_amdgcn_global_load_lds(src + 512 * k, (lds_ptr_t)(dst + 1024 * k), 16, 0, 0);
                     }
                 };
                 for (int j = 0; j < min(ahead - 1, steps); ++j) request(j);
+                if (c0 == e0) edges();  // (while the ring fills)
 #pragma unroll 1
                 for (int j = 0; j < steps; ++j) {
                     // step j is there for all, and everyone is done with the one before
                     if (ahead == 2 || steps - 1 - j < ahead - 2) ring_barrier<0>();
-                    else ring_barrier<2 * US * (PG_SLOTS / US - 2)>();  // (ks 1)
+                    else ring_barrier<MV * US * (PG_SLOTS / US - 2)>();  // (ks 1)
                     if (j + ahead - 1 < steps) request(j + ahead - 1);
                     const int i = per * j + US * kl;
                     if (!works || i >= n) continue;
@@ -578,7 +643,7 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
 #pragma unroll
                     for (int u = 0; u < US; ++u)
                         all &= i + u < n && __builtin_amdgcn_readfirstlane(s_pg[min(i + u, n - 1)]) >= 0;
-                    if (all) {
+                    if (all && (US == U || US == 1)) {
                         ring_units<T, US>(tl, q, slots);
                         continue;
                     }
@@ -590,21 +655,14 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                 }
                 __syncthreads();  // (the page numbers and the ring have been read)
             }
+            if (e0 == e1) edges();
         };
         if (ks == 4) go_round(std::integral_constant<int, 1>{});
         else go_round(std::integral_constant<int, 2>{});
-        if (works)
-#pragma unroll 1
-            for (int e = kl; e < e0 - S.i0 + S.i1 - e1; e += ks) {
-                const int i = e < e0 - S.i0 ? S.i0 + e : e1 + e - (e0 - S.i0);
-                const int pg = __builtin_amdgcn_readfirstlane(seg_page(a, S, i));
-                if (pg < 0) continue;
-                const size_t at = seg_at(a, S, i, pg);
-                edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
-            }
         PgLeft* left = (PgLeft*)ring;
         if (ks > 1) {
-            if (x != run.b0) __syncthreads();  // (where no ring came between: the states before have been read)
+            if (states) __syncthreads();  // (where no ring came between: the states before have been read)
+            states = true;
             if (works && kl > 0)
 #pragma unroll
                 for (int i = 0; i < T; ++i) put_tile(left[(w - tg) * T + i], tl[i]);
@@ -618,7 +676,6 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                 if (tw + 16 * i < S.vend) write_tile(a, S, tw + 16 * i, tl[i], x4_sum(tl[i].l));
             }
         }
-        x += S.i1 - S.i0;
     }
 }
 
@@ -641,17 +698,19 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
     if (t == 0) s_abort = ab;
     __syncthreads();
     if (s_abort || s >= a.b.n_seqs || h >= a.p.nKV * a.G) return;  // (h: a whole wave, and the block has no barrier then)
-    const SeqUnits su = seq_units(a, s);
+    int r0;
+    const int m = pg_rows(a.b, s, r0);
+    const SeqUnits su = seq_units(a, m, r0, pg_len(a.p, s));
     const int local = r - su.r0;
     if (local < 0 || local >= su.m) return;
     uint16_t* out = a.out + r * a.ldo + h * HD;
     const int g = h / a.G, v = local * a.G + h - g * a.G, c = v / a.cols, cc = v - c * a.cols;
-    const int64_t S = a.off[s] + ((int64_t)g * su.ncg + c) * su.nu, E = S + su.nu;
+    const int64_t S = a.off[s] + ((int64_t)g * su.ncg + c) * (su.nu + a.extra), E = S + su.nu + a.extra;
     if (su.nu == 0) {
         if (WAVES == 1 ? lane < 32 : t < 32) *(uint2*)(out + 4 * d) = make_uint2(0u, 0u);
         return;
     }
-    const int bA = (int)(S / per), n = (int)((E - 1) / per) - bA + 1;
+    const int bA = (int)((S + a.extra) / per), n = (int)((E - 1) / per) - bA + 1;
     if (n == 1) return;
     const int k = WAVES == 1 ? lane >> 5 : t >> 5;
     float M = -INFINITY, l = 0.0f;
@@ -662,7 +721,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
         float2 ml[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            // (a block before the run's last begins with this segment, or its last segment is this one)
+            // (a block that begins in this segment has it first, another one last)
             const int64_t b = bA + min(i + j * GR, n - 1);
             const size_t at = ((size_t)b * 2 + (S <= b * per ? 0 : 1)) * a.cols + cc;
             ml[j] = a.pml[at];
@@ -724,7 +783,8 @@ size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     const int nv = a.b.max_rows * a.G;
     a.cols = nv <= 16 ? 16 : nv <= 32 ? 32 : std::min((nv + 31) / 32 * 32, 256);
     a.blocks = a.cols <= 32 ? 512 : 256;  // two a CU, or one
-    a.least = 4;
+    a.extra = a.cols <= 32 ? 2 : 6;
+    a.least = a.extra + 4;
     Arena ar{base, 0};
     a.off = (int64_t*)ar.take((PG_MAX_SEQS + 2) * sizeof(int64_t));
     a.pml = (float2*)ar.take((size_t)a.blocks * 2 * a.cols * sizeof(float2));
@@ -732,19 +792,21 @@ size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     return ar.off;
 }
 
+template <int T, int NW>
 static hipError_t launch_shared(const PgAttnArgs& a, hipStream_t st) {
     static std::atomic<uint64_t> raised{0};  // the devices whose LDS limit is raised
     constexpr int lds = PG_SLOTS * PG_SLOT_BYTES;
+    constexpr auto kernel = k_paged_attn_shared<T, NW>;
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(raised.load(std::memory_order_relaxed) & bit)) {
-        e = hipFuncSetAttribute((const void*)k_paged_attn_shared, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         raised.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL(k_paged_attn_shared, dim3(a.blocks), dim3(512), lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), lds, st, a);
     return hipSuccess;
 }
 
@@ -757,7 +819,7 @@ hipError_t launch_paged_attn(const PgAttnArgs& a, hipStream_t st) {
     } else if (a.cols == 32) {
         hipLaunchKernelGGL(k_paged_attn_own<2>, dim3(a.blocks), dim3(256), 0, st, a);
     } else {
-        const hipError_t e = launch_shared(a, st);
+        const hipError_t e = a.cols > 128 ? launch_shared<4, 4>(a, st) : launch_shared<2, 8>(a, st);
         if (e != hipSuccess) return e;
     }
     const int heads = a.p.nKV * a.G;
