@@ -57,17 +57,31 @@ struct PgTile {
 // the rounding.
 #define SLACK 6.0f
 #define LIFT 9.0f
-// Scores past FAR: a weight's one fma differs from the rounded score by more than the slack allows, so
-// the reference is taken off the rounded scores, in the branch that moves it.
+// Scores past FAR, whose steps in fp32 are an eighth and more: a weight's one fma differs from the rounded
+// score by more than the slack allows, so the reference is taken off the rounded score.
 #define FAR 1048576.0f
+
+// x *= f in place.  (Behind a branch the compiler keeps the accumulators in two places and copies all of
+// them at every step.)  The values are results of matrix instructions: scale_ready() first, which waits for these
+// to be there, and scaled() before the next ones read them.
+__device__ __forceinline__ void scale_ready() { asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory"); }
+__device__ __forceinline__ void scale(f4& x, float f) {
+    float a = x[0], b = x[1], c = x[2], d = x[3];
+    asm volatile("v_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3"
+                 : "+v"(a), "+v"(b), "+v"(c), "+v"(d)
+                 : "v"(f));
+    x = (f4){a, b, c, d};
+}
+__device__ __forceinline__ void scaled() { asm volatile("s_nop 7" ::: "memory"); }
 
 // Softmax of U units' scores of T tiles against the running states, in two parts.  S[y][2 u + t]: tile y's
 // vector ln against tokens 8 lq + 4 t + r of unit u, without the scale; masked ones -inf.
-// The references moved, for all tiles in one branch; c: what makes exp2(fma(S, SC2, c)) the weights.
+// The references moved, for all tiles in one branch; c: what makes exp2(S SC2 - c) the weights.  True: some
+// score is far.
 template <int T, int U>
-__device__ __forceinline__ void move_refs(PgTile* tl, f4 (*S)[2 * U], float* c) {
-    float s[T], ref[T];
-    bool rare = false;
+__device__ __forceinline__ bool move_refs(PgTile* tl, const f4 (*S)[2 * U], float* c) {
+    float s[T];
+    bool rare = false, far = false;
 #pragma unroll
     for (int y = 0; y < T; ++y) {
         float x = fmaxf(S[y][0][0], S[y][0][1]);
@@ -75,46 +89,58 @@ __device__ __forceinline__ void move_refs(PgTile* tl, f4 (*S)[2 * U], float* c) 
         for (int i = 1; i < 4 * U; ++i)
             x = fmaxf(fmaxf(x, S[y][i >> 1][2 * (i & 1)]), S[y][i >> 1][2 * (i & 1) + 1]);
         s[y] = product(x4_max(x), SC2);
-        rare |= (s[y] > tl[y].m + SLACK) | (fabsf(s[y]) > FAR);
-        ref[y] = tl[y].m;
+        rare |= s[y] > tl[y].m + SLACK;
     }
     if (__any(rare)) {
+        scale_ready();
 #pragma unroll
         for (int y = 0; y < T; ++y) {
-            const bool far = fabsf(s[y]) > FAR && s[y] > -INFINITY;  // (-inf: every score is masked)
             const float mn = fmaxf(tl[y].m, s[y]);
             const float alpha = tl[y].m == mn ? 1.0f : __builtin_amdgcn_exp2f(tl[y].m - mn);  // (both may be -inf)
             tl[y].m = mn;
             tl[y].l *= alpha;
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] *= alpha;
-            ref[y] = far ? 0.0f : mn;
-            if (!__any(far)) continue;
-#pragma unroll
-            for (int t = 0; t < 2 * U; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    S[y][t][r] = far ? (product(S[y][t][r], SC2) - mn) * (1.0f / SC2) : S[y][t][r];
+            for (int dt = 0; dt < 8; ++dt) scale(tl[y].o[dt], alpha);
         }
+        scaled();
     }
 #pragma unroll
-    for (int y = 0; y < T; ++y)
+    for (int y = 0; y < T; ++y) {
         // no key seen: any finite reference (a masked score still gives 0, a NaN stays one)
-        c[y] = LIFT - (ref[y] == -INFINITY ? 0.0f : ref[y]);
+        c[y] = (tl[y].m == -INFINITY ? 0.0f : tl[y].m) - LIFT;
+        far |= fabsf(c[y]) > FAR;
+    }
+    return __any(far);
 }
 // p[u]: unit u's weights as the B operand of the product with V.
-template <int U>
+template <int U, bool FARS>
 __device__ __forceinline__ void unit_weights(PgTile& T, const f4* S, float c, u4v* p) {
     float sum = 0.0f;
+    const float ref = T.m == -INFINITY ? 0.0f : T.m;
+    auto weight = [&](float x) {
+        if (!FARS) return __builtin_amdgcn_exp2f(fmaf(x, SC2, -c));
+        // (the lift last: far from 0 it would be lost in the reference)
+        return __builtin_amdgcn_exp2f(product(x, SC2) - ref + LIFT);
+    };
 #pragma unroll
     for (int i = 0; i < 4 * U; ++i) {
-        const f2v w = {__builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1)], SC2, c)),
-                       __builtin_amdgcn_exp2f(fmaf(S[i >> 1][2 * (i & 1) + 1], SC2, c))};
+        const f2v w = {weight(S[i >> 1][2 * (i & 1)]), weight(S[i >> 1][2 * (i & 1) + 1])};
         sum += w.x;
         sum += w.y;
         p[i >> 2][i & 3] = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, h2v));
     }
     T.l += sum;
+}
+template <int T, int U>
+__device__ __forceinline__ void softmax(PgTile* tl, const f4 (*S)[2 * U], u4v (*p)[U]) {
+    float c[T];
+    if (move_refs<T, U>(tl, S, c)) {
+#pragma unroll
+        for (int y = 0; y < T; ++y) unit_weights<U, true>(tl[y], S[y], c[y], p[y]);
+    } else {
+#pragma unroll
+        for (int y = 0; y < T; ++y) unit_weights<U, false>(tl[y], S[y], c[y], p[y]);
+    }
 }
 
 // The query vectors of a tile.
@@ -275,21 +301,28 @@ __device__ __forceinline__ int seg_page(const PgAttnArgs& a, const PgSeg& S, int
 // Halves from a layer's first to the segment's unit i in page pg.
 __device__ __forceinline__ size_t seg_at(const PgAttnArgs& a, const PgSeg& S, int i, int pg) {
     const int in = ((S.su.lo + i) * PG_UNIT) & (a.p.page - 1);
-    return ((size_t)pg * a.p.nKV + S.g) * a.p.head_halves() + (size_t)(in >> 5) * PG_UNIT_HALVES;
+    return (((size_t)pg * a.p.nKV + S.g) << (a.p.shift + 7)) + (size_t)(in >> 5) * PG_UNIT_HALVES;
 }
 
-// Query vector v (lanes without one take the group's first, unused) and what its row sees.
-__device__ __forceinline__ void load_vector(const PgAttnArgs& a, const PgSeg& S, int v, u4v q[4], PgCol& col) {
+// Query vector v (lanes without one take the group's first, unused).
+__device__ __forceinline__ void load_vector(const PgAttnArgs& a, const PgSeg& S, int v, u4v q[4]) {
     const int lq = (threadIdx.x & 63) >> 4;
-    col.on = v < S.vend;
-    const int r = col.on ? v / a.G : 0, h = S.g * a.G + (col.on ? v - r * a.G : 0);
+    const bool on = v < S.vend;
+    const int r = on ? v / a.G : 0, h = S.g * a.G + (on ? v - r * a.G : 0);
     const uint16_t* qp = a.q + (S.su.r0 + r) * a.ldq + h * HD + 8 * lq;
 #pragma unroll
     for (int k = 0; k < 4; ++k) q[k] = *(const u4v*)(qp + 32 * k);
+}
+// What its row sees.
+__device__ __forceinline__ PgCol load_col(const PgAttnArgs& a, const PgSeg& S, int v) {
+    PgCol col;
+    col.on = v < S.vend;
+    const int r = col.on ? v / a.G : 0;
     col.anc = pg_anc(a.b, S.su.r0 + r, r);
     const int depth = pg_depth(col.anc, r);
     if (S.su.m < 64) col.anc &= (1ull << S.su.m) - 1;  // (a row that there is not is nobody's ancestor)
     col.first = a.window > 0 ? max(0, S.su.L + depth - a.window + 1) : 0;
+    return col;
 }
 
 // Scores of tokens that vector ln does not see taken out (ok: those that it sees).
@@ -390,25 +423,24 @@ __device__ __forceinline__ void edge_unit(PgTile* tl, const u4v (*q)[4], const P
         }
         const uint32_t ok = col[y].mask(pos, L);
         mask_scores(sc[0], ok);
-        float c;
-        u4v pw;
-        move_refs<1, 1>(&tl[y], sc, &c);
-        unit_weights<1>(tl[y], sc[0], c, &pw);
+        u4v pw[1][1];
+        softmax<1, 1>(&tl[y], sc, pw);
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw), tl[y].o[dt]);
+        for (int dt = 0; dt < 8; ++dt) tl[y].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[0][0]), tl[y].o[dt]);
         if (bad) add_bad(tl[y], vu, bad, ok);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// Up to 16 T query vectors a sequence and head.  A block of four waves takes its run of units, a segment at a
+// Up to 16 query vectors a sequence and head.  A block of four waves takes its run of units, a segment at a
 // time; a wave takes every fourth unit of it, straight from the pages into registers: a unit's bytes lie in
 // the order of the operands.  The next unit's K goes out behind a unit's scores, its V behind the output
 // products.  Page numbers of 64 units come with one request a lane.  The states meet in LDS.
-template <int T>
+// Bound by HBM: one sequence of 131000 tokens and 4 heads takes 48 us; its 268 MB alone would
+// take 45 at the rate of a streaming read.
 __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
     __shared__ PgPlan plan;
-    __shared__ PgLeft s_left[3][T];
+    __shared__ PgLeft s_left[3];
     PgRun run;
     if (!plan_run<256>(a, plan, run)) return;
     const int t = threadIdx.x, lane = t & 63, ln = lane & 15, w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -418,19 +450,15 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
     for (int64_t x = run.b0; x < run.b1;) {
         const PgSeg S = next_seg(a, plan, run, x);
         if (S.i1 <= S.i0) continue;
-        PgTile tl[T];
-        PgCol col[T];
-        u4v q[T][4];
+        PgTile tl;
+        u4v q[1][4];
         bool fresh = true;
         for (int ub = S.i0 + w; ub < S.i1 || fresh; ub += 256) {
             const int mine = ub + 4 * lane;
             const int pl = mine < S.i1 ? seg_page(a, S, mine) : -1;
             if (fresh) {
-#pragma unroll
-                for (int i = 0; i < T; ++i) {
-                    load_vector(a, S, S.v0 + 16 * i + ln, q[i], col[i]);
-                    tl[i].clear();
-                }
+                load_vector(a, S, S.v0 + ln, q[0]);
+                tl.clear();
                 fresh = false;
             }
             const int first = S.su.lo + mine;
@@ -444,28 +472,19 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                 for (int k = 0; k < 8; ++k) r[k] = p[64 * k];
             };
             auto step = [&](int nx, auto more) {  // the unit in registers; unit nx requested behind it
-                f4 sc[T][2];
-                float c[T];
+                f4 sc[1][2];
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
-#pragma unroll
-                    for (int j = 0; j < T; ++j) sc[j][tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+                    sc[0][tt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int j = 0; j < T; ++j)
-                            sc[j][tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[j][k]), sc[j][tt]);
+                        sc[0][tt] = mfma16x16x32(as_h8(kr[4 * tt + k]), as_h8(q[0][k]), sc[0][tt]);
                 }
                 if constexpr (more.value) request(kr, kl, nx);
-                u4v pw[T];
-                move_refs<T, 1>(tl, sc, c);
+                u4v pw[1][1];
+                softmax<1, 1>(&tl, sc, pw);
 #pragma unroll
-                for (int j = 0; j < T; ++j) unit_weights<1>(tl[j], sc[j], c[j], &pw[j]);
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-                    for (int j = 0; j < T; ++j)
-                        tl[j].o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[j]), tl[j].o[dt]);
+                for (int dt = 0; dt < 8; ++dt) tl.o[dt] = mfma16x16x32(as_h8(vr[dt]), as_h8(pw[0][0]), tl.o[dt]);
                 if constexpr (more.value) request(vr, vl, nx);
             };
             if (todo) {
@@ -476,26 +495,24 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
                 for (todo &= todo - 1; todo; todo &= todo - 1) step(__builtin_ctzll(todo), std::true_type{});
                 step(0, std::false_type{});
             }
+            if (!edge) continue;
+            const PgCol col = load_col(a, S, S.v0 + ln);
 #pragma unroll 1
             for (uint64_t e = edge; e; e &= e - 1) {
                 const int i = __builtin_ctzll(e);
                 const size_t at = seg_at(a, S, ub + 4 * i, __builtin_amdgcn_readlane(pl, i));
-                edge_unit<T>(tl, q, col, kl + at, vl + at, (S.su.lo + ub + 4 * i) * PG_UNIT, S.su.L);
+                edge_unit<1>(&tl, q, &col, kl + at, vl + at, (S.su.lo + ub + 4 * i) * PG_UNIT, S.su.L);
             }
         }
         if (!fresh_block) __syncthreads();  // (the states of the segment before have been read)
         fresh_block = false;
-        if (w > 0)
-#pragma unroll
-            for (int i = 0; i < T; ++i) put_tile(s_left[w - 1][i], tl[i]);
+        if (w > 0) put_tile(s_left[w - 1], tl);
         __syncthreads();
-        if (w == 0)
-#pragma unroll
-            for (int i = 0; i < T; ++i) {
+        if (w == 0) {
 #pragma unroll 1
-                for (int k = 0; k < 3; ++k) add_tile(s_left[k][i], tl[i]);
-                write_tile(a, S, S.v0 + 16 * i, tl[i], x4_sum(tl[i].l));
-            }
+            for (int k = 0; k < 3; ++k) add_tile(s_left[k], tl);
+            write_tile(a, S, S.v0, tl, x4_sum(tl.l));
+        }
     }
 }
 
@@ -516,10 +533,11 @@ __device__ __forceinline__ void ring_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// U units of LDS against a wave's T tiles.  Four operands are on their way while the four before them are
-// multiplied (left to itself the compiler requests them all at once, and spills).
-template <int T, int U>
-__device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const char* slot) {
+// U units of LDS against a wave's T tiles; next: what goes out behind the scores.  Four operands are on their
+// way while the four before them are multiplied (left to itself the compiler requests them all at once, and
+// spills).
+template <int T, int U, typename F>
+__device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const char* slot, F next) {
     const u4v* base = (const u4v*)slot + (threadIdx.x & 63);
     f4 sc[T][2 * U];
     u4v r[2][4];
@@ -545,11 +563,10 @@ __device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const 
             for (int y = 0; y < T; ++y) sc[y][i] = mfma16x16x32(as_h8(r[i & 1][k]), as_h8(q[y][k]), sc[y][i]);
         __builtin_amdgcn_sched_barrier(0);
     }
-    float c[T];
+    next();
+    __builtin_amdgcn_sched_barrier(0);
     u4v pw[T][U];
-    move_refs<T, U>(tl, sc, c);
-#pragma unroll
-    for (int y = 0; y < T; ++y) unit_weights<U>(tl[y], sc[y], c[y], pw[y]);
+    softmax<T, U>(tl, sc, pw);
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
         if (i + 1 < 2 * U) v_at(i + 1, r[(i + 1) & 1]);
@@ -565,10 +582,9 @@ __device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const 
     }
 }
 
-template <int T, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void k_paged_attn_shared(PgAttnArgs a) {
-    constexpr int NT = 64 * NW, MV = 16 / NW;  // KB of a unit that a wave moves
-    constexpr int U = T > 2 ? 1 : 2;           // units a softmax takes together
+__global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
+    constexpr int T = 2, NW = 8, NT = 64 * NW;  // tiles a wave, waves
+    constexpr int MV = 16 / NW;                 // KB of a unit that a wave moves
     extern __shared__ __align__(16) char ring[];  // [PG_SLOTS][K 8 KB, V 8 KB]; then the states
     __shared__ PgPlan plan;
     __shared__ int s_pg[PG_CHUNK];
@@ -590,25 +606,27 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_paged_attn_shared(PgAttnArg
         const int kl = w / tg, tw = S.v0 + 16 * T * (w - kl * tg);  // the wave's share of the keys, its first vector
         const bool works = kl < ks;
         PgTile tl[T];
-        PgCol col[T];
         u4v q[T][4];
 #pragma unroll
         for (int i = 0; i < T; ++i) {
-            load_vector(a, S, tw + 16 * i + ln, q[i], col[i]);
+            load_vector(a, S, tw + 16 * i + ln, q[i]);
             tl[i].clear();
         }
         // units i0 .. e0 - 1 and e1 .. i1 - 1 are not seen whole by every row
         const int e0 = min(max(S.clean0 - S.su.lo, S.i0), S.i1), e1 = min(max(S.clean1 - S.su.lo, e0), S.i1);
         auto edges = [&]() __attribute__((always_inline)) {
-            if (works)
+            if (!works || kl >= e0 - S.i0 + S.i1 - e1) return;
+            PgCol col[T];
+#pragma unroll
+            for (int i = 0; i < T; ++i) col[i] = load_col(a, S, tw + 16 * i + ln);
 #pragma unroll 1
-                for (int e = kl; e < e0 - S.i0 + S.i1 - e1; e += ks) {
-                    const int i = e < e0 - S.i0 ? S.i0 + e : e1 + e - (e0 - S.i0);
-                    const int pg = __builtin_amdgcn_readfirstlane(seg_page(a, S, i));
-                    if (pg < 0) continue;
-                    const size_t at = seg_at(a, S, i, pg);
-                    edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
-                }
+            for (int e = kl; e < e0 - S.i0 + S.i1 - e1; e += ks) {
+                const int i = e < e0 - S.i0 ? S.i0 + e : e1 + e - (e0 - S.i0);
+                const int pg = __builtin_amdgcn_readfirstlane(seg_page(a, S, i));
+                if (pg < 0) continue;
+                const size_t at = seg_at(a, S, i, pg);
+                edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
+            }
         };
         auto go_round = [&](auto us_) __attribute__((always_inline)) {
             constexpr int US = us_.value;  // units a group of waves takes a step
@@ -635,23 +653,27 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void k_paged_attn_shared(PgAttnArg
                     // step j is there for all, and everyone is done with the one before
                     if (ahead == 2 || steps - 1 - j < ahead - 2) ring_barrier<0>();
                     else ring_barrier<MV * US * (PG_SLOTS / US - 2)>();  // (ks 1)
-                    if (j + ahead - 1 < steps) request(j + ahead - 1);
+                    const bool more = j + ahead - 1 < steps;
+                    auto next = [&]() __attribute__((always_inline)) {
+                        if (more) request(j + ahead - 1);
+                    };
                     const int i = per * j + US * kl;
-                    if (!works || i >= n) continue;
-                    const char* slots = ring + ((j & (ahead - 1)) * per + US * kl) * PG_SLOT_BYTES;
-                    bool all = true;
+                    bool all = works && i + US <= n;
+                    if (all)
 #pragma unroll
-                    for (int u = 0; u < US; ++u)
-                        all &= i + u < n && __builtin_amdgcn_readfirstlane(s_pg[min(i + u, n - 1)]) >= 0;
-                    if (all && (US == U || US == 1)) {
-                        ring_units<T, US>(tl, q, slots);
+                        for (int u = 0; u < US; ++u) all &= __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0;
+                    const char* slots = ring + ((j & (ahead - 1)) * per + US * kl) * PG_SLOT_BYTES;
+                    if (all) {
+                        ring_units<T, US>(tl, q, slots, next);
                         continue;
                     }
+                    next();
                     if constexpr (US > 1)
+                        if (works)
 #pragma unroll 1
-                        for (int u = 0; u < US; ++u)
-                            if (i + u < n && __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0)
-                                ring_units<T, 1>(tl, q, slots + u * PG_SLOT_BYTES);
+                            for (int u = 0; u < US; ++u)
+                                if (i + u < n && __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0)
+                                    ring_units<T, 1>(tl, q, slots + u * PG_SLOT_BYTES, []() {});
                 }
                 __syncthreads();  // (the page numbers and the ring have been read)
             }
@@ -779,11 +801,18 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
                                         pack2(f2h(o[2] * inv), f2h(o[3] * inv)));
 }
 
+// Up to 16 vectors the blocks are of the first kernel, which needs no barriers: 131000 tokens, one vector a head
+// 47.9 us against 51.6, 64 sequences of 200..8000 tokens 54.0 against 64, one of 300 10.7 against 18.  Past
+// 16 the ring's: the first kernel with two tiles spills (eight rows at 8000 tokens, four heads a group: 50
+// us against 32), and its waves would all read every unit.  One block of 256 vectors, though two of 128 would
+// divide the work more evenly: as fast (53.2 and 53.1 us), with half the reads.
+// A segment's beginning (its rows' queries, page numbers, the ring filled, the result written) costs as much
+// as 10 units of the ring (17 rows of 16 sequences 32.3 us; counted as 6 units 36) or 2 of the first kernel.
 size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     const int nv = a.b.max_rows * a.G;
-    a.cols = nv <= 16 ? 16 : nv <= 32 ? 32 : std::min((nv + 31) / 32 * 32, 256);
-    a.blocks = a.cols <= 32 ? 512 : 256;  // two a CU, or one
-    a.extra = a.cols <= 32 ? 2 : 6;
+    a.cols = nv <= 16 ? 16 : std::min((nv + 31) / 32 * 32, 256);
+    a.blocks = a.cols == 16 ? 512 : 256;  // two a CU, or one
+    a.extra = a.cols == 16 ? 2 : 10;
     a.least = a.extra + 4;
     Arena ar{base, 0};
     a.off = (int64_t*)ar.take((PG_MAX_SEQS + 2) * sizeof(int64_t));
@@ -792,21 +821,19 @@ size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     return ar.off;
 }
 
-template <int T, int NW>
 static hipError_t launch_shared(const PgAttnArgs& a, hipStream_t st) {
     static std::atomic<uint64_t> raised{0};  // the devices whose LDS limit is raised
     constexpr int lds = PG_SLOTS * PG_SLOT_BYTES;
-    constexpr auto kernel = k_paged_attn_shared<T, NW>;
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(raised.load(std::memory_order_relaxed) & bit)) {
-        e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        e = hipFuncSetAttribute((const void*)k_paged_attn_shared, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
         raised.fetch_or(bit, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL(kernel, dim3(a.blocks), dim3(64 * NW), lds, st, a);
+    hipLaunchKernelGGL(k_paged_attn_shared, dim3(a.blocks), dim3(512), lds, st, a);
     return hipSuccess;
 }
 
@@ -815,11 +842,9 @@ hipError_t launch_paged_attn(const PgAttnArgs& a, hipStream_t st) {
         a.blocks > PG_MAX_BLOCKS)
         return hipErrorInvalidValue;
     if (a.cols == 16) {
-        hipLaunchKernelGGL(k_paged_attn_own<1>, dim3(a.blocks), dim3(256), 0, st, a);
-    } else if (a.cols == 32) {
-        hipLaunchKernelGGL(k_paged_attn_own<2>, dim3(a.blocks), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(k_paged_attn_own, dim3(a.blocks), dim3(256), 0, st, a);
     } else {
-        const hipError_t e = a.cols > 128 ? launch_shared<4, 4>(a, st) : launch_shared<2, 8>(a, st);
+        const hipError_t e = launch_shared(a, st);
         if (e != hipSuccess) return e;
     }
     const int heads = a.p.nKV * a.G;
