@@ -82,6 +82,14 @@ struct AcceptPart {
     float m;
     int at;
 };
+// A sequence's last row, for the launch that samples from what is left of it (row -1: nothing to do).
+struct AcceptLast {
+    double Z;          // its sum
+    uint64_t refused;  // drafts below it, by row of the sequence
+    float m;           // its greatest logit
+    int first, row;    // of the sequence, and the row
+    int count;         // blocks that have stored their chunk's sum
+};
 struct AcceptArgs {
     PgRows b;
     const float* logits;
@@ -99,8 +107,8 @@ struct AcceptArgs {
     // workspace
     AcceptPart* part;  // [rows][chunks]
     double* csum;      // [n_seqs][chunks] what is left of the last row's probabilities
-    int32_t* count;    // [n_seqs] blocks that have stored theirs
-    int chunks;
+    AcceptLast* last;  // [n_seqs]
+    int chunks;        // of a row
     const int* abort;
 };
 size_t accept_rows_layout(AcceptArgs& a, void* base);

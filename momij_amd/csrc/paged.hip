@@ -183,12 +183,26 @@ __device__ __forceinline__ int block_scan(int v, int* wsum, int* total) {
 __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int32_t* out, const int* abort) {
     __shared__ int wsum[16];
     __shared__ int ids[PG_NEED * PG_MAX_SEQS];
+    __shared__ int s_abort;
     const int s = threadIdx.x;
-    if (block_aborted(abort)) {  // nobody is served (the copies that follow go by these records)
-        if (s < p.n_seqs) *(int4*)(out + 4 * s) = make_int4(0, 0, -1, -1);
-        return;
-    }
-    int old[PG_NEED], need = 0, count = 0, first = 0, L = 0, m = 0;
+    const bool ab = aborted(abort);
+    int4 next[4];  // counts of 16 pages, requested a round ahead
+    auto request = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = base + 16 * s + 4 * k;
+            next[k] = make_int4(1, 1, 1, 1);
+            if (at + 3 < p.n_pages) {
+                next[k] = *(const int4*)(p.refs + at);
+            } else {
+                if (at < p.n_pages) next[k].x = p.refs[at];
+                if (at + 1 < p.n_pages) next[k].y = p.refs[at + 1];
+                if (at + 2 < p.n_pages) next[k].z = p.refs[at + 2];
+            }
+        }
+    };
+    request(0);
+    int old[PG_NEED], refs[PG_NEED], need = 0, count = 0, first = 0, L = 0, m = 0;
     bool fits = false;
     if (s < p.n_seqs) {
         int r0;
@@ -198,15 +212,24 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
         const int last = (L + m - 1) >> p.shift;
         fits = m > 0 && last < p.stride;
 #pragma unroll
+        for (int i = 0; i < PG_NEED; ++i) old[i] = fits && first + i <= last ? pg_page(p, s, first + i) : -1;
+#pragma unroll
+        for (int i = 0; i < PG_NEED; ++i) refs[i] = old[i] >= 0 ? p.refs[old[i]] : 0;
+#pragma unroll
         for (int i = 0; i < PG_NEED; ++i) {
-            old[i] = fits && first + i <= last ? pg_page(p, s, first + i) : -1;
-            if (fits && first + i <= last && (old[i] < 0 || p.refs[old[i]] != 1)) {
+            if (fits && first + i <= last && refs[i] != 1) {
                 need |= 1 << i;
                 ++count;
             }
             // (a page that others name too: one reference less, below)
-            if (old[i] >= 0 && p.refs[old[i]] <= 1) old[i] = -1;
+            if (refs[i] <= 1) old[i] = -1;
         }
+    }
+    if (s == 0) s_abort = ab;
+    __syncthreads();
+    if (s_abort) {  // nobody is served (the copies that follow go by these records)
+        if (s < p.n_seqs) *(int4*)(out + 4 * s) = make_int4(0, 0, -1, -1);
+        return;
     }
     int want, found = 0;
     const int upto = block_scan(count, wsum, &want);
@@ -214,15 +237,10 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
         int free = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int at = base + 16 * s + 4 * k;
-            if (at + 3 < p.n_pages) {
-                const int4 c = *(const int4*)(p.refs + at);
-                free |= ((c.x == 0) | (c.y == 0) << 1 | (c.z == 0) << 2 | (c.w == 0) << 3) << (4 * k);
-            } else {
-                for (int i = 0; i < 4; ++i)
-                    if (at + i < p.n_pages && p.refs[at + i] == 0) free |= 1 << (4 * k + i);
-            }
+            const int4 c = next[k];
+            free |= ((c.x == 0) | (c.y == 0) << 1 | (c.z == 0) << 2 | (c.w == 0) << 3) << (4 * k);
         }
+        request(base + 1024 * 16);
         int total;
         int at = found + block_scan(__popc(free), wsum, &total) - __popc(free);
         for (; free && at < want; free &= free - 1, ++at) ids[at] = base + 16 * s + __builtin_ctz(free);
@@ -253,25 +271,33 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
 }
 
 // The committed tokens of the pages that were shared, copied to their new ones: block (layer and K or
-// V, sequence), all heads, 16 bytes a thread and turn; groups of eight tokens behind the last committed
-// one stay.  A piece of K holds eight dims of a token (group (piece / 4) % 4 of its unit), one of V eight
-// tokens of a dim (group (piece / 16) % 4).
+// V, head, sequence), 16 bytes a thread and piece, four pieces under way (all heads in one block, a piece at a
+// time: one branch of 24 layers 7.2 us); groups of eight tokens behind the last committed one stay.  A piece of
+// K holds eight dims of a token (group (piece / 4) % 4 of its unit), one of V eight tokens of a dim (group
+// (piece / 16) % 4).
 // (An abort does not stop it: the table names the new pages already.)
 __global__ __launch_bounds__(256) void k_pages_copy(PgPool p, const int32_t* moved) {
-    const int s = blockIdx.y, from = moved[4 * s + 2], to = moved[4 * s + 3];
+    const int s = blockIdx.z, from = moved[4 * s + 2], to = moved[4 * s + 3];
     if ((unsigned)from >= (unsigned)p.n_pages || (unsigned)to >= (unsigned)p.n_pages) return;
     const int fill = pg_len(p, s) & (p.page - 1);
     const bool isv = blockIdx.x & 1;
     uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
-    const size_t page_halves = p.nKV * p.head_halves();
-    const u4v* src = (const u4v*)(base + from * page_halves);
-    u4v* dst = (u4v*)(base + to * page_halves);
-    const int units = (fill + 31) >> 5, per = units * 512, n = per * p.nKV;  // (512 pieces a unit)
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int g = i / per, x = i - g * per;
-        const int token = 32 * (x >> 9) + 8 * (isv ? (x >> 4) & 3 : (x >> 2) & 3);
-        const size_t at = (size_t)g * (p.head_halves() / 8) + x;
-        if (token < fill) dst[at] = src[at];
+    const u4v* src = (const u4v*)(base + ((size_t)from * p.nKV + blockIdx.y) * p.head_halves());
+    u4v* dst = (u4v*)(base + ((size_t)to * p.nKV + blockIdx.y) * p.head_halves());
+    const int n = ((fill + 31) >> 5) * 512;  // (512 pieces a unit)
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        u4v x[4];
+        bool on[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = i + 256 * k;
+            const int token = 32 * (at >> 9) + 8 * (isv ? (at >> 4) & 3 : (at >> 2) & 3);
+            on[k] = token < fill;
+            if (on[k]) x[k] = src[at];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (on[k]) dst[i + 256 * k] = x[k];
     }
 }
 
@@ -281,78 +307,72 @@ __global__ __launch_bounds__(256) void k_pages_copy(PgPool p, const int32_t* mov
 __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const int32_t* accepted,
                                                       const int32_t* path, int32_t* lens_out,
                                                       const int* abort) {
-    __shared__ int s_from[MJ_ROWS], s_to[MJ_ROWS], s_n;
-    if (block_aborted(abort)) return;
+    __shared__ int64_t s_from[MJ_ROWS], s_to[MJ_ROWS];
+    __shared__ int s_n, s_abort;
     const int s = blockIdx.y, t = threadIdx.x;
+    const bool isv = blockIdx.x & 1, ab = aborted(abort);
     int r0;
     const int m = pg_rows(b, s, r0), L = pg_len(p, s);
     const int kept = m > 0 ? max(0, min(accepted[s], m - 1) + 1) : 0;
-    if (blockIdx.x == 0 && t == 0 && lens_out) lens_out[s] = min(L + kept, p.room());
-    if (!path || kept == 0) return;
-    if (t < 64) {  // rows that move, in order
+    if (t < 64) {  // rows that move, in order: where they lie in their page's first head, and where they go
         int from = t;
-        if (t < kept) from = path[r0 + t];
-        const bool move = t < kept && from != t && from >= 0 && from < m;
+        if (path && t < kept) from = path[r0 + t];
+        bool move = path && t < kept && from != t && from >= 0 && from < m;
+        int64_t src = 0, dst = 0;
+        if (move) {
+            const int a = L + from, c = L + t, pa = pg_page(p, s, a >> p.shift), pc = pg_page(p, s, c >> p.shift);
+            const int ta = a & (p.page - 1), tc = c & (p.page - 1);
+            move = pa >= 0 && pc >= 0;
+            src = (int64_t)((size_t)pa * p.nKV * p.head_halves()) + (isv ? pg_v_at(ta, 0) : pg_k_at(ta, 0));
+            dst = (int64_t)((size_t)pc * p.nKV * p.head_halves()) + (isv ? pg_v_at(tc, 0) : pg_k_at(tc, 0));
+        }
         const uint64_t which = __ballot(move);
         const int at = __popcll(which & ((1ull << t) - 1));
         if (move) {
-            s_from[at] = L + from;
-            s_to[at] = L + t;
+            s_from[at] = src;
+            s_to[at] = dst;
         }
-        if (t == 0) s_n = __popcll(which);
+        if (t == 0) {
+            s_n = __popcll(which);
+            s_abort = ab;
+        }
     }
     __syncthreads();
+    if (s_abort) return;
+    if (blockIdx.x == 0 && blockIdx.z == 0 && t == 0 && lens_out) lens_out[s] = min(L + kept, p.room());
     const int n = s_n;
     if (n == 0) return;
-    const bool isv = blockIdx.x & 1;
     uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
-    auto place = [&](int slot) -> int64_t {  // a token's page, or -1
-        const int pg = pg_page(p, s, slot >> p.shift);
-        return pg < 0 ? -1 : (int64_t)((size_t)pg * p.nKV * p.head_halves());
-    };
-    if (!isv) {
-        const int c = t & 15;
-        int64_t src[4], dst[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = 16 * i + (t >> 4);
-            src[i] = dst[i] = -1;
-            if (j < n) {
-                src[i] = place(s_from[j]);
-                dst[i] = place(s_to[j]);
-                if (src[i] < 0) dst[i] = -1;
-                src[i] += pg_k_at(s_from[j] & (p.page - 1), 8 * c);
-                if (dst[i] >= 0) dst[i] += pg_k_at(s_to[j] & (p.page - 1), 8 * c);
-            }
-        }
-        for (int g = 0; g < p.nKV; ++g) {
+    for (int g = blockIdx.z; g < p.nKV; g += gridDim.z) {
+        uint16_t* head = base + g * p.head_halves();
+        if (!isv) {
+            const int d = pg_k_at(0, 8 * (t & 15));
             u4v x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (dst[i] >= 0) x[i] = *(const u4v*)(base + src[i] + g * p.head_halves());
+            for (int i = 0; i < 4; ++i) {
+                const int j = 16 * i + (t >> 4);
+                if (j < n) x[i] = *(const u4v*)(head + s_from[j] + d);
+            }
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (dst[i] >= 0) *(u4v*)(base + dst[i] + g * p.head_halves()) = x[i];
-        }
-        return;
-    }
-    const int d = t & 127;
-    for (int g = 0; g < p.nKV; ++g) {
-        uint16_t* head = base + g * p.head_halves();
-        uint16_t x[32];
+            for (int i = 0; i < 4; ++i) {
+                const int j = 16 * i + (t >> 4);
+                if (j < n) *(u4v*)(head + s_to[j] + d) = x[i];
+            }
+        } else {
+            const int d = pg_v_at(0, t & 127);
+            uint16_t x[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int j = 2 * i + (t >> 7);
-            const int64_t at = j < n ? place(s_from[j]) : -1;
-            if (at >= 0) x[i] = head[at + pg_v_at(s_from[j] & (p.page - 1), d)];
-        }
-        __syncthreads();
+            for (int i = 0; i < 32; ++i) {
+                const int j = 2 * i + (t >> 7);
+                if (j < n) x[i] = head[s_from[j] + d];
+            }
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int j = 2 * i + (t >> 7);
-            const int64_t at = j < n ? place(s_to[j]) : -1;
-            if (at >= 0 && place(s_from[j]) >= 0) head[at + pg_v_at(s_to[j] & (p.page - 1), d)] = x[i];
+            for (int i = 0; i < 32; ++i) {
+                const int j = 2 * i + (t >> 7);
+                if (j < n) head[s_to[j] + d] = x[i];
+            }
         }
     }
 }
@@ -383,7 +403,7 @@ hipError_t launch_pages_reserve(const PgPool& p, const PgRows& b, int32_t* out, 
                                 hipStream_t st) {
     if (p.n_seqs > PG_MAX_SEQS || b.max_rows > MJ_ROWS || p.page < 32) return hipErrorInvalidValue;
     hipLaunchKernelGGL(k_pages_reserve, dim3(1), dim3(1024), 0, st, p, b, out, abort);
-    hipLaunchKernelGGL(k_pages_copy, dim3(2 * p.n_layers, p.n_seqs), dim3(256), 0, st, p, out);
+    hipLaunchKernelGGL(k_pages_copy, dim3(2 * p.n_layers, p.nKV, p.n_seqs), dim3(256), 0, st, p, out);
     return hipGetLastError();
 }
 
@@ -393,7 +413,8 @@ hipError_t launch_pages_commit(const PgPool& p, const PgRows& b, const int32_t* 
     if (b.max_rows > MJ_ROWS) return hipErrorInvalidValue;
     const bool here = lens_out == p.lens;
     if (path || !here)
-        hipLaunchKernelGGL(k_pages_commit, dim3(path ? 2 * p.n_layers : 1, p.n_seqs), dim3(256), 0, st, p, b,
+        hipLaunchKernelGGL(k_pages_commit, dim3(path ? 2 * p.n_layers : 1, p.n_seqs, path ? p.nKV : 1), dim3(256), 0,
+                           st, p, b,
                            accepted, path, here ? nullptr : lens_out, abort);
     if (here)
         hipLaunchKernelGGL(k_pages_lens, dim3((p.n_seqs + 255) / 256), dim3(256), 0, st, p, b, accepted,
