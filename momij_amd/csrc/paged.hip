@@ -123,11 +123,12 @@ __device__ __forceinline__ void give_back(const PgPool& p, int s, int first) {
 }
 
 __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t* len, const int* abort) {
-    if (block_aborted(abort)) return;
-    const int s = blockIdx.x, want = len[s];
-    if (want < 0) return;
-    const int n = min(want, pg_len(p, s));
+    __shared__ int s_abort;
+    const bool ab = aborted(abort);
+    const int s = blockIdx.x, want = len[s], n = min(want, pg_len(p, s));
+    if (threadIdx.x == 0) s_abort = ab;
     __syncthreads();
+    if (s_abort || want < 0) return;
     if (threadIdx.x == 0) p.lens[s] = n;
     give_back(p, s, (n + p.page - 1) >> p.shift);
 }
@@ -136,8 +137,12 @@ __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t*
 // ones named once more.  Counts only change by atomics, so the order of the blocks does not matter; a
 // source that is itself a destination would be read while it is written, and is not taken.
 __global__ __launch_bounds__(256) void k_pages_fork(PgPool p, const int32_t* from, const int* abort) {
-    if (block_aborted(abort)) return;
+    __shared__ int s_abort;
+    const bool ab = aborted(abort);
     const int s = blockIdx.x, f = from[s];
+    if (threadIdx.x == 0) s_abort = ab;
+    __syncthreads();
+    if (s_abort) return;
     if ((unsigned)f >= (unsigned)p.n_seqs || f == s) return;
     const int ff = from[f];
     if ((unsigned)ff < (unsigned)p.n_seqs && ff != f) return;
@@ -301,9 +306,11 @@ __global__ __launch_bounds__(256) void k_pages_copy(PgPool p, const int32_t* mov
     }
 }
 
-// The rows of an accepted path moved to consecutive places: block (layer and K or V, sequence), a head at a
-// time; every row is read before any is written.  A thread takes 16 bytes of K, or one dim of V, of a
-// row and turn.
+// The rows of an accepted path moved to consecutive places: block (layer and K or V, sequence, four heads).
+// A thread takes 16 bytes of K, or one dim of V, of a head's row; 64 of these rows a turn, all read before any
+// is written.  (A head a block: 17 us for 64 sequences and 24 layers; a head a turn, with the places looked
+// up for each: 26 us.)
+#define COMMIT_HEADS 4
 __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const int32_t* accepted,
                                                       const int32_t* path, int32_t* lens_out,
                                                       const int* abort) {
@@ -343,36 +350,37 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
     const int n = s_n;
     if (n == 0) return;
     uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
-    for (int g = blockIdx.z; g < p.nKV; g += gridDim.z) {
-        uint16_t* head = base + g * p.head_halves();
+    const int h0 = COMMIT_HEADS * blockIdx.z, h1 = min(h0 + COMMIT_HEADS, p.nKV), turn = 64 / n;
+    for (int g0 = h0; g0 < h1; g0 += turn) {
+        const int rows = n * min(turn, h1 - g0);
+        auto at = [&](int j, const int64_t* place) __attribute__((always_inline)) {
+            const int g = j / n;
+            return base + (size_t)(g0 + g) * p.head_halves() + place[j - g * n];
+        };
         if (!isv) {
             const int d = pg_k_at(0, 8 * (t & 15));
             u4v x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = 16 * i + (t >> 4);
-                if (j < n) x[i] = *(const u4v*)(head + s_from[j] + d);
+                if (j < rows) x[i] = *(const u4v*)(at(j, s_from) + d);
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = 16 * i + (t >> 4);
-                if (j < n) *(u4v*)(head + s_to[j] + d) = x[i];
+                if (j < rows) *(u4v*)(at(j, s_to) + d) = x[i];
             }
         } else {
-            const int d = pg_v_at(0, t & 127);
+            const int d = pg_v_at(0, t & 127), j0 = __builtin_amdgcn_readfirstlane(t >> 7);
             uint16_t x[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int j = 2 * i + (t >> 7);
-                if (j < n) x[i] = head[s_from[j] + d];
-            }
+            for (int i = 0; i < 32; ++i)
+                if (2 * i + j0 < rows) x[i] = at(2 * i + j0, s_from)[d];
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int j = 2 * i + (t >> 7);
-                if (j < n) head[s_to[j] + d] = x[i];
-            }
+            for (int i = 0; i < 32; ++i)
+                if (2 * i + j0 < rows) at(2 * i + j0, s_to)[d] = x[i];
         }
     }
 }
@@ -412,10 +420,11 @@ hipError_t launch_pages_commit(const PgPool& p, const PgRows& b, const int32_t* 
                                hipStream_t st) {
     if (b.max_rows > MJ_ROWS) return hipErrorInvalidValue;
     const bool here = lens_out == p.lens;
-    if (path || !here)
-        hipLaunchKernelGGL(k_pages_commit, dim3(path ? 2 * p.n_layers : 1, p.n_seqs, path ? p.nKV : 1), dim3(256), 0,
-                           st, p, b,
-                           accepted, path, here ? nullptr : lens_out, abort);
+    if (path || !here) {
+        const dim3 grid(path ? 2 * p.n_layers : 1, p.n_seqs, path ? (p.nKV + COMMIT_HEADS - 1) / COMMIT_HEADS : 1);
+        hipLaunchKernelGGL(k_pages_commit, grid, dim3(256), 0, st, p, b, accepted, path, here ? nullptr : lens_out,
+                           abort);
+    }
     if (here)
         hipLaunchKernelGGL(k_pages_lens, dim3((p.n_seqs + 255) / 256), dim3(256), 0, st, p, b, accepted,
                            abort);
