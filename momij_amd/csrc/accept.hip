@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void k_accept_stats(AcceptArgs a) {
     __shared__ int s_at, s_abort;
     const int t = threadIdx.x, lane = t & 63, w = t >> 6, r = blockIdx.y;
     // what leads to the row's temperature goes out before its logits: they come last, and nothing after them
-    const bool ab = aborted(a.abort);
+    const int ab = abort_word(a.abort);
     const int end = lane < a.b.n_seqs ? a.b.start[lane + 1] : INT32_MAX;
     const float* x = a.logits + r * a.ld;
     const int v0 = blockIdx.x * AC_CHUNK;
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     __shared__ int s_cur, s_abort;
     __shared__ LeftShared<AC_WALK> s_left;
     const int s = blockIdx.x, t = threadIdx.x;
-    const bool ab = aborted(a.abort);
+    const int ab = abort_word(a.abort);
     int r0;
     const int n = pg_rows(a.b, s, r0);
     const float T = a.temperature[s], u_sample = a.u_sample[s];
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
     const int s = blockIdx.y, c = blockIdx.x, t = threadIdx.x;
     const AcceptLast last = a.last[s];
     if (last.row < 0) return;
-    const bool ab = aborted(a.abort);
+    const int ab = abort_word(a.abort);
     const float T = a.temperature[s], u_sample = a.u_sample[s];
     if (t < 32) s_tab[t] = root32(t);
     if (t == 0) s_abort = ab;

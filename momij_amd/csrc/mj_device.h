@@ -270,6 +270,9 @@ __device__ __forceinline__ bool block_aborted(const int* flag) {
     __syncthreads();
     return s_abort != 0;
 }
+// The word alone, for a block that requests it beside its first data: thread 0's goes to LDS, and that one
+// decides for all, as above.
+__device__ __forceinline__ int abort_word(const int* flag) { return flag ? *flag : 0; }
 
 // ------------------------------------------------------------------------------------------
 // Canonical arithmetic for sampled acceptance.  The CPU oracle evaluates the identical IEEE

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
         wa = *(const u4v*)(nw + 8 * pa);
         wb = *(const u4v*)(nw + 8 * pb);
     }
-    const int ab = a.abort ? *a.abort : 0;
+    const int ab = abort_word(a.abort);
     if (t == 0) s_abort = ab;
     const int s = pg_seq(a.b, r);
     int r0 = 0, m = 0, L = 0;
@@ -124,7 +124,7 @@ __device__ __forceinline__ void give_back(const PgPool& p, int s, int first) {
 
 __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t* len, const int* abort) {
     __shared__ int s_abort;
-    const bool ab = aborted(abort);
+    const int ab = abort_word(abort);
     const int s = blockIdx.x, want = len[s], n = min(want, pg_len(p, s));
     if (threadIdx.x == 0) s_abort = ab;
     __syncthreads();
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t*
 // source that is itself a destination would be read while it is written, and is not taken.
 __global__ __launch_bounds__(256) void k_pages_fork(PgPool p, const int32_t* from, const int* abort) {
     __shared__ int s_abort;
-    const bool ab = aborted(abort);
+    const int ab = abort_word(abort);
     const int s = blockIdx.x, f = from[s];
     if (threadIdx.x == 0) s_abort = ab;
     __syncthreads();
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
     __shared__ int ids[PG_NEED * PG_MAX_SEQS];
     __shared__ int s_abort;
     const int s = threadIdx.x;
-    const bool ab = aborted(abort);
+    const int ab = abort_word(abort);
     int4 next[4];  // counts of 16 pages, requested a round ahead
     auto request = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
@@ -317,7 +317,8 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
     __shared__ int64_t s_from[MJ_ROWS], s_to[MJ_ROWS];
     __shared__ int s_n, s_abort;
     const int s = blockIdx.y, t = threadIdx.x;
-    const bool isv = blockIdx.x & 1, ab = aborted(abort);
+    const bool isv = blockIdx.x & 1;
+    const int ab = abort_word(abort);
     int r0;
     const int m = pg_rows(b, s, r0), L = pg_len(p, s);
     const int kept = m > 0 ? max(0, min(accepted[s], m - 1) + 1) : 0;

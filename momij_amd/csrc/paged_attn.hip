@@ -203,7 +203,7 @@ struct PgRun {
 template <int NT>
 __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, PgPlan& P, PgRun& run) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = a.b.n_seqs;
-    const int ab = a.abort ? *a.abort : 0;
+    const int ab = abort_word(a.abort);
     int64_t before = 0;
     for (int c = 0; c < n; c += NT) {
         int64_t u = 0;
@@ -522,6 +522,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
 // the waves split the keys: `ks` groups of waves have all tiles each, and the groups' states meet in LDS at a
 // segment's end.  A group takes two units a step (one where ks is 4 and the ring holds two steps of one):
 // the softmax's own steps (the maximum over the lanes, the test of the reference) come once for both.
+// Where there is one group, the second wave of each SIMD passes the barrier between its weights and its product
+// with V instead of before the scores, so that the one multiplies while the other takes exponentials (four
+// chunks of 64 rows at 4000 .. 16000 tokens: 48.1 us, in step 49.7; the step before is read a while longer, so
+// the ring holds one step less ahead).  Bound by instructions: a step of 64 keys and 256 vectors takes 2.5 us,
+// of pages in this XCD's cache 2.4, without the product with V 2.2, and its matrix instructions would take
+// 0.85.  Tried: four tiles a wave in four waves (half the LDS reads, no second wave to fill in) 66 us, columns
+// of 128 as fast, references moved at every step 56, a wave priority for one of the two no change.
 #define PG_SLOTS 8
 #define PG_SLOT_BYTES (4 * PG_UNIT_HALVES)
 #define PG_CHUNK 1024  // page numbers in LDS
@@ -533,27 +540,22 @@ __device__ __forceinline__ void ring_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// U units of LDS against a wave's T tiles; next: what goes out behind the scores.  Four operands are on their
-// way while the four before them are multiplied (left to itself the compiler requests them all at once, and
-// spills).
+// U units of LDS against a wave's T tiles, in two halves: scores and weights, then the product with V.  Four
+// operands are on their way while the four before them are multiplied (left to itself the compiler requests
+// them all at once, and spills).  next: what goes out behind the scores.
 template <int T, int U, typename F>
-__device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const char* slot, F next) {
+__device__ __forceinline__ void ring_weights(PgTile* tl, const u4v (*q)[4], const char* slot, u4v (*pw)[U], F next) {
     const u4v* base = (const u4v*)slot + (threadIdx.x & 63);
     f4 sc[T][2 * U];
     u4v r[2][4];
-    auto k_at = [&](int i, u4v* x) {  // K operands 4 i .. 4 i + 3
+    auto at = [&](int i, u4v* x) __attribute__((always_inline)) {  // operands 4 i .. 4 i + 3
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = base[1024 * (i >> 1) + 256 * (i & 1) + 64 * k];
     };
-    auto v_at = [&](int i, u4v* x) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = base[1024 * (i >> 1) + 512 + 256 * (i & 1) + 64 * k];
-    };
-    k_at(0, r[0]);
+    at(0, r[0]);
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
-        if (i + 1 < 2 * U) k_at(i + 1, r[(i + 1) & 1]);
-        else v_at(0, r[(i + 1) & 1]);
+        if (i + 1 < 2 * U) at(i + 1, r[(i + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int y = 0; y < T; ++y) sc[y][i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -565,11 +567,21 @@ __device__ __forceinline__ void ring_units(PgTile* tl, const u4v (*q)[4], const 
     }
     next();
     __builtin_amdgcn_sched_barrier(0);
-    u4v pw[T][U];
     softmax<T, U>(tl, sc, pw);
+    __builtin_amdgcn_sched_barrier(0);
+}
+template <int T, int U>
+__device__ __forceinline__ void ring_values(PgTile* tl, const char* slot, u4v (*pw)[U]) {
+    const u4v* base = (const u4v*)slot + 512 + (threadIdx.x & 63);
+    u4v r[2][4];
+    auto at = [&](int i, u4v* x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = base[1024 * (i >> 1) + 256 * (i & 1) + 64 * k];
+    };
+    at(0, r[0]);
 #pragma unroll
     for (int i = 0; i < 2 * U; ++i) {
-        if (i + 1 < 2 * U) v_at(i + 1, r[(i + 1) & 1]);
+        if (i + 1 < 2 * U) at(i + 1, r[(i + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -628,9 +640,11 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                 edge_unit<T>(tl, q, col, kl0 + at, vl0 + at, (S.su.lo + i) * PG_UNIT, S.su.L);
             }
         };
-        auto go_round = [&](auto us_) __attribute__((always_inline)) {
-            constexpr int US = us_.value;  // units a group of waves takes a step
-            const int per = US * ks, ahead = PG_SLOTS / per;
+        auto go_round = [&](auto us_, auto two_) __attribute__((always_inline)) {
+            constexpr int US = us_.value;     // units a group of waves takes a step
+            constexpr bool TWO = two_.value;  // one group of waves: half of them a product behind
+            const int per = US * ks, slots = PG_SLOTS / per, ahead = slots - 1 - TWO;
+            const bool late = TWO && w >= NW / 2;
             for (int c0 = e0; c0 < e1; c0 += PG_CHUNK) {
                 const int n = min(e1 - c0, PG_CHUNK), steps = (n + per - 1) / per;
                 for (int i = t; i < n; i += NT) s_pg[i] = seg_page(a, S, c0 + i);
@@ -640,31 +654,37 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                     for (int u = 0; u < per; ++u) {
                         const int i = min(step * per + u, n - 1), pg = __builtin_amdgcn_readfirstlane(s_pg[i]);
                         const uint16_t* src = mover + seg_at(a, S, c0 + i, max(pg, 0));  // (page 0 for none: unread)
-                        char* dst = ring + ((step & (ahead - 1)) * per + u) * PG_SLOT_BYTES + 1024 * MV * w;
+                        char* dst = ring + ((step & (slots - 1)) * per + u) * PG_SLOT_BYTES + 1024 * MV * w;
 #pragma unroll
                         for (int k = 0; k < MV; ++k)
                             __builtin_amdgcn_global_load_lds(src + 512 * k, (lds_ptr_t)(dst + 1024 * k), 16, 0, 0);
                     }
                 };
-                for (int j = 0; j < min(ahead - 1, steps); ++j) request(j);
+                for (int j = 0; j < min(ahead, steps); ++j) request(j);
                 if (c0 == e0) edges();  // (while the ring fills)
+                // step j is there for all, and everyone is done with the one whose slots are filled next
+                auto there = [&](int j) __attribute__((always_inline)) {
+                    if (ahead == 1 || steps - 1 - j < ahead - 1) ring_barrier<0>();
+                    else ring_barrier<MV * US * (PG_SLOTS / US - 2 - TWO)>();  // (ks 1)
+                };
 #pragma unroll 1
                 for (int j = 0; j < steps; ++j) {
-                    // step j is there for all, and everyone is done with the one before
-                    if (ahead == 2 || steps - 1 - j < ahead - 2) ring_barrier<0>();
-                    else ring_barrier<MV * US * (PG_SLOTS / US - 2)>();  // (ks 1)
-                    const bool more = j + ahead - 1 < steps;
+                    if (!late || j == 0) there(j);
+                    const bool more = j + ahead < steps;
                     auto next = [&]() __attribute__((always_inline)) {
-                        if (more) request(j + ahead - 1);
+                        if (more) request(j + ahead);
                     };
                     const int i = per * j + US * kl;
                     bool all = works && i + US <= n;
                     if (all)
 #pragma unroll
                         for (int u = 0; u < US; ++u) all &= __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0;
-                    const char* slots = ring + ((j & (ahead - 1)) * per + US * kl) * PG_SLOT_BYTES;
+                    const char* here = ring + ((j & (slots - 1)) * per + US * kl) * PG_SLOT_BYTES;
                     if (all) {
-                        ring_units<T, US>(tl, q, slots, next);
+                        u4v pw[T][US];
+                        ring_weights<T, US>(tl, q, here, pw, next);
+                        if (late && j + 1 < steps) there(j + 1);
+                        ring_values<T, US>(tl, here, pw);
                         continue;
                     }
                     next();
@@ -672,15 +692,22 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                         if (works)
 #pragma unroll 1
                             for (int u = 0; u < US; ++u)
-                                if (i + u < n && __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0)
-                                    ring_units<T, 1>(tl, q, slots + u * PG_SLOT_BYTES, []() {});
+                                if (i + u < n && __builtin_amdgcn_readfirstlane(s_pg[i + u]) >= 0) {
+                                    u4v p1[T][1];
+                                    ring_weights<T, 1>(tl, q, here + u * PG_SLOT_BYTES, p1, []() {});
+                                    ring_values<T, 1>(tl, here + u * PG_SLOT_BYTES, p1);
+                                }
+                    if (late && j + 1 < steps) there(j + 1);
                 }
                 __syncthreads();  // (the page numbers and the ring have been read)
             }
             if (e0 == e1) edges();
         };
-        if (ks == 4) go_round(std::integral_constant<int, 1>{});
-        else go_round(std::integral_constant<int, 2>{});
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+        if (ks == 4) go_round(One{}, std::false_type{});
+        else if (ks == 2) go_round(Two{}, std::false_type{});
+        else go_round(Two{}, std::true_type{});
         PgLeft* left = (PgLeft*)ring;
         if (ks > 1) {
             if (states) __syncthreads();  // (where no ring came between: the states before have been read)
@@ -714,7 +741,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
     __shared__ int s_abort;
     const int t = threadIdx.x, lane = t & 63, d = t & 31, r = blockIdx.x;
     const int h = WAVES == 1 ? 4 * blockIdx.y + (t >> 6) : blockIdx.y;
-    const int ab = a.abort ? *a.abort : 0;
+    const int ab = abort_word(a.abort);
     const int64_t per = a.off[a.b.n_seqs + 1];
     const int s = pg_seq(a.b, r);
     if (t == 0) s_abort = ab;
