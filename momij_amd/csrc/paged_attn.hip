@@ -645,7 +645,7 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
             constexpr bool TWO = two_.value;  // one group of waves: half of them a product behind
             const int per = US * ks, slots = PG_SLOTS / per, ahead = slots - 1 - TWO;
             const bool late = TWO && w >= NW / 2;
-            for (int c0 = e0; c0 < e1; c0 += PG_CHUNK) {
+            for (int c0 = e0; c0 == e0 || c0 < e1; c0 += PG_CHUNK) {  // (once for the edges alone)
                 const int n = min(e1 - c0, PG_CHUNK), steps = (n + per - 1) / per;
                 for (int i = t; i < n; i += NT) s_pg[i] = seg_page(a, S, c0 + i);
                 __syncthreads();  // (and the ring is free)
@@ -701,7 +701,6 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
                 }
                 __syncthreads();  // (the page numbers and the ring have been read)
             }
-            if (e0 == e1) edges();
         };
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;
