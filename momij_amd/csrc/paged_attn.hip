@@ -186,6 +186,11 @@ __device__ __forceinline__ void add_bad(PgTile& T, const uint16_t* vu, uint32_t 
     }
 }
 
+// a / b of numbers from 0 up.  (A division of 64 bits takes half a microsecond.)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // The batch as a block needs it: units before each sequence, and its rows and length as they were read.
 struct PgPlan {
     int64_t off[PG_MAX_SEQS + 1], wsum[8];
@@ -237,7 +242,7 @@ __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, PgPlan& P, PgRun& 
     }
     __syncthreads();
     if (P.abort) return false;
-    run.per = max((before + a.blocks - 1) / a.blocks, (int64_t)a.least);
+    run.per = max(quotient(before + a.blocks - 1, a.blocks), (int64_t)a.least);
     if (blockIdx.x == 0)
         for (int i = t; i <= n + 1; i += NT) a.off[i] = i <= n ? P.off[i] : run.per;
     run.b0 = blockIdx.x * run.per;
@@ -275,7 +280,7 @@ __device__ __forceinline__ PgSeg next_seg(const PgAttnArgs& a, const PgPlan& P, 
     if (rel >> 31) {
         gc = (int)(rel / len);
         at = (int)(rel - (int64_t)gc * len);
-    } else {  // (a division of 64 bits takes half a microsecond)
+    } else {
         gc = (int)((uint32_t)rel / (uint32_t)len);
         at = (int)rel - gc * len;
     }
@@ -758,7 +763,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
         if (WAVES == 1 ? lane < 32 : t < 32) *(uint2*)(out + 4 * d) = make_uint2(0u, 0u);
         return;
     }
-    const int bA = (int)((S + a.extra) / per), n = (int)((E - 1) / per) - bA + 1;
+    const int bA = (int)quotient(S + a.extra, per), n = (int)quotient(E - 1, per) - bA + 1;
     if (n == 1) return;
     const int k = WAVES == 1 ? lane >> 5 : t >> 5;
     float M = -INFINITY, l = 0.0f;
