@@ -341,7 +341,7 @@ mj_status mj_attn_block_kv8(mj_ctx* ctx, const mj_attn_config* cfg, const mj_att
 typedef struct mj_pages {
     int n_layers;
     int n_kv_heads;
-    int n_pages;
+    int n_pages;      /* at most 2^28 */
     int page_tokens;  /* 32, 64, 128 or 256 */
     /* fp16 [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096]: units of 32 tokens by 128 dims in the
      * order the matrix instructions take them.  Of token t of a unit and dim d,

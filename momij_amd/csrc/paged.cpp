@@ -14,6 +14,7 @@ constexpr int kMaxGroup = 64;            // query heads a KV head
 constexpr int kMaxTokens = 1 << 30;      // tokens a table row can hold
 constexpr int kMaxRowsInAll = 65535;
 constexpr int kMaxVocab = 1 << 23;
+constexpr int kMaxPages = 1 << 28;       // (16 KB each at least)
 
 mj_status check_pages(mj_ctx* ctx, const mj_pages* c, const char* what, PgPool& p) {
     if (!c || !c->k || !c->v || !c->table || !c->lens || !c->refs)
@@ -21,7 +22,7 @@ mj_status check_pages(mj_ctx* ctx, const mj_pages* c, const char* what, PgPool& 
     if (c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128 && c->page_tokens != 256)
         return mj_fail(ctx, MJ_UNSUPPORTED_SHAPE, "%s: page_tokens=%d (32, 64, 128 or 256)", what,
                        c->page_tokens);
-    if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->n_layers < 1 ||
+    if (c->n_kv_heads < 1 || c->n_kv_heads > 1024 || c->n_pages < 1 || c->n_pages > kMaxPages || c->n_layers < 1 ||
         c->n_layers > PG_MAX_LAYERS || c->n_seqs < 1 || c->n_seqs > PG_MAX_SEQS || c->table_stride < 1 ||
         (int64_t)c->table_stride * c->page_tokens > kMaxTokens)
         return mj_fail(ctx, MJ_INVALID_ARG,

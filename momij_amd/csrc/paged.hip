@@ -1,6 +1,8 @@
 // paged.hip -- the pages of many sequences: appending a batch's normed and rotated rows, making room
 // (with a copy of shared pages), sharing, giving back, and moving accepted rows together.
 // (Attention over the pages: paged_attn.hip.)
+#include <algorithm>
+
 #include "mj_device.h"
 #include "mj_paged.h"
 
@@ -276,33 +278,49 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
 }
 
 // The committed tokens of the pages that were shared, copied to their new ones: block (layer and K or
-// V, head, sequence), 16 bytes a thread and piece, four pieces under way (all heads in one block, a piece at a
-// time: one branch of 24 layers 7.2 us); groups of eight tokens behind the last committed one stay.  A piece of
-// K holds eight dims of a token (group (piece / 4) % 4 of its unit), one of V eight tokens of a dim (group
-// (piece / 16) % 4).
+// V, head, some of the sequences), 16 bytes a thread and piece, four pieces under way (all heads in one block, a
+// piece at a time: one branch of 24 layers 7.2 us, so 5); groups of eight tokens behind the last committed one
+// stay.  A piece of K holds eight dims of a token (group (piece / 4) % 4 of its unit), one of V eight tokens of
+// a dim (group (piece / 16) % 4).  In most steps few sequences or none have a page to copy: of many, a block
+// looks through 64 records at once, and the launch has no more blocks than find their place in a few us.
 // (An abort does not stop it: the table names the new pages already.)
+#define COPY_BLOCKS 16384
 __global__ __launch_bounds__(256) void k_pages_copy(PgPool p, const int32_t* moved) {
-    const int s = blockIdx.z, from = moved[4 * s + 2], to = moved[4 * s + 3];
-    if ((unsigned)from >= (unsigned)p.n_pages || (unsigned)to >= (unsigned)p.n_pages) return;
-    const int fill = pg_len(p, s) & (p.page - 1);
+    const int t = threadIdx.x, lane = t & 63, step = gridDim.z;
     const bool isv = blockIdx.x & 1;
-    uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
-    const u4v* src = (const u4v*)(base + ((size_t)from * p.nKV + blockIdx.y) * p.head_halves());
-    u4v* dst = (u4v*)(base + ((size_t)to * p.nKV + blockIdx.y) * p.head_halves());
-    const int n = ((fill + 31) >> 5) * 512;  // (512 pieces a unit)
-    for (int i = threadIdx.x; i < n; i += 1024) {
-        u4v x[4];
-        bool on[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int at = i + 256 * k;
-            const int token = 32 * (at >> 9) + 8 * (isv ? (at >> 4) & 3 : (at >> 2) & 3);
-            on[k] = token < fill;
-            if (on[k]) x[k] = src[at];
+    uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves() + blockIdx.y * p.head_halves();
+    const size_t page_halves = p.nKV * p.head_halves();
+    for (int s0 = blockIdx.z; s0 < p.n_seqs; s0 += 64 * step) {
+        const int mine = s0 + lane * step;
+        int from = -1, to = -1, len = 0;
+        if (mine < p.n_seqs) {
+            const int2 m = *(const int2*)(moved + 4 * mine + 2);
+            from = m.x;
+            to = m.y;
+            len = pg_len(p, mine);
         }
+        const bool has = (unsigned)from < (unsigned)p.n_pages && (unsigned)to < (unsigned)p.n_pages;
+        for (uint64_t todo = __ballot(has); todo; todo &= todo - 1) {
+            const int l = __builtin_ctzll(todo);
+            const int fill = __builtin_amdgcn_readlane(len, l) & (p.page - 1);
+            const u4v* src = (const u4v*)(base + __builtin_amdgcn_readlane(from, l) * page_halves);
+            u4v* dst = (u4v*)(base + __builtin_amdgcn_readlane(to, l) * page_halves);
+            const int n = ((fill + 31) >> 5) * 512;  // (512 pieces a unit)
+            for (int i = t; i < n; i += 1024) {
+                u4v x[4];
+                bool on[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (on[k]) dst[i + 256 * k] = x[k];
+                for (int k = 0; k < 4; ++k) {
+                    const int at = i + 256 * k;
+                    const int token = 32 * (at >> 9) + 8 * (isv ? (at >> 4) & 3 : (at >> 2) & 3);
+                    on[k] = token < fill;
+                    if (on[k]) x[k] = src[at];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (on[k]) dst[i + 256 * k] = x[k];
+            }
+        }
     }
 }
 
@@ -412,7 +430,8 @@ hipError_t launch_pages_reserve(const PgPool& p, const PgRows& b, int32_t* out, 
                                 hipStream_t st) {
     if (p.n_seqs > PG_MAX_SEQS || b.max_rows > MJ_ROWS || p.page < 32) return hipErrorInvalidValue;
     hipLaunchKernelGGL(k_pages_reserve, dim3(1), dim3(1024), 0, st, p, b, out, abort);
-    hipLaunchKernelGGL(k_pages_copy, dim3(2 * p.n_layers, p.nKV, p.n_seqs), dim3(256), 0, st, p, out);
+    const int z = std::max(1, std::min(p.n_seqs, COPY_BLOCKS / (2 * p.n_layers * p.nKV)));
+    hipLaunchKernelGGL(k_pages_copy, dim3(2 * p.n_layers, p.nKV, z), dim3(256), 0, st, p, out);
     return hipGetLastError();
 }
 

@@ -614,7 +614,6 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
     const uint16_t* vl0 = a.p.v + a.layer * a.p.layer_halves();
     // the first half of the waves moves K, the other V
     const uint16_t* mover = (w < NW / 2 ? kl0 : vl0) + 512 * MV * (w % (NW / 2)) + 8 * lane;
-    bool states = false;  // the ring holds states of the segment before
     for (int64_t x = run.b0; x < run.b1;) {
         const PgSeg S = next_seg(a, plan, run, x);
         if (S.i1 <= S.i0) continue;
@@ -714,8 +713,6 @@ __global__ __launch_bounds__(512, 2) void k_paged_attn_shared(PgAttnArgs a) {
         else go_round(Two{}, std::true_type{});
         PgLeft* left = (PgLeft*)ring;
         if (ks > 1) {
-            if (states) __syncthreads();  // (where no ring came between: the states before have been read)
-            states = true;
             if (works && kl > 0)
 #pragma unroll
                 for (int i = 0; i < T; ++i) put_tile(left[(w - tg) * T + i], tl[i]);

@@ -117,6 +117,37 @@ def test_wide_rows(ctx):
     assert go(ctx, rows, **d) == want(rows, **d)
 
 
+@pytest.mark.parametrize("u", [0.0, 0.3, 0.7, 1.0 - 2.0 ** -24])
+@pytest.mark.parametrize("refused", [1, 2, 3, 20, 63])
+@pytest.mark.parametrize("near", [True, False])
+def test_refusals_below_one_row(ctx, refused, near, u):
+    """Drafts that were certain, all of one row and all refused, in the same chunk of ids or in many: the
+    token is sampled from what they leave."""
+    V, rows = 30011, [refused + 1]
+    d = make(rows, V, refused)
+    ids = torch.arange(refused) * (7 if near else V // refused - 1) + 4090
+    d["tokens"][1:] = (ids % V).int().cuda()
+    d["logits"] = d["logits"].clone()
+    d["logits"][0, d["tokens"][1:].long()] += 3.0  # a good part of the row
+    d["ua"].fill_(1.0)  # (u rest > e where the row has another id)
+    d["us"].fill_(u)
+    got = go(ctx, rows, parents=[[-1] + [0] * refused], **d)
+    assert got == want(rows, parents=[[-1] + [0] * refused], **d)
+    assert got[0] == [0] and got[2][0] not in d["tokens"][1:].tolist()
+
+
+@pytest.mark.parametrize("rows,parents,q", [([3], None, False), ([3], None, True), ([6], [[-1, 0, 0, 0, 0, 1]], False)],
+                         ids=["certain", "drawn", "tree"])
+def test_the_largest_vocabulary(ctx, rows, parents, q):
+    """2048 chunks of ids: several a thread of the block that samples."""
+    V = 1 << 23
+    for ua, us in ((1.0, 0.25), (0.0, 0.9999)):
+        d = make(rows, V, 5, q, spread=6.0)
+        d["ua"].fill_(ua)
+        d["us"].fill_(us)
+        assert go(ctx, rows, parents=parents, **d) == want(rows, parents=parents, **d), (ua, us)
+
+
 @pytest.mark.parametrize("u", [0.0, 0.5, 1.0 - 2.0 ** -24])
 @pytest.mark.parametrize("q", [False, True])
 def test_ends_of_the_uniforms(ctx, u, q):

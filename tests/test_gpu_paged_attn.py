@@ -164,6 +164,25 @@ def test_uneven_batch(ctx, M, nq):
     check(cache, rows, chains(rows), q, out, nq)
 
 
+@pytest.mark.parametrize("M,hole", [(1, None), (3, None), (5, 1300), (9, None), (17, 1301), (64, None), (64, 2040)])
+def test_runs_of_many_units(ctx, M, hole):
+    """So much work that a block's run is longer than the page numbers it holds at once; 24 sequences with the
+    pages of one.  hole: a block of the table that names no page (units are missing in the middle of a run)."""
+    L, n = 131000 - M, 24
+    one, gen, _ = make(ctx, [L], [M], 64, 4, seed=M)
+    table = one.table.repeat(n, 1).contiguous()
+    if hole is not None:
+        table[:, hole] = -1
+    cache = PagedCache.over(ctx, one.k, one.v, table, one.lens.repeat(n), one.refs)
+    q = (torch.randn((n * M, 16 * D), generator=gen, device="cuda") * 2).half()
+    out = torch.full_like(q, 7.0)
+    ctx.paged_attn(cache, 0, batch_of([M] * n), q, 16, out)
+    src = one  # (its own table still names every page: the reference leaves the hole out itself)
+    for s in (0, 1, 11, n - 1):
+        check(src, [M], chains([M]), q[s * M:(s + 1) * M], out[s * M:(s + 1) * M], 16,
+              holes=[] if hole is None else [(0, hole)])
+
+
 def test_1024_sequences(ctx):
     lens = [(37 * i) % 90 for i in range(1024)]
     rows = [1 + (i % 3 == 0) for i in range(1024)]

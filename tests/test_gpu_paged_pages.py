@@ -93,6 +93,43 @@ def test_many_calls_in_turn(ctx, n, n_pages, page, seed):
     assert not cache.refs.any() and bool((cache.table == -1).all())
 
 
+@pytest.mark.parametrize("n,layers,nkv", [(100, 24, 8), (1024, 1024, 1)])
+def test_few_copies_of_many_sequences(ctx, n, layers, nkv):
+    """More sequences, layers and heads than a launch has blocks: branches here and there, each of which
+    gets a page of its own with the committed tokens of every layer and head."""
+    page, L, n_pages = 32, 20, 16
+    shape = (layers, n_pages, nkv, 1, 4096)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(n)
+    k, v = (torch.randn(shape, generator=gen, device="cuda", dtype=torch.float16) for _ in range(2))
+    table, lens, refs = np.full((n, 2), -1), np.zeros(n, int), np.zeros(n_pages, int)
+    table[3, 0], lens[3], refs[9] = 9, L, 1
+    cache = PagedCache.over(ctx, k, v, cuda(table), cuda(lens), cuda(refs))
+    to = [0, 5, 63, 64, n // 2 - 1, n // 2, n - 2, n - 1]
+    src = np.full(n, -1)
+    src[to] = 3
+    ctx.pages_fork(cache, cuda(src))
+    before = [x.clone() for x in (k, v)]
+    out = torch.zeros((n, 4), dtype=torch.int32, device="cuda")
+    ctx.pages_reserve(cache, starts([1 if s in to or s == 3 else 0 for s in range(n)]), out)
+    ctx.sync()
+    got = out.tolist()
+    new = [p for p in range(n_pages) if p != 9]
+    at = 0
+    for s in range(n):  # (all leave the shared page, also the source: its count is that before the call)
+        if s in to or s == 3:
+            assert got[s] == [1, 1, 9, new[at]], s
+            at += 1
+        else:
+            assert got[s] == [0, 0, -1, -1], s
+    i = [x.cuda() for x in R.unit_at(torch.arange(24))]
+    for x, b, j in zip((k, v), before, i):
+        b = b.view(layers, n_pages, nkv, 4096)
+        for p in new[:at]:
+            b[:, p, :, j.reshape(-1)] = b[:, 9, :, j.reshape(-1)]
+        assert torch.equal(x.view(layers, n_pages, nkv, 4096), b)
+
+
 def test_lengths_themselves_give_back_what_was_reserved(ctx):
     cache = filled(ctx, 3, 12)
     out = torch.zeros((3, 4), dtype=torch.int32, device="cuda")

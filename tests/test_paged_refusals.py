@@ -107,7 +107,7 @@ ON_BATCHES = [append, attn, reserve, commit, accept]
 
 @pytest.mark.parametrize("bad", [
     dict(k=None), dict(v=None), dict(table=None), dict(lens=None), dict(refs=None), dict(n_kv=0),
-    dict(n_kv=1025), dict(n_pages=0), dict(n_layers=0), dict(n_layers=4097), dict(n_seqs=0), dict(n_seqs=1025),
+    dict(n_kv=1025), dict(n_pages=0), dict(n_pages=(1 << 28) + 1), dict(n_layers=0), dict(n_layers=4097), dict(n_seqs=0), dict(n_seqs=1025),
     dict(n_seqs=-1), dict(stride=0), dict(stride=(1 << 24) + 1), dict(page=256, stride=(1 << 22) + 1),
     dict(k=20 * P + 8), dict(v=30 * P + 2), dict(table=P + 4), dict(lens=2 * P + 4), dict(refs=3 * P + 8)],
     ids=str)
