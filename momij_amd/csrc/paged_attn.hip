@@ -835,13 +835,16 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
 // us against 32), and its waves would all read every unit.  One block of 256 vectors, though two of 128 would
 // divide the work more evenly: as fast (53.2 and 53.1 us), with half the reads.
 // A segment's beginning (its rows' queries, page numbers, the ring filled, the result written) costs as much
-// as 10 units of the ring (17 rows of 16 sequences 32.3 us; counted as 6 units 36) or 2 of the first kernel.
+// as 10 units of the ring (17 rows of 16 sequences 32.3 us; counted as 6 units 36) or 8 of the first kernel (64
+// sequences of 200..8000 tokens 51.5 us, as 2 units 53.1, as 16 52.5).
+// A block takes four units at least, those that count for beginnings among them, so a short segment still has
+// several blocks (nine rows of four sequences of 200..400 tokens 18 us; with four units of keys at least 23).
 size_t paged_attn_plan(PgAttnArgs& a, void* base) {
     const int nv = a.b.max_rows * a.G;
     a.cols = nv <= 16 ? 16 : std::min((nv + 31) / 32 * 32, 256);
     a.blocks = a.cols == 16 ? 512 : 256;  // two a CU, or one
-    a.extra = a.cols == 16 ? 2 : 10;
-    a.least = a.extra + 4;
+    a.extra = a.cols == 16 ? 8 : 10;
+    a.least = 4;
     Arena ar{base, 0};
     a.off = (int64_t*)ar.take((PG_MAX_SEQS + 2) * sizeof(int64_t));
     a.pml = (float2*)ar.take((size_t)a.blocks * 2 * a.cols * sizeof(float2));
