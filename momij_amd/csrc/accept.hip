@@ -354,7 +354,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     __shared__ float s_m[MJ_ROWS];
     __shared__ int s_at[MJ_ROWS];
     __shared__ uint64_t s_refused;
-    __shared__ int s_cur, s_abort;
+    __shared__ int s_cur, s_any, s_abort;
     __shared__ LeftShared<AC_WALK> s_left;
     const int s = blockIdx.x, t = threadIdx.x;
     const int ab = abort_word(a.abort);
@@ -465,11 +465,13 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
                 kids &= kids - 1;
             }
         }
-        if (refused >> t & 1) s_left.out[__popcll(refused & ((1ull << t) - 1))] = tok;
+        const uint64_t out = refused & __ballot((unsigned)tok < (unsigned)a.V);  // (others have nothing to leave out)
+        if (out >> t & 1) s_left.out[__popcll(out & ((1ull << t) - 1))] = tok;
         if (t < n) a.path[r0 + t] = way;
         if (t == 0) {
             s_cur = cur;
-            s_refused = refused;
+            s_refused = out;
+            s_any = refused != 0;
             a.accepted[s] = acc;
             if (greedy || !(s_Z[cur] > 0.0)) a.token[s] = s_Z[cur] > 0.0 ? s_at[cur] : -1;
         }
@@ -477,10 +479,10 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     __syncthreads();
     const int cur = s_cur, row = r0 + cur;
     const uint64_t refused = s_refused;
-    const int n_out = __popcll(refused);
+    const int n_out = (int)__popcll(refused);
     const double Z = s_Z[cur];
     if (greedy || !(Z > 0.0)) return;
-    const int mode = n_out == 0 ? LAST_P : a.q ? LAST_RESIDUAL : LAST_WITHOUT;
+    const int mode = a.q && s_any ? LAST_RESIDUAL : n_out ? LAST_WITHOUT : LAST_P;
     if (mode == LAST_RESIDUAL || n_out > AC_FEW) {
         if (t == 0) {
             a.last[s].refused = refused;

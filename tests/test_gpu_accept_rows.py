@@ -209,6 +209,21 @@ def test_drafts_that_are_no_ids(ctx):
     assert got == want(rows, **d) and got[0] == [0, 0]
 
 
+@pytest.mark.parametrize("V", [500, 20001])
+@pytest.mark.parametrize("form", ["certain", "drawn", "tree"])
+def test_drafts_far_from_any_id(ctx, V, form):
+    """Below the first id and past the last by more than a chunk of ids, alone and beside drafts that are."""
+    far = [-1, -4096, -4097, -5000, -2 ** 31, V, V + 4096, V + 100000, 2 ** 31 - 1, 2 ** 31 - 4096]
+    for i, bad in enumerate(far):
+        parents = [[-1, 0, 0, 0, 2]] if form == "tree" else None
+        rows = [5] if parents else [2, 3]
+        d = make(rows, V, i, form == "drawn")
+        d["ua"].fill_(0.999)
+        d["tokens"][1] = bad
+        d["tokens"][4] = bad
+        assert go(ctx, rows, parents=parents, **d) == want(rows, parents=parents, **d), bad
+
+
 def test_draft_distributions_at_their_ends(ctx):
     """q of 0, below 0 and NaN at the draft: never accepted; q that covers p: the row's own probabilities
     stand in where nothing is left; q of 1 at the draft: what is left is p without it."""
