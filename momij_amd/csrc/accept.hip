@@ -211,10 +211,10 @@ __device__ __forceinline__ double of_lane(double v, int lane) {
 // LDS of a block that samples.
 template <int NT>
 struct LeftShared {
-    double w[NT / 64], fix[AC_FEW], before;
+    double w[NT / 64], fix[AC_FEW], gone_e[MJ_ROWS], before;
     uint32_t gone[AC_CHUNK / 32];
     int out[MJ_ROWS];  // the refused drafts of the row
-    int first[NT / 64], last[NT / 64], chunk;
+    int first[NT / 64], last[NT / 64], chunk, bad;
 };
 // What the walk left of a row's probabilities: methods are for a whole block.
 template <int NT>
@@ -282,9 +282,10 @@ struct Left {
         return all;
     }
     // The id where the sums pass u times all, -1 where nothing has any weight; in one thread, the others
-    // get -2.  of_chunk(c): what chunk c has left.
-    template <typename F>
-    __device__ __forceinline__ int sample(double u, F of_chunk) {
+    // get -2.  of_chunk(c): what chunk c has left; again(): the same in every thread, after all have asked for
+    // their chunks: whether they have to ask once more.
+    template <typename F, typename G>
+    __device__ __forceinline__ int sample(double u, F of_chunk, G again) {
         const int t = threadIdx.x, per = (chunks + NT - 1) / NT;
         double all = 0.0, upto = 0.0, share = 0.0;
         bool plain = mode == LAST_P;
@@ -298,6 +299,7 @@ struct Left {
             share = 0.0;
             for (int i = 0; i < per; ++i) share += has(per * t + i);
             upto = block_scan64<NT>(share, S.w, &all);
+            if (!plain && again()) continue;
             if (all > 0.0 || plain) break;
             plain = true;  // nothing left: the row's own probabilities
             mode = LAST_P;
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
         const uint64_t can = __ballot(q > 0.0f);
         int cur = 0, acc = 0, way = t == 0 ? 0 : -1;
         uint64_t refused = 0, kids = __ballot(par == 0);
-        double rest = s_Z[0];
+        double rest = s_Z[0], gone = 0.0;
         while (kids) {
             const int r = __builtin_ctzll(kids);
             const double er = of_lane(e, r);
@@ -460,16 +462,22 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
             } else {
                 refused |= 1ull << r;
                 rest -= er;
+                if (t == r) gone = er;
                 // (an equal sibling after it has nothing left)
                 if (par == cur && tok == __builtin_amdgcn_readlane(tok, r)) e = 0.0;
                 kids &= kids - 1;
             }
         }
         const uint64_t out = refused & __ballot((unsigned)tok < (unsigned)a.V);  // (others have nothing to leave out)
-        if (out >> t & 1) s_left.out[__popcll(out & ((1ull << t) - 1))] = tok;
+        if (out >> t & 1) {
+            const int at = __popcll(out & ((1ull << t) - 1));
+            s_left.out[at] = tok;
+            s_left.gone_e[at] = gone;
+        }
         if (t < n) a.path[r0 + t] = way;
         if (t == 0) {
             s_cur = cur;
+            s_left.bad = rest < s_Z[cur] * 0x1p-10;
             s_refused = out;
             s_any = refused != 0;
             a.accepted[s] = acc;
@@ -495,17 +503,34 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     }
     Left<AC_WALK> left{a.logits + row * a.ld, nullptr, a.part + (size_t)row * a.chunks, 0.0, Weights(k, s_m[cur], s_tab),
               a.V, a.chunks, mode, n_out, s_left};
-    for (int i = 0; i < n_out; ++i) {
-        const double z = left.chunk(s_left.out[i] / AC_CHUNK);
-        if (t == 0) s_left.fix[i] = z;
-        __syncthreads();
-    }
-    const int id = left.sample((double)u_sample, [&](int c) __attribute__((always_inline)) {
-        for (int i = 0; i < n_out; ++i)
-            if (s_left.out[i] / AC_CHUNK == c) return s_left.fix[i];
-        const AcceptPart p = left.parts[c];
-        return p.s * left.e(p.m);
-    });
+    // The drafts' weights are known and taken off their chunks' sums, which have an error of 2^-53 of
+    // themselves; where that is not small against what is left, the chunks are gone through again.
+    bool exact = false;
+    const int id = left.sample(
+        (double)u_sample,
+        [&](int c) __attribute__((always_inline)) {
+            const AcceptPart p = left.parts[c];
+            const double z = p.s * left.e(p.m);
+            double less = 0.0;
+            for (int i = 0; i < n_out; ++i)
+                if (s_left.out[i] / AC_CHUNK == c) {
+                    if (exact) return s_left.fix[i];
+                    less += s_left.gone_e[i];
+                }
+            if (less > 0.0 && z - less < z * 0x1p-20) s_left.bad = 1;
+            return z - less;
+        },
+        [&]() __attribute__((always_inline)) {
+            __syncthreads();
+            if (exact || !s_left.bad) return false;
+            exact = true;
+            for (int i = 0; i < n_out; ++i) {
+                const double z = left.chunk(s_left.out[i] / AC_CHUNK);
+                if (t == 0) s_left.fix[i] = z;
+                __syncthreads();
+            }
+            return true;
+        });
     if (id > -2) a.token[s] = id;
 }
 
@@ -547,9 +572,12 @@ __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
     }
     __syncthreads();
     if (!s_last) return;
-    const int id = left.sample((double)u_sample, [&](int i) __attribute__((always_inline)) {
-        return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    });
+    const int id = left.sample(
+        (double)u_sample,
+        [&](int i) __attribute__((always_inline)) {
+            return __hip_atomic_load(sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        },
+        []() { return false; });
     if (id > -2) a.token[s] = id;
 }
 

@@ -742,20 +742,33 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
     __shared__ int s_abort;
     const int t = threadIdx.x, lane = t & 63, d = t & 31, r = blockIdx.x;
     const int h = WAVES == 1 ? 4 * blockIdx.y + (t >> 6) : blockIdx.y;
-    const int ab = abort_word(a.abort);
-    const int64_t per = a.off[a.b.n_seqs + 1];
+    // Of up to 64 sequences all that a row's may need is requested at once, a sequence a lane.
+    const int ab = abort_word(a.abort), n_seqs = a.b.n_seqs, mine = min(lane, n_seqs - 1);
+    const int64_t per = a.off[n_seqs + 1];
+    int r0, m = pg_rows(a.b, mine, r0), L = pg_len(a.p, mine);
+    int64_t S = a.off[mine];
     const int s = pg_seq(a.b, r);
     if (t == 0) s_abort = ab;
     __syncthreads();
-    if (s_abort || s >= a.b.n_seqs || h >= a.p.nKV * a.G) return;  // (h: a whole wave, and the block has no barrier then)
-    int r0;
-    const int m = pg_rows(a.b, s, r0);
-    const SeqUnits su = seq_units(a, m, r0, pg_len(a.p, s));
+    if (s_abort || s >= n_seqs || h >= a.p.nKV * a.G) return;  // (h: a whole wave, and the block has no barrier then)
+    if (n_seqs <= 64) {
+        m = __builtin_amdgcn_readlane(m, s);
+        r0 = __builtin_amdgcn_readlane(r0, s);
+        L = __builtin_amdgcn_readlane(L, s);
+        S = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(S >> 32), s) << 32 |
+                      (uint32_t)__builtin_amdgcn_readlane((int)S, s));
+    } else {
+        m = pg_rows(a.b, s, r0);
+        L = pg_len(a.p, s);
+        S = a.off[s];
+    }
+    const SeqUnits su = seq_units(a, m, r0, L);
     const int local = r - su.r0;
     if (local < 0 || local >= su.m) return;
     uint16_t* out = a.out + r * a.ldo + h * HD;
     const int g = h / a.G, v = local * a.G + h - g * a.G, c = v / a.cols, cc = v - c * a.cols;
-    const int64_t S = a.off[s] + ((int64_t)g * su.ncg + c) * (su.nu + a.extra), E = S + su.nu + a.extra;
+    S += ((int64_t)g * su.ncg + c) * (su.nu + a.extra);
+    const int64_t E = S + su.nu + a.extra;
     if (su.nu == 0) {
         if (WAVES == 1 ? lane < 32 : t < 32) *(uint2*)(out + 4 * d) = make_uint2(0u, 0u);
         return;

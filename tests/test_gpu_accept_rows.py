@@ -209,6 +209,30 @@ def test_drafts_that_are_no_ids(ctx):
     assert got == want(rows, **d) and got[0] == [0, 0]
 
 
+@pytest.mark.parametrize("refused", [1, 2, 3])
+@pytest.mark.parametrize("u", [0.0, 1e-9, 0.4, 0.99])
+@pytest.mark.parametrize("others", [True, False])
+def test_refused_drafts_that_were_almost_all(ctx, refused, u, others):
+    """What is left of a chunk of ids, or of the row, is lost in the drafts' own weight."""
+    V = 12301
+    rows, parents = [refused + 1], [[-1] + [0] * refused]
+    d = make(rows, V, refused)
+    x = torch.randn(rows[0], V, generator=torch.Generator().manual_seed(refused)) - 27.0
+    ids = [100 + 50 * i for i in range(refused)]
+    x[0, ids] = 0.0
+    if others:  # as much in another chunk
+        x[0, 9000:9010] = 0.0
+    d["logits"], d["T"] = x.cuda(), torch.ones(1, device="cuda")
+    d["tokens"][1:] = cuda(ids)
+    d["ua"].fill_(1.0)
+    d["us"].fill_(u)
+    if not others:
+        d["ua"][refused] = 2.0  # (the last of them would be accepted for any u below 1)
+    got = go(ctx, rows, parents=parents, **d)
+    assert got == want(rows, parents=parents, **d)
+    assert got[0] == [0] and got[2][0] not in ids
+
+
 @pytest.mark.parametrize("V", [500, 20001])
 @pytest.mark.parametrize("form", ["certain", "drawn", "tree"])
 def test_drafts_far_from_any_id(ctx, V, form):
