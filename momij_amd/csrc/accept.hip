@@ -18,7 +18,9 @@
 #define AC_CHUNK 4096  // ids a block takes
 #define AC_PER (AC_CHUNK / 256)
 #define AC_GREEDY 1e-5f
-#define AC_FEW 2  // refused drafts that are taken out of their chunks one after another
+// Refused drafts that the walk takes out of their chunks itself: a chunk gone through again takes its block 2 us,
+// so that of more the third launch, all chunks at once, is not longer.
+#define AC_FEW 2
 
 // 2^(i / 32), 0 <= i < 32, in 64 bits: 12 terms of the series of exp(i ln 2 / 32 - ln 2 / 2) (the next is
 // below 7e-15), times sqrt 2.
@@ -92,7 +94,9 @@ __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY;
 // Four floats from any place.
 typedef float __attribute__((ext_vector_type(4), aligned(4))) f4_any;
 
-// Sum of e, greatest logit and its lowest place of AC_CHUNK ids of a row.
+// Sum of e, greatest logit and its lowest place of AC_CHUNK ids of a row.  Bound by memory and by its
+// operations in 64 bits alike: 324 rows of 151936 ids take 37 to 40 us, 33 at the rate of a streaming read, and
+// the VALU is busy 70% of it (64 roots, the place carried beside the maximum and a load an id: 53 us).
 __global__ __launch_bounds__(256) void k_accept_stats(AcceptArgs a) {
     __shared__ double s_tab[32], s_s[4];
     __shared__ float s_m[4];
@@ -349,7 +353,8 @@ struct Left {
 // The rows' totals and the walk over the drafts, a block a sequence; and the token, where it is the greatest
 // logit's, or is sampled from the row's sums by chunks as they are or with a few drafts taken out.
 // One block's steps one after another bound it, its instructions' own way to it among them: with 256 threads of
-// 16 ids each, four times the instructions, a sequence took 14 us, so 11.5.
+// 16 ids each, four times the instructions, a sequence took 14 us, so 11.5 (10 without a chunk gone through
+// again).
 #define AC_WALK 1024
 __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     __shared__ double s_tab[32], s_Z[MJ_ROWS];
@@ -534,7 +539,9 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     if (id > -2) a.token[s] = id;
 }
 
-// What is left of the other sequences' last rows, a block a chunk; the block that comes last samples.
+// What is left of the other sequences' last rows, a block a chunk; the block that comes last samples.  Bound
+// by its operations (48 rows of 151936 ids with distributions, 58 MB, 20 us, VALU 64% busy; by 1024 threads of
+// four ids, one block a CU, 43, by 256 of 16 30).
 #define AC_LEFT 512
 __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
     __shared__ double s_tab[32];

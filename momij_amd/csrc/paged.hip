@@ -13,7 +13,8 @@
 // a lane, both dims of a rotated pair in one lane; angles in turns in 64 bits), with the row's sequence,
 // length and depth from the device: every wave counts the sequences that end at or before the row, 64 a
 // step, so the position is two dependent rounds of requests away and the row's data are on their way
-// meanwhile.  A token's V goes to 128 places 16 bytes apart (eight tokens of a dim lie together).
+// meanwhile.  A token's V goes to 128 places 16 bytes apart (eight tokens of a dim lie together).  A row takes
+// 3.6 us, 64 chains of up to 9 rows 6.2.
 __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
     __shared__ float2 cs[MJ_ROPE_F];
     __shared__ int s_abort;
@@ -186,7 +187,9 @@ __device__ __forceinline__ int block_scan(int v, int* wsum, int* total) {
 
 // Room for the batch's rows, one block: a thread a sequence counts the blocks that it lacks, a scan gives
 // each its place among them, and the pool's counts are gone through for as many free pages, 16 a thread
-// and round, so that the k-th lacking block takes the k-th free page.
+// and round, so that the k-th lacking block takes the k-th free page.  Bound by requests one after another (a
+// sequence's rows and length, its table, the counts of these pages) and three scans: 5 us for 4 sequences, 6 for
+// 64; the counts of the first 16384 pages come meanwhile.
 __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int32_t* out, const int* abort) {
     __shared__ int wsum[16];
     __shared__ int ids[PG_NEED * PG_MAX_SEQS];
