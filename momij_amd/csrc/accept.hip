@@ -22,7 +22,8 @@
 // so that of more the third launch, all chunks at once, is not longer.
 #define AC_FEW 2
 
-// 2^(i / 32), 0 <= i < 32, in 64 bits: 12 terms of the series of exp(i ln 2 / 32 - ln 2 / 2) (the next is
+// 2^(i / 32), 0 <= i < 32, in 64 bits, with i << 15 taken off the upper half: n << 15 added there gives 2^(n / 32)
+// for any n = i in the lowest five bits (32 << 15 is one in the exponent).  12 terms of the series of exp(i ln 2 / 32 - ln 2 / 2) (the next is
 // below 7e-15), times sqrt 2.
 __device__ __forceinline__ double root32(int i) {
     const double r = (double)(i - 16) * 0.02166084939249829;
@@ -38,7 +39,8 @@ __device__ __forceinline__ double root32(int i) {
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
-    return p * 1.4142135623730951;
+    p *= 1.4142135623730951;
+    return __hiloint2double(__double2hiint(p) - (i << 15), __double2loint(p));
 }
 
 // e of many logits of one row: y = (x - m) 32 log2(e) / T = n + r, |r| <= 1/2; 2^(n / 32) from a table and the
@@ -64,7 +66,7 @@ struct Weights {
         p = fma(p, r, 0.021660849391723976);
         p = fma(p, r, 1.0);
         root = tab[n & 31];
-        root = __hiloint2double(__double2hiint(root) + ((n & ~31) << 15), __double2loint(root));
+        root = __hiloint2double(__double2hiint(root) + (n << 15), __double2loint(root));
     }
     // 0 below 2^-1000, for -inf and for NaN
     __device__ __forceinline__ double operator()(float x) const {
@@ -87,9 +89,6 @@ __device__ __forceinline__ double wave_sum64(double v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, MJ_WAVE);
     return v;
 }
-
-// What a row's logits count as: a NaN as the least.
-__device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
 
 // Four floats from any place.
 typedef float __attribute__((ext_vector_type(4), aligned(4))) f4_any;
@@ -244,8 +243,8 @@ struct Left {
     }
     // of id d of a chunk, of logit x and draft's probability q
     __device__ __forceinline__ double weight(float x, float q, int d) const {
-        double z = e(logit(x));
-        if (mode == LAST_RESIDUAL) z = fmax(z * inv - (q > 0.0f ? (double)q : 0.0), 0.0);
+        double z = e(x);
+        if (mode == LAST_RESIDUAL) z = fmax(fma(z, inv, -(double)fmaxf(q, 0.0f)), 0.0);  // (a NaN counts as 0)
         if (mode == LAST_WITHOUT && (S.gone[d >> 5] >> (d & 31)) & 1) z = 0.0;
         return z;
     }
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     if (t < 64) {
         double e = 0.0;
         if (par >= 0 && (unsigned)tok < (unsigned)a.V && s_Z[par] > 0.0)
-            e = greedy ? (tok == s_at[par] ? 1.0 : 0.0) : Weights(k, s_m[par], s_tab)(logit(x));
+            e = greedy ? (tok == s_at[par] ? 1.0 : 0.0) : Weights(k, s_m[par], s_tab)(x);
         const double uq = (double)u * (double)q;
         const uint64_t can = __ballot(q > 0.0f);
         int cur = 0, acc = 0, way = t == 0 ? 0 : -1;
