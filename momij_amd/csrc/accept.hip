@@ -94,8 +94,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 typedef float __attribute__((ext_vector_type(4), aligned(4))) f4_any;
 
 // Sum of e, greatest logit and its lowest place of AC_CHUNK ids of a row.  Bound by memory and by its
-// operations in 64 bits alike: 324 rows of 151936 ids take 37 to 40 us, 33 at the rate of a streaming read, and
-// the VALU is busy 70% of it (64 roots, the place carried beside the maximum and a load an id: 53 us).
+// operations in 64 bits alike: 324 rows of 151936 ids take 36 to 39 us, 33 at the rate of a streaming read, and
+// the VALU is busy 69% of it (64 roots, the place carried beside the maximum and a load an id: 53 us).
 __global__ __launch_bounds__(256) void k_accept_stats(AcceptArgs a) {
     __shared__ double s_tab[32], s_s[4];
     __shared__ float s_m[4];
@@ -539,8 +539,8 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
 }
 
 // What is left of the other sequences' last rows, a block a chunk; the block that comes last samples.  Bound
-// by its operations (48 rows of 151936 ids with distributions, 58 MB, 20 us, VALU 64% busy; by 1024 threads of
-// four ids, one block a CU, 43, by 256 of 16 30).
+// by its operations and a block's few steps one after another (48 rows of 151936 ids with distributions, 58 MB, 20
+// us, VALU 58% busy; by 1024 threads of four ids, one block a CU, 43, by 256 of 16 30).
 #define AC_LEFT 512
 __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
     __shared__ double s_tab[32];
