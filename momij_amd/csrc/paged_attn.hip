@@ -203,8 +203,8 @@ struct PgRun {
     int64_t b0, b1, per;
     int s;  // the sequence that the run begins in
 };
-// One round of requests and a scan for every NT sequences; a.off gets the units for the join.  False: the
-// call was aborted.
+// One round of requests and a scan for every NT sequences; a.off gets the units for the join (also of a call
+// that is aborted: the word may be cleared before the join reads it).  False: the call was aborted.
 template <int NT>
 __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, PgPlan& P, PgRun& run) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6, n = a.b.n_seqs;
@@ -241,10 +241,10 @@ __device__ __forceinline__ bool plan_run(const PgAttnArgs& a, PgPlan& P, PgRun& 
         before = all;
     }
     __syncthreads();
-    if (P.abort) return false;
     run.per = max(quotient(before + a.blocks - 1, a.blocks), (int64_t)a.least);
     if (blockIdx.x == 0)
         for (int i = t; i <= n + 1; i += NT) a.off[i] = i <= n ? P.off[i] : run.per;
+    if (P.abort) return false;
     run.b0 = blockIdx.x * run.per;
     run.b1 = min(before, run.b0 + run.per);
     run.s = 0;

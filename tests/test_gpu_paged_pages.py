@@ -10,7 +10,7 @@ import paged_ref as R
 from momij_amd._lib import MomijError
 from momij_amd.ops import Context
 from momij_amd.paged import PagedCache, RowBatch
-from test_gpu_paged_attn import batch_of, cfg, chains, check, cuda, norm_rope
+from test_gpu_paged_attn import batch_of, cfg, chains, check, cuda, make, norm_rope
 
 pytestmark = pytest.mark.gpu
 D = 128
@@ -429,3 +429,41 @@ def test_an_abort_serves_nobody(ctx):
     ctx.pages_reserve(cache, starts([3, 3]), out)
     ctx.sync()
     assert out[:, 0].tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("M", [1, 9, 64])
+def test_an_aborted_step_leaves_its_arrays(ctx, M):
+    """The word set: nothing is attended, accepted or kept; cleared, the same calls on the same workspaces are
+    right."""
+    nq, nkv, V = 16, 4, 5000
+    lens, rows = [700, 90], [M, M]
+    cache, gen, _ = make(ctx, lens, rows, 64, nkv, seed=M)
+    q = torch.randn((2 * M, nq * D), generator=gen, device="cuda").half()
+    logits = torch.randn((2 * M, V), generator=gen, device="cuda")
+    tokens = torch.randint(0, V, (2 * M,), generator=gen, device="cuda").int()
+    T, u, us = (torch.full((k,), 0.5, device="cuda") for k in (2, 2 * M, 2))
+    out, acc, path, tok = torch.full_like(q, 7.0), cuda([55] * 2), cuda([55] * (2 * M)), cuda([55] * 2)
+    ws = [torch.full((size,), 0xA5, dtype=torch.uint8, device="cuda")
+          for size in (ctx.paged_workspace(nq, nkv, M), ctx.accept_workspace(2, 2 * M, V))]
+    batch = batch_of(rows)
+
+    def step():
+        ctx.paged_attn(cache, 0, batch, q, nq, out, ws=ws[0])
+        ctx.accept_rows(batch, logits, tokens, T, u, us, acc, path, tok, ws=ws[1])
+        ctx.pages_commit(cache, batch, acc)
+
+    torch.cuda.synchronize()
+    ctx.set_abort(True)
+    step()
+    torch.cuda.synchronize()
+    ctx.set_abort(False)
+    with pytest.raises(MomijError):
+        ctx.sync()
+    assert bool((out == 7.0).all()) and cache.lens.tolist() == lens
+    assert acc.tolist() + path.tolist() + tok.tolist() == [55] * (4 + 2 * M)
+    acc.fill_(-1)
+    ctx.paged_attn(cache, 0, batch, q, nq, out, ws=ws[0])
+    check(cache, rows, chains(rows), q, out, nq)
+    ctx.accept_rows(batch, logits, tokens, T, u, us, acc, path, tok, ws=ws[1])
+    ctx.sync()
+    assert all(0 <= t < V for t in tok.tolist())
