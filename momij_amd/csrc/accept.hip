@@ -43,23 +43,26 @@ __device__ __forceinline__ double root32(int i) {
     return __hiloint2double(__double2hiint(p) - (i << 15), __double2loint(p));
 }
 
-// e of many logits of one row: y = (x - m) 32 log2(e) / T = n + r, |r| <= 1/2; 2^(n / 32) from a table and the
+// e of many logits of one row: (x - m) a = n + r, a = 32 log2(e) / T, |r| <= 1/2; 2^(n / 32) from a table and the
 // exponent, 2^(r / 32) from a polynomial of degree 4 (its coefficients fitted to the least greatest error,
-// 8e-14; the series' own would have 1.2e-12).  n comes out of the low bits of y + 1.5 2^52.  The table is 256
-// bytes, each LDS bank once, so that lanes never wait for one another; of 64 entries and one term less they
-// did.  Infinities share the row.
+// 8e-14; the series' own would have 1.2e-12).  The difference d = x - m of two floats is exact at 0 and off by 2^-53
+// of itself elsewhere, so e is 1 at m wherever the row lies (a x - a m, with a m rounded first, is off by 2^-53 a m:
+// at logits of 1e15 and more by whole steps of n).  n comes out of the low bits of a d + 1.5 2^52, r out of a second
+// fma with the same product.  The table is 256 bytes, each LDS bank once, so that lanes never wait for one another; of
+// 64 entries and one term less they did.  Infinities share the row.
 struct Weights {
-    double a, c;  // y = a x + c
+    double a, least;  // a d = -32000 at `least`: what lies below has no weight
     float m;
     const double* tab;
     __device__ __forceinline__ Weights(double k, float top, const double* t) : m(top), tab(t) {
-        a = k * 46.16624130844683;  // 32 log2(e)
-        c = top < INFINITY ? -a * (double)top : 0.0;
+        // (an infinite temperature: a is not 0, so that -inf stays below everything, and any finite a d is)
+        a = fmax(k * 46.16624130844683, 1e-60);  // 32 log2(e)
+        least = -32000.0 / a;
     }
     __device__ __forceinline__ bool finite() const { return m < INFINITY; }
-    // 2^(y / 32) as a product
-    __device__ __forceinline__ void factors(double y, double& p, double& root) const {
-        const double t = y + 6755399441055744.0, r = y - (t - 6755399441055744.0);
+    // 2^(a d / 32) as a product
+    __device__ __forceinline__ void factors(double d, double& p, double& root) const {
+        const double t = fma(d, a, 6755399441055744.0), r = fma(d, a, 6755399441055744.0 - t);
         const int n = __double2loint(t);
         p = fma(r, 9.172541587776638e-09, 1.6938633817694331e-06);
         p = fma(p, r, 0.0002345961982133178);
@@ -71,15 +74,15 @@ struct Weights {
     // 0 below 2^-1000, for -inf and for NaN
     __device__ __forceinline__ double operator()(float x) const {
         if (!finite()) return x == m ? 1.0 : 0.0;
-        const double y = fma((double)x, a, c);
+        const double d = (double)x - (double)m;
         double p, root;
-        factors(y, p, root);
-        return y > -32000.0 ? p * root : 0.0;
+        factors(d, p, root);
+        return d > least ? p * root : 0.0;
     }
     // sum + e, of a finite row's sum: what is 0 above counts as 2^-1000, which is lost in the sum (that has a 1)
     __device__ __forceinline__ double onto(double sum, float x) const {
         double p, root;
-        factors(fmax(fma((double)x, a, c), -32000.0), p, root);
+        factors(fmax((double)x - (double)m, least), p, root);
         return fma(p, root, sum);
     }
 };
