@@ -354,6 +354,12 @@ typedef struct mj_pages {
     int table_stride; /* blocks a sequence can have; times page_tokens at most 2^30 */
     int32_t* lens;    /* [n_seqs] committed tokens */
     int32_t* refs;    /* [n_pages] how many entries name the page; 0: it is free */
+    /* [n_seqs] what the last mj_pages_reserve with rows of a sequence said of it: 1 it had room, 0 it had
+     * none; others (to begin with, and after the sequence was forked into or cut): not known.  By this append
+     * and commit leave out whoever has no room.  NULL: not known of any.  Where it is not known the counts
+     * decide: rows that go to a page with refs above 1 are not written, and a step of which one row has no page, or
+     * such a page, is not kept. */
+    int32_t* served;
 } mj_pages;
 
 /* The rows of a pass: sequence s has rows row_start[s] .. row_start[s + 1] - 1 (none: it takes no
@@ -376,7 +382,8 @@ typedef struct mj_batch {
  * lacks nothing is always served).  A shared page loses a reference for each sequence that leaves it, all
  * counted as before the call; of the block that holds committed tokens these are copied in all layers
  * (in groups of eight).  out int32 [n_seqs][4]: 1 if served, pages taken, then the page copied from
- * and to (-1: none). */
+ * and to (-1: none).  A sequence with rows that is not served has no part in the step: nothing of it is appended
+ * or kept (its attention and its drafts' acceptance are formed, of what there is, and mean nothing). */
 mj_status mj_pages_reserve(mj_ctx* ctx, const mj_pages* pages, const mj_batch* batch, int32_t* out);
 /* Sequence s becomes a branch of from[s]: what it had is given back, the pages of the source's committed
  * tokens gain a reference, the length is the source's.  from [n_seqs]: outside [0, n_seqs), or s itself:
@@ -389,13 +396,15 @@ mj_status mj_pages_truncate(mj_ctx* ctx, const mj_pages* pages, const int32_t* l
 /* The accepted rows of a pass kept: rows path[0] .. path[accepted] of a sequence (accepted [n_seqs], path
  * [rows] at the sequence's first row, as mj_accept_rows gives them) are moved to its tokens L, L + 1, ...
  * in all layers, and lens_out[s] = L + accepted + 1 (accepted below 0, or no rows: L).  path NULL: the rows
- * of a chain, in place already.  An entry that names no row of the sequence moves nothing.  lens_out
- * [n_seqs] may be pages->lens. */
+ * of a chain, in place already.  An entry that names no row of the sequence moves nothing.  A sequence whose
+ * rows were not all appended, because it had no room, keeps none: lens_out[s] = L.  lens_out [n_seqs] may be
+ * pages->lens. */
 mj_status mj_pages_commit(mj_ctx* ctx, const mj_pages* pages, const mj_batch* batch,
                           const int32_t* accepted, const int32_t* path, int32_t* lens_out);
 
 /* mj_qkv_append for a batch: queries and keys normed (a NULL weight: not), rotated at their positions,
- * keys and values written to layer `layer` of the sequences' pages.  qkv fp16 [rows] rows of ld_qkv halves
+ * keys and values written to layer `layer` of the sequences' pages (of a sequence without room: not, and never
+ * over another sequence's tokens).  qkv fp16 [rows] rows of ld_qkv halves
  * (0: packed; else a multiple of 8), q_out fp16 [rows][n_heads * 128], not over qkv.  Reads n_heads,
  * n_kv_heads, head_dim, rope_dim, rope_base and eps of cfg. */
 mj_status mj_paged_append(mj_ctx* ctx, const mj_attn_config* cfg, const mj_pages* pages, int layer,

@@ -113,7 +113,8 @@ class KvRingStruct(C.Structure):
 
 class Pages(C.Structure):
     _fields_ = [("n_layers", i32), ("n_kv_heads", i32), ("n_pages", i32), ("page_tokens", i32), ("k", vp),
-                ("v", vp), ("table", vp), ("n_seqs", i32), ("table_stride", i32), ("lens", vp), ("refs", vp)]
+                ("v", vp), ("table", vp), ("n_seqs", i32), ("table_stride", i32), ("lens", vp), ("refs", vp),
+                ("served", vp)]
 
 
 class Batch(C.Structure):

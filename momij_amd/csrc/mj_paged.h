@@ -11,6 +11,9 @@
 #define PG_MAX_SEQS 1024
 #define PG_MAX_LAYERS 4096
 #define PG_NEED 3           // blocks that MJ_ROWS rows touch at most (pages of 32 and more)
+#define PG_REFUSED 0        // of a sequence: the last call for room had none for its rows
+#define PG_SERVED 1         // it had
+#define PG_UNKNOWN -1       // nobody asked since its pages were another's too, or cut
 
 struct PgPool {
     uint16_t* k;  // [n_layers][n_pages][nKV][page * 128]
@@ -18,6 +21,7 @@ struct PgPool {
     int32_t* table;  // [n_seqs][stride]
     int32_t* lens;   // [n_seqs]
     int32_t* refs;   // [n_pages]
+    int32_t* served;  // [n_seqs] or nullptr: PG_REFUSED, PG_SERVED, others
     int nKV, n_pages, page, shift, n_seqs, stride, n_layers;  // page = 1 << shift tokens
     __host__ __device__ size_t head_halves() const { return (size_t)page * 128; }
     __host__ __device__ size_t layer_halves() const { return (size_t)n_pages * nKV * page * 128; }
@@ -127,6 +131,28 @@ __device__ __forceinline__ int pg_page(const PgPool& p, int s, int j) {
     if ((unsigned)j >= (unsigned)p.stride) return -1;
     const int pg = p.table[(size_t)s * p.stride + j];
     return (unsigned)pg < (unsigned)p.n_pages ? pg : -1;
+}
+// Whether rows of a sequence may be written to a page of its table.  Where it was served: from its length on its
+// pages hold nothing that is another's (those that others named were left then; a branch made since has
+// the tokens before that length only, and its own call for room gives it other pages; a branch's and a cut
+// sequence's word is PG_UNKNOWN).  Where it is not known, the page's count tells.
+__device__ __forceinline__ int pg_word(const PgPool& p, int s) { return p.served ? p.served[s] : PG_UNKNOWN; }
+__device__ __forceinline__ bool pg_own(const PgPool& p, int word, int pg) {
+    return word == PG_SERVED || (word != PG_REFUSED && p.refs[pg] <= 1);
+}
+// Whether all of m rows from the length L on could be written.
+__device__ __forceinline__ bool pg_stored(const PgPool& p, int s, int L, int m) {
+    const int word = pg_word(p, s), first = L >> p.shift, n = m > 0 ? ((L + m - 1) >> p.shift) - first + 1 : 0;
+    int pg[PG_NEED];
+#pragma unroll
+    for (int i = 0; i < PG_NEED; ++i) pg[i] = i < n ? pg_page(p, s, first + i) : 0;
+    bool all = true, own = true;
+#pragma unroll
+    for (int i = 0; i < PG_NEED; ++i) {
+        all &= pg[i] >= 0;
+        own &= i >= n || p.refs[max(pg[i], 0)] <= 1;
+    }
+    return all && (word == PG_SERVED || (word != PG_REFUSED && own));
 }
 // The sequence that row r belongs to (n_seqs: none), by one round of loads of a whole wave.
 __device__ __forceinline__ int pg_seq(const PgRows& b, int r) {

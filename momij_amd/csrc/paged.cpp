@@ -28,12 +28,12 @@ mj_status check_pages(mj_ctx* ctx, const mj_pages* c, const char* what, PgPool& 
         return mj_fail(ctx, MJ_INVALID_ARG,
                        "%s: n_layers=%d n_kv_heads=%d n_pages=%d n_seqs=%d table_stride=%d", what,
                        c->n_layers, c->n_kv_heads, c->n_pages, c->n_seqs, c->table_stride);
-    if (!aligned16({c->k, c->v, c->table, c->lens, c->refs}))
+    if (!aligned16({c->k, c->v, c->table, c->lens, c->refs, c->served}))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: the pages' arrays need 16-byte alignment", what);
     int shift = 5;
     while (1 << shift < c->page_tokens) ++shift;
-    p = PgPool{(uint16_t*)c->k, (uint16_t*)c->v, c->table, c->lens, c->refs, c->n_kv_heads, c->n_pages,
-               c->page_tokens, shift, c->n_seqs, c->table_stride, c->n_layers};
+    p = PgPool{(uint16_t*)c->k, (uint16_t*)c->v, c->table, c->lens, c->refs, c->served, c->n_kv_heads,
+               c->n_pages, c->page_tokens, shift, c->n_seqs, c->table_stride, c->n_layers};
     return MJ_OK;
 }
 
@@ -91,6 +91,7 @@ bool over_any(Span a, std::initializer_list<Span> others) {
 Span table_of(const PgPool& p) { return {p.table, (size_t)p.n_seqs * p.stride * 4}; }
 Span lens_of(const PgPool& p) { return {p.lens, (size_t)p.n_seqs * 4}; }
 Span refs_of(const PgPool& p) { return {p.refs, (size_t)p.n_pages * 4}; }
+Span served_of(const PgPool& p) { return {p.served, (size_t)p.n_seqs * 4}; }
 Span starts_of(const PgRows& b) { return {b.start, (size_t)(b.n_seqs + 1) * 4}; }
 
 }  // namespace
@@ -197,7 +198,8 @@ mj_status mj_pages_reserve(mj_ctx* ctx, const mj_pages* pages, const mj_batch* b
     if (s == MJ_OK) s = check_batch(ctx, batch, p.n_seqs, what, b);
     if (s != MJ_OK) return s;
     if (!out || !aligned16({out}) ||
-        over_any({out, (size_t)p.n_seqs * 16}, {table_of(p), lens_of(p), refs_of(p), starts_of(b)}))
+        over_any({out, (size_t)p.n_seqs * 16},
+                 {table_of(p), lens_of(p), refs_of(p), served_of(p), starts_of(b)}))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: out null, unaligned or over another array", what);
     OnDevice on(ctx->device);
     return mj_hip(ctx, launch_pages_reserve(p, b, out, ctx->abort_dev, ctx->stream), what);
@@ -210,7 +212,7 @@ mj_status mj_pages_fork(mj_ctx* ctx, const mj_pages* pages, const int32_t* from)
     mj_status s = check_pages(ctx, pages, what, p);
     if (s != MJ_OK) return s;
     if (!from || ((uintptr_t)from & 3) ||
-        over_any({from, (size_t)p.n_seqs * 4}, {table_of(p), lens_of(p), refs_of(p)}))
+        over_any({from, (size_t)p.n_seqs * 4}, {table_of(p), lens_of(p), refs_of(p), served_of(p)}))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: from null, unaligned or over another array", what);
     OnDevice on(ctx->device);
     return mj_hip(ctx, launch_pages_fork(p, from, ctx->abort_dev, ctx->stream), what);
@@ -223,7 +225,7 @@ mj_status mj_pages_truncate(mj_ctx* ctx, const mj_pages* pages, const int32_t* l
     mj_status s = check_pages(ctx, pages, what, p);
     if (s != MJ_OK) return s;
     // (each sequence's own number is read before its length is written: len may be the lengths)
-    if (!len || ((uintptr_t)len & 3) || over_any({len, (size_t)p.n_seqs * 4}, {table_of(p), refs_of(p)}) ||
+    if (!len || ((uintptr_t)len & 3) || over_any({len, (size_t)p.n_seqs * 4}, {table_of(p), refs_of(p), served_of(p)}) ||
         (len != p.lens && over_any({len, (size_t)p.n_seqs * 4}, {lens_of(p)})))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: len null, unaligned or over another array", what);
     OnDevice on(ctx->device);
@@ -242,7 +244,7 @@ mj_status mj_pages_commit(mj_ctx* ctx, const mj_pages* pages, const mj_batch* ba
     const Span acc{accepted, (size_t)p.n_seqs * 4}, way{path, (size_t)b.rows * 4};
     const Span to{lens_out, (size_t)p.n_seqs * 4};
     if (!accepted || !lens_out || ((uintptr_t)accepted & 3) || ((uintptr_t)path & 3) ||
-        ((uintptr_t)lens_out & 3) || over_any(to, {table_of(p), refs_of(p), starts_of(b), acc, way}) ||
+        ((uintptr_t)lens_out & 3) || over_any(to, {table_of(p), refs_of(p), served_of(p), starts_of(b), acc, way}) ||
         (lens_out != p.lens && over_any(to, {lens_of(p)})))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: null or unaligned pointer, or lens_out over another array",
                        what);

@@ -35,10 +35,11 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
     const int ab = abort_word(a.abort);
     if (t == 0) s_abort = ab;
     const int s = pg_seq(a.b, r);
-    int r0 = 0, m = 0, L = 0;
+    int r0 = 0, m = 0, L = 0, word = PG_UNKNOWN;
     if (s < a.b.n_seqs) {
         m = pg_rows(a.b, s, r0);
         L = pg_len(a.p, s);
+        word = pg_word(a.p, s);
     }
     const int local = r - r0;
     const bool row = local >= 0 && local < m;
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
         return;
     }
     const int slot = L + local, pg = pg_page(a.p, s, slot >> a.p.shift), tok = slot & (a.p.page - 1);
-    if (pg < 0) return;
+    if (pg < 0 || !pg_own(a.p, word, pg)) return;
     const int g = vec - a.nQ - (isv ? a.p.nKV : 0);
     const size_t at = a.layer * a.p.layer_halves() + ((size_t)pg * a.p.nKV + g) * a.p.head_halves();
     if (!isv) {
@@ -132,7 +133,10 @@ __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t*
     if (threadIdx.x == 0) s_abort = ab;
     __syncthreads();
     if (s_abort || want < 0) return;
-    if (threadIdx.x == 0) p.lens[s] = n;
+    if (threadIdx.x == 0) {
+        p.lens[s] = n;
+        if (p.served) p.served[s] = PG_UNKNOWN;
+    }
     give_back(p, s, (n + p.page - 1) >> p.shift);
 }
 
@@ -160,7 +164,10 @@ __global__ __launch_bounds__(256) void k_pages_fork(PgPool p, const int32_t* fro
         if (pg >= 0) atomicAdd(&p.refs[pg], 1);
         dst[j] = pg;
     }
-    if (threadIdx.x == 0) p.lens[s] = L;
+    if (threadIdx.x == 0) {
+        p.lens[s] = L;
+        if (p.served) p.served[s] = PG_UNKNOWN;
+    }
 }
 
 // Inclusive sum over a block of 1024 threads; *total: of all of them.
@@ -238,7 +245,10 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
     if (s == 0) s_abort = ab;
     __syncthreads();
     if (s_abort) {  // nobody is served (the copies that follow go by these records)
-        if (s < p.n_seqs) *(int4*)(out + 4 * s) = make_int4(0, 0, -1, -1);
+        if (s < p.n_seqs) {
+            *(int4*)(out + 4 * s) = make_int4(0, 0, -1, -1);
+            if (p.served && m > 0) p.served[s] = PG_REFUSED;
+        }
         return;
     }
     int want, found = 0;
@@ -278,6 +288,7 @@ __global__ __launch_bounds__(1024) void k_pages_reserve(PgPool p, PgRows b, int3
             }
     }
     *(int4*)(out + 4 * s) = res;
+    if (p.served && m > 0) p.served[s] = served ? PG_SERVED : PG_REFUSED;
 }
 
 // The committed tokens of the pages that were shared, copied to their new ones: block (layer and K or
@@ -332,6 +343,10 @@ __global__ __launch_bounds__(256) void k_pages_copy(PgPool p, const int32_t* mov
 // is written.  (A head a block: 17 us for 64 sequences and 24 layers; a head a turn, with the places looked
 // up for each: 26 us.)
 #define COMMIT_HEADS 4
+// How many rows of a sequence are kept, if they were all written (pg_stored).
+__device__ __forceinline__ int kept_rows(int s, int m, const int32_t* accepted) {
+    return m > 0 ? max(0, min(accepted[s], m - 1) + 1) : 0;
+}
 __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const int32_t* accepted,
                                                       const int32_t* path, int32_t* lens_out,
                                                       const int* abort) {
@@ -342,7 +357,8 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
     const int ab = abort_word(abort);
     int r0;
     const int m = pg_rows(b, s, r0), L = pg_len(p, s);
-    const int kept = m > 0 ? max(0, min(accepted[s], m - 1) + 1) : 0;
+    const bool stored = pg_stored(p, s, L, m);  // (its requests beside those for the path)
+    const int kept = kept_rows(s, m, accepted);
     if (t < 64) {  // rows that move, in order: where they lie in their page's first head, and where they go
         int from = t;
         if (path && t < kept) from = path[r0 + t];
@@ -362,13 +378,13 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
             s_to[at] = dst;
         }
         if (t == 0) {
-            s_n = __popcll(which);
+            s_n = stored ? __popcll(which) : 0;
             s_abort = ab;
         }
     }
     __syncthreads();
     if (s_abort) return;
-    if (blockIdx.x == 0 && blockIdx.z == 0 && t == 0 && lens_out) lens_out[s] = min(L + kept, p.room());
+    if (blockIdx.x == 0 && blockIdx.z == 0 && t == 0 && lens_out) lens_out[s] = stored ? min(L + kept, p.room()) : L;
     const int n = s_n;
     if (n == 0) return;
     uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
@@ -415,8 +431,7 @@ __global__ __launch_bounds__(256) void k_pages_lens(PgPool p, PgRows b, const in
     if (s >= p.n_seqs) return;
     int r0;
     const int m = pg_rows(b, s, r0), L = pg_len(p, s);
-    const int kept = m > 0 ? max(0, min(accepted[s], m - 1) + 1) : 0;
-    p.lens[s] = min(L + kept, p.room());
+    p.lens[s] = pg_stored(p, s, L, m) ? min(L + kept_rows(s, m, accepted), p.room()) : L;
 }
 
 hipError_t launch_pages_fork(const PgPool& p, const int32_t* from, const int* abort, hipStream_t st) {

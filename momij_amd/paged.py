@@ -6,7 +6,7 @@ A step of a batch in use (row_start int32 [n_seqs + 1], tokens and uniforms on t
 
     cache = PagedCache(ctx, n_seqs, n_pages, n_kv_heads, blocks, n_layers)
     batch = RowBatch(row_start, rows, max_rows, anc)            # anc None: chains
-    ctx.pages_reserve(cache, batch, reserved)                   # reserved[:, 0]: who has room
+    ctx.pages_reserve(cache, batch, reserved)                   # reserved[:, 0]: who has room; others stay as they are
     for l in range(n_layers):
         ctx.paged_append(cfg, cache, l, batch, qkv, q_norm_w, k_norm_w, q)
         ctx.paged_attn(cache, l, batch, q, n_heads, out, window)
@@ -19,6 +19,7 @@ A step of a batch in use (row_start int32 [n_seqs + 1], tokens and uniforms on t
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import nullcontext
 
 import torch
 
@@ -65,7 +66,8 @@ class RowBatch:
 class PagedCache:
     """A pool of n_pages pages for n_seqs sequences of at most `blocks` pages each: k and v fp16
     [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096], table int32 [n_seqs][blocks] (-1: none), lens
-    int32 [n_seqs], refs int32 [n_pages]."""
+    int32 [n_seqs], refs int32 [n_pages], served int32 [n_seqs] (by it a sequence that pages_reserve had no room
+    for is left out of the step; views of one pool that share a step share it)."""
 
     def __init__(self, ctx, n_seqs: int, n_pages: int, n_kv_heads: int, blocks: int, n_layers: int = 1,
                  page_tokens: int = 64):
@@ -77,37 +79,42 @@ class PagedCache:
         shape = (n_layers, n_pages, n_kv_heads, page_tokens // UNIT, 128 * UNIT)
         k, v = (zeros(*shape, dtype=torch.float16) for _ in range(2))
         table = zeros(n_seqs, blocks).fill_(-1)
-        lens, refs = zeros(n_seqs), zeros(n_pages)
+        lens, refs, served = zeros(n_seqs), zeros(n_pages), zeros(n_seqs).fill_(-1)
         torch.cuda.synchronize(device)  # they are in place for the context's stream
-        self._bind(ctx, k, v, table, lens, refs)
+        self._bind(ctx, k, v, table, lens, refs, served)
 
     @classmethod
-    def over(cls, ctx, k, v, table, lens, refs):
-        """Over tensors that are there already."""
+    def over(cls, ctx, k, v, table, lens, refs, served=None):
+        """Over tensors that are there already (served None: a new one, not known of any sequence)."""
         self = object.__new__(cls)
-        self._bind(ctx, k, v, table, lens, refs)
+        if served is None:
+            with torch.cuda.stream(ctx.stream) if lens.is_cuda else nullcontext():
+                served = torch.full_like(lens, -1)
+        self._bind(ctx, k, v, table, lens, refs, served)
         return self
 
-    def _bind(self, ctx, k, v, table, lens, refs):
+    def _bind(self, ctx, k, v, table, lens, refs, served):
         if k.dim() < 4 or k.shape != v.shape and k.shape[:3] != v.shape[:3] or k.numel() != v.numel():
             raise ValueError("pages: k and v [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096]")
         self.n_layers, self.n_pages, self.n_kv_heads = (int(x) for x in k.shape[:3])
         tokens = k.numel() // max(self.n_layers * self.n_pages * self.n_kv_heads * 128, 1)
         shapes = [(k, torch.float16, None), (v, torch.float16, None), (table, torch.int32, 2),
-                  (lens, torch.int32, 1), (refs, torch.int32, 1)]
+                  (lens, torch.int32, 1), (refs, torch.int32, 1), (served, torch.int32, 1)]
         for t, dtype, dim in shapes:
             if t.dtype != dtype or not t.is_contiguous() or dim not in (None, t.dim()) or (
                     t.get_device() != ctx.device):
                 raise ValueError(f"pages: contiguous {dtype} on device {ctx.device}, not {t.dtype} "
                                  f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
         self.n_seqs, self.blocks = (int(x) for x in table.shape)
-        if tokens % UNIT or lens.numel() != self.n_seqs or refs.numel() != self.n_pages:
+        if tokens % UNIT or refs.numel() != self.n_pages or lens.numel() != self.n_seqs or (
+                served.numel() != self.n_seqs):
             raise ValueError(f"pages of {tokens} tokens, {lens.numel()} lengths of {self.n_seqs} sequences, "
                              f"{refs.numel()} counts of {self.n_pages} pages")
         self.ctx, self.device, self.page_tokens = ctx, ctx.device, tokens
-        self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
+        self.k, self.v, self.table, self.lens, self.refs, self.served = k, v, table, lens, refs, served
         self._ref = C.byref(_lib.Pages(self.n_layers, self.n_kv_heads, self.n_pages, tokens, ptr(k), ptr(v),
-                                       ptr(table), self.n_seqs, self.blocks, ptr(lens), ptr(refs)))
+                                       ptr(table), self.n_seqs, self.blocks, ptr(lens), ptr(refs),
+                                       ptr(served)))
 
     def on(self, device: int):
         """The struct for a call on `device`."""
