@@ -360,18 +360,32 @@ __device__ __forceinline__ uint32_t clear_bad(u4v v[8]) {
     return __builtin_amdgcn_readfirstlane(my);
 }
 
+// Four outputs as fp16.  A mean of V lies among its numbers, but the weights under it are rounded and those in the
+// sum are not: up to 2^-11 more, by which fp16's greatest number would round to an infinity.
+__device__ __forceinline__ uint2 outputs(f4 o, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = o[i] * inv;
+        const uint32_t over = (__float_as_uint(x) & 0x7FFFFFFFu) - 0x477FF000u;  // from 65520 on
+        h[i] = (uint16_t)(f2h(x) - (over < 0x7F800000u - 0x477FF000u ? 1 : 0));  // (infinities and NaN stay)
+    }
+    return make_uint2(pack2(h[0], h[1]), pack2(h[2], h[3]));
+}
+
 // A tile's state out: its vectors v .. v + 15 finished, or as a partial result.
 __device__ __forceinline__ void write_tile(const PgAttnArgs& a, const PgSeg& S, int v, const PgTile& T, float l) {
     const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
     if (v + ln >= S.vend) return;
     if (S.whole) {
         const int r = (v + ln) / a.G, h = S.g * a.G + (v + ln) - r * a.G;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
         uint16_t* o = a.out + (S.su.r0 + r) * a.ldo + h * HD + 4 * lq;
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
-            *(uint2*)(o + 16 * dt) = make_uint2(pack2(f2h(T.o[dt][0] * inv), f2h(T.o[dt][1] * inv)),
-                                                pack2(f2h(T.o[dt][2] * inv), f2h(T.o[dt][3] * inv)));
+        for (int dt = 0; dt < 8; ++dt) {
+            *(uint2*)(o + 16 * dt) = outputs(T.o[dt], l);
+            __builtin_amdgcn_sched_barrier(0);  // (all of them at once take registers that the steps need)
+        }
         return;
     }
     const size_t at = (size_t)S.slot * a.cols + (v - S.v0) + ln;
@@ -837,9 +851,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
             o += s_o[i][d] * f;
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros)
-    *(uint2*)(out + 4 * d) = make_uint2(pack2(f2h(o[0] * inv), f2h(o[1] * inv)),
-                                        pack2(f2h(o[2] * inv), f2h(o[3] * inv)));
+    *(uint2*)(out + 4 * d) = outputs(o, l);
 }
 
 // Up to 16 vectors the blocks are of the first kernel, which needs no barriers: 131000 tokens, one vector a head
