@@ -97,7 +97,8 @@ class PagedCache:
         if k.dim() < 4 or k.shape != v.shape and k.shape[:3] != v.shape[:3] or k.numel() != v.numel():
             raise ValueError("pages: k and v [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096]")
         self.n_layers, self.n_pages, self.n_kv_heads = (int(x) for x in k.shape[:3])
-        tokens = k.numel() // max(self.n_layers * self.n_pages * self.n_kv_heads * 128, 1)
+        heads = self.n_layers * self.n_pages * self.n_kv_heads
+        tokens = k.numel() // max(heads * 128, 1)
         shapes = [(k, torch.float16, None), (v, torch.float16, None), (table, torch.int32, 2),
                   (lens, torch.int32, 1), (refs, torch.int32, 1), (served, torch.int32, 1)]
         for t, dtype, dim in shapes:
@@ -106,9 +107,9 @@ class PagedCache:
                 raise ValueError(f"pages: contiguous {dtype} on device {ctx.device}, not {t.dtype} "
                                  f"{tuple(t.shape)} of strides {t.stride()} on {t.device}")
         self.n_seqs, self.blocks = (int(x) for x in table.shape)
-        if tokens % UNIT or refs.numel() != self.n_pages or lens.numel() != self.n_seqs or (
-                served.numel() != self.n_seqs):
-            raise ValueError(f"pages of {tokens} tokens, {lens.numel()} lengths of {self.n_seqs} sequences, "
+        if tokens % UNIT or k.numel() != heads * tokens * 128 or refs.numel() != self.n_pages or (
+                lens.numel() != self.n_seqs) or served.numel() != self.n_seqs:
+            raise ValueError(f"pages of {tokens} tokens ({k.numel()} halves), {lens.numel()} lengths of {self.n_seqs} sequences, "
                              f"{refs.numel()} counts of {self.n_pages} pages")
         self.ctx, self.device, self.page_tokens = ctx, ctx.device, tokens
         self.k, self.v, self.table, self.lens, self.refs, self.served = k, v, table, lens, refs, served

@@ -48,3 +48,10 @@ def test_outputs_over_it(call):  # noqa: F811
         fork(call, BAD, p=known(), src=at)
         truncate(call, BAD, p=known(), lens=at)
         commit(call, BAD, p=known(), lens=at)
+
+
+@pytest.mark.parametrize("shape", [(2, 4100), (1, 8200), (2, 4096 + 1), (8192 + 64,), (64, 130)])
+def test_pages_of_no_whole_tokens(ctx, shape):  # noqa: F811
+    """Halves of a head's page that are no multiple of a token's: the pages behind would be looked for elsewhere."""
+    with pytest.raises(ValueError):
+        cache_of(ctx, **{x: z(2, 8, 2, *shape) for x in "kv"})
