@@ -88,11 +88,23 @@ bool over_any(Span a, std::initializer_list<Span> others) {
         if (o.p && o.bytes && overlap(a.p, a.bytes, o.p, o.bytes)) return true;
     return false;
 }
+// Whether rows of `width` bytes at p in steps of ld lie over one of others (columns beside the rows do not count).
+bool rows_over_any(const void* p, int64_t ld, int64_t width, int rows, std::initializer_list<Span> others) {
+    for (const Span& o : others) {
+        if (!o.p || !o.bytes || !overlap(p, (rows - 1) * ld + width, o.p, o.bytes)) continue;
+        const int64_t d = (intptr_t)o.p - (intptr_t)p;
+        if (d < 0 || d % ld < width || d % ld + (int64_t)o.bytes > ld) return true;
+    }
+    return false;
+}
+Span k_of(const PgPool& p) { return {p.k, p.n_layers * p.layer_halves() * 2}; }
+Span v_of(const PgPool& p) { return {p.v, p.n_layers * p.layer_halves() * 2}; }
 Span table_of(const PgPool& p) { return {p.table, (size_t)p.n_seqs * p.stride * 4}; }
 Span lens_of(const PgPool& p) { return {p.lens, (size_t)p.n_seqs * 4}; }
 Span refs_of(const PgPool& p) { return {p.refs, (size_t)p.n_pages * 4}; }
 Span served_of(const PgPool& p) { return {p.served, (size_t)p.n_seqs * 4}; }
 Span starts_of(const PgRows& b) { return {b.start, (size_t)(b.n_seqs + 1) * 4}; }
+Span masks_of(const PgRows& b) { return {b.anc, (size_t)b.rows * 8}; }
 
 }  // namespace
 
@@ -126,6 +138,10 @@ mj_status mj_paged_append(mj_ctx* ctx, const mj_attn_config* cfg, const mj_pages
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: null or unaligned pointer", what);
     if (rows_overlap(qkv, ld_qkv * 2, width * 2, q_out, cfg->n_heads * 256, cfg->n_heads * 256, a.b.rows))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: q_out over qkv", what);
+    if (over_any({q_out, (size_t)a.b.rows * cfg->n_heads * 256},
+                 {k_of(a.p), v_of(a.p), table_of(a.p), lens_of(a.p), refs_of(a.p), served_of(a.p), starts_of(a.b),
+                  masks_of(a.b), {q_norm_w, 256}, {k_norm_w, 256}}))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: q_out over another array", what);
     a.qkv = (const uint16_t*)qkv;
     a.ld = ld_qkv;
     a.qw = (const uint16_t*)q_norm_w;
@@ -173,6 +189,10 @@ mj_status mj_paged_attn(mj_ctx* ctx, const mj_pages* pages, int layer, const mj_
     if (s != MJ_OK) return s;
     if (rows_overlap(q, ld_q * 2, width * 2, out, ld_out * 2, width * 2, a.b.rows))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: out over q", what);
+    const std::initializer_list<Span> read = {k_of(a.p),    v_of(a.p),      table_of(a.p), lens_of(a.p),
+                                              refs_of(a.p), served_of(a.p), starts_of(a.b), masks_of(a.b)};
+    if (rows_over_any(out, ld_out * 2, width * 2, a.b.rows, read))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: out over another array", what);
     a.q = (const uint16_t*)q;
     a.ldq = ld_q;
     a.out = (uint16_t*)out;
@@ -183,8 +203,12 @@ mj_status mj_paged_attn(mj_ctx* ctx, const mj_pages* pages, int layer, const mj_
     a.abort = ctx->abort_dev;
     OnDevice on(ctx->device);
     void* base = nullptr;
-    s = take_ws(ctx, ws, ws_bytes, paged_attn_plan(a, nullptr), what, &base);
+    const size_t need = paged_attn_plan(a, nullptr);
+    s = take_ws(ctx, ws, ws_bytes, need, what, &base);
     if (s != MJ_OK) return s;
+    if (ws && (over_any({ws, need}, read) || rows_over_any(q, ld_q * 2, width * 2, a.b.rows, {{ws, need}}) ||
+               rows_over_any(out, ld_out * 2, width * 2, a.b.rows, {{ws, need}})))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: the workspace over another array", what);
     paged_attn_plan(a, base);
     return mj_hip(ctx, launch_paged_attn(a, ctx->stream), what);
 }
@@ -199,7 +223,7 @@ mj_status mj_pages_reserve(mj_ctx* ctx, const mj_pages* pages, const mj_batch* b
     if (s != MJ_OK) return s;
     if (!out || !aligned16({out}) ||
         over_any({out, (size_t)p.n_seqs * 16},
-                 {table_of(p), lens_of(p), refs_of(p), served_of(p), starts_of(b)}))
+                 {k_of(p), v_of(p), table_of(p), lens_of(p), refs_of(p), served_of(p), starts_of(b)}))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: out null, unaligned or over another array", what);
     OnDevice on(ctx->device);
     return mj_hip(ctx, launch_pages_reserve(p, b, out, ctx->abort_dev, ctx->stream), what);
@@ -244,7 +268,7 @@ mj_status mj_pages_commit(mj_ctx* ctx, const mj_pages* pages, const mj_batch* ba
     const Span acc{accepted, (size_t)p.n_seqs * 4}, way{path, (size_t)b.rows * 4};
     const Span to{lens_out, (size_t)p.n_seqs * 4};
     if (!accepted || !lens_out || ((uintptr_t)accepted & 3) || ((uintptr_t)path & 3) ||
-        ((uintptr_t)lens_out & 3) || over_any(to, {table_of(p), refs_of(p), served_of(p), starts_of(b), acc, way}) ||
+        ((uintptr_t)lens_out & 3) || over_any(to, {k_of(p), v_of(p), table_of(p), refs_of(p), served_of(p), starts_of(b), acc, way}) ||
         (lens_out != p.lens && over_any(to, {lens_of(p)})))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: null or unaligned pointer, or lens_out over another array",
                        what);
@@ -291,12 +315,12 @@ mj_status mj_accept_rows(mj_ctx* ctx, const mj_batch* batch, const float* logits
         (R && (!logits || !tokens || !u_accept || !path)))
         return mj_fail(ctx, MJ_INVALID_ARG, "%s: null or unaligned pointer", what);
     const Span out[3] = {{accepted, n * 4}, {path, R * 4}, {token, n * 4}};
+    const std::initializer_list<Span> read = {starts_of(a.b), masks_of(a.b), {tokens, R * 4}, {temperature, n * 4},
+                                              {u_accept, R * 4}, {u_sample, n * 4},
+                                              {logits, R ? ((R - 1) * ld_logits + V) * 4 : 0},
+                                              {q, R ? ((R - 1) * ld_q + V) * 4 : 0}};
     for (int i = 0; i < 3; ++i)
-        if (out[i].bytes &&
-            over_any(out[i], {starts_of(a.b), {a.b.anc, R * 8}, {tokens, R * 4}, {temperature, n * 4},
-                              {u_accept, R * 4}, {u_sample, n * 4}, out[(i + 1) % 3],
-                              {logits, R ? ((R - 1) * ld_logits + V) * 4 : 0},
-                              {q, R ? ((R - 1) * ld_q + V) * 4 : 0}}))
+        if (out[i].bytes && (over_any(out[i], read) || over_any(out[i], {out[(i + 1) % 3]})))
             return mj_fail(ctx, MJ_INVALID_ARG, "%s: an output over another array", what);
     a.logits = logits;
     a.ld = ld_logits;
@@ -313,8 +337,11 @@ mj_status mj_accept_rows(mj_ctx* ctx, const mj_batch* batch, const float* logits
     a.abort = ctx->abort_dev;
     OnDevice on(ctx->device);
     void* base = nullptr;
-    s = take_ws(ctx, ws, ws_bytes, accept_rows_layout(a, nullptr), what, &base);
+    const size_t need = accept_rows_layout(a, nullptr);
+    s = take_ws(ctx, ws, ws_bytes, need, what, &base);
     if (s != MJ_OK) return s;
+    if (ws && (over_any({ws, need}, read) || over_any({ws, need}, {out[0], out[1], out[2]})))
+        return mj_fail(ctx, MJ_INVALID_ARG, "%s: the workspace over another array", what);
     accept_rows_layout(a, base);
     return mj_hip(ctx, launch_accept_rows(a, ctx->stream), what);
 }
