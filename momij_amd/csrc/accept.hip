@@ -54,10 +54,11 @@ struct Weights {
     double a, least;  // a d = -32000 at `least`: what lies below has no weight
     float m;
     const double* tab;
-    __device__ __forceinline__ Weights(double k, float top, const double* t) : m(top), tab(t) {
+    // k: 1 / T
+    __device__ __forceinline__ Weights(double T, double k, float top, const double* t) : m(top), tab(t) {
         // (an infinite temperature: a is not 0, so that -inf stays below everything, and any finite a d is)
         a = fmax(k * 46.16624130844683, 1e-60);  // 32 log2(e)
-        least = -32000.0 / a;
+        least = fmax(T * -693.1471805599453, -3.2e64);
     }
     __device__ __forceinline__ bool finite() const { return m < INFINITY; }
     // 2^(a d / 32) as a product
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256) void k_accept_stats(AcceptArgs a) {
             atomicMin(&s_at, at);
         }
         if (T > AC_GREEDY) {
-            const Weights e(1.0 / (double)T, m, s_tab);
+            const Weights e(T, 1.0 / (double)T, m, s_tab);
             if (e.finite()) {
 #pragma unroll
                 for (int i = 0; i < AC_PER; ++i) sum = e.onto(sum, y[i >> 2][i & 3]);
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     const int n = pg_rows(a.b, s, r0);
     const float T = a.temperature[s], u_sample = a.u_sample[s];
     const bool greedy = !(T > AC_GREEDY);
-    const double k = greedy ? 1.0 : 1.0 / (double)T;
+    const double temp = greedy ? 1.0 : (double)T, k = 1.0 / temp;
     // drafts and their logits, on their way while the totals are formed
     int par = -1, tok = -1;
     float x = -INFINITY, q = 1.0f, u = 0.0f;
@@ -421,7 +422,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
                     m = part[i].m;
                     at = part[i].at;
                 }
-            const Weights e(k, m, s_tab);
+            const Weights e(temp, k, m, s_tab);
             Z *= e(before);
 #pragma unroll
             for (int i = 0; i < 4; ++i) Z += c0 + 16 * i < a.chunks ? part[i].s * e(part[i].m) : 0.0;
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
                 at = oa;
             }
         }
-        Z *= Weights(k, m, s_tab)(mine);
+        Z *= Weights(temp, k, m, s_tab)(mine);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) Z += __shfl_xor(Z, o, 16);
         if ((t & 15) == 0) {
@@ -450,7 +451,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     if (t < 64) {
         double e = 0.0;
         if (par >= 0 && (unsigned)tok < (unsigned)a.V && s_Z[par] > 0.0)
-            e = greedy ? (tok == s_at[par] ? 1.0 : 0.0) : Weights(k, s_m[par], s_tab)(x);
+            e = greedy ? (tok == s_at[par] ? 1.0 : 0.0) : Weights(temp, k, s_m[par], s_tab)(x);
         const double uq = (double)u * (double)q;
         const uint64_t can = __ballot(q > 0.0f);
         int cur = 0, acc = 0, way = t == 0 ? 0 : -1;
@@ -508,8 +509,8 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
         }
         return;
     }
-    Left<AC_WALK> left{a.logits + row * a.ld, nullptr, a.part + (size_t)row * a.chunks, 0.0, Weights(k, s_m[cur], s_tab),
-              a.V, a.chunks, mode, n_out, s_left};
+    Left<AC_WALK> left{a.logits + row * a.ld, nullptr, a.part + (size_t)row * a.chunks, 0.0,
+              Weights(temp, k, s_m[cur], s_tab), a.V, a.chunks, mode, n_out, s_left};
     // The drafts' weights are known and taken off their chunks' sums, which have an error of 2^-53 of
     // themselves; where that is not small against what is left, the chunks are gone through again.
     bool exact = false;
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
               a.q ? a.q + last.row * a.ldq : nullptr,
               a.part + (size_t)last.row * a.chunks,
               1.0 / last.Z,
-              Weights(1.0 / (double)T, last.m, s_tab),
+              Weights(T, 1.0 / (double)T, last.m, s_tab),
               a.V,
               a.chunks,
               a.q ? LAST_RESIDUAL : LAST_WITHOUT,
