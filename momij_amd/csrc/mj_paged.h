@@ -136,23 +136,34 @@ __device__ __forceinline__ int pg_page(const PgPool& p, int s, int j) {
 // pages hold nothing that is another's (those that others named were left then; a branch made since has
 // the tokens before that length only, and its own call for room gives it other pages; a branch's and a cut
 // sequence's word is PG_UNKNOWN).  Where it is not known, the page's count tells.
-__device__ __forceinline__ int pg_word(const PgPool& p, int s) { return p.served ? p.served[s] : PG_UNKNOWN; }
-__device__ __forceinline__ bool pg_own(const PgPool& p, int word, int pg) {
-    return word == PG_SERVED || (word != PG_REFUSED && p.refs[pg] <= 1);
+__device__ __forceinline__ int pg_word(const PgPool& p, int s) {
+    const int word = p.served ? p.served[s] : PG_UNKNOWN;
+    return word == PG_SERVED || word == PG_REFUSED ? word : PG_UNKNOWN;
 }
-// Whether all of m rows from the length L on could be written.
+__device__ __forceinline__ bool pg_own(int word, int refs) {  // refs: of the page, or the greatest of several
+    return word == PG_SERVED || (word == PG_UNKNOWN && refs <= 1);
+}
+// Whether all of m rows from the length L on could be written.  (No branches: one after another the requests of three
+// blocks took 1.5 us.)
 __device__ __forceinline__ bool pg_stored(const PgPool& p, int s, int L, int m) {
     const int word = pg_word(p, s), first = L >> p.shift, n = m > 0 ? ((L + m - 1) >> p.shift) - first + 1 : 0;
-    int pg[PG_NEED];
+    const int32_t* row = p.table + (size_t)s * p.stride;
+    int pg[PG_NEED], refs[PG_NEED];
 #pragma unroll
-    for (int i = 0; i < PG_NEED; ++i) pg[i] = i < n ? pg_page(p, s, first + i) : 0;
-    bool all = true, own = true;
+    for (int i = 0; i < PG_NEED; ++i) pg[i] = row[min(first + i, p.stride - 1)];
+    bool all = first + n <= p.stride;
+    int most = 0;
 #pragma unroll
     for (int i = 0; i < PG_NEED; ++i) {
-        all &= pg[i] >= 0;
-        own &= i >= n || p.refs[max(pg[i], 0)] <= 1;
+        const bool there = (unsigned)pg[i] < (unsigned)p.n_pages;
+        all &= there | (i >= n);
+        pg[i] = there ? pg[i] : 0;
     }
-    return all && (word == PG_SERVED || (word != PG_REFUSED && own));
+#pragma unroll
+    for (int i = 0; i < PG_NEED; ++i) refs[i] = p.refs[pg[i]];
+#pragma unroll
+    for (int i = 0; i < PG_NEED; ++i) most = max(most, i < n ? refs[i] : 0);
+    return all & pg_own(word, most);
 }
 // The sequence that row r belongs to (n_seqs: none), by one round of loads of a whole wave.
 __device__ __forceinline__ int pg_seq(const PgRows& b, int r) {

@@ -43,6 +43,8 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
     }
     const int local = r - r0;
     const bool row = local >= 0 && local < m;
+    // (the page on its way before the angles, its count before the norm)
+    const int slot = L + local, pg = row ? pg_page(a.p, s, slot >> a.p.shift) : -1, tok = slot & (a.p.page - 1);
     if (t < a.half && row) {
         const int64_t pos = (int64_t)L + pg_depth(pg_anc(a.b, r, local), local);
         const double turn = (double)pos * a.turns[t];
@@ -52,6 +54,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
     }
     __syncthreads();
     if (s_abort || !row) return;
+    const int named = word == PG_UNKNOWN && pg >= 0 ? a.p.refs[pg] : 0;
     if (!isv) {
         float xa[8], xb[8], ss = 0.0f;
 #pragma unroll
@@ -91,8 +94,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PgAppendArgs a) {
         *(u4v*)(dst + 8 * pb) = vb;
         return;
     }
-    const int slot = L + local, pg = pg_page(a.p, s, slot >> a.p.shift), tok = slot & (a.p.page - 1);
-    if (pg < 0 || !pg_own(a.p, word, pg)) return;
+    if (pg < 0 || !pg_own(word, named)) return;
     const int g = vec - a.nQ - (isv ? a.p.nKV : 0);
     const size_t at = a.layer * a.p.layer_halves() + ((size_t)pg * a.p.nKV + g) * a.p.head_halves();
     if (!isv) {
@@ -351,13 +353,12 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
                                                       const int32_t* path, int32_t* lens_out,
                                                       const int* abort) {
     __shared__ int64_t s_from[MJ_ROWS], s_to[MJ_ROWS];
-    __shared__ int s_n, s_abort;
+    __shared__ int s_n, s_abort, s_stored;
     const int s = blockIdx.y, t = threadIdx.x;
     const bool isv = blockIdx.x & 1;
     const int ab = abort_word(abort);
     int r0;
     const int m = pg_rows(b, s, r0), L = pg_len(p, s);
-    const bool stored = pg_stored(p, s, L, m);  // (its requests beside those for the path)
     const int kept = kept_rows(s, m, accepted);
     if (t < 64) {  // rows that move, in order: where they lie in their page's first head, and where they go
         int from = t;
@@ -378,14 +379,17 @@ __global__ __launch_bounds__(256) void k_pages_commit(PgPool p, PgRows b, const 
             s_to[at] = dst;
         }
         if (t == 0) {
-            s_n = stored ? __popcll(which) : 0;
+            s_n = __popcll(which);
             s_abort = ab;
         }
+    } else if (t < 128) {  // (the second wave's requests beside the first one's)
+        const bool stored = pg_stored(p, s, L, m);
+        if (t == 64) s_stored = stored;
     }
     __syncthreads();
     if (s_abort) return;
-    if (blockIdx.x == 0 && blockIdx.z == 0 && t == 0 && lens_out) lens_out[s] = stored ? min(L + kept, p.room()) : L;
-    const int n = s_n;
+    if (blockIdx.x == 0 && blockIdx.z == 0 && t == 0 && lens_out) lens_out[s] = s_stored ? min(L + kept, p.room()) : L;
+    const int n = s_stored ? s_n : 0;
     if (n == 0) return;
     uint16_t* base = (isv ? p.v : p.k) + (blockIdx.x >> 1) * p.layer_halves();
     const int h0 = COMMIT_HEADS * blockIdx.z, h1 = min(h0 + COMMIT_HEADS, p.nKV), turn = 64 / n;
