@@ -358,7 +358,8 @@ typedef struct mj_pages {
      * none; others (to begin with, and after the sequence was forked into or cut): not known.  By this append
      * and commit leave out whoever has no room.  NULL: not known of any.  Where it is not known the counts
      * decide: rows that go to a page with refs above 1 are not written, and a step of which one row has no page, or
-     * such a page, is not kept. */
+     * such a page, is not kept.  (Then a branch made between a step's append and its commit has the step dropped;
+     * with 1 it does not.)  Who changes the table by other means than these calls sets it to -1. */
     int32_t* served;
 } mj_pages;
 

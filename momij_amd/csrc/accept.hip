@@ -99,7 +99,7 @@ typedef float __attribute__((ext_vector_type(4), aligned(4))) f4_any;
 
 // Sum of e, greatest logit and its lowest place of AC_CHUNK ids of a row.  Bound by memory and by its
 // operations in 64 bits alike: 324 rows of 151936 ids take 36 to 39 us, 33 at the rate of a streaming read, and
-// the VALU is busy 69% of it (64 roots, the place carried beside the maximum and a load an id: 53 us).
+// the VALU is busy 73% of it (64 roots, the place carried beside the maximum and a load an id: 53 us).
 __global__ __launch_bounds__(256) void k_accept_stats(AcceptArgs a) {
     __shared__ double s_tab[32], s_s[4];
     __shared__ float s_m[4];
@@ -356,8 +356,8 @@ struct Left {
 // The rows' totals and the walk over the drafts, a block a sequence; and the token, where it is the greatest
 // logit's, or is sampled from the row's sums by chunks as they are or with a few drafts taken out.
 // One block's steps one after another bound it, its instructions' own way to it among them: with 256 threads of
-// 16 ids each, four times the instructions, a sequence took 14 us, so 11.5 (10 without a chunk gone through
-// again).
+// 16 ids each, four times the instructions, a sequence took 14 us, so 11.5, and 9.7 where no chunk is gone
+// through again.
 #define AC_WALK 1024
 __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
     __shared__ double s_tab[32], s_Z[MJ_ROWS];
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(AC_WALK) void k_accept_walk(AcceptArgs a) {
 
 // What is left of the other sequences' last rows, a block a chunk; the block that comes last samples.  Bound
 // by its operations and a block's few steps one after another (48 rows of 151936 ids with distributions, 58 MB, 20
-// us, VALU 58% busy; by 1024 threads of four ids, one block a CU, 43, by 256 of 16 30).
+// us, VALU 64% busy; by 1024 threads of four ids, one block a CU, 43, by 256 of 16 30).
 #define AC_LEFT 512
 __global__ __launch_bounds__(AC_LEFT) void k_accept_left(AcceptArgs a) {
     __shared__ double s_tab[32];

@@ -455,8 +455,8 @@ __device__ __forceinline__ void edge_unit(PgTile* tl, const u4v (*q)[4], const P
 // time; a wave takes every fourth unit of it, straight from the pages into registers: a unit's bytes lie in
 // the order of the operands.  The next unit's K goes out behind a unit's scores, its V behind the output
 // products.  Page numbers of 64 units come with one request a lane.  The states meet in LDS.
-// Bound by HBM: one sequence of 131000 tokens and 4 heads takes 48 us; its 268 MB alone would
-// take 45 at the rate of a streaming read.
+// Bound by HBM: one sequence of 131000 tokens and 4 heads takes 50 us (least 49); its 268 MB alone
+// would take 45 at the rate of a streaming read.
 __global__ __launch_bounds__(256, 2) void k_paged_attn_own(PgAttnArgs a) {
     __shared__ PgPlan plan;
     __shared__ PgLeft s_left[3];
@@ -855,13 +855,14 @@ __global__ __launch_bounds__(256) void k_paged_join(PgAttnArgs a) {
 }
 
 // Up to 16 vectors the blocks are of the first kernel, which needs no barriers: 131000 tokens, one vector a head
-// 47.9 us against 51.6, 64 sequences of 200..8000 tokens 54.0 against 64, one of 300 10.7 against 18.  Past
-// 16 the ring's: the first kernel with two tiles spills (eight rows at 8000 tokens, four heads a group: 50
+// 50.4 us against 54.0, 64 sequences of 200..8000 tokens 55.6 against 62.9, one of 300 7.3 against 11.5.  (The greatest
+// count of rows decides for the whole batch: a chunk of 64 rows among 63 of one takes 99 us, the two in calls of their
+// own 78.)  Past 16 the ring's: the first kernel with two tiles spills (eight rows at 8000 tokens, four heads a group: 50
 // us against 32), and its waves would all read every unit.  One block of 256 vectors, though two of 128 would
 // divide the work more evenly: as fast (53.2 and 53.1 us), with half the reads.
 // A segment's beginning (its rows' queries, page numbers, the ring filled, the result written) costs as much
-// as 10 units of the ring (17 rows of 16 sequences 32.3 us; counted as 6 units 36) or 8 of the first kernel (64
-// sequences of 200..8000 tokens 51.5 us, as 2 units 53.1, as 16 52.5).
+// as 10 units of the ring (17 rows of 16 sequences 28.7 us; counted as 6 units 30.5) or 8 of the first kernel
+// (64 sequences of 200..8000 tokens 55.6 us, as 2 units 57.5, as 16 56.8).
 // A block takes four units at least, those that count for beginnings among them, so a short segment still has
 // several blocks (nine rows of four sequences of 200..400 tokens 18 us; with four units of keys at least 23).
 size_t paged_attn_plan(PgAttnArgs& a, void* base) {

@@ -66,8 +66,9 @@ class RowBatch:
 class PagedCache:
     """A pool of n_pages pages for n_seqs sequences of at most `blocks` pages each: k and v fp16
     [n_layers][n_pages][n_kv_heads][page_tokens / 32][4096], table int32 [n_seqs][blocks] (-1: none), lens
-    int32 [n_seqs], refs int32 [n_pages], served int32 [n_seqs] (by it a sequence that pages_reserve had no room
-    for is left out of the step; views of one pool that share a step share it)."""
+    int32 [n_seqs], refs int32 [n_pages], served int32 [n_seqs]: whether pages_reserve had room for the
+    sequence's rows (1, 0; -1: not known), by which the others are left out of the step.  Views of one pool
+    that make a step together share it; who changes the table by hand sets it to -1."""
 
     def __init__(self, ctx, n_seqs: int, n_pages: int, n_kv_heads: int, blocks: int, n_layers: int = 1,
                  page_tokens: int = 64):
