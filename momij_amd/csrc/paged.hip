@@ -131,13 +131,13 @@ __device__ __forceinline__ void give_back(const PgPool& p, int s, int first) {
 __global__ __launch_bounds__(256) void k_pages_truncate(PgPool p, const int32_t* len, const int* abort) {
     __shared__ int s_abort;
     const int ab = abort_word(abort);
-    const int s = blockIdx.x, want = len[s], n = min(want, pg_len(p, s));
+    const int s = blockIdx.x, want = len[s], L = pg_len(p, s), n = min(want, L);
     if (threadIdx.x == 0) s_abort = ab;
     __syncthreads();
     if (s_abort || want < 0) return;
     if (threadIdx.x == 0) {
         p.lens[s] = n;
-        if (p.served) p.served[s] = PG_UNKNOWN;
+        if (p.served && n < L) p.served[s] = PG_UNKNOWN;
     }
     give_back(p, s, (n + p.page - 1) >> p.shift);
 }

@@ -190,10 +190,12 @@ def test_the_one_that_is_left_alone_on_its_page(ctx, how):  # noqa: F811
     kept(cache, before)
 
 
+@pytest.mark.parametrize("give_back", [False, True])
 @pytest.mark.parametrize("when", ["before append", "before commit"])
-def test_a_branch_in_the_middle_of_a_step(ctx, when):  # noqa: F811
-    """A sequence that has room keeps its step, though a branch of its committed tokens is made meanwhile; the
-    branch is the committed tokens, also after it has gone on itself."""
+def test_a_branch_in_the_middle_of_a_step(ctx, when, give_back):  # noqa: F811
+    """A sequence that has room keeps its step, though a branch of its committed tokens is made meanwhile (and pages
+    behind the lengths are given back: the rows' is not one); the branch is the committed tokens, also after it has
+    gone on itself."""
     cache = filled(ctx, 2, 6, NKV, 6, 2, 32)
     Step(ctx, cache, [45, 0])()
     step = Step(ctx, cache, [6, 0], seed=1)
@@ -205,6 +207,8 @@ def test_a_branch_in_the_middle_of_a_step(ctx, when):  # noqa: F811
     step.accept()
     if when == "before commit":
         ctx.pages_fork(cache, cuda([-1, 0]))
+    if give_back:
+        ctx.pages_truncate(cache, cache.lens)
     step.commit()
     ctx.sync()
     assert cache.lens.tolist() == [51, 45]
@@ -341,6 +345,54 @@ def test_many_steps_of_a_pool_that_runs_out(ctx, n, n_pages, page, seed):  # noq
         book.truncate(cut)
         told = [t[:book.lens[s]] for s, t in enumerate(told)]
     assert refusals > 0
+
+
+@pytest.mark.parametrize("seed", range(3))
+@pytest.mark.parametrize("n,n_pages,page", [(9, 14, 32), (40, 60, 64)])
+def test_branches_in_the_middle_of_steps(ctx, n, n_pages, page, seed):  # noqa: F811
+    """Branches made before a step's append or before its commit: the source's step goes on, a branch that had rows
+    in it has lost them, and nobody's tokens are another's."""
+    rng = np.random.default_rng(50 + seed)
+    cache = filled(ctx, n, n_pages, NKV, 5, 1, page, seed)
+    book = book_of(cache)
+    told = [torch.zeros((0, NKV, D), dtype=torch.float64, device="cuda") for _ in range(n)]
+    made = 0
+    for i in range(14):
+        rows = [int(x) for x in np.where(rng.random(n) < 0.5, rng.integers(1, 12, n), 0)]
+        rows[0] = max(rows[0], 1)
+        step = Step(ctx, cache, rows, seed=100 * seed + i)
+        step.reserve()
+        want, _ = book.reserve(rows)
+        assert step.reserved.tolist() == want
+        src = [int(x) for x in np.where(rng.random(n) < 0.15, rng.integers(0, n, n), -1)]
+        goes = [src[s] >= 0 and src[s] != s and not (src[src[s]] >= 0 and src[src[s]] != src[s]) for s in range(n)]
+        when = i % 2
+        for phase in range(2):
+            if phase == when:
+                ctx.pages_fork(cache, cuda(src))
+                book.fork(src)
+                told = [told[src[s]] if goes[s] else told[s] for s in range(n)]
+                made += sum(goes)
+            if phase == 0:
+                step.append()
+        step.accepted.copy_(cuda([int(rng.integers(0, m)) if m else -1 for m in rows]))
+        step.commit("chain")
+        at = 0
+        for s, m in enumerate(rows):
+            k = step.accepted[s].item() + 1
+            if m and want[s][0] and not goes[s]:
+                book.lens[s] += k
+                told[s] = torch.cat([told[s], step.qkv[0][at:at + k].reshape(k, -1, D)[:, NQ + NKV:].double()])
+            at += m
+        same(cache, book)
+        assert book.named() == book.refs
+        for s in range(n):
+            assert torch.equal(R.rows_of(cache, 0, s, torch.arange(book.lens[s], device="cuda"))[1], told[s]), (i, s)
+        cut = [0 if rng.random() < 0.15 else -1 for _ in range(n)]
+        ctx.pages_truncate(cache, cuda(cut))
+        book.truncate(cut)
+        told = [t[:book.lens[s]] for s, t in enumerate(told)]
+    assert made > 5
 
 
 def test_an_aborted_call_for_room(ctx):  # noqa: F811
